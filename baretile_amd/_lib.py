@@ -67,6 +67,33 @@ class RopeArgs(ctypes.Structure):  # bt_rope_args
               ("pad_", c_int32)]
 
 
+class PagesArgs(ctypes.Structure):  # bt_pages
+  _fields_ = [("values", c_uint64), ("scales", c_uint64), ("pages", c_int32), ("page", c_int32), ("kv", c_int32),
+              ("head_dim", c_int32)]
+
+
+class PlanArgs(ctypes.Structure):  # bt_plan_args
+  _fields_ = [("tables", c_uint64), ("cached", c_uint64), ("fresh", c_uint64), ("free_pages", c_uint64),
+              ("taken", c_uint64), ("starts", c_uint64), ("lengths", c_uint64), ("places", c_uint64),
+              ("slots", c_uint64), ("taken_out", c_uint64), ("parts", c_uint64), ("tables_sr", c_int64),
+              ("requests", c_int32), ("width", c_int32), ("n_free", c_int32), ("rows", c_int32), ("page", c_int32),
+              ("pages", c_int32), ("most", c_int32), ("target", c_int32)]
+
+
+class BatchArgs(ctypes.Structure):  # bt_batch
+  _fields_ = [("tables", c_uint64), ("starts", c_uint64), ("lengths", c_uint64), ("parts", c_uint64),
+              ("tables_sr", c_int64), ("requests", c_int32), ("width", c_int32), ("rows", c_int32), ("most", c_int32),
+              ("target", c_int32), ("pad_", c_int32)]
+
+
+class VerifyArgs(ctypes.Structure):  # bt_verify_args
+  _fields_ = [("logits", c_uint64), ("probs", c_uint64), ("t", c_uint64), ("uniforms", c_uint64), ("ids", c_uint64),
+              ("starts", c_uint64), ("tokens", c_uint64), ("counts", c_uint64), ("scratch", c_uint64),
+              ("scratch_bytes", c_uint64), ("logits_sr", c_int64), ("probs_sr", c_int64), ("t_sr", c_int64),
+              ("uniforms_sr", c_int64), ("requests", c_int32), ("rows", c_int32), ("vocab", c_int32),
+              ("pad_", c_int32)]
+
+
 RT = c_void_p
 U64, I64 = c_uint64, c_int64
 # name: argument types. Every function returns an int status.
@@ -101,6 +128,12 @@ SIGNATURES = {
   "bt_gather": [RT, c_int, U64, I64, I64, I64, U64, I64, U64, I64],
   "bt_put": [RT, c_int, U64, I64, I64, I64, I64, I64, U64, I64, U64, I64, I64],
   "bt_topk": [RT, c_int, U64, I64, I64, I64, I64, I64, c_int32, c_int32, U64, I64, I64, U64, U64],
+  "bt_pages_plan": [RT, POINTER(PlanArgs)],
+  "bt_pages_put": [RT, POINTER(PagesArgs), POINTER(BatchArgs), U64, I64, I64],
+  "bt_pages_read": [RT, POINTER(PagesArgs), U64],
+  "bt_pages_attend_scratch": [POINTER(PagesArgs), POINTER(BatchArgs), c_int32, c_int32, POINTER(c_uint64)],
+  "bt_pages_attend": [RT, POINTER(PagesArgs), POINTER(BatchArgs), U64, I64, I64, U64, I64, I64, c_int32, c_int32, U64, U64],
+  "bt_verify_scratch": [POINTER(VerifyArgs), POINTER(c_uint64)], "bt_verify": [RT, POINTER(VerifyArgs)],
 }
 
 _lib = None

@@ -1,0 +1,950 @@
+// A paged 8-bit KV cache: the step's plan (block tables, row starts, places, slots) from request lengths, keys and values
+// put into their pages, attention over the pages, and the pages read back.
+//
+// A page holds `page` tokens of every key and value head under one id. A head's values are e4m3 codes (4 exponent and 3
+// mantissa bits, at most 448) times one power of two for the page and head, so each is exact in bf16 and the conversion
+// v_cvt_scalef32_pk_bf16_fp8 applies the scale: half an instruction a value, where a block float's decoding takes 2.5.
+// Keys are kept by row, [page][head width], and values by dimension, [head width][page], so that both products of
+// attention read their operands from memory as they lie, 16 bytes a lane, with no transposition and no trip through LDS:
+//   S^T = K Q^T: lane (n, g) (n = l % 16, g = l / 16) holds for tile kt (of 4 in a block of 64 keys) the key
+//     16 (n / 4) + 4 kt + n % 4, dims 64 j + 16 g .. + 15 (the contraction takes dims in any order that both operands share);
+//   so in the result lane (n, g) holds keys 16 g + 4 kt + i, i < 4, against pair n: 16 keys in a row over the 4 tiles;
+//   O^T = V^T P^T: the second operand is the lane's own P, the first 16 bytes of dim 16 c + n: keys 16 g .. + 15.
+// O^T's column is the lane's pair as well, so the running maximum rescales it with no move between lanes.
+#include "common.h"
+#include <algorithm>
+
+namespace bt {
+
+typedef short bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int KB = 64;          // keys of a block
+constexpr int MOST_PARTS = 64;  // parts of one request
+constexpr int MOST_REQUESTS = 2048;
+
+// ---- the plan ------------------------------------------------------------------------------------------------------
+
+struct PlanArgs {
+  int32_t *tables;
+  const int32_t *cached, *fresh, *free_pages, *taken;
+  int32_t *starts, *lengths, *places, *slots, *taken_out, *parts;
+  int64_t tables_sr;
+  int32_t requests, width, n_free, rows, page_log2, pages, most, target;
+};
+
+__device__ __forceinline__ int pages_of(int n, int lg) { return (n + (1 << lg) - 1) >> lg; }
+
+// The sum of x over the lower threads of the block, and the block's total. `sums`: a word of LDS a wave.
+template <int NT> __device__ __forceinline__ int block_exclusive(int x, int *sums, int *total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int inc = x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const int up = __shfl_up(inc, d, 64);
+    if (lane >= d) inc += up;
+  }
+  __syncthreads();
+  if (lane == 63) sums[w] = inc;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) {
+    const int s = sums[i];
+    before += i < w ? s : 0, all += s;
+  }
+  *total = all;
+  return before + inc - x;
+}
+
+// The request that owns row j: the last one that starts at or before it.
+__device__ __forceinline__ int owner_of(const int *starts, int requests, int j) {
+  int lo = 0, hi = requests;  // starts[lo] <= j < starts[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= j) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// The place and slot of row j (-1 past the last request's).
+__device__ __forceinline__ void plan_row(const PlanArgs &a, int j, int start, int cached, int id_or_free, bool real) {
+  const int place = cached + j - start, mask = (1 << a.page_log2) - 1;
+  a.places[j] = real ? place : -1;
+  a.slots[j] = real && id_or_free >= 0 ? (id_or_free << a.page_log2) + (place & mask) : -1;
+}
+
+// One block. Requests are scanned 1024 at a time: first their rows, cut to `most` each and to the rows there are, and the
+// pages they take; then, with the keys' blocks counted, the parts that attention cuts each request's keys into: as many
+// parts over all requests as `target`, of whole blocks of 64 keys, so that uneven lengths make parts of even length.
+// Latency bounds it: three scans of about a microsecond and two trips to memory.
+constexpr int PLAN_NT = 1024;
+constexpr int PLAN_ROWS = 2048;  // rows that the plan's one block writes itself; more go to plan_rows_kernel's many
+__global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
+  __shared__ int starts[MOST_REQUESTS + 1], first[MOST_REQUESTS], from[MOST_REQUESTS + 1], cache[MOST_REQUESTS];
+  __shared__ int sums[PLAN_NT / 64];
+  const int lg = a.page_log2, room = (int)min((int64_t)a.width << lg, (int64_t)0x40000000);
+  const int taken = a.taken ? gload(a.taken) : 0;
+  int rows = 0, takes = 0, blocks = 0;
+  for (int base = 0; base < a.requests; base += PLAN_NT) {
+    const int r = base + threadIdx.x;
+    int c = 0, n = 0, total;
+    if (r < a.requests) c = min(max(gload(a.cached + r), 0), room), n = min(max(gload(a.fresh + r), 0), a.most);
+    // at most 2^20 rows and 2^20 a request: a sum over 1024 requests keeps to 31 bits
+    const int s = rows + block_exclusive<PLAN_NT>(n, sums, &total);
+    const int s0 = min(s, a.rows), s1 = min(s + n, a.rows);
+    rows = min(rows + total, a.rows);
+    n = s1 - s0;
+    int k = 0, need = 0;
+    if (r < a.requests) {
+      const int end = min(pages_of(c + n, lg), a.width);
+      k = pages_of(c, lg);
+      const int32_t *row = a.tables + r * a.tables_sr;
+      while (k < end && (uint32_t)row[k] < (uint32_t)a.pages) k++;
+      need = max(end - k, 0);
+      starts[r] = s0, first[r] = k, cache[r] = c;
+      a.starts[r] = s0, a.lengths[r] = c + n;
+    }
+    const int off = block_exclusive<PLAN_NT>(need, sums, &total);
+    if (r < a.requests) from[r] = takes + off;
+    takes += total;
+    block_exclusive<PLAN_NT>(n > 0 ? (min(c + n, room) + KB - 1) / KB : 0, sums, &total);
+    blocks += total;
+  }
+  const int last = rows;
+  if (threadIdx.x == 0) {
+    starts[a.requests] = last, from[a.requests] = takes;
+    a.starts[a.requests] = last;
+    a.taken_out[0] = taken + takes;
+  }
+  const int per = max(1, (blocks + a.target - 1) / a.target);
+  int made = 0;
+  __syncthreads();
+  for (int base = 0; base < a.requests; base += PLAN_NT) {
+    const int r = base + threadIdx.x;
+    int parts = 0, total;
+    if (r < a.requests) {
+      const int n = starts[r + 1] - starts[r], nb = n > 0 ? (min(cache[r] + n, room) + KB - 1) / KB : 0;
+      const int mine = max(per, (nb + MOST_PARTS - 1) / MOST_PARTS);
+      parts = (nb + mine - 1) / mine;
+    }
+    const int off = block_exclusive<PLAN_NT>(parts, sums, &total);
+    if (r < a.requests) a.parts[r] = made + off;
+    made += total;
+  }
+  if (threadIdx.x == 0) a.parts[a.requests] = made, a.parts[a.requests + 1] = per;
+  auto page_at = [&](int e) {  // the free list's page e, or -1
+    if ((uint32_t)e >= (uint32_t)a.n_free) return -1;
+    const int id = gload(a.free_pages + e);
+    return (uint32_t)id < (uint32_t)a.pages ? id : -1;
+  };
+  for (int e = threadIdx.x; e < takes; e += PLAN_NT) {
+    const int r = owner_of(from, a.requests, e);
+    a.tables[r * a.tables_sr + first[r] + e - from[r]] = page_at(taken + e);
+  }
+  if (a.rows > PLAN_ROWS) return;
+  for (int j = threadIdx.x; j < a.rows; j += PLAN_NT) {
+    const bool real = j < last;
+    const int r = real ? owner_of(starts, a.requests, j) : 0;
+    const int on = (cache[r] + j - starts[r]) >> lg;
+    int id = -1;
+    if (real && on < a.width) {
+      if (on >= first[r]) id = page_at(taken + from[r] + on - first[r]);
+      else id = gload(a.tables + r * a.tables_sr + on);
+      if ((uint32_t)id >= (uint32_t)a.pages) id = -1;
+    }
+    plan_row(a, j, starts[r], cache[r], id, real);
+  }
+}
+
+// The rows' places and slots from the finished tables.
+__global__ void __launch_bounds__(256) plan_rows_kernel(const PlanArgs a) {
+  const int j = blockIdx.x * 256 + threadIdx.x;
+  if (j >= a.rows) return;
+  const bool real = j < gload(a.starts + a.requests);
+  const int r = real ? owner_of(a.starts, a.requests, j) : 0;
+  const int start = a.starts[r], cached = a.lengths[r] - (a.starts[r + 1] - start);
+  const int on = (cached + j - start) >> a.page_log2;
+  int id = real && on < a.width ? gload(a.tables + r * a.tables_sr + on) : -1;
+  if ((uint32_t)id >= (uint32_t)a.pages) id = -1;
+  plan_row(a, j, start, cached, id, real);
+}
+
+// ---- rows into pages ------------------------------------------------------------------------------------------------
+
+struct PoolArgs {
+  uint8_t *values;
+  float *scales;
+  int32_t pages, page_log2, kv;
+};
+struct BatchArgs {
+  const int32_t *tables, *starts, *lengths, *parts;
+  int64_t tables_sr;
+  int32_t requests, width, rows;
+};
+
+// What one request of a batch is: its first row, rows and length, and which of its pieces a block takes.
+struct Piece {
+  int r, k, row0, n, len;
+};
+// The request whose pieces `before(i, starts[i])` .. `before(i + 1, ..)` hold piece `at`, found by the wave's lanes
+// together, 64 requests a trip to memory (a search by halves would be a trip a step).
+template <class F> __device__ __forceinline__ bool find_piece(const BatchArgs &b, int at, int lane, F before, Piece *p) {
+  for (int base = 0; base < b.requests; base += 64) {
+    const int i = min(base + lane, b.requests - 1);
+    const int s0 = gload(b.starts + i), s1 = gload(b.starts + i + 1), len = gload(b.lengths + i);
+    const int lo = before(i, s0), hi = before(i + 1, s1);
+    const uint64_t hit = __ballot(base + lane < b.requests && lo <= at && at < hi);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      p->r = base + l;
+      p->k = at - __builtin_amdgcn_readlane(lo, l);
+      p->row0 = __builtin_amdgcn_readlane(s0, l);
+      p->n = __builtin_amdgcn_readlane(s1, l) - p->row0;
+      p->len = __builtin_amdgcn_readlane(len, l);
+      return true;
+    }
+  }
+  return false;
+}
+
+// Two codes of x0, x1 in the low half: nearest even, at most 448 in size (a NaN, which no code stands for in a cache, 448).
+__device__ __forceinline__ uint32_t codes_of(float x0, float x1) {
+  x0 = __builtin_copysignf(fminf(fabsf(x0), 448.0f), x0), x1 = __builtin_copysignf(fminf(fabsf(x1), 448.0f), x1);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x0, x1, 0, false) & 0xFFFFu;
+}
+__device__ __forceinline__ uint32_t codes_of4(float x0, float x1, float x2, float x3) {
+  return codes_of(x0, x1) | codes_of(x2, x3) << 16;
+}
+// Four codes under another scale: times `by`, a power of two of at most 1.
+__device__ __forceinline__ uint32_t rescaled4(uint32_t w, float by) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w, true);
+  return codes_of4(lo[0] * by, lo[1] * by, hi[0] * by, hi[1] * by);
+}
+
+// The smallest power of two s with amax <= 448 s = 1.75 * 2^8 s, from 2^-100 to 2^119 (so that every value is a normal
+// bf16). amax is finite.
+__device__ __forceinline__ float scale_of(float amax) {
+  const uint32_t b = __float_as_uint(amax);
+  const int e = (int)(b >> 23) - ((b & 0x7FFFFFu) > 0x600000u ? 7 : 8);  // biased by 127
+  return __uint_as_float((uint32_t)min(max(e, 27), 246) << 23);
+}
+
+// A block: the rows that one request puts into one page of one head. Its rows are loaded once (up to 16 loads of 16 bytes
+// a thread, all at once), their largest finite size gives the scale, and a page that already holds rows and whose scale
+// grows has them rounded again. Values turn by dimension in LDS, so they are stored as whole words.
+template <int HD>
+__global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
+                                                        int64_t x_sr) {
+  constexpr int U = HD / 8, MOST = 256 * U / 256;  // 16-byte units of a row, loads a thread for the largest page
+  __shared__ float tops[4];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (256 + 4)];
+  const int tid = threadIdx.x, lane = tid & 63, lg = c.page_log2, page = 1 << lg, heads = 2 * c.kv;
+  const int at = blockIdx.x / heads, h = blockIdx.x - at * heads;
+  Piece p;
+  // request r owns pieces starts[r] / page + 2 r and on: at least as many as the pages its rows touch
+  if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> lg) + 2 * i; }, &p)) return;
+  const int cached = p.len - p.n, on = (cached >> lg) + p.k;
+  const int from = max(cached, on << lg), count = min(p.len, (on + 1) << lg) - from;
+  if (count <= 0 || on >= b.width) return;
+  const int id = gload(b.tables + p.r * b.tables_sr + on);
+  if ((uint32_t)id >= (uint32_t)c.pages) return;
+  const int held = from & (page - 1), units = count * U;
+  const uint16_t *src = x + h * x_sb + (int64_t)(p.row0 + from - cached) * x_sr;
+  float *scale_at = c.scales + (int64_t)id * heads + h;
+  const float old = held ? gload(scale_at) : 0.0f;
+  u32x4 v[MOST];
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    const int e = tid + 256 * i;
+    if (256 * i < units) v[i] = e < units ? gload((const u32x4 *)(src + e / U * x_sr + e % U * 8)) : u32x4{0, 0, 0, 0};
+  }
+#pragma unroll
+  for (int i = 0; i < MOST; i++)
+    if (256 * i < units)
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t lo = v[i][k] << 16 & 0x7FFFFFFFu, hi = v[i][k] & 0x7FFF0000u;
+        top = fmaxf(top, lo < 0x7F800000u ? __uint_as_float(lo) : 0.0f);
+        top = fmaxf(top, hi < 0x7F800000u ? __uint_as_float(hi) : 0.0f);
+      }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if (lane == 0) tops[tid >> 6] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+  const float s = fmaxf(scale_of(top), old), inv = __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, exact
+  const float by = old * inv;
+  uint8_t *to = c.values + ((int64_t)id * heads + h << lg) * HD;
+  if (h < c.kv) {  // keys: whole rows
+    if (held && by != 1.0f)
+      for (int e = tid; e < held * HD / 16; e += 256) {
+        u32x4 w = *(const u32x4 *)(to + 16 * e);
+#pragma unroll
+        for (int k = 0; k < 4; k++) w[k] = rescaled4(w[k], by);
+        *(u32x4 *)(to + 16 * e) = w;
+      }
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int e = tid + 256 * i;
+      if (256 * i < units && e < units) {
+        uint2 w;
+        const auto val = [&](int k) { return __uint_as_float(k & 1 ? v[i][k / 2] & 0xFFFF0000u : v[i][k / 2] << 16) * inv; };
+        w.x = codes_of4(val(0), val(1), val(2), val(3)), w.y = codes_of4(val(4), val(5), val(6), val(7));
+        *(uint2 *)(to + held * HD + 8 * e) = w;
+      }
+    }
+  } else {  // values: each dimension's codes lie along the page
+    const int line = page + 4;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int e = tid + 256 * i;
+      if (256 * i < units && e < units) {
+        const int row = held + e / U, dim = e % U * 8;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          const uint32_t w = codes_of(__uint_as_float(v[i][k] << 16) * inv, __uint_as_float(v[i][k] & 0xFFFF0000u) * inv);
+          turned[(dim + 2 * k) * line + row] = (uint8_t)w, turned[(dim + 2 * k + 1) * line + row] = (uint8_t)(w >> 8);
+        }
+      }
+    }
+    __syncthreads();
+    // whole words of 4 rows: from the page's start where its rows are rounded again, else from the word with the first new row
+    const int w0 = held && by != 1.0f ? 0 : held / 4, w1 = (held + count + 3) / 4, words = w1 - w0;
+    for (int e = tid; e < words * HD; e += 256) {
+      const int dim = e / words, w = w0 + e - dim * words;
+      uint32_t *word = (uint32_t *)(to + (dim << lg)) + w;
+      const uint32_t now = *(const uint32_t *)(turned + dim * line + 4 * w);
+      const int kept = min(max(held - 4 * w, 0), 4), end = min(held + count - 4 * w, 4);
+      if (kept == 0 && end == 4) {
+        *word = now;
+      } else {  // rows kept before the new ones, and what lies behind them
+        const uint32_t was = *word, before = by != 1.0f && kept ? rescaled4(was, by) : was;
+        const auto low = [](int n) { return n >= 4 ? 0xFFFFFFFFu : (1u << 8 * n) - 1; };
+        const uint32_t fresh = low(end) & ~low(kept);
+        *word = (now & fresh) | (before & low(kept)) | (was & ~low(end));
+      }
+    }
+  }
+  if (tid == 0) *scale_at = s;
+}
+
+// A block: one page of one head as bf16 rows.
+template <int HD>
+__global__ void __launch_bounds__(256) read_pages_kernel(const PoolArgs c, uint16_t *out) {
+  __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (256 + 4)];
+  const int tid = threadIdx.x, lg = c.page_log2, page = 1 << lg, heads = 2 * c.kv;
+  const int64_t unit = blockIdx.x;
+  const int h = (int)(unit % heads);
+  const uint8_t *from = c.values + (unit << lg) * HD;
+  uint16_t *to = out + (unit << lg) * HD;
+  const float s = gload(c.scales + unit);
+  const auto pair = [&](uint32_t w, bool up) {
+    return up ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, true))
+              : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
+  };
+  if (h < c.kv) {
+    for (int e = tid; e < page * HD / 8; e += 256) {
+      const uint2 w = gload((const uint2 *)(from + 8 * e));
+      *(uint4 *)(to + 8 * e) = make_uint4(pair(w.x, false), pair(w.x, true), pair(w.y, false), pair(w.y, true));
+    }
+    return;
+  }
+  const int line = page + 4, wl = lg - 2;
+  for (int e = tid; e < HD << wl; e += 256) {
+    const int dim = e >> wl, w = e & ((1 << wl) - 1);
+    *(uint32_t *)(turned + dim * line + 4 * w) = gload((const uint32_t *)(from + (dim << lg)) + w);
+  }
+  __syncthreads();
+  for (int e = tid; e < page * HD / 8; e += 256) {
+    const int row = e / (HD / 8), dim = e % (HD / 8) * 8;
+    uint32_t w[2] = {0, 0};
+#pragma unroll
+    for (int k = 0; k < 8; k++) w[k / 4] |= (uint32_t)turned[(dim + k) * line + row] << 8 * (k % 4);
+    *(uint4 *)(to + 8 * e) = make_uint4(pair(w[0], false), pair(w[0], true), pair(w[1], false), pair(w[1], true));
+  }
+}
+
+// ---- attention over pages --------------------------------------------------------------------------------------------
+
+struct AttendArgs {
+  PoolArgs c;
+  BatchArgs b;
+  const uint16_t *q;
+  uint16_t *out;
+  float *scratch;
+  int64_t q_sh, q_sr, o_sh, o_sr;
+  int32_t rep, window, items, few;  // items: the most parts a plan makes; few: the most query pairs that parts are for
+  FastDiv drep;
+};
+
+// Rows behind the last request's are zeros: block `at` clears 16 of them, every head.
+template <int HD> __device__ __forceinline__ void clear_rows(const AttendArgs &a, int at, int tid, int threads) {
+  const int last = gload(a.b.starts + a.b.requests), heads = a.c.kv * a.rep;
+  for (int j = max(16 * at, last); j < min(16 * at + 16, a.b.rows); j++)
+    for (int e = tid; e < heads * (HD / 8); e += threads) {
+      const int h = e / (HD / 8);
+      *(uint4 *)(a.out + h * a.o_sh + j * a.o_sr + e % (HD / 8) * 8) = make_uint4(0, 0, 0, 0);
+    }
+}
+
+// 64 of a request's pages from page `p0` on, one a lane: its id (-1: none, whose keys are hidden) and the head's scales.
+struct PageRun {
+  int id;
+  float ks, vs;
+};
+__device__ __forceinline__ PageRun page_run(const AttendArgs &a, int r, int kvh, int p0, int lane) {
+  const int p = p0 + lane;
+  PageRun w;
+  w.id = p < a.b.width ? gload(a.b.tables + r * a.b.tables_sr + p) : -1;
+  if ((uint32_t)w.id >= (uint32_t)a.c.pages) w.id = -1;
+  const float *s = a.c.scales + (int64_t)max(w.id, 0) * (2 * a.c.kv) + kvh;
+  w.ks = gload(s), w.vs = gload(s + a.c.kv);
+  return w;
+}
+
+__device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t lo, uint32_t hi, float s) {
+  u32x4 w;
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, true));
+  w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, false));
+  w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s, true));
+  return __builtin_bit_cast(bf16x8, w);
+}
+__device__ __forceinline__ uint32_t pack_rne(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){lo, hi}, bf16x2));
+}
+__device__ __forceinline__ float max_groups(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float sum_groups(float x) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+constexpr float LOG2E = 1.4426950408889634f;
+constexpr float INF = __builtin_inff();
+
+// 16 query pairs' running softmax: the reference maximum of the lane's pair in log2 units (p = 2^(s log2 e - m)), the sum
+// of the lane's own p, and O^T. The reference moves only where a block's maximum passes it by 2^8 (O / l is the same for
+// any reference, and p stays below 256), so most blocks rescale nothing.
+template <int HD> struct Running {
+  float m, l;
+  f32x4 o[HD / 16];
+  __device__ __forceinline__ void clear() {
+    m = -INF, l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < HD / 16; c++) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  // s: the block's scores, hidden keys at -inf; p: the lane's 16 weights as bf16, the second operand of the two 32-key
+  // steps of O^T. They are rounded to nearest; l sums them unrounded, in 32 bits.
+  __device__ __forceinline__ void weigh(const f32x4 (&s)[4], bf16x8 (&p)[2]) {
+    float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
+#pragma unroll
+    for (int kt = 1; kt < 4; kt++) top = fmaxf(top, fmaxf(fmaxf(s[kt][0], s[kt][1]), fmaxf(s[kt][2], s[kt][3])));
+    top = max_groups(top) * LOG2E;
+    if (__any(top > m + 8.0f)) {
+      const float now = fmaxf(m, top), by = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - now);
+      m = now, l *= by;
+#pragma unroll
+      for (int c = 0; c < HD / 16; c++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) o[c][i] *= by;
+    }
+    const float ref = m == -INF ? 0.0f : m;  // no key of the pair seen yet: every weight is 2^-inf = 0
+    u32x4 w[2];
+#pragma unroll
+    for (int kt = 0; kt < 4; kt++) {
+      float e[4];
+#pragma unroll
+      for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], LOG2E, -ref));
+      l += (e[0] + e[1]) + (e[2] + e[3]);
+      w[kt / 2][kt % 2 * 2] = pack_rne(e[0], e[1]), w[kt / 2][kt % 2 * 2 + 1] = pack_rne(e[2], e[3]);
+    }
+    p[0] = __builtin_bit_cast(bf16x8, w[0]), p[1] = __builtin_bit_cast(bf16x8, w[1]);
+  }
+};
+
+// The lane's query pair, its row of q in the operand's order, and the keys it sees.
+template <int HD> struct Query {
+  bf16x8 f[HD / 32];
+  int lo, hi;
+  __device__ __forceinline__ void load(const AttendArgs &a, const Piece &p, int kvh, int pair, int g) {
+    const bool real = pair < p.n * a.rep;
+    const int pp = real ? pair : 0, i = (int)fdiv((uint32_t)pp, a.drep), h = kvh * a.rep + pp - i * a.rep;
+    const uint16_t *q = a.q + h * a.q_sh + (p.row0 + i) * a.q_sr + 16 * g;
+#pragma unroll
+    for (int k = 0; k < HD / 32; k++) f[k] = gload((const bf16x8 *)(q + 64 * (k / 2) + 8 * (k % 2)));
+    hi = real ? p.len - p.n + i : -1;  // the row's place
+    lo = a.window > 0 ? max(hi - a.window + 1, 0) : 0;
+  }
+};
+
+// Where pair `pair`'s output row starts.
+__device__ __forceinline__ uint16_t *out_row(const AttendArgs &a, const Piece &p, int kvh, int pair) {
+  const int i = (int)fdiv((uint32_t)pair, a.drep), h = kvh * a.rep + pair - i * a.rep;
+  return a.out + h * a.o_sh + (p.row0 + i) * a.o_sr;
+}
+
+// One block of 64 keys against QT tiles of pairs. key: the lane's first key (its 16 are in a row), seen: whether their page
+// is one; keys(kt, j) and values(c): the lane's 16 codes of each piece; between: run once the scores are made.
+template <int HD, int QT, class Keys, class Values, class Between>
+__device__ __forceinline__ void fold_block(const Query<HD> (&q)[QT], Running<HD> (&st)[QT], int key, bool seen, float ks, float vs,
+                                           Keys keys, Values values, Between between) {
+  constexpr int J = HD / 64;
+  f32x4 s[QT][4];
+#pragma unroll
+  for (int kt = 0; kt < 4; kt++) {
+    bf16x8 kf[2 * J];
+#pragma unroll
+    for (int j = 0; j < J; j++) {
+      const u32x4 w = keys(kt, j);
+      kf[2 * j] = fp8_to_bf16(w[0], w[1], ks), kf[2 * j + 1] = fp8_to_bf16(w[2], w[3], ks);
+    }
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      s[t][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int k = 0; k < 2 * J; k++) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k], q[t].f[k], s[t][kt], 0, 0, 0);
+    }
+  }
+  between();
+  bf16x8 w[QT][2];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int lo = q[t].lo - key, hi = seen ? q[t].hi - key : -1;
+    if (!__all(lo <= 0 && hi >= 15)) {
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (4 * kt + i < lo || 4 * kt + i > hi) s[t][kt][i] = -INF;
+    }
+    st[t].weigh(s[t], w[t]);
+  }
+#pragma unroll
+  for (int c = 0; c < HD / 16; c++) {
+    const u32x4 x = values(c);
+    const bf16x8 v0 = fp8_to_bf16(x[0], x[1], vs), v1 = fp8_to_bf16(x[2], x[3], vs);
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      st[t].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, w[t][0], st[t].o[c], 0, 0, 0);
+      st[t].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, w[t][1], st[t].o[c], 0, 0, 0);
+    }
+  }
+}
+// The finished rows of a tile: O / l in bf16, 4 dims a store. A row that sees no key is zeros; a NaN stays one.
+template <int HD> __device__ __forceinline__ void store_rows(const AttendArgs &a, const Piece &p, int kvh, int pair, int g,
+                                                             const Running<HD> &st, float l) {
+  const float inv = l > 0.0f ? 1.0f / l : l;
+  uint16_t *out = out_row(a, p, kvh, pair) + 4 * g;
+#pragma unroll
+  for (int c = 0; c < HD / 16; c++)
+    *(uint2 *)(out + 16 * c) = make_uint2(pack_rne(st.o[c][0] * inv, st.o[c][1] * inv),
+                                          pack_rne(st.o[c][2] * inv, st.o[c][3] * inv));
+}
+
+// Few query pairs a request: a wave a part. A part is a run of whole blocks of 64 keys of one request, against QT tiles of
+// 16 of its pairs, so every key and value is read and converted once for all of them. A block's keys are requested while
+// the block before weighs its scores, its values while it multiplies, so 16 KB (heads of 128) are always in flight.
+template <int HD, int QT>
+__global__ void __launch_bounds__(64) pages_few_kernel(const AttendArgs a) {
+  constexpr int J = HD / 64, C = HD / 16;
+  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  if (blockIdx.x >= (uint32_t)(a.items * a.c.kv)) return clear_rows<HD>(a, blockIdx.x - a.items * a.c.kv, lane, 64);
+  const int item = blockIdx.x / a.c.kv, kvh = blockIdx.x - item * a.c.kv;
+  const int per = gload(a.b.parts + a.b.requests + 1);
+  Piece p;
+  const int32_t *at = a.b.parts;
+  if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p)) return;
+  const int pairs = p.n * a.rep;
+  if (pairs > a.few) return;
+  const int room = min(p.len, a.b.width << lg), nb = (room + KB - 1) / KB;
+  const int mine = max(per, (nb + MOST_PARTS - 1) / MOST_PARTS), parts = (nb + mine - 1) / mine;
+  int b0 = p.k * mine;
+  const int b1 = min(b0 + mine, nb);
+  if (a.window > 0) b0 = max(b0, max(p.len - p.n - a.window + 1, 0) / KB);
+  Query<HD> q[QT];
+  Running<HD> st[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) q[t].load(a, p, kvh, 16 * t + n, g), st[t].clear();
+  if (b0 < b1) {
+    const int64_t head = (int64_t)HD << lg;  // codes of one page of one head
+    int p0 = b0 * KB >> lg;
+    PageRun run = page_run(a, p.r, kvh, p0, lane);
+    u32x4 kw[4][J], vw[C];
+    float ks, vs, ks_next = 0, vs_next = 0;
+    int id_v, id_v_next = 0;
+    const auto turn = [&](int b) {  // the 64 pages that block b's keys lie in, if they are not there yet
+      if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, run = page_run(a, p.r, kvh, p0, lane);
+    };
+    const auto fetch_keys = [&](int b, float &s) {
+      const int key = b * KB + 16 * (n >> 2), from = (key >> lg) - p0;
+      const int id = max(__shfl(run.id, from, 64), 0);
+      s = __shfl(run.ks, from, 64);
+      const uint8_t *k = a.c.values + ((int64_t)id * (2 * a.c.kv) + kvh) * head + ((key & mask) + (n & 3)) * HD + 16 * g;
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+        for (int j = 0; j < J; j++) kw[kt][j] = __builtin_nontemporal_load((const u32x4 *)(k + 4 * kt * HD + 64 * j));
+    };
+    const auto fetch_values = [&](int b, float &s, int &valid) {
+      const int key = b * KB + 16 * g, from = (key >> lg) - p0;
+      valid = __shfl(run.id, from, 64);
+      s = __shfl(run.vs, from, 64);
+      const uint8_t *v = a.c.values + ((int64_t)max(valid, 0) * (2 * a.c.kv) + a.c.kv + kvh) * head + (n << lg) + (key & mask);
+#pragma unroll
+      for (int c = 0; c < C; c++) vw[c] = __builtin_nontemporal_load((const u32x4 *)(v + (c << (lg + 4))));
+    };
+    fetch_keys(b0, ks);
+    fetch_values(b0, vs, id_v);
+    for (int b = b0; b < b1; b++) {
+      const bool more = b + 1 < b1;
+      fold_block<HD, QT>(q, st, b * KB + 16 * g, id_v >= 0, ks, vs, [&](int kt, int j) { return kw[kt][j]; },
+                         [&](int c) { return vw[c]; }, [&] {
+                           if (more) turn(b + 1), fetch_keys(b + 1, ks_next);
+                         });
+      if (more) fetch_values(b + 1, vs_next, id_v_next);
+      ks = ks_next, vs = vs_next, id_v = id_v_next;
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int pair = 16 * t + n;
+    const float l = sum_groups(st[t].l);
+    if (pair >= pairs) continue;
+    if (parts == 1) {
+      store_rows<HD>(a, p, kvh, pair, g, st[t], l);
+    } else {  // the part's sums for the combine: O by pair, then the pairs' maxima and sums
+      float *to = a.scratch + ((int64_t)item * a.c.kv + kvh) * (16 * QT * (HD + 2));
+#pragma unroll
+      for (int c = 0; c < C; c++) *(f32x4 *)(to + pair * HD + 16 * c + 4 * g) = st[t].o[c];
+      if (g == 0) to[16 * QT * HD + 2 * pair] = st[t].m, to[16 * QT * HD + 2 * pair + 1] = l;
+    }
+  }
+}
+
+// Joins a request's parts: block (request, key head, pair), its 4 waves a quarter of the parts each, then each other's
+// sums through LDS: M = max m, L = sum 2^(m - M) l, out = sum 2^(m - M) O / L.
+template <int HD, int QT>
+__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a, int most_pairs) {
+  constexpr int V = HD / 64, STRIDE = 16 * QT * (HD + 2), TURN = 8;
+  __shared__ float ms[4], ls[4], os[4][HD];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int u = blockIdx.x;
+  const int pair = u % most_pairs;
+  u /= most_pairs;
+  const int kvh = u % a.c.kv, r = u / a.c.kv;
+  const int row0 = gload(a.b.starts + r), n = gload(a.b.starts + r + 1) - row0, first = gload(a.b.parts + r);
+  const int parts = gload(a.b.parts + r + 1) - first;
+  if (parts <= 1 || pair >= n * a.rep || n * a.rep > a.few) return;
+  const float *from = a.scratch + ((int64_t)first * a.c.kv + kvh) * STRIDE;
+  const int64_t step = (int64_t)a.c.kv * STRIDE;
+  float M = -INF, L = 0.0f, O[V];
+#pragma unroll
+  for (int i = 0; i < V; i++) O[i] = 0.0f;
+  for (int b = w; b < parts; b += 4 * TURN) {
+    float m[TURN], l[TURN], o[TURN][V];
+#pragma unroll
+    for (int j = 0; j < TURN; j++) {  // past the last part it is read again and left out
+      const float *s = from + min(b + 4 * j, parts - 1) * step;
+      m[j] = gload(s + 16 * QT * HD + 2 * pair), l[j] = gload(s + 16 * QT * HD + 2 * pair + 1);
+#pragma unroll
+      for (int i = 0; i < V; i++) o[j][i] = gload(s + pair * HD + V * lane + i);
+    }
+    float top = M;
+#pragma unroll
+    for (int j = 0; j < TURN; j++) {
+      if (b + 4 * j >= parts) m[j] = -INF, l[j] = 0.0f;
+      top = fmaxf(top, m[j]);
+    }
+    const float keep = M == -INF ? 0.0f : __builtin_amdgcn_exp2f(M - top);
+    L *= keep;
+#pragma unroll
+    for (int i = 0; i < V; i++) O[i] *= keep;
+#pragma unroll
+    for (int j = 0; j < TURN; j++) {
+      if (m[j] == -INF && l[j] == 0.0f) continue;  // nothing seen; its O was not written
+      const float by = __builtin_amdgcn_exp2f(m[j] - top);
+      L += by * l[j];
+#pragma unroll
+      for (int i = 0; i < V; i++) O[i] += by * o[j][i];
+    }
+    M = top;
+  }
+  if (lane == 0) ms[w] = M, ls[w] = L;
+#pragma unroll
+  for (int i = 0; i < V; i++) os[w][V * lane + i] = O[i];
+  __syncthreads();
+  if (threadIdx.x >= HD / 2) return;
+  const float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
+  float sum = 0.0f, x = 0.0f, y = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (ms[i] == -INF && ls[i] == 0.0f) continue;
+    const float by = __builtin_amdgcn_exp2f(ms[i] - top);
+    sum += by * ls[i], x += by * os[i][2 * threadIdx.x], y += by * os[i][2 * threadIdx.x + 1];
+  }
+  const float inv = sum > 0.0f ? 1.0f / sum : sum;
+  const int i = (int)fdiv((uint32_t)pair, a.drep), h = kvh * a.rep + pair - i * a.rep;
+  *(uint32_t *)(a.out + h * a.o_sh + (row0 + i) * a.o_sr + 2 * threadIdx.x) = pack_rne(x * inv, y * inv);
+}
+
+// Many query pairs a request (a prompt's rows): a block of 4 waves takes 128 pairs of one key head, 32 a wave, so every
+// fragment that a wave converts feeds two matrix instructions. Blocks of 64 keys and values pass through LDS as codes, one
+// barrier a block, the next block's codes held in registers meanwhile. 16-byte units are placed so that the 16 lanes of a
+// read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2) (heads of 64: u ^ (r / 16)), values'
+// unit u of dim d at u ^ (d / 4) % 4.
+template <int HD>
+__global__ void __launch_bounds__(256, 2) pages_many_kernel(const AttendArgs a, int tiles) {
+  constexpr int C = HD / 16, UK = HD / 16, NU = HD * KB / 16 / 256;  // units of a key's row; units a thread
+  __shared__ __attribute__((aligned(16))) uint8_t kl[2][KB * HD], vl[2][KB * HD];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int slot = tiles - 1 - blockIdx.x / a.c.kv, kvh = blockIdx.x % a.c.kv;  // the longest rows first
+  Piece p;
+  // request r owns tiles starts[r] * rep / 128 + r and on: at least as many as its pairs fill
+  if (!find_piece(a.b, slot, lane, [&](int i, int s) { return (int)((uint32_t)s * (uint32_t)a.rep >> 7) + i; }, &p)) return;
+  const int pairs = p.n * a.rep, pair0 = 128 * p.k;
+  if (pairs <= a.few || pair0 >= pairs) return;
+  Query<HD> q[2];
+  Running<HD> st[2];
+#pragma unroll
+  for (int t = 0; t < 2; t++) q[t].load(a, p, kvh, pair0 + 32 * wave + 16 * t + n, g), st[t].clear();
+  const int cached = p.len - p.n, room = min(p.len, a.b.width << lg);
+  const auto place = [&](int pair) { return cached + (int)fdiv((uint32_t)min(pair, pairs - 1), a.drep); };
+  const auto low = [&](int at) { return a.window > 0 ? max(at - a.window + 1, 0) : 0; };
+  const int b0 = low(place(pair0)) / KB, b1 = min(place(pair0 + 127), room - 1) / KB + 1;
+  // the wave's own keys: blocks outside them it only helps to bring in
+  const int wlo = low(place(pair0 + 32 * wave)), whi = pair0 + 32 * wave < pairs ? place(pair0 + 32 * wave + 31) : -1;
+  const int64_t head = (int64_t)HD << lg;
+  int p0 = b0 * KB >> lg;
+  PageRun run = page_run(a, p.r, kvh, p0, lane);
+  u32x4 kr[NU], vr[NU];
+  const auto fetch = [&](int b) {
+    if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, run = page_run(a, p.r, kvh, p0, lane);
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+      const int u = tid + 256 * i;
+      const int key = b * KB + u / UK, kid = max(__shfl(run.id, (key >> lg) - p0, 64), 0);
+      kr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)kid * (2 * a.c.kv) + kvh) * head + (key & mask) * HD + u % UK * 16));
+      const int vkey = b * KB + 16 * (u & 3), vid = max(__shfl(run.id, (vkey >> lg) - p0, 64), 0);
+      vr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)vid * (2 * a.c.kv) + a.c.kv + kvh) * head + (u / 4 << lg) + (vkey & mask)));
+    }
+  };
+  const auto turned = [](int row) { return HD == 128 ? row >> 4 << 1 | (row >> 1 & 1) : row >> 4; };
+  const auto store = [&](int to) {
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+      const int u = tid + 256 * i, row = u / UK, dim = u / 4;
+      *(u32x4 *)(kl[to] + row * HD + 16 * (u % UK ^ turned(row))) = kr[i];
+      *(u32x4 *)(vl[to] + dim * KB + 16 * ((u & 3) ^ (dim >> 2 & 3))) = vr[i];
+    }
+  };
+  if (b0 < b1) fetch(b0), store(0);
+  __syncthreads();
+  for (int b = b0; b < b1; b++) {
+    const int now = (b - b0) & 1;
+    const int fk = ((b * KB + 16 * (n >> 2)) >> lg) - p0, fv = ((b * KB + 16 * g) >> lg) - p0;
+    const float ks = __shfl(run.ks, fk, 64), vs = __shfl(run.vs, fv, 64);
+    const bool seen = __shfl(run.id, fv, 64) >= 0;
+    if (b + 1 < b1) fetch(b + 1);
+    if (b * KB <= whi && b * KB + KB > wlo) {
+      const uint8_t *k = kl[now], *v = vl[now];
+      fold_block<HD, 2>(q, st, b * KB + 16 * g, seen, ks, vs,
+                        [&](int kt, int j) {
+                          const int row = 16 * (n >> 2) + 4 * kt + (n & 3);
+                          return *(const u32x4 *)(k + row * HD + 16 * ((4 * j + g) ^ turned(row)));
+                        },
+                        [&](int c) { return *(const u32x4 *)(v + (16 * c + n) * KB + 16 * (g ^ (n >> 2))); }, [] {});
+    }
+    if (b + 1 < b1) store(now ^ 1);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int pair = pair0 + 32 * wave + 16 * t + n;
+    const float l = sum_groups(st[t].l);
+    if (pair < pairs) store_rows<HD>(a, p, kvh, pair, g, st[t], l);
+  }
+}
+
+// ---- entry points ----------------------------------------------------------------------------------------------------
+
+static int check_pool(const bt_pages *c, PoolArgs *out) {
+  if (!c || !c->values || !c->scales) return fail(BT_EINVAL, "a paged cache needs its values and scales");
+  if (c->head_dim != 64 && c->head_dim != 128) return fail(BT_EINVAL, "a paged cache's heads are 64 or 128 wide, not %d", c->head_dim);
+  int lg = 0;
+  while (lg < 9 && (1 << lg) != c->page) lg++;
+  if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", c->page);
+  if (c->kv < 1 || c->kv > 1024 || c->pages < 1 || (int64_t)c->pages * c->page > 0x7FFFFFFFll)
+    return fail(BT_EINVAL, "a paged cache of %d pages of %d tokens and %d key heads", c->pages, c->page, c->kv);
+  if (c->values % 16 || c->scales % 4) return fail(BT_EINVAL, "a paged cache's values are 16-byte aligned, its scales 4-byte");
+  if (out) *out = PoolArgs{(uint8_t *)(uintptr_t)c->values, (float *)(uintptr_t)c->scales, c->pages, lg, c->kv};
+  return BT_OK;
+}
+
+constexpr int MOST_ROWS = 1 << 20;
+
+static int check_batch(const bt_batch *b, BatchArgs *out) {
+  if (!b || !b->tables || !b->starts || !b->lengths || !b->parts) return fail(BT_EINVAL, "a batch needs its tables, starts, lengths and parts");
+  if ((b->tables | b->starts | b->lengths | b->parts) % 4) return fail(BT_EINVAL, "a batch's tensors are int32-aligned");
+  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 || b->most < 1 ||
+      b->target < 1 || b->target > MOST_ROWS)
+    return fail(BT_EINVAL, "a batch of %d requests (1 to %d), %d rows (1 to %d), tables %d wide, %d rows a request at most, %d parts",
+                b->requests, MOST_REQUESTS, b->rows, MOST_ROWS, b->width, b->most, b->target);
+  if (out)
+    *out = BatchArgs{(const int32_t *)(uintptr_t)b->tables, (const int32_t *)(uintptr_t)b->starts, (const int32_t *)(uintptr_t)b->lengths,
+                     (const int32_t *)(uintptr_t)b->parts, b->tables_sr, b->requests, b->width, b->rows};
+  return BT_OK;
+}
+
+// How a call is cut: `few`, the most pairs of a request whose keys are cut into parts, in `tiles` of 16; `many`, whether
+// requests may have more (their rows then share blocks of 128 pairs).
+struct AttendPlan {
+  int few, tiles, items;
+  bool many, join;
+  uint64_t scratch;
+};
+static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int window, AttendPlan *p) {
+  if (int s = check_pool(c, nullptr)) return s;
+  if (int s = check_batch(b, nullptr)) return s;
+  if (heads < 1 || heads % c->kv || window < 0 || (int64_t)heads * b->rows > 0x3FFFFFFF)
+    return fail(BT_EINVAL, "paged attention of %d heads over %d key heads, %d rows, window %d", heads, c->kv, b->rows, window);
+  const int rep = heads / c->kv;
+  const int64_t most = (int64_t)std::min(b->most, b->rows) * rep;
+  p->many = most > 64;
+  p->few = p->many ? 32 : (int)most;
+  p->tiles = p->few <= 16 ? 1 : p->few <= 32 ? 2 : 4;
+  p->items = b->target + b->requests;
+  const int64_t keys = (int64_t)b->width * c->page;
+  p->join = keys > KB;
+  const uint64_t bytes = (uint64_t)p->items * c->kv * (16 * p->tiles * (c->head_dim + 2)) * 4;
+  p->scratch = p->join ? bytes : 0;
+  if ((int64_t)p->items * c->kv > 0x3FFFFFFF) return fail(BT_EINVAL, "paged attention in %d parts of %d key heads", p->items, c->kv);
+  return BT_OK;
+}
+
+template <int HD, int QT> static int launch_few(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  const int clear = (a.b.rows + 15) / 16;
+  pages_few_kernel<HD, QT><<<(unsigned)(p.items * a.c.kv + clear), 64, 0, s>>>(a);
+  BT_LAUNCHED("paged attention");
+  if (p.join) {
+    pages_join_kernel<HD, QT><<<(unsigned)(a.b.requests * a.c.kv * p.few), 256, 0, s>>>(a, p.few);
+    BT_LAUNCHED("paged attention's join");
+  }
+  return BT_OK;
+}
+template <int HD> static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  const int status = p.tiles == 1 ? launch_few<HD, 1>(a, p, s) : p.tiles == 2 ? launch_few<HD, 2>(a, p, s) : launch_few<HD, 4>(a, p, s);
+  if (status || !p.many) return status;
+  const int tiles = (int)((int64_t)a.b.rows * a.rep >> 7) + a.b.requests;
+  pages_many_kernel<HD><<<(unsigned)(tiles * a.c.kv), 256, 0, s>>>(a, tiles);
+  BT_LAUNCHED("paged attention");
+  return BT_OK;
+}
+
+}  // namespace bt
+
+using namespace bt;
+
+extern "C" {
+
+int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  if (!a || !a->tables || !a->cached || !a->fresh || !a->free_pages || !a->starts || !a->lengths || !a->places || !a->slots ||
+      !a->taken_out || !a->parts)
+    return fail(BT_EINVAL, "a plan needs its tables, lengths, free pages and results");
+  if ((a->tables | a->cached | a->fresh | a->free_pages | a->taken | a->starts | a->lengths | a->places | a->slots | a->taken_out |
+       a->parts) % 4)
+    return fail(BT_EINVAL, "a plan's tensors are int32-aligned");
+  int lg = 0;
+  while (lg < 9 && (1 << lg) != a->page) lg++;
+  if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", a->page);
+  if (a->requests < 1 || a->requests > MOST_REQUESTS || a->width < 1 || a->n_free < 1 || a->rows < 1 || a->rows > MOST_ROWS ||
+      a->most < 1 || a->target < 1 || a->pages < 1 || (int64_t)a->pages * a->page > 0x7FFFFFFFll)
+    return fail(BT_EINVAL, "a plan of %d requests (1 to %d), %d rows (1 to %d), %d a request at most, tables %d wide, %d free of %d pages",
+                a->requests, MOST_REQUESTS, a->rows, MOST_ROWS, a->most, a->width, a->n_free, a->pages);
+  const auto at = [](uint64_t p) { return (int32_t *)(uintptr_t)p; };
+  const PlanArgs k{at(a->tables), at(a->cached), at(a->fresh), at(a->free_pages), at(a->taken), at(a->starts), at(a->lengths),
+                   at(a->places), at(a->slots), at(a->taken_out), at(a->parts), a->tables_sr, a->requests, a->width, a->n_free,
+                   a->rows, lg, a->pages, std::min(a->most, a->rows), a->target};
+  plan_kernel<<<1, PLAN_NT, 0, r->stream>>>(k);
+  BT_LAUNCHED("a plan");
+  if (a->rows > PLAN_ROWS) {
+    plan_rows_kernel<<<(unsigned)ceil_div(a->rows, 256), 256, 0, r->stream>>>(k);
+    BT_LAUNCHED("a plan's rows");
+  }
+  return BT_OK;
+}
+
+int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t x, int64_t x_sb, int64_t x_sr) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  PoolArgs c;
+  BatchArgs b;
+  if (int s = check_pool(pool, &c)) return s;
+  if (int s = check_batch(batch, &b)) return s;
+  if (!x || x % 16 || x_sb % 8 || x_sr % 8) return fail(BT_EINVAL, "a paged cache takes rows on 16-byte boundaries");
+  const int64_t blocks = (int64_t)((b.rows >> c.page_log2) + 2 * b.requests) * 2 * c.kv;
+  if (blocks > 0x7FFFFFFF) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, 2 * c.kv);
+  const uint16_t *src = (const uint16_t *)(uintptr_t)x;
+  if (pool->head_dim == 64) put_pages_kernel<64><<<(unsigned)blocks, 256, 0, r->stream>>>(c, b, src, x_sb, x_sr);
+  else put_pages_kernel<128><<<(unsigned)blocks, 256, 0, r->stream>>>(c, b, src, x_sb, x_sr);
+  BT_LAUNCHED("a paged put");
+  return BT_OK;
+}
+
+int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  PoolArgs c;
+  if (int s = check_pool(pool, &c)) return s;
+  if (!out || out % 16) return fail(BT_EINVAL, "pages are read to a 16-byte aligned tensor");
+  const int64_t blocks = (int64_t)c.pages * 2 * c.kv;
+  if (blocks > 0x7FFFFFFF) return fail(BT_EINVAL, "%d pages of %d heads are too many to read at once", c.pages, 2 * c.kv);
+  if (pool->head_dim == 64) read_pages_kernel<64><<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out);
+  else read_pages_kernel<128><<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out);
+  BT_LAUNCHED("reading pages");
+  return BT_OK;
+}
+
+int bt_pages_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t heads, int32_t window, uint64_t *bytes) {
+  if (!bytes) return fail(BT_EINVAL, "no result pointer");
+  AttendPlan p;
+  if (int s = plan_attend(pool, batch, heads, window, &p)) return s;
+  *bytes = p.scratch;
+  return BT_OK;
+}
+
+int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr, uint64_t out,
+                    int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch, uint64_t scratch_bytes) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  AttendPlan p;
+  if (int s = plan_attend(pool, batch, heads, window, &p)) return s;
+  AttendArgs a;
+  check_pool(pool, &a.c), check_batch(batch, &a.b);
+  if (!q || !out || q % 16 || q_sh % 8 || q_sr % 8 || out % 16 || o_sh % 8 || o_sr % 8)
+    return fail(BT_EINVAL, "paged attention needs q and out rows on 16-byte boundaries");
+  if (p.scratch && (!scratch || scratch % 16 || scratch_bytes < p.scratch))
+    return fail(BT_EINVAL, "paged attention needs %llu bytes of 16-byte aligned scratch", (unsigned long long)p.scratch);
+  a.q = (const uint16_t *)(uintptr_t)q, a.out = (uint16_t *)(uintptr_t)out, a.scratch = (float *)(uintptr_t)scratch;
+  a.q_sh = q_sh, a.q_sr = q_sr, a.o_sh = o_sh, a.o_sr = o_sr;
+  a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few;
+  a.drep = make_fastdiv((uint32_t)a.rep);
+  return pool->head_dim == 64 ? launch_attend<64>(a, p, r->stream) : launch_attend<128>(a, p, r->stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,425 @@
+"""The paged 8-bit cache and the verification of drafts on the GPU, against oracle/pages.py in 64 bits: plans, puts and tokens
+exactly, attention within what its roundings allow. Needs a GPU."""
+import numpy as np
+import pytest
+
+from baretile_amd.models import serve
+from baretile_amd.pages import Pages
+from baretile_amd.tensor import Recording, Tensor, jit
+from oracle import bfp as B, pages as P
+
+pytestmark = pytest.mark.gpu
+
+
+def row(rt, a): return Tensor.of(rt, [[int(v) for v in a]], "int32")
+
+
+def ints(t): return np.array(t.tolist()).reshape(t.shape[-2:]).squeeze(0) if t.rows == 1 else np.array(t.tolist())
+
+
+def planned(rt, pool, tables, cached, new, free, rows, taken=None, most=None):
+  """A plan made on the device and checked against the oracle's: (batch, the oracle's results)."""
+  t = Tensor.of(rt, np.asarray(tables), "int32")
+  b = pool.plan(t, row(rt, cached), row(rt, new), row(rt, free), rows, row(rt, [taken]) if taken is not None else None, most)
+  want = P.plan(tables, cached, new, free, rows, pool.page, pool.pages, taken or 0, most)
+  got = [ints(t).reshape(np.shape(tables)), *(ints(v) for v in (b.starts, b.lengths, b.places, b.slots)), int(ints(b.taken)[0])]
+  for g, w, name in zip(got, want, ("tables", "starts", "lengths", "places", "slots", "taken")):
+    assert np.array_equal(g, w), (name, g, w)
+  return b, want
+
+
+def bf16_rows(rng, *shape):
+  x = rng.normal(0, 1, shape) * np.exp(rng.normal(0, 0.7, (*shape[:-1], 1)))
+  return B.bf16(x)
+
+
+# ---- plans
+
+@pytest.mark.parametrize("requests, page, most, rows", [(1, 16, None, 1), (1, 64, None, 40), (5, 16, None, 33), (7, 32, 3, 50), (64, 64, None, 64),
+                                                        (65, 16, 2, 300), (300, 128, None, 900), (1100, 16, 4, 2048), (2048, 16, None, 4100),
+                                                        (3, 256, None, 2500)])
+def test_plan(rt, requests, page, most, rows):
+  rng = np.random.default_rng(requests + rows)
+  pool = Pages(rt, 5000, 1, 64, page)
+  width = 12
+  cached, new = rng.integers(0, page * 6, requests), rng.integers(0, max(2, 2 * rows // requests), requests)
+  free = rng.permutation(5000)
+  # every request's pages for what it has cached, some with a spare page behind, some with a hole
+  tables, at = np.full((requests, width), -1), 0
+  for r in range(requests):
+    n = min(-(-int(cached[r]) // page) + int(rng.integers(0, 3) == 0), width)
+    tables[r, :n] = rng.integers(0, 5000, n)
+    if n and rng.integers(0, 5) == 0: tables[r, rng.integers(0, n)] = rng.choice([-1, 5000, 2 ** 31 - 1, -2 ** 31])
+  planned(rt, pool, tables, cached, new, free, rows, most=most)
+  planned(rt, pool, tables, cached, new, free[:3], rows, taken=2, most=most)  # the free list runs out
+
+
+def test_plan_with_odd_lengths(rt):
+  pool = Pages(rt, 20, 1, 64, 16)
+  none = np.full((4, 3), -1)
+  free = np.arange(20)
+  planned(rt, pool, none, [0, 0, 0, 0], [0, 0, 0, 0], free, 5)  # nothing to do
+  planned(rt, pool, none, [-5, 0, 2 ** 31 - 1, 48], [3, -2, 4, 1], free, 20)  # below 0, and past the tables' width
+  planned(rt, pool, none, [0, 0, 0, 0], [2 ** 31 - 1] * 4, free, 40)  # more than the rows
+  planned(rt, pool, none, [0, 15, 16, 17], [1, 1, 1, 1], [99, -1, 3, 20], 4)  # free pages that are none
+  planned(rt, pool, none, [0, 0, 0, 0], [5, 5, 5, 5], free, 20, taken=-3)
+  planned(rt, pool, none, [0, 0, 0, 0], [40, 1, 1, 1], free, 20, taken=19)
+
+
+def test_plan_leaves_refused_drafts_their_pages(rt):
+  pool = Pages(rt, 20, 1, 64, 16)
+  b, want = planned(rt, pool, np.full((2, 4), -1), [0, 0], [30, 20], np.arange(20), 50)
+  assert want[5] == 4
+  planned(rt, pool, want[0], [14, 20], [5, 5], np.arange(20), 10, taken=4)  # the first request's second page is its own still
+
+
+# ---- puts
+
+def whole(pool): return np.array(pool.values().tolist()).reshape(pool.pages, 2 * pool.kv, pool.page, pool.head)
+
+
+def scales(pool): return np.array(pool.scales.tolist())
+
+
+@pytest.mark.parametrize("hd, kv, page", [(64, 1, 16), (128, 2, 32), (64, 3, 64), (128, 1, 128), (128, 2, 256), (64, 2, 256)])
+def test_put(rt, hd, kv, page):
+  rng = np.random.default_rng(hd + kv + page)
+  pool = Pages(rt, 24, kv, hd, page)
+  values, s = np.zeros((24, 2 * kv, page, hd)), np.full((24, 2 * kv), 2.0 ** -100)
+  tables, lengths, taken = np.full((5, 6), -1), np.zeros(5, int), 0
+  free = rng.permutation(24)
+  for step, new in enumerate(([page + 3, 1, 0, 2 * page, 5], [1, 1, 1, 1, 1], [0, page - 1, 2, 1, 7], [1, 2, 0, 17, 3], [3, 1, 4, 1, 1])):
+    rows = sum(new) + 2
+    x = bf16_rows(rng, 2 * kv, rows, hd) * 4.0 ** (step % 3)  # later rows larger, then smaller: scales that grow and stay
+    b, (tables, starts, lengths, _, _, taken) = planned(rt, pool, tables, lengths, new, free, rows, taken)
+    pool.put(b, Tensor.of(rt, x))
+    P.put(values, s, tables, starts, lengths, x)
+    assert np.array_equal(whole(pool), values), step
+    assert np.array_equal(scales(pool), s), step
+  assert (values != 0).any(axis=(1, 2, 3)).sum() == taken  # pages of no request stay as they were
+
+
+def test_put_of_odd_values(rt):
+  pool = Pages(rt, 3, 1, 64, 16)
+  x = np.zeros((2, 20, 64))
+  x[0, 0, :8] = [np.inf, -np.inf, np.nan, 3.0, -1e-3, 448, -449, 1e-30]  # infinities and NaNs don't count for the scale
+  x[1, 1, 0], x[1, 2, 0], x[1, 3, :2] = 3e38, 1e-38, [np.nan, -np.inf]
+  x[0, 16] = B.bf16(2.0 ** -133 * np.arange(64))  # smaller than any scale's grid
+  x[1, 17, :4] = [np.inf, np.inf, np.nan, 0]  # nothing finite but zeros
+  bits = (np.asarray(x, np.float32).view(np.uint32) >> 16).astype(np.uint16)
+  x = (bits.astype(np.uint32) << 16).view(np.float32)
+  b, (tables, starts, lengths, *_) = planned(rt, pool, np.full((1, 2), -1), [0], [20], np.arange(3), 20)
+  values, s = np.zeros((3, 2, 16, 64)), np.full((3, 2), 2.0 ** -100)
+  pool.put(b, Tensor.frombytes(rt, 20, 64, bits.tobytes(), 2))
+  P.put(values, s, tables, starts, lengths, x)
+  assert np.array_equal(whole(pool), values) and np.array_equal(scales(pool), s)
+
+
+def test_put_a_token_at_a_time(rt):
+  rng = np.random.default_rng(3)
+  pool = Pages(rt, 4, 2, 128, 32)
+  values, s = np.zeros((4, 4, 32, 128)), np.full((4, 4), 2.0 ** -100)
+  tables = np.full((1, 4), -1)
+  x = bf16_rows(rng, 4, 70, 128) * np.exp(rng.normal(0, 2, (1, 70, 1)))  # sizes all over: scales that grow often
+  x = B.bf16(x)
+  taken = 0
+  for i in range(70):
+    b, (tables, starts, lengths, _, _, taken) = planned(rt, pool, tables, [i], [1], [2, 0, 3, 1], 1, taken)
+    pool.put(b, Tensor.of(rt, x[:, i:i + 1]))
+    P.put(values, s, tables, starts, lengths, x[:, i:i + 1])
+  assert np.array_equal(whole(pool), values) and np.array_equal(scales(pool), s)
+
+
+def test_put_drops_rows_without_a_page_and_takes_strided_rows(rt):
+  rng = np.random.default_rng(4)
+  pool = Pages(rt, 5, 1, 64, 16)
+  tables = np.array([[2, -1, 7], [0, 1, -1]])
+  cached, new = [10, 20], [30, 20]
+  x = bf16_rows(rng, 2, 60, 192)  # wider rows, of which the middle is put
+  b, (made, starts, lengths, *_) = planned(rt, pool, tables, cached, new, [9, 4], 60)
+  values, s = np.zeros((5, 2, 16, 64)), np.full((5, 2), 2.0 ** -100)
+  pool.put(b, Tensor.of(rt, x)[:, :, 64:128])
+  P.put(values, s, made, starts, lengths, x[:, :, 64:128])
+  assert np.array_equal(whole(pool), values) and np.array_equal(scales(pool), s)
+
+
+# ---- attention
+
+def bound(q, values, weighed, out):
+  """How far an output may be from the oracle's: the weights' rounding to bf16 (2^-8 of the weighed |v|), the output's, and the fp32
+  scores' (4 roundings of a sum of hd products, doubled for the weights' sum)."""
+  size = np.linalg.norm(q, axis=-1).max() * np.linalg.norm(values, axis=-1).max()
+  return weighed * (2.0 ** -8 + 8 * q.shape[-1] * 2.0 ** -24 * (1 + size)) + 2.0 ** -8 * np.abs(out) + 1e-30
+
+
+def filled(rt, rng, heads, kv, hd, page, lengths, width=None, spare=3):
+  """A pool with rows of every request in it, (pool, values, tables)."""
+  width = width or max(1, -(-max(lengths) // page))
+  pages = sum(-(-n // page) for n in lengths) + spare
+  pool = Pages(rt, pages, kv, hd, page)
+  values, s = np.zeros((pages, 2 * kv, page, hd)), np.full((pages, 2 * kv), 2.0 ** -100)
+  rows = max(1, sum(lengths))
+  x = bf16_rows(rng, 2 * kv, rows, hd)
+  b, (tables, starts, _, _, _, taken) = planned(rt, pool, np.full((len(lengths), width), -1), [0] * len(lengths), lengths, rng.permutation(pages), rows)
+  pool.put(b, Tensor.of(rt, x))
+  P.put(values, s, tables, starts, lengths, x)
+  return pool, values, tables, taken
+
+
+def attended(rt, rng, heads, kv, hd, page, lengths, new, window=0, spare=0, tables=None, merged=False, most=None):
+  pool, values, made, taken = filled(rt, rng, heads, kv, hd, page, lengths)
+  if tables is not None: made = tables(made)
+  rows = sum(new) + spare
+  q = B.bf16(rng.normal(0, 1, (heads, rows, hd)) * 1.5 / np.sqrt(hd))
+  b, (made, starts, total, *_) = planned(rt, pool, made, [n - m for n, m in zip(lengths, new)], new, [-1], rows, most=most)
+  out = pool.attend(Tensor.of(rt, q), b, window, merged)
+  got = np.array(out.tolist())
+  if merged: got = got.reshape(rows, heads, hd).transpose(1, 0, 2)
+  got = got.reshape(heads, rows, hd)
+  want, weighed = P.attend(q, values, made, starts, total, window)
+  assert np.all(np.abs(got - want) <= bound(q, values, weighed, want)), np.abs(got - want).max()
+  return got, want
+
+
+@pytest.mark.parametrize("heads, kv, hd, page", [(8, 2, 64, 16), (4, 4, 128, 32), (32, 8, 128, 64), (9, 3, 64, 128), (7, 1, 128, 256), (20, 1, 64, 16)])
+@pytest.mark.parametrize("lengths, new", [([1], [1]), ([300], [1]), ([64, 0, 1, 65, 500], [1, 0, 1, 1, 1]), ([700, 63, 129], [5, 3, 0]),
+                                          ([200, 90], [9, 7])])
+def test_attend_few_rows(rt, heads, kv, hd, page, lengths, new):
+  attended(rt, np.random.default_rng(heads + page + sum(lengths)), heads, kv, hd, page, lengths, new, spare=2, merged=page == 64)
+
+
+@pytest.mark.parametrize("heads, kv, hd, page", [(8, 2, 64, 16), (4, 1, 128, 64), (6, 2, 128, 32), (3, 3, 64, 256)])
+@pytest.mark.parametrize("lengths, new", [([130], [130]), ([333, 1, 200], [140, 1, 90]), ([520, 64], [71, 64])])
+def test_attend_many_rows(rt, heads, kv, hd, page, lengths, new):
+  attended(rt, np.random.default_rng(heads + page + sum(lengths)), heads, kv, hd, page, lengths, new, spare=17)
+
+
+@pytest.mark.parametrize("window", [1, 7, 64, 100, 1000])
+@pytest.mark.parametrize("lengths, new", [([300, 40], [1, 3]), ([400, 150], [100, 70])])
+def test_attend_window(rt, window, lengths, new):
+  attended(rt, np.random.default_rng(window), 8, 2, 64, 16, lengths, new, window)
+
+
+@pytest.mark.parametrize("new", [[1, 3, 1], [90, 80, 1]])
+def test_attend_hides_pages_that_are_none(rt, new):
+  def holes(t):
+    t = t.copy()
+    t[0, 1], t[0, 4], t[1, 0], t[2, :] = -1, 10 ** 6, -2 ** 31, -1
+    return t
+  got, want = attended(rt, np.random.default_rng(5), 8, 2, 64, 16, [200, 120, 30], new, tables=holes)
+  assert not want[:, -1].any()  # a request with no page at all: its row sees nothing
+
+
+def test_attend_long(rt):
+  attended(rt, np.random.default_rng(6), 4, 1, 64, 64, [40000, 100], [1, 2])
+
+
+def test_attend_a_row_that_is_not_a_number(rt):
+  rng = np.random.default_rng(7)
+  for new in ([2, 2], [40, 40]):
+    pool, values, tables, _ = filled(rt, rng, 4, 2, 64, 16, [300, 90])
+    rows = sum(new)
+    q = B.bf16(rng.normal(0, 0.2, (4, rows, 64)))
+    bits = B.bf16_bits(q)
+    bits[1, 1, 3], bits[2, new[0], 0] = 0x7FC0, 0x7F80  # one row's head with a NaN, one with an infinity
+    b, (tables, starts, total, *_) = planned(rt, pool, tables, [300 - new[0], 90 - new[1]], new, [-1], rows)
+    got = np.array(pool.attend(Tensor.frombytes(rt, rows, 64, bits.tobytes(), 4), b).tolist())
+    want, weighed = P.attend(q, values, tables, starts, total)
+    ok = np.ones((4, rows), bool)
+    ok[1, 1] = ok[2, new[0]] = False
+    assert np.isnan(got[~ok]).all()
+    assert np.all(np.abs(got - want)[ok] <= bound(q, values, weighed, want)[ok])
+
+
+def test_attend_takes_strided_queries_and_masks_what_a_page_held_before(rt):
+  rng = np.random.default_rng(8)
+  pool, values, tables, _ = filled(rt, rng, 8, 2, 64, 16, [100])
+  # the request ends; another takes its last page and half fills it: the rows behind it are the old request's
+  page = int(tables[0, 6])
+  b, (t, starts, total, *_) = planned(rt, pool, np.full((1, 1), -1), [0], [5], [page], 5)
+  x = bf16_rows(rng, 4, 5, 64)
+  pool.put(b, Tensor.of(rt, x))
+  s = scales(pool)
+  values[page] = 0
+  P.put(values, s, t, starts, total, x)
+  q = B.bf16(rng.normal(0, 0.2, (5, 8 * 64)))
+  got = np.array(pool.attend(Tensor.of(rt, q).split(8), b).tolist())
+  q = q.reshape(5, 8, 64).transpose(1, 0, 2)
+  want, weighed = P.attend(q, values, t, starts, total)
+  assert np.all(np.abs(got - want) <= bound(q, values, weighed, want))
+
+
+def test_attend_repeats_itself(rt):
+  rng = np.random.default_rng(9)
+  pool, _, tables, _ = filled(rt, rng, 8, 2, 128, 64, [3000, 50, 900])
+  q = Tensor.of(rt, B.bf16(rng.normal(0, 0.2, (8, 12, 128))))
+  b, _ = planned(rt, pool, tables, [2996, 46, 896], [4, 4, 4], [-1], 12)
+  first = pool.attend(q, b).tobytes()
+  for _ in range(5): assert pool.attend(q, b).tobytes() == first
+
+
+# ---- verification
+
+def verified(rt, logits, ids, starts, uniforms, probs=None, t=None):
+  of = lambda a: Tensor.of(rt, np.asarray(a, np.float32), "fp32")
+  tokens, counts = serve.verify(of(logits), row(rt, ids), row(rt, starts), of(uniforms), of(probs) if probs is not None else None,
+                                of(np.reshape(t, (-1, 1))) if t is not None else None)
+  as32 = lambda a: np.asarray(a, np.float32)
+  want = P.verify(as32(logits), ids, starts, as32(uniforms), None if probs is None else as32(probs), None if t is None else as32(t))
+  got = ints(tokens), ints(counts)
+  assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1]), (got, want)
+  return got
+
+
+def soft(x): return np.exp(x - x.max(-1, keepdims=True)) / np.exp(x - x.max(-1, keepdims=True)).sum(-1, keepdims=True)
+
+
+def near(rng, logits):  # draft probabilities near the row before's
+  return soft(np.roll(logits, 1, 0) + 0.7 * rng.normal(0, 1, logits.shape)).astype(np.float32)
+
+
+@pytest.mark.parametrize("vocab", [1, 2, 63, 1000, 2048, 2049, 49152, 131072, 200001])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify(rt, vocab, drawn):
+  rng = np.random.default_rng(vocab)
+  starts = [0, 5, 5, 6, 14]
+  rows = 16
+  logits = 3 * rng.normal(0, 1, (rows, vocab)).astype(np.float32)
+  probs = near(rng, logits)
+  ids = [int(np.searchsorted(np.cumsum(p.astype(np.float64)), rng.random() * 0.999)) for p in probs] if drawn else np.roll(logits, 1, 0).argmax(1)
+  for _ in range(3):
+    verified(rt, logits, np.minimum(ids, vocab - 1), starts, rng.random((2, rows)).astype(np.float32), probs if drawn else None,
+             rng.uniform(0.5, 2, rows).astype(np.float32))
+
+
+def test_verify_many_requests(rt):
+  rng = np.random.default_rng(1)
+  starts = np.concatenate([[0], np.cumsum(rng.integers(0, 5, 150))])
+  rows = int(starts[-1]) + 3
+  logits = 2 * rng.normal(0, 1, (rows, 3001)).astype(np.float32)
+  probs = near(rng, logits)
+  ids = [int(rng.choice(3001, p=p.astype(np.float64) / p.sum(dtype=np.float64))) for p in probs]
+  verified(rt, logits, ids, starts, rng.random((2, rows)).astype(np.float32), probs)
+
+
+def test_verify_draws_from_all_of_the_distribution(rt):
+  # one request a uniform, over a grid of them: the drawn tokens' counts are the distribution's, to the grid's step
+  n = 1 << 11
+  p = np.array([0.5, 0.0, 0.25, 0.125, 0.125])
+  logits = np.tile(np.where(p > 0, np.log(np.maximum(p, 1e-9)), -np.inf), (n, 1))
+  u = np.stack([np.zeros(n), (np.arange(n) + 0.5) / n])
+  tokens, _ = verified(rt, logits, [0] * n, range(n + 1), u)
+  assert np.array_equal(np.bincount(tokens, minlength=5), p * n)
+
+
+def test_verify_at_its_edges(rt):
+  rng = np.random.default_rng(2)
+  inf, nan = np.inf, np.nan
+  low = np.finfo(np.float32).min
+  v = 300
+  logits = rng.normal(0, 1, (24, v)).astype(np.float32)
+  logits[0], logits[1], logits[2] = -inf, low, nan  # nothing; everything alike; nothing
+  logits[3, 7], logits[4, [3, 9]] = inf, inf
+  logits[5, 100:], logits[6, :] = -inf, -inf
+  logits[6, 250] = -1e30  # one token left
+  logits[7, 5] = nan
+  for u0 in (0.0, 0.5, 1 - 2.0 ** -24):
+    for u1 in (0.0, 0.5, 1 - 2.0 ** -24):
+      u = np.array([[u0] * 24, [u1] * 24], np.float32)
+      verified(rt, logits, [7] * 24, range(25), u)  # every row on its own
+      verified(rt, logits, [7] * 24, range(0, 25, 2), u)  # drafts against odd rows
+      verified(rt, logits, [7] * 24, range(0, 25, 3), u, soft(rng.normal(0, 1, (24, v))))
+  ids = [0, -1, v, 2 ** 31 - 1, -2 ** 31, 5] * 4  # drafts that are no tokens
+  verified(rt, logits, ids, [0, 12, 24], rng.random((2, 24)), soft(rng.normal(0, 1, (24, v))))
+  # inverse temperatures: 0 takes any token with a weight, infinity the largest, the first of equals; below 0 and NaN are 0
+  logits[10, 20], logits[10, 30] = 50, 50
+  verified(rt, logits, logits.argmax(1), [0, 12, 24], rng.random((2, 24)), None, [0, inf, 1, -1, nan, inf, 0, 1e30, inf, 1e-30, inf, 3] * 2)
+  # the same distribution on both sides: refused by rounding or not at all, something is drawn
+  q = np.roll(soft(logits[12:].astype(np.float64)), 1, 0)
+  verified(rt, logits[12:], [9] * 12, [0, 12], np.full((2, 12), 1 - 2.0 ** -24), q)
+
+
+def test_verify_reads_starts_within_its_rows(rt):
+  logits = Tensor.of(rt, np.zeros((4, 10)), "fp32")
+  u = Tensor.of(rt, np.full((2, 4), 0.55), "fp32")
+  for starts in ([0, 9], [-5, 2], [3, 1], [2 ** 31 - 1, -2 ** 31]):
+    tokens, counts = serve.verify(logits, row(rt, [1, 2, 3, 4]), row(rt, starts), u)
+    assert len(ints(tokens)) == 4 and len(ints(counts)) == 1  # (starts that no plan makes: any tokens, but nothing outside)
+
+
+# ---- together
+
+def test_a_recorded_step_follows_its_lengths(rt):
+  # plan, put, attention and verification recorded once; each replay takes the lengths, rows and numbers of its own
+  rng = np.random.default_rng(10)
+  heads, kv, hd, page, R, rows, vocab = 8, 2, 64, 16, 3, 9, 500
+  pool = Pages(rt, 40, kv, hd, page)
+  free = rng.permutation(40)
+  tables, fr = Tensor.of(rt, np.full((R, 10), -1), "int32"), row(rt, free)
+  cached, new, taken = row(rt, [0] * R), row(rt, [0] * R), row(rt, [0])
+  x, q = Tensor.zeros(rt, rows, hd, 2 * kv), Tensor.zeros(rt, rows, hd, heads)
+  logits, ids, u = Tensor.zeros(rt, rows, vocab, dtype="fp32"), row(rt, [0] * rows), Tensor.zeros(rt, 2, rows, dtype="fp32")
+  def step():
+    b = pool.plan(tables, cached, new, fr, rows, taken, most=4)
+    pool.put(b, x)
+    o = pool.attend(q, b)
+    tokens, counts = serve.verify(logits, ids, b.starts, u)
+    taken.assign(b.taken)
+    cached.assign(b.lengths - 0)
+    return b, o, tokens, counts
+  step()
+  rt.wait()
+  for t, v in ((tables, np.full((R, 10), -1)), (cached, [[0] * R]), (taken, [[0]])): t.assign(Tensor.of(rt, np.array(v), "int32"))
+  rec = Recording(rt)
+  with rec: out = step()
+  values, s = np.zeros((40, 2 * kv, page, hd)), np.full((40, 2 * kv), 2.0 ** -100)
+  want_tables, want_cached, want_taken = np.full((R, 10), -1), np.zeros(R, int), 0
+  for i in range(8):
+    n = rng.integers(0, 6, R)  # some past `most`
+    xs, qs = bf16_rows(rng, 2 * kv, rows, hd) * 2.0 ** i, B.bf16(rng.normal(0, 0.2 / 2.0 ** i, (heads, rows, hd)))
+    ls, ds, us = rng.normal(0, 2, (rows, vocab)).astype(np.float32), rng.integers(0, vocab, rows), rng.random((2, rows)).astype(np.float32)
+    new.assign(row(rt, n))
+    x.assign(Tensor.of(rt, xs))
+    q.assign(Tensor.of(rt, qs))
+    logits.assign(Tensor.of(rt, ls, "fp32"))
+    ids.assign(row(rt, ds))
+    u.assign(Tensor.of(rt, us, "fp32"))
+    rec.send()
+    rt.wait()
+    want_tables, starts, total, places, slots, want_taken = P.plan(want_tables, want_cached, n, free, rows, page, 40, want_taken, 4)
+    P.put(values, s, want_tables, starts, total, xs)
+    want, weighed = P.attend(qs, values, want_tables, starts, total)
+    b, o, tokens, counts = out
+    assert np.array_equal(np.array(tables.tolist()), want_tables) and np.array_equal(ints(b.slots), slots)
+    assert np.array_equal(whole(pool), values)
+    assert np.all(np.abs(np.array(o.tolist()) - want) <= bound(qs, values, weighed, want)), i
+    vt, vc = P.verify(ls, ds, starts, us)
+    assert np.array_equal(ints(tokens), vt) and np.array_equal(ints(counts), vc)
+    want_cached = total
+
+
+def test_refusals(rt):
+  pool = Pages(rt, 10, 2, 64, 16)
+  tables, r = Tensor.of(rt, np.full((2, 4), -1), "int32"), lambda *v: row(rt, v)
+  b = pool.plan(tables, r(0, 0), r(1, 1), r(*range(10)), 4)
+  x, q = Tensor.zeros(rt, 4, 64, 4), Tensor.zeros(rt, 4, 64, 8)
+  for bad in (dict(page=24), dict(head=32), dict(kv=0), dict(pages=0), dict(pages=1 << 28)):
+    with pytest.raises(ValueError): Pages(rt, **(dict(pages=10, kv=2, head=64, page=16) | bad))
+  for args in ((Tensor.zeros(rt, 2, 4), r(0, 0), r(1, 1), r(1), 4), (tables, r(0), r(1, 1), r(1), 4), (tables, r(0, 0), r(1, 1, 1), r(1), 4),
+               (tables, r(0, 0), r(1, 1), tables, 4), (tables, r(0, 0), r(1, 1), r(1), 0), (tables, r(0, 0), r(1, 1), r(1), (1 << 20) + 1),
+               (tables, r(0, 0), r(1, 1), r(1), 4, r(0, 0)), (tables, r(0, 0), r(1, 1), r(1), 4, None, 0), (tables.T, r(0, 0, 0, 0), r(1, 1, 1, 1), r(1), 4),
+               ([[1]], r(0), r(1), r(1), 4), (Tensor.zeros(rt, 2049, 1, dtype="int32"), Tensor.zeros(rt, 1, 2049, dtype="int32"),
+                                              Tensor.zeros(rt, 1, 2049, dtype="int32"), r(1), 4)):
+    with pytest.raises(ValueError): pool.plan(*args)
+  for bad in (Tensor.zeros(rt, 4, 64, 2), Tensor.zeros(rt, 3, 64, 4), Tensor.zeros(rt, 4, 128, 4), Tensor.zeros(rt, 4, 64, 4, "fp32"), None):
+    with pytest.raises(ValueError, match="put needs"): pool.put(b, bad)
+  for bad in (Tensor.zeros(rt, 4, 64, 7), Tensor.zeros(rt, 3, 64, 8), Tensor.zeros(rt, 4, 64, 8, "fp32"), None):
+    with pytest.raises(ValueError, match="attend needs"): pool.attend(bad, b)
+  with pytest.raises(ValueError, match="window"): pool.attend(q, b, -1)
+  other = Pages(rt, 10, 2, 64, 32)
+  for f in (lambda: other.put(b, x), lambda: other.attend(q, b), lambda: pool.put(None, x)):
+    with pytest.raises(ValueError, match="batch must be planned"): f()
+  logits, ids, starts, u = Tensor.zeros(rt, 4, 50, dtype="fp32"), r(1, 2, 3, 4), r(0, 4), Tensor.zeros(rt, 2, 4, dtype="fp32")
+  for args in ((Tensor.zeros(rt, 4, 50), ids, starts, u), (logits, r(1), starts, u), (logits, ids, r(0), u), (logits, ids, starts, logits),
+               (logits, ids, starts, u, u), (logits, ids, starts, u, None, u), (logits, ids, None, u)):
+    with pytest.raises((ValueError, AttributeError)): serve.verify(*args)
