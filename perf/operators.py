@@ -400,7 +400,7 @@ def _prepare_own(s):
   else:
     qs = [_tensor(q) for q in s["q"]]
     def step(): return [pool.attend(q, batch, window=case["window"], merged=True) for pool, q in zip(pools, qs)]
-  o["keep"] = (pools, table, batch, cached, new, free, taken)
+  o["keep"] = (pools, table, batch, cached, new, free, taken, step)  # (step: its queries or rows)
   rt.wait()
   if rows <= 512: o["rec"], o["out"] = _replayed(step)
   else: o["step"] = step
