@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
   top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   const float s = fmaxf(scale_of(top), old), inv = __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, exact
   const float by = old * inv;
-  uint8_t *to = c.values + ((int64_t)id * heads + h << lg) * HD;
+  uint8_t *to = c.values + (((int64_t)id * heads + h) << lg) * HD;
   if (h < c.kv) {  // keys: whole rows
     if (held && by != 1.0f)
       for (int e = tid; e < held * HD / 16; e += 256) {

@@ -4,42 +4,47 @@
 // of the token after row j, and q_j the distribution that the draft fed at row j was drawn from. Row j's draft d is
 // accepted where u0_j q_j(d) < p_{j-1}(d). The first refusal, after row j, draws from max(p_j - q_{j+1}, 0); where every
 // draft was accepted the last row draws from p: the first token whose running sum passes u1_j times the whole. Tokens
-// so drawn are distributed as the target's own (speculative sampling, Leviathan, Kalman and Matias, 2023).
+// so drawn are distributed as the target's own (speculative sampling: Leviathan, Kalman and Matias, 2023).
 //
-// A token depends on which side of a border a sum falls, so weights, sums and comparisons are in 64 bits throughout
-// (matrix-free work that reads each logit once: HBM bounds it, then the 64-bit exponential). Three launches: each row's
-// chunks give a maximum and a sum; each request's chunks find the first refusal from those and sum what is left to draw
-// from; then one block a request finds the chunk and the token.
+// A token depends on which side of a border a sum falls, so weights, sums and comparisons are in 64 bits throughout, and
+// what is drawn from stays unnormalized, so that equal weights add without rounding. Three launches: every row's chunks, a wave
+// each, give a maximum and a sum (each logit read once, weighed once against its chunk's maximum); each request's chunks find
+// the first refusal from those and sum what is left (only where a draft was refused and its distribution given does that
+// read the row again); then a wave a request picks the chunk and the token.
 #include "common.h"
 #include <algorithm>
 
 namespace bt {
 
-struct VerifyArgs {
-  const float *logits, *probs, *t, *uniforms;
-  const int32_t *ids, *starts;
-  int32_t *tokens, *counts;
-  int64_t logits_sr, probs_sr, t_sr, uniforms_sr;
-  int32_t requests, rows, vocab, chunks, chunk;  // a row's chunks, and their tokens
-  struct ChunkStat *stats;                       // [rows][chunks]
-  double *left;                                  // [requests][chunks]
-  struct Refusal *refusals;                      // [requests]
-};
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 // A chunk's largest logit, where it first is, and the sum of exp(t (x - m)).
 struct ChunkStat {
   double s;
   float m;
   int32_t at;
 };
-// Where a request draws: `accepted` drafts, row's maximum and sum of exp(t (x - m)), whether a draft was refused.
-struct Refusal {
-  double z;
+// Where a request draws: after `accepted` drafts, from `row`, with the row's maximum and sum.
+struct Draw {
+  double z, t2;
   float m;
-  int32_t accepted, refused, at;
+  int32_t accepted, row, refused, without, token;  // without: the token that a certain draft takes out, or -1; token:
+};                                                 // where there is nothing to draw, the one to take (-1: none)
+struct VerifyArgs {
+  const float *logits, *probs, *t, *uniforms;
+  const int32_t *ids, *starts;
+  int32_t *tokens, *counts;
+  ChunkStat *stats;  // [rows][chunks]
+  Draw *draws;       // [requests]
+  double *left;      // [requests][chunks]: what is left to draw from
+  int64_t logits_sr, probs_sr, t_sr, uniforms_sr;
+  int32_t requests, rows, vocab, chunks;
 };
 
-constexpr int VT = 256;
+constexpr int WAVES = 4;   // of a block; a chunk each
+constexpr int KEPT = 64;   // rows of a request whose sums a block keeps
 constexpr float NONE = -__builtin_inff();
+constexpr int NOWHERE = 0x7FFFFFFF;
 
 // A logit as it counts: NaN as -inf, +inf as the largest finite.
 __device__ __forceinline__ float logit(float x) { return x != x ? NONE : fminf(x, 3.4028234663852886e38f); }
@@ -49,260 +54,331 @@ __device__ __forceinline__ float inverse(const VerifyArgs &a, int row) {
   return t > 0.0f ? t : 0.0f;
 }
 __device__ __forceinline__ bool greedy(float t) { return t > 3.4028234663852886e38f; }
-// exp(t (x - m)), 0 for a logit that has no weight.
-__device__ __forceinline__ double weight(float x, float m, float t) {
-  return x == NONE ? 0.0 : exp((double)t * ((double)x - (double)m));
+// t log2(e), as weight() takes it.
+__device__ __forceinline__ double in_log2(float t) { return (double)t * 1.4426950408889634074; }
+
+// exp(t (x - m)) as 2^(x - m) t2, t2 = t log2(e): 2^n by the exponent and 2^f, |f| <= 1/2, by the polynomial of degree 9 through
+// it at the Chebyshev points, its constant set to 1 so that the largest weigh exactly that (3.3e-14 relative; a draw over 2^17
+// tokens falls on the other side of a border less than once in 10^8). 16 64-bit instructions, where exp() takes about 40 and bounded the first launch. -inf and what is below
+// 2^-1074 give 0.
+__device__ __forceinline__ double weight(float x, float m, double t2) {
+  const double y = fmax(((double)x - (double)m) * t2, -2000.0), n = rint(y), f = y - n;
+  double p = 0x1.b6571e229927fp-24;
+  p = fma(p, f, 0x1.63ef9699120e2p-20);
+  p = fma(p, f, 0x1.ffcb767842e11p-17);
+  p = fma(p, f, 0x1.43088e2580989p-13);
+  p = fma(p, f, 0x1.5d87fe908fb19p-10);
+  p = fma(p, f, 0x1.3b2ab72b175e1p-7);
+  p = fma(p, f, 0x1.c6b08d7044117p-5);
+  p = fma(p, f, 0x1.ebfbdff8149f2p-3);
+  p = fma(p, f, 0x1.62e42fefa39f7p-1);
+  p = fma(p, f, 1.0);
+  return __builtin_amdgcn_ldexp(p, (int)n);
 }
 
+// Reductions over a wave's lanes with no trip through LDS (as wave_sum in common.h): lane swaps by 32 and 16, then DPP moves
+// within rows of 16, each step pairing lanes symmetrically, so every lane ends with the same bits.
+template <int CTRL> __device__ __forceinline__ double moved(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)b, CTRL, 0xF, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp((int)(b >> 32), (int)(b >> 32), CTRL, 0xF, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 __device__ __forceinline__ double wave_sum64(double x) {
-#pragma unroll
-  for (int d = 32; d; d /= 2) x += __shfl_xor(x, d, 64);
-  return x;
+  const auto pair = [](uint32_t lo, uint32_t hi) { return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
+  uint64_t b = __builtin_bit_cast(uint64_t, x);
+  auto lo = __builtin_amdgcn_permlane32_swap((uint32_t)b, (uint32_t)b, false, false);
+  auto hi = __builtin_amdgcn_permlane32_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  x = pair(lo[0], hi[0]) + pair(lo[1], hi[1]);
+  b = __builtin_bit_cast(uint64_t, x);
+  lo = __builtin_amdgcn_permlane16_swap((uint32_t)b, (uint32_t)b, false, false);
+  hi = __builtin_amdgcn_permlane16_swap((uint32_t)(b >> 32), (uint32_t)(b >> 32), false, false);
+  x = pair(lo[0], hi[0]) + pair(lo[1], hi[1]);
+  x += moved<0x128>(x);  // row_ror 8
+  x += moved<0x141>(x);  // row_half_mirror
+  x += moved<0x4E>(x);   // quad_perm [2, 3, 0, 1]
+  return x + moved<0xB1>(x);  // quad_perm [1, 0, 3, 2]
 }
-__device__ __forceinline__ double block_sum64(double x, double *sums) {
-  x = wave_sum64(x);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = x;
-  __syncthreads();
-  double all = 0.0;
-#pragma unroll
-  for (int i = 0; i < VT / 64; i++) all += sums[i];
-  return all;
+template <class F> __device__ __forceinline__ uint32_t wave_fold(uint32_t x, F f) {
+  const auto a = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = f(a[0], a[1]);
+  const auto b = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = f(b[0], b[1]);
+  x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x128, 0xF, 0xF, false));
+  x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x141, 0xF, 0xF, false));
+  x = f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0x4E, 0xF, 0xF, false));
+  return f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, 0xB1, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float wave_max(float x) {
+  return __uint_as_float(wave_fold(__float_as_uint(x), [](uint32_t a, uint32_t b) {
+    return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b)));
+  }));
+}
+__device__ __forceinline__ int wave_min(int x) {
+  return (int)wave_fold((uint32_t)x, [](uint32_t a, uint32_t b) { return (uint32_t)min((int)a, (int)b); });
+}
+// The sum over the lanes before this one: shifts within rows of 16, then each row's last sum to the rows after it.
+template <int CTRL, int ROWS> __device__ __forceinline__ double shifted(double x) {  // 0 where no lane gives a value
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xF, false);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xF, false);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double wave_before(double x) {
+  double upto = x;
+  upto += shifted<0x111, 0xF>(upto);  // row_shr 1, 2, 4, 8
+  upto += shifted<0x112, 0xF>(upto);
+  upto += shifted<0x114, 0xF>(upto);
+  upto += shifted<0x118, 0xF>(upto);
+  upto += shifted<0x142, 0xA>(upto);  // row_bcast 15 into rows 1 and 3
+  upto += shifted<0x143, 0xC>(upto);  // row_bcast 31 into rows 2 and 3
+  return upto - x;
 }
 
-// Block (row, chunk): PER logits a thread, all loaded at once.
-template <int PER> __global__ void __launch_bounds__(VT) verify_stats_kernel(const VerifyArgs a) {
-  __shared__ double sums[VT / 64];
-  __shared__ float tops[VT / 64];
-  __shared__ int ats[VT / 64];
-  const int row = blockIdx.x / a.chunks, c = blockIdx.x - row * a.chunks, tid = threadIdx.x;
-  if (row >= gload(a.starts + a.requests)) return;  // row < rows by the grid
-  const int v0 = c * a.chunk, end = min(a.vocab, v0 + a.chunk);
-  const float *x = a.logits + row * a.logits_sr;
-  const float t = inverse(a, row);
-  float v[PER], top = NONE;
+// PER values of a chunk of 64 PER, four in a row a lane at a time where rows allow 16-byte loads (WIDE), else one; `none`
+// past the row's end. place(i) is value i's.
+template <int PER, bool WIDE> struct Chunk {
+  static __device__ __forceinline__ int place(int lane, int i) { return WIDE ? i / 4 * 256 + 4 * lane + i % 4 : 64 * i + lane; }
+  static __device__ __forceinline__ void load(float (&v)[PER], const float *row, int v0, int vocab, int lane, float none) {
+    if constexpr (WIDE) {  // rows end on 16 bytes too
 #pragma unroll
-  for (int i = 0; i < PER; i++) {
-    const int e = v0 + tid + VT * i;
-    v[i] = e < end ? gload(x + e) : NONE;
+      for (int i = 0; i < PER; i += 4) {
+        const int e = v0 + place(lane, i);
+        f32x4 w = {none, none, none, none};
+        if (e < vocab) w = gload((const f32x4 *)(row + e));
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[i + k] = w[k];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const int e = v0 + place(lane, i);
+        v[i] = e < vocab ? gload(row + e) : none;
+      }
+    }
   }
+};
+
+// Wave (row, chunk): no LDS, no barrier.
+template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) verify_stats_kernel(const VerifyArgs a) {
+  const int lane = threadIdx.x & 63, at = blockIdx.x * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = at / a.chunks, c = at - row * a.chunks, v0 = c * 64 * PER;
+  if (row >= min(gload(a.starts + a.requests), a.rows)) return;
+  float v[PER], top = NONE;
+  Chunk<PER, WIDE>::load(v, a.logits + row * a.logits_sr, v0, a.vocab, lane, NONE);
+  const float t = inverse(a, row);
 #pragma unroll
   for (int i = 0; i < PER; i++) top = fmaxf(top, v[i] = logit(v[i]));
-#pragma unroll
-  for (int d = 32; d; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-  if ((tid & 63) == 0) tops[tid >> 6] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  int at = 0x7FFFFFFF;
-#pragma unroll
-  for (int i = PER - 1; i >= 0; i--)
-    if (v[i] == top) at = v0 + tid + VT * i;
-#pragma unroll
-  for (int d = 32; d; d /= 2) at = min(at, __shfl_xor(at, d, 64));
-  if ((tid & 63) == 0) ats[tid >> 6] = at;
+  top = wave_max(top);
   double s = 0.0;
-  if (!greedy(t))
+  int first = NOWHERE;
+  if (greedy(t)) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) s += weight(v[i], top, t);
-  s = block_sum64(s, sums);
-  if (tid == 0) a.stats[(int64_t)row * a.chunks + c] = ChunkStat{s, top, min(min(ats[0], ats[1]), min(ats[2], ats[3]))};
+    for (int i = PER - 1; i >= 0; i--)
+      if (v[i] == top) first = v0 + Chunk<PER, WIDE>::place(lane, i);
+    first = wave_min(first);
+  } else if (top != NONE) {
+    const double t2 = in_log2(t);
+#pragma unroll
+    for (int i = 0; i < PER; i++) s += weight(v[i], top, t2);
+    s = wave_sum64(s);
+  }
+  if (lane == 0) a.stats[(int64_t)row * a.chunks + c] = ChunkStat{s, top, first};
 }
 
-// A row's maximum, its first place and its sum, from its chunks' (64 at most), by a wave; the chunk sums are added in order of lanes.
+// A row's maximum, its first place (greedy rows) and its sum, by a wave from the row's chunks.
 struct RowStat {
   double z;
   float m;
   int at;
 };
 __device__ __forceinline__ RowStat row_stat(const VerifyArgs &a, int row, float t, int lane) {
-  ChunkStat s{0.0, NONE, 0x7FFFFFFF};
-  if (lane < a.chunks) s = a.stats[(int64_t)row * a.chunks + lane];
-  RowStat r;
-  r.m = s.m;
+  const ChunkStat *stats = a.stats + (int64_t)row * a.chunks;
+  constexpr int G = 4;  // chunks a lane loads at once: all of up to 256
+  RowStat r{0.0, NONE, NOWHERE};
+  ChunkStat s[G];
 #pragma unroll
-  for (int d = 32; d; d /= 2) r.m = fmaxf(r.m, __shfl_xor(r.m, d, 64));
-  r.at = s.m == r.m ? s.at : 0x7FFFFFFF;
+  for (int i = 0; i < G; i++) {
+    s[i] = stats[min(lane + 64 * i, a.chunks - 1)];  // past the last it is read again and left out
+    if (lane + 64 * i < a.chunks) r.m = fmaxf(r.m, s[i].m);
+  }
+  for (int c = lane + 64 * G; c < a.chunks; c += 64) r.m = fmaxf(r.m, stats[c].m);
+  r.m = wave_max(r.m);
+  if (r.m == NONE) return r;
+  const double t2 = in_log2(t);
+  const auto add = [&](const ChunkStat &k) {
+    if (greedy(t)) r.at = k.m == r.m ? min(r.at, k.at) : r.at;
+    else r.z += k.s * weight(k.m, r.m, t2);
+  };
 #pragma unroll
-  for (int d = 32; d; d /= 2) r.at = min(r.at, __shfl_xor(r.at, d, 64));
-  r.z = wave_sum64(greedy(t) ? 0.0 : s.s * weight(s.m, r.m, t));
+  for (int i = 0; i < G; i++)
+    if (lane + 64 * i < a.chunks) add(s[i]);
+  for (int c = lane + 64 * G; c < a.chunks; c += 64) add(stats[c]);
+  if (greedy(t)) r.at = wave_min(r.at);
+  else r.z = wave_sum64(r.z);
   return r;
 }
 
-// What the thread's PER tokens from e on, `step` apart, may still be drawn with: p, or where a draft was refused what p has
-// over q. Every load is issued before the first is used.
-template <int PER>
-__device__ __forceinline__ void left_of(const VerifyArgs &a, const Refusal &f, int row, float t, int e, int step, int end,
-                                        double (&out)[PER]) {
+// What chunk c's tokens may still be drawn with, times z: p, or where a draft was refused what p has over q.
+template <int PER, bool WIDE> __device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int c, int lane, double (&out)[PER]) {
   float x[PER], q[PER];
-  const double inv = 1.0 / f.z;
+  const int v0 = c * 64 * PER;
   const bool drawn = f.refused && a.probs;
-  const float *logits = a.logits + row * a.logits_sr, *probs = drawn ? a.probs + (row + 1) * a.probs_sr : logits;
-#pragma unroll
-  for (int i = 0; i < PER; i++) x[i] = e + i * step < end ? gload(logits + e + i * step) : NONE;
-  if (drawn) {
-#pragma unroll
-    for (int i = 0; i < PER; i++) q[i] = e + i * step < end ? gload(probs + e + i * step) : 0.0f;
-  } else {
-    const int d = f.refused ? gload(a.ids + row + 1) : -1;
-#pragma unroll
-    for (int i = 0; i < PER; i++) q[i] = e + i * step == d ? 1.0f : 0.0f;
-  }
+  Chunk<PER, WIDE>::load(x, a.logits + f.row * a.logits_sr, v0, a.vocab, lane, NONE);
+  if (drawn) Chunk<PER, WIDE>::load(q, a.probs + (f.row + 1) * a.probs_sr, v0, a.vocab, lane, 0.0f);
 #pragma unroll
   for (int i = 0; i < PER; i++) {
-    const double p = weight(logit(x[i]), f.m, t) * inv;
-    out[i] = q[i] != q[i] ? p : p > (double)q[i] ? p - (double)q[i] : 0.0;
+    const double p = weight(logit(x[i]), f.m, f.t2);
+    if (drawn) out[i] = q[i] != q[i] ? p : fmax(fma(-(double)q[i], f.z, p), 0.0);
+    else out[i] = v0 + Chunk<PER, WIDE>::place(lane, i) == f.without ? 0.0 : p;
   }
 }
-// The first row of request r, and its rows; within the rows there are, whatever starts holds.
+// The first row of request r, and its rows: within those there are, whatever starts holds.
 __device__ __forceinline__ int request_rows(const VerifyArgs &a, int r, int *n) {
   const int s0 = gload(a.starts + r), s1 = gload(a.starts + r + 1), start = min(max(s0, 0), a.rows);
   *n = min(max(s1, start), a.rows) - start;
   return start;
 }
 
-// Block (request, chunk): the first refused draft, then the chunk's sum of what is left.
-template <int PER> __global__ void __launch_bounds__(VT) verify_left_kernel(const VerifyArgs a) {
-  __shared__ double sums[VT / 64];
-  __shared__ int refused;
-  __shared__ Refusal found;
-  const int r = blockIdx.x / a.chunks, c = blockIdx.x - r * a.chunks, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+// Block (request, 4 chunks): the first refused draft, found by every block for itself, then what is left of a chunk a wave.
+template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) verify_left_kernel(const VerifyArgs a) {
+  __shared__ RowStat kept[KEPT];
+  __shared__ int refusal;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int blocks = (a.chunks + WAVES - 1) / WAVES, r = blockIdx.x / blocks, c = (blockIdx.x - r * blocks) * WAVES + w;
   int n;
   const int start = request_rows(a, r, &n);
-  if (n <= 0) return;
-  if (tid == 0) refused = n;
+  if (n == 0) return;
+  if (tid == 0) refusal = n;
   __syncthreads();
-  for (int i = 1 + w; i < n; i += VT / 64) {  // draft i, against the row before it
-    const int row = start + i - 1, d = gload(a.ids + row + 1);
+  for (int i = 1 + w; i <= n; i += WAVES) {  // draft i, against the row before it; past the last, that row's sums alone
+    const int row = start + i - 1;
     const float t = inverse(a, row);
-    const bool is = (uint32_t)d < (uint32_t)a.vocab;
-    const float x = is ? logit(gload(a.logits + row * a.logits_sr + d)) : NONE;
-    const double q = a.probs ? (is ? (double)gload(a.probs + (row + 1) * a.probs_sr + d) : 1.0) : 1.0;
-    const double u = gload(a.uniforms + row + 1);
-    const RowStat s = row_stat(a, row, t, lane);
-    const bool ok = is && s.m != NONE && (greedy(t) ? d == s.at : u * q < weight(x, s.m, t) / s.z);
-    if (!ok) {
-      if (lane == 0) atomicMin(&refused, i);
-      break;
+    int d = -1;
+    float u = 0.0f, x = NONE, q = 1.0f;
+    bool is = false;
+    if (i < n) {
+      d = gload(a.ids + row + 1), u = gload(a.uniforms + row + 1);
+      is = (uint32_t)d < (uint32_t)a.vocab;
+      const int at = is ? d : 0;
+      x = logit(gload(a.logits + row * a.logits_sr + at));
+      q = a.probs ? gload(a.probs + (row + 1) * a.probs_sr + at) : 1.0f;
     }
+    const RowStat s = row_stat(a, row, t, lane);
+    if (lane == 0 && i <= KEPT) kept[i - 1] = s;
+    if (i < n && is && s.m != NONE && (greedy(t) ? d == s.at : (double)u * (double)q * s.z < weight(x, s.m, in_log2(t)))) continue;
+    if (lane == 0) atomicMin(&refusal, i);
+    break;
   }
   __syncthreads();
-  if (w == 0) {
-    const int accepted = refused - 1, row = start + accepted;
-    const RowStat s = row_stat(a, row, inverse(a, row), lane);
-    if (lane == 0) found = Refusal{s.z, s.m, accepted, refused < n, s.at};
-  }
-  __syncthreads();
-  const Refusal f = found;
-  if (tid == 0 && c == 0) a.refusals[r] = f;
-  const int row = start + f.accepted;
-  const float t = inverse(a, row);
-  if (greedy(t) || f.m == NONE) return;
-  const int v0 = c * a.chunk, end = min(a.vocab, v0 + a.chunk);
-  if (!f.refused) {  // the chunk's share of p is known already
-    const ChunkStat k = a.stats[(int64_t)row * a.chunks + c];
-    if (tid == 0) a.left[(int64_t)r * a.chunks + c] = k.s * weight(k.m, f.m, t) / f.z;
-    return;
-  }
-  double left[PER], s = 0.0;
-  left_of<PER>(a, f, row, t, v0 + tid, VT, end, left);
+  Draw f;
+  f.accepted = refusal - 1, f.row = start + f.accepted, f.refused = refusal < n;
+  const float t = inverse(a, f.row);
+  const RowStat s = refusal <= KEPT ? kept[refusal - 1] : row_stat(a, f.row, t, lane);
+  f.z = s.z, f.m = s.m, f.t2 = in_log2(t), f.without = f.refused && !a.probs ? gload(a.ids + f.row + 1) : -1;
+  const bool known = s.m == NONE || greedy(t);
+  f.token = s.m == NONE ? -1 : greedy(t) ? s.at : NOWHERE;
+  if (c == 0 && lane == 0) a.draws[r] = f;
+  if (known || c >= a.chunks) return;
+  double sum = 0.0;
+  if ((f.refused && a.probs) || (f.without >= 0 && f.without / (64 * PER) == c)) {
+    double v[PER];
+    left_of<PER, WIDE>(a, f, c, lane, v);
 #pragma unroll
-  for (int i = 0; i < PER; i++) s += left[i];
-  s = block_sum64(s, sums);
-  if (tid == 0) a.left[(int64_t)r * a.chunks + c] = s;
+    for (int i = 0; i < PER; i++) sum += v[i];
+    sum = wave_sum64(sum);
+  } else {  // p's share of the chunk is known
+    const ChunkStat k = a.stats[(int64_t)f.row * a.chunks + c];
+    sum = k.s * weight(k.m, f.m, f.t2);
+  }
+  if (lane == 0) a.left[(int64_t)r * a.chunks + c] = sum;
 }
 
-// Block (request): the token, then the request's rows of the result.
-template <int PER> __global__ void __launch_bounds__(VT) verify_draw_kernel(const VerifyArgs a) {
-  __shared__ double sums[VT / 64], goal;
-  __shared__ int chunk, token, other, lasts[VT / 64];
-  const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+// Wave (request): the chunk, the token, and the request's rows of the result.
+template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_kernel(const VerifyArgs a) {
+  const int r = blockIdx.x, lane = threadIdx.x;
+  if (r == a.requests) {  // rows behind the last request's
+    for (int j = max(0, gload(a.starts + a.requests)) + lane; j < a.rows; j += 64) a.tokens[j] = -1;
+    return;
+  }
   int n;
   const int start = request_rows(a, r, &n);
-  if (r == 0)  // rows behind the last request's
-    for (int j = max(0, gload(a.starts + a.requests)) + tid; j < a.rows; j += VT) a.tokens[j] = -1;
-  if (n <= 0) {
-    if (tid == 0) a.counts[r] = 0;
+  if (n == 0) {
+    if (lane == 0) a.counts[r] = 0;
     return;
   }
-  Refusal f = a.refusals[r];
-  const int row = start + f.accepted;
-  const float t = inverse(a, row);
-  if (f.m == NONE || greedy(t)) {
-    if (tid == 0) token = f.m == NONE ? -1 : f.at;
-  } else {
-    if (tid < 64) {
-      double s = lane < a.chunks ? a.left[(int64_t)r * a.chunks + lane] : 0.0;
-      double all = wave_sum64(s);
-      if (!(all > 0.0)) {  // p nowhere over q, yet a draft refused (by rounding): all of p is drawn from
-        const ChunkStat k = lane < a.chunks ? a.stats[(int64_t)row * a.chunks + lane] : ChunkStat{0.0, NONE, 0};
-        s = k.s * weight(k.m, f.m, t) / f.z, all = wave_sum64(s);
-        if (lane == 0) other = 1;
-      } else if (lane == 0) {
-        other = 0;
-      }
-      double upto = s;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const double up = __shfl_up(upto, d, 64);
-        if (lane >= d) upto += up;
-      }
-      const double aim = (double)gload(a.uniforms + a.uniforms_sr + row) * all;
-      // the first chunk whose running sum passes the aim; by rounding none may, then the last with any weight
-      const uint64_t past = __ballot(upto > aim && s > 0.0), any = __ballot(s > 0.0);
-      const int pick = past ? __builtin_ctzll(past) : any ? 63 - __builtin_clzll(any) : 0;
-      if (lane == pick) chunk = pick, goal = aim - (upto - s);
+  Draw f = a.draws[r];
+  if (f.token == NOWHERE) {
+    const double *left = a.left + (int64_t)r * a.chunks;
+    const float u = gload(a.uniforms + a.uniforms_sr + f.row);
+    const int each = (a.chunks + 63) / 64, c0 = lane * each, c1 = min(c0 + each, a.chunks);  // the lane's chunks
+    double s = 0.0;
+#pragma unroll 4
+    for (int c = c0; c < c1; c++) s += gload(left + c);
+    double all = wave_sum64(s);
+    const bool none = !(all > 0.0);  // p nowhere over q, yet a draft refused (by rounding): all of p is drawn from
+    const ChunkStat *stats = a.stats + (int64_t)f.row * a.chunks;
+    const auto chunk = [&](int c) { return none ? stats[c].s * weight(stats[c].m, f.m, f.t2) : gload(left + c); };
+    if (none) {
+      f.refused = 0, f.without = -1, s = 0.0;
+      for (int c = c0; c < c1; c++) s += chunk(c);
+      all = wave_sum64(s);
     }
-    __syncthreads();
-    if (other) f.refused = 0;
-    // PER tokens in a row a thread; its running sum over the threads before it, as the block's order has it
-    const int v0 = chunk * a.chunk + tid * PER, w = tid >> 6;
-    double left[PER], s = 0.0;
-    left_of<PER>(a, f, row, t, v0, 1, min(a.vocab, (chunk + 1) * a.chunk), left);
-    int last = -1;
-#pragma unroll
-    for (int i = 0; i < PER; i++) s += left[i], last = left[i] > 0.0 ? v0 + i : last;
-    double upto = s;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double up = __shfl_up(upto, d, 64);
-      if (lane >= d) upto += up;
+    double goal = (double)u * all, upto = wave_before(s), from = 0.0;
+    // the first chunk whose running sum passes the goal; by rounding none may, then the last with any weight
+    int pick = NOWHERE, last = -1;
+#pragma unroll 4
+    for (int c = c0; c < c1; c++) {
+      const double l = chunk(c);
+      if (l > 0.0) last = c;
+      if (pick == NOWHERE && l > 0.0 && upto + l > goal) pick = c, from = upto;
+      upto += l;
     }
+    uint64_t who = __ballot(pick != NOWHERE);
+    if (who) {
+      const int l = __builtin_ctzll(who);
+      pick = __shfl(pick, l, 64), goal -= __shfl(from, l, 64);
+    } else {
+      who = __ballot(last >= 0);
+      pick = who ? __shfl(last, 63 - __builtin_clzll(who), 64) : 0, goal = __builtin_inf();
+    }
+    pick = __builtin_amdgcn_readfirstlane(pick);
+    // the chunk's tokens in order: RUN in a row a lane, 64 RUN a turn
+    constexpr int RUN = WIDE ? 4 : 1, TURNS = PER / RUN;
+    double v[PER], before[TURNS], carry = 0.0;
+    left_of<PER, WIDE>(a, f, pick, lane, v);
 #pragma unroll
-    for (int d = 32; d; d /= 2) last = max(last, __shfl_xor(last, d, 64));
-    if (lane == 63) sums[w] = upto, lasts[w] = last;
-    if (tid == 0) token = 0x7FFFFFFF;
-    __syncthreads();
-    double before = 0.0;
+    for (int i = 0; i < TURNS; i++) {
+      double mine = 0.0;
 #pragma unroll
-    for (int i = 0; i < VT / 64; i++) before += i < w ? sums[i] : 0.0;
-    before += upto - s;
-    if (before + s > goal) {  // the first token past the goal is the lowest that any thread finds
-      int pick = 0x7FFFFFFF;
-      double sum = before;
+      for (int k = 0; k < RUN; k++) mine += v[RUN * i + k];
+      before[i] = wave_before(mine);
+      const double turn = __shfl(before[i] + mine, 63, 64);
+      before[i] += carry, carry += turn;
+    }
+    int best = NOWHERE;
+    last = -1;
 #pragma unroll
-      for (int i = 0; i < PER; i++) {
-        sum += left[i];
-        if (pick == 0x7FFFFFFF && left[i] > 0.0 && sum > goal) pick = v0 + i;
+    for (int i = 0; i < PER; i++) {
+      const int e = pick * 64 * PER + Chunk<PER, WIDE>::place(lane, i);
+      before[i / RUN] += v[i];
+      if (v[i] > 0.0) {
+        last = e;
+        if (best == NOWHERE && before[i / RUN] > goal) best = e;
       }
-      atomicMin(&token, pick);
     }
-    __syncthreads();
-    if (tid == 0 && token == 0x7FFFFFFF)  // by rounding none passes it: the last with any weight
-      token = max(max(lasts[0], lasts[1]), max(lasts[2], lasts[3]));
+    best = wave_min(best);
+    f.token = best != NOWHERE ? best : -wave_min(-last);
   }
-  __syncthreads();
-  for (int i = tid; i < n; i += VT)
-    a.tokens[start + i] = i < f.accepted ? gload(a.ids + start + i + 1) : i == f.accepted ? token : -1;
-  if (tid == 0) a.counts[r] = f.accepted + (token >= 0);
+  for (int i = lane; i < n; i += 64)
+    a.tokens[start + i] = i < f.accepted ? gload(a.ids + start + i + 1) : i == f.accepted ? f.token : -1;
+  if (lane == 0) a.counts[r] = f.accepted + (f.token >= 0);
 }
 
-// How a call's rows are cut: 64 chunks at most (a lane a chunk where they join).
-static void verify_chunks(const bt_verify_args *a, int *chunk, int *chunks) {
-  int per = 8;  // logits a thread
-  while ((int64_t)per * VT * 64 < a->vocab) per *= 2;
-  *chunk = per * VT;
-  *chunks = ceil_div(a->vocab, *chunk);
-}
+// Logits a lane of a chunk's 64: 8 up to 2^22 logits, where larger chunks would leave waves too few to fill the card (5 rows of
+// 49152 12.3 us), else 16, which spreads a chunk's maximum and sums over more of them (112 rows of 131072 in 32 requests: the three
+// launches 13.1, 8.5 and 5.9 us; with 32 a lane, whose draw is one wave's long run, 14.4, 10.4 and 9.3).
+static int verify_per(const bt_verify_args *a) { return (int64_t)a->rows * a->vocab <= 1 << 22 ? 8 : 16; }
 static int check_verify(const bt_verify_args *a) {
   if (!a || !a->logits || !a->ids || !a->starts || !a->uniforms || !a->tokens || !a->counts)
     return fail(BT_EINVAL, "verifying drafts needs logits, ids, starts, uniforms and results");
@@ -312,18 +388,17 @@ static int check_verify(const bt_verify_args *a) {
     return fail(BT_EINVAL, "verifying %d requests' %d rows of %d logits (each 1 to 2^20)", a->requests, a->rows, a->vocab);
   return BT_OK;
 }
+static int verify_chunks(const bt_verify_args *a) { return ceil_div(a->vocab, 64 * verify_per(a)); }
 static uint64_t verify_bytes(const bt_verify_args *a) {
-  int chunk, chunks;
-  verify_chunks(a, &chunk, &chunks);
-  return (uint64_t)a->rows * chunks * sizeof(ChunkStat) + (uint64_t)a->requests * (chunks * 8 + sizeof(Refusal));
+  return (uint64_t)a->rows * verify_chunks(a) * sizeof(ChunkStat) + (uint64_t)a->requests * (sizeof(Draw) + 8 * verify_chunks(a));
 }
 
-template <int PER> static int launch_verify(const VerifyArgs &k, hipStream_t s) {
-  verify_stats_kernel<PER><<<(unsigned)(k.rows * k.chunks), VT, 0, s>>>(k);
+template <int PER, bool WIDE> static int launch_verify(const VerifyArgs &k, hipStream_t s) {
+  verify_stats_kernel<PER, WIDE><<<(unsigned)ceil_div((int64_t)k.rows * k.chunks, WAVES), 64 * WAVES, 0, s>>>(k);
   BT_LAUNCHED("verifying drafts");
-  verify_left_kernel<PER><<<(unsigned)(k.requests * k.chunks), VT, 0, s>>>(k);
+  verify_left_kernel<PER, WIDE><<<(unsigned)(k.requests * ceil_div(k.chunks, WAVES)), 64 * WAVES, 0, s>>>(k);
   BT_LAUNCHED("verifying drafts");
-  verify_draw_kernel<PER><<<(unsigned)k.requests, VT, 0, s>>>(k);
+  verify_draw_kernel<PER, WIDE><<<(unsigned)(k.requests + 1), 64, 0, s>>>(k);
   BT_LAUNCHED("verifying drafts");
   return BT_OK;
 }
@@ -352,20 +427,16 @@ int bt_verify(bt_runtime *rt, const bt_verify_args *a) {
   k.logits = f(a->logits), k.probs = f(a->probs), k.t = f(a->t), k.uniforms = f(a->uniforms);
   k.ids = (const int32_t *)(uintptr_t)a->ids, k.starts = (const int32_t *)(uintptr_t)a->starts;
   k.tokens = (int32_t *)(uintptr_t)a->tokens, k.counts = (int32_t *)(uintptr_t)a->counts;
+  k.chunks = verify_chunks(a);
+  k.stats = (ChunkStat *)(uintptr_t)a->scratch;
+  k.draws = (Draw *)(k.stats + (int64_t)a->rows * k.chunks), k.left = (double *)(k.draws + a->requests);
   k.logits_sr = a->logits_sr, k.probs_sr = a->probs_sr, k.t_sr = a->t_sr, k.uniforms_sr = a->uniforms_sr;
   k.requests = a->requests, k.rows = a->rows, k.vocab = a->vocab;
-  verify_chunks(a, &k.chunk, &k.chunks);
-  k.stats = (ChunkStat *)(uintptr_t)a->scratch;
-  k.refusals = (Refusal *)(k.stats + (int64_t)a->rows * k.chunks);
-  k.left = (double *)(k.refusals + a->requests);
-  const int64_t blocks = (int64_t)std::max(a->rows, a->requests) * k.chunks;
-  if (blocks > 0x7FFFFFFF) return fail(BT_EINVAL, "verifying %d rows of %d logits is too large", a->rows, a->vocab);
-  switch (k.chunk / VT) {
-    case 8: return launch_verify<8>(k, r->stream);
-    case 16: return launch_verify<16>(k, r->stream);
-    case 32: return launch_verify<32>(k, r->stream);
-    default: return launch_verify<64>(k, r->stream);
-  }
+  if ((int64_t)std::max(a->rows, a->requests) * k.chunks > 0x7FFFFFFF)
+    return fail(BT_EINVAL, "verifying %d rows of %d logits is too large", a->rows, a->vocab);
+  const bool wide = a->logits % 16 == 0 && a->logits_sr % 4 == 0 && a->probs % 16 == 0 && a->probs_sr % 4 == 0 && a->vocab % 4 == 0;
+  if (verify_per(a) == 8) return wide ? launch_verify<8, true>(k, r->stream) : launch_verify<8, false>(k, r->stream);
+  return wide ? launch_verify<16, true>(k, r->stream) : launch_verify<16, false>(k, r->stream);
 }
 
 }  // extern "C"

@@ -95,19 +95,20 @@ def attend(q, values, tables, starts, lengths, window=0):
 
 
 def verify(logits, ids, starts, uniforms, probs=None, t=None):
-  """(tokens, counts) as serve.verify gives them."""
+  """(tokens, counts) as serve.verify gives them. What is drawn from is not normalized, in extended precision, so that equal weights
+  add exactly and a number on the border between two falls where it should."""
   rows, vocab = logits.shape
   x = np.where(np.isnan(logits), -np.inf, np.minimum(logits.astype(np.float64), np.finfo(np.float32).max))
   tokens, counts = np.full(rows, -1), []
   t = np.ones(rows) if t is None else np.asarray(t, np.float64).reshape(rows)
   t = np.where(t > 0, t, 0)
 
-  def choice(j):  # p of row j, or None where it has no token
-    if not (x[j] > -np.inf).any(): return None
-    if t[j] == np.inf: return np.eye(1, vocab, np.argmax(x[j]))[0]
+  def choice(j):  # (weights of row j, their sum: p times it), or (None, 0) where it has no token
+    if not (x[j] > -np.inf).any(): return None, 0
+    if t[j] == np.inf: return np.eye(1, vocab, np.argmax(x[j]))[0], 1
     with np.errstate(invalid="ignore"):
-      e = np.where(x[j] > -np.inf, np.exp(t[j] * (x[j] - x[j].max())), 0)
-    return e / e.sum()
+      e = np.where(x[j] > -np.inf, np.exp(np.longdouble(t[j]) * (x[j] - x[j].max())), 0)
+    return e, e.sum()
 
   def draw(w, u):
     upto = np.cumsum(w)
@@ -116,20 +117,20 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None):
   for s, e in zip(starts[:-1], starts[1:]):
     a, n, made = 0, e - s, -1
     while n > 0:
-      p = choice(s + a)
+      p, z = choice(s + a)
       if a == n - 1:
         if p is not None: made = draw(p, uniforms[1, s + a])
         break
       d = ids[s + a + 1]
-      q = probs[s + a + 1].astype(np.float64) if probs is not None else np.zeros(vocab)
+      q = probs[s + a + 1].astype(np.longdouble) if probs is not None else np.zeros(vocab)
       inside = 0 <= d < vocab
       if probs is None and inside: q[d] = 1
-      if p is not None and inside and np.float64(uniforms[0, s + a + 1]) * q[d] < p[d]:
+      if p is not None and inside and uniforms[0, s + a + 1] * q[d] * z < p[d]:
         tokens[s + a] = d
         a += 1
         continue
       if p is not None:
-        left = np.maximum(p - q, 0) if t[s + a] < np.inf else p
+        left = p if t[s + a] == np.inf else np.maximum(p - q * z, 0) if probs is not None else np.where(q > 0, 0, p)
         made = draw(left if left.sum() > 0 else p, uniforms[1, s + a])
       break
     if n > 0: tokens[s + a] = made

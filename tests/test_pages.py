@@ -78,7 +78,7 @@ def test_verify_refuses(bad):
             "vocab": 1000}
   n = ctypes.c_uint64()
   _lib.call("verify_scratch", ctypes.byref(_lib.VerifyArgs(**fields)), ctypes.byref(n))
-  assert n.value == 5 * 16 + 8 + 24
+  assert n.value == 5 * 2 * 16 + 40 + 2 * 8  # 1000 logits are two chunks of 512
   with pytest.raises(ValueError, match="verifying"):
     _lib.call("verify_scratch", ctypes.byref(_lib.VerifyArgs(**(fields | bad))), ctypes.byref(n))
 
