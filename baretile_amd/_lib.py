@@ -77,13 +77,12 @@ class PlanArgs(ctypes.Structure):  # bt_plan_args
               ("taken", c_uint64), ("starts", c_uint64), ("lengths", c_uint64), ("places", c_uint64),
               ("slots", c_uint64), ("taken_out", c_uint64), ("parts", c_uint64), ("tables_sr", c_int64),
               ("requests", c_int32), ("width", c_int32), ("n_free", c_int32), ("rows", c_int32), ("page", c_int32),
-              ("pages", c_int32), ("most", c_int32), ("target", c_int32)]
+              ("pages", c_int32), ("most", c_int32), ("kv", c_int32)]
 
 
 class BatchArgs(ctypes.Structure):  # bt_batch
   _fields_ = [("tables", c_uint64), ("starts", c_uint64), ("lengths", c_uint64), ("parts", c_uint64),
-              ("tables_sr", c_int64), ("requests", c_int32), ("width", c_int32), ("rows", c_int32), ("most", c_int32),
-              ("target", c_int32), ("pad_", c_int32)]
+              ("tables_sr", c_int64), ("requests", c_int32), ("width", c_int32), ("rows", c_int32), ("most", c_int32)]
 
 
 class VerifyArgs(ctypes.Structure):  # bt_verify_args

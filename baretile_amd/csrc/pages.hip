@@ -4,8 +4,10 @@
 // A page holds `page` tokens of every key and value head under one id. A head's values are e4m3 codes (4 exponent and 3
 // mantissa bits, at most 448) times one power of two for the page and head, so each is exact in bf16 and the conversion
 // v_cvt_scalef32_pk_bf16_fp8 applies the scale: half an instruction a value, where a block float's decoding takes 2.5.
-// Keys are kept by row, [page][head width], and values by dimension, [head width][page], so that both products of
-// attention read their operands from memory as they lie, 16 bytes a lane, with no transposition and no trip through LDS:
+// Keys are kept by row, 64 dims at a time, [head width / 64][page][64], and values by dimension, [head width][page], so that both
+// products of attention read their operands from memory as they lie, 16 bytes a lane, with no transposition and no trip
+// through LDS, and each load of a wave covers whole lines (rows of 128 dims, of which a load takes half a line each: 8
+// requests of 8191 keys 20.8 us, by halves 19.5; 32 of 4096 47.5 and 45.4):
 //   S^T = K Q^T: lane (n, g) (n = l % 16, g = l / 16) holds for tile kt (of 4 in a block of 64 keys) the key
 //     16 (n / 4) + 4 kt + n % 4, dims 64 j + 16 g .. + 15 (the contraction takes dims in any order that both operands share);
 //   so in the result lane (n, g) holds keys 16 g + 4 kt + i, i < 4, against pair n: 16 keys in a row over the 4 tiles;
@@ -23,7 +25,9 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KB = 64;          // keys of a block
-constexpr int MOST_PARTS = 64;  // parts of one request
+constexpr int MOST_PARTS = 32;  // parts of one request
+constexpr int SHORT = 8 * KB;   // keys that tables of one part a request hold at most
+constexpr int WAVES = 2048;     // waves that attention's parts are for, over all key heads
 constexpr int MOST_REQUESTS = 2048;
 
 // ---- the plan ------------------------------------------------------------------------------------------------------
@@ -33,7 +37,7 @@ struct PlanArgs {
   const int32_t *cached, *fresh, *free_pages, *taken;
   int32_t *starts, *lengths, *places, *slots, *taken_out, *parts;
   int64_t tables_sr;
-  int32_t requests, width, n_free, rows, page_log2, pages, most, target;
+  int32_t requests, width, n_free, rows, page_log2, pages, most, target, least;
 };
 
 __device__ __forceinline__ int pages_of(int n, int lg) { return (n + (1 << lg) - 1) >> lg; }
@@ -80,7 +84,8 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int j, int start, in
 
 // One block. Requests are scanned 1024 at a time: first their rows, cut to `most` each and to the rows there are, and the
 // pages they take; then, with the keys' blocks counted, the parts that attention cuts each request's keys into: as many
-// parts over all requests as `target`, of whole blocks of 64 keys, so that uneven lengths make parts of even length.
+// parts over all requests as `target`, of whole blocks of 64 keys and `least` of them, so that uneven lengths make parts of
+// even length.
 // Latency bounds it: three scans of about a microsecond and two trips to memory.
 constexpr int PLAN_NT = 1024;
 constexpr int PLAN_ROWS = 2048;  // rows that the plan's one block writes itself; more go to plan_rows_kernel's many
@@ -121,7 +126,7 @@ __global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
     a.starts[a.requests] = last;
     a.taken_out[0] = taken + takes;
   }
-  const int per = max(1, (blocks + a.target - 1) / a.target);
+  const int per = max(a.least, ((blocks + a.target - 1) / a.target + 3) & ~3);
   int made = 0;
   __syncthreads();
   for (int base = 0; base < a.requests; base += PLAN_NT) {
@@ -281,13 +286,13 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
   const float s = fmaxf(scale_of(top), old), inv = __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, exact
   const float by = old * inv;
   uint8_t *to = c.values + (((int64_t)id * heads + h) << lg) * HD;
-  if (h < c.kv) {  // keys: whole rows
+  if (h < c.kv) {  // keys: 64 dims of a row are 4 units of 16
     if (held && by != 1.0f)
       for (int e = tid; e < held * HD / 16; e += 256) {
-        u32x4 w = *(const u32x4 *)(to + 16 * e);
+        u32x4 *at = (u32x4 *)(to + (e / 4 / held << (lg + 6)) + e / 4 % held * 64 + e % 4 * 16), w = *at;
 #pragma unroll
         for (int k = 0; k < 4; k++) w[k] = rescaled4(w[k], by);
-        *(u32x4 *)(to + 16 * e) = w;
+        *at = w;
       }
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
@@ -296,7 +301,7 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
         uint2 w;
         const auto val = [&](int k) { return __uint_as_float(k & 1 ? v[i][k / 2] & 0xFFFF0000u : v[i][k / 2] << 16) * inv; };
         w.x = codes_of4(val(0), val(1), val(2), val(3)), w.y = codes_of4(val(4), val(5), val(6), val(7));
-        *(uint2 *)(to + held * HD + 8 * e) = w;
+        *(uint2 *)(to + (e % U / 8 << (lg + 6)) + (held + e / U) * 64 + e % 8 * 8) = w;
       }
     }
   } else {  // values: each dimension's codes lie along the page
@@ -349,9 +354,10 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const PoolArgs c, uint1
               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, false));
   };
   if (h < c.kv) {
-    for (int e = tid; e < page * HD / 8; e += 256) {
+    for (int e = tid; e < page * HD / 8; e += 256) {  // e: 8 codes as they lie
       const uint2 w = gload((const uint2 *)(from + 8 * e));
-      *(uint4 *)(to + 8 * e) = make_uint4(pair(w.x, false), pair(w.x, true), pair(w.y, false), pair(w.y, true));
+      const int row = e / 8 & (page - 1), dim = (e >> (lg + 3)) * 64 + e % 8 * 8;
+      *(uint4 *)(to + row * HD + dim) = make_uint4(pair(w.x, false), pair(w.x, true), pair(w.y, false), pair(w.y, true));
     }
     return;
   }
@@ -379,7 +385,8 @@ struct AttendArgs {
   uint16_t *out;
   float *scratch;
   int64_t q_sh, q_sr, o_sh, o_sr;
-  int32_t rep, window, items, few;  // items: the most parts a plan makes; few: the most query pairs that parts are for
+  int32_t rep, window, items, few, groups;  // items: the most parts a plan makes; few: the most query pairs that parts
+                                             // are for, in `groups` that fold the keys apart
   FastDiv drep;
 };
 
@@ -554,30 +561,38 @@ template <int HD> __device__ __forceinline__ void store_rows(const AttendArgs &a
                                           pack_rne(st.o[c][2] * inv, st.o[c][3] * inv));
 }
 
-// Few query pairs a request: a wave a part. A part is a run of whole blocks of 64 keys of one request, against QT tiles of
-// 16 of its pairs, so every key and value is read and converted once for all of them. A block's keys are requested while
-// the block before weighs its scores, its values while it multiplies, so 16 KB (heads of 128) are always in flight.
-template <int HD, int QT>
-__global__ void __launch_bounds__(64) pages_few_kernel(const AttendArgs a) {
+// Few query pairs a request: a block of NW waves a part. A part is a run of whole blocks of 64 keys of one request, against QT
+// tiles of 16 of its pairs, so every key and value is read and converted once for all of them; the waves take its
+// blocks in turn and join by halves through LDS, lane by lane, since every wave's state lies in the same lanes. A block's keys are
+// requested while the block before weighs its scores, its values while it multiplies, so 16 KB a wave (heads of 128) are always
+// in flight. Two waves a SIMD: held to their registers (the compiler's own choice put O into accumulation registers as
+// well, which left one of QT = 2: 16 requests of 5 rows of 4 heads over 2048 keys 20.1 us, 15.2 so).
+template <int HD, int QT, int NW>
+__global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs a) {
   constexpr int J = HD / 64, C = HD / 16;
-  const int lane = threadIdx.x, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
-  if (blockIdx.x >= (uint32_t)(a.items * a.c.kv)) return clear_rows<HD>(a, blockIdx.x - a.items * a.c.kv, lane, 64);
-  const int item = blockIdx.x / a.c.kv, kvh = blockIdx.x - item * a.c.kv;
+  __shared__ __attribute__((aligned(16))) f32x4 joined[NW / 2][QT * C][64];
+  __shared__ float joined_m[NW / 2][QT][64], joined_l[NW / 2][QT][64];
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int units = a.items * a.c.kv, group = blockIdx.x / units, unit = blockIdx.x - group * units;
+  if (group >= a.groups) return clear_rows<HD>(a, blockIdx.x - a.groups * units, tid, 64 * NW);
+  const int item = unit / a.c.kv, kvh = unit - item * a.c.kv, pair0 = 16 * QT * group;
   const int per = gload(a.b.parts + a.b.requests + 1);
   Piece p;
   const int32_t *at = a.b.parts;
   if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p)) return;
   const int pairs = p.n * a.rep;
-  if (pairs > a.few) return;
+  if (pairs > a.few || pair0 >= pairs) return;
   const int room = min(p.len, a.b.width << lg), nb = (room + KB - 1) / KB;
   const int mine = max(per, (nb + MOST_PARTS - 1) / MOST_PARTS), parts = (nb + mine - 1) / mine;
   int b0 = p.k * mine;
   const int b1 = min(b0 + mine, nb);
   if (a.window > 0) b0 = max(b0, max(p.len - p.n - a.window + 1, 0) / KB);
+  b0 += wave;
   Query<HD> q[QT];
   Running<HD> st[QT];
 #pragma unroll
-  for (int t = 0; t < QT; t++) q[t].load(a, p, kvh, 16 * t + n, g), st[t].clear();
+  for (int t = 0; t < QT; t++) q[t].load(a, p, kvh, pair0 + 16 * t + n, g), st[t].clear();
   if (b0 < b1) {
     const int64_t head = (int64_t)HD << lg;  // codes of one page of one head
     int p0 = b0 * KB >> lg;
@@ -592,11 +607,11 @@ __global__ void __launch_bounds__(64) pages_few_kernel(const AttendArgs a) {
       const int key = b * KB + 16 * (n >> 2), from = (key >> lg) - p0;
       const int id = max(__shfl(run.id, from, 64), 0);
       s = __shfl(run.ks, from, 64);
-      const uint8_t *k = a.c.values + ((int64_t)id * (2 * a.c.kv) + kvh) * head + ((key & mask) + (n & 3)) * HD + 16 * g;
+      const uint8_t *k = a.c.values + ((int64_t)id * (2 * a.c.kv) + kvh) * head + ((key & mask) + (n & 3)) * 64 + 16 * g;
 #pragma unroll
       for (int kt = 0; kt < 4; kt++)
 #pragma unroll
-        for (int j = 0; j < J; j++) kw[kt][j] = __builtin_nontemporal_load((const u32x4 *)(k + 4 * kt * HD + 64 * j));
+        for (int j = 0; j < J; j++) kw[kt][j] = __builtin_nontemporal_load((const u32x4 *)(k + 4 * kt * 64 + (j << (lg + 6))));
     };
     const auto fetch_values = [&](int b, float &s, int &valid) {
       const int key = b * KB + 16 * g, from = (key >> lg) - p0;
@@ -608,96 +623,113 @@ __global__ void __launch_bounds__(64) pages_few_kernel(const AttendArgs a) {
     };
     fetch_keys(b0, ks);
     fetch_values(b0, vs, id_v);
-    for (int b = b0; b < b1; b++) {
-      const bool more = b + 1 < b1;
+    for (int b = b0; b < b1; b += NW) {
+      const bool more = b + NW < b1;
       fold_block<HD, QT>(q, st, b * KB + 16 * g, id_v >= 0, ks, vs, [&](int kt, int j) { return kw[kt][j]; },
                          [&](int c) { return vw[c]; }, [&] {
-                           if (more) turn(b + 1), fetch_keys(b + 1, ks_next);
+                           if (more) turn(b + NW), fetch_keys(b + NW, ks_next);
                          });
-      if (more) fetch_values(b + 1, vs_next, id_v_next);
+      if (more) fetch_values(b + NW, vs_next, id_v_next);
       ks = ks_next, vs = vs_next, id_v = id_v_next;
     }
   }
 #pragma unroll
+  for (int half = NW / 2; half; half /= 2) {
+    if (wave >= half && wave < 2 * half) {
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        joined_m[wave - half][t][lane] = st[t].m, joined_l[wave - half][t][lane] = st[t].l;
+#pragma unroll
+        for (int c = 0; c < C; c++) joined[wave - half][t * C + c][lane] = st[t].o[c];
+      }
+    }
+    __syncthreads();
+    if (wave < half) {
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        const float m = joined_m[wave][t][lane], top = fmaxf(st[t].m, m);
+        const float mine = st[t].m == -INF ? 0.0f : __builtin_amdgcn_exp2f(st[t].m - top);
+        const float other = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        st[t].m = top, st[t].l = st[t].l * mine + joined_l[wave][t][lane] * other;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          const f32x4 o = joined[wave][t * C + c][lane];
+#pragma unroll
+          for (int i = 0; i < 4; i++) st[t].o[c][i] = st[t].o[c][i] * mine + o[i] * other;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (wave) return;
+#pragma unroll
   for (int t = 0; t < QT; t++) {
-    const int pair = 16 * t + n;
+    const int pair = pair0 + 16 * t + n;
     const float l = sum_groups(st[t].l);
     if (pair >= pairs) continue;
     if (parts == 1) {
       store_rows<HD>(a, p, kvh, pair, g, st[t], l);
-    } else {  // the part's sums for the combine: O by pair, then the pairs' maxima and sums
-      float *to = a.scratch + ((int64_t)item * a.c.kv + kvh) * (16 * QT * (HD + 2));
+    } else {  // the part's sums for the join: the pair's O, then its maximum and sum
+      float *to = a.scratch + (int64_t)unit * a.few * (HD + 4) + pair * (HD + 4);
 #pragma unroll
-      for (int c = 0; c < C; c++) *(f32x4 *)(to + pair * HD + 16 * c + 4 * g) = st[t].o[c];
-      if (g == 0) to[16 * QT * HD + 2 * pair] = st[t].m, to[16 * QT * HD + 2 * pair + 1] = l;
+      for (int c = 0; c < C; c++) *(f32x4 *)(to + 16 * c + 4 * g) = st[t].o[c];
+      if (g == 0) to[HD] = st[t].m, to[HD + 1] = l;
     }
   }
 }
 
-// Joins a request's parts: block (request, key head, pair), its 4 waves a quarter of the parts each, then each other's
-// sums through LDS: M = max m, L = sum 2^(m - M) l, out = sum 2^(m - M) O / L.
-template <int HD, int QT>
-__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a, int most_pairs) {
-  constexpr int V = HD / 64, STRIDE = 16 * QT * (HD + 2), TURN = 8;
-  __shared__ float ms[4], ls[4], os[4][HD];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  int u = blockIdx.x;
-  const int pair = u % most_pairs;
-  u /= most_pairs;
-  const int kvh = u % a.c.kv, r = u / a.c.kv;
+// Joins a request's parts: a wave (request, key head, pair), 4 a block; M = max m, L = sum 2^(m - M) l, out = sum 2^(m - M) O / L.
+// 16 parts' sums are requested at once, so that the usual plan is one trip to memory.
+template <int HD>
+__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
+  constexpr int V = HD / 64, TURN = 16;
+  const int lane = threadIdx.x & 63;
+  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = unit / a.few;
+  const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
+  if (r >= a.b.requests) return;
   const int row0 = gload(a.b.starts + r), n = gload(a.b.starts + r + 1) - row0, first = gload(a.b.parts + r);
   const int parts = gload(a.b.parts + r + 1) - first;
-  if (parts <= 1 || pair >= n * a.rep || n * a.rep > a.few) return;
-  const float *from = a.scratch + ((int64_t)first * a.c.kv + kvh) * STRIDE;
-  const int64_t step = (int64_t)a.c.kv * STRIDE;
+  if (parts <= 1 || first + parts > a.items || pair >= n * a.rep || n * a.rep > a.few) return;
+  const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
+  const float *from = a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4);
   float M = -INF, L = 0.0f, O[V];
 #pragma unroll
   for (int i = 0; i < V; i++) O[i] = 0.0f;
-  for (int b = w; b < parts; b += 4 * TURN) {
+  for (int b = 0; b < parts; b += TURN) {
     float m[TURN], l[TURN], o[TURN][V];
 #pragma unroll
-    for (int j = 0; j < TURN; j++) {  // past the last part it is read again and left out
-      const float *s = from + min(b + 4 * j, parts - 1) * step;
-      m[j] = gload(s + 16 * QT * HD + 2 * pair), l[j] = gload(s + 16 * QT * HD + 2 * pair + 1);
+    for (int j = 0; j < TURN; j++) {
+      m[j] = -INF, l[j] = 0.0f;
 #pragma unroll
-      for (int i = 0; i < V; i++) o[j][i] = gload(s + pair * HD + V * lane + i);
+      for (int i = 0; i < V; i++) o[j][i] = 0.0f;
+      if (b + j < parts) {  // (the whole wave's branch)
+        const float *s = from + (b + j) * step;
+        m[j] = gload(s + HD), l[j] = gload(s + HD + 1);
+#pragma unroll
+        for (int i = 0; i < V; i++) o[j][i] = gload(s + V * lane + i);
+      }
     }
     float top = M;
 #pragma unroll
-    for (int j = 0; j < TURN; j++) {
-      if (b + 4 * j >= parts) m[j] = -INF, l[j] = 0.0f;
-      top = fmaxf(top, m[j]);
-    }
+    for (int j = 0; j < TURN; j++) top = fmaxf(top, m[j]);
     const float keep = M == -INF ? 0.0f : __builtin_amdgcn_exp2f(M - top);
     L *= keep;
 #pragma unroll
     for (int i = 0; i < V; i++) O[i] *= keep;
 #pragma unroll
     for (int j = 0; j < TURN; j++) {
-      if (m[j] == -INF && l[j] == 0.0f) continue;  // nothing seen; its O was not written
-      const float by = __builtin_amdgcn_exp2f(m[j] - top);
+      const float by = m[j] == -INF ? 0.0f : __builtin_amdgcn_exp2f(m[j] - top);  // 0: nothing seen (0 of a NaN stays one)
       L += by * l[j];
 #pragma unroll
       for (int i = 0; i < V; i++) O[i] += by * o[j][i];
     }
     M = top;
   }
-  if (lane == 0) ms[w] = M, ls[w] = L;
-#pragma unroll
-  for (int i = 0; i < V; i++) os[w][V * lane + i] = O[i];
-  __syncthreads();
-  if (threadIdx.x >= HD / 2) return;
-  const float top = fmaxf(fmaxf(ms[0], ms[1]), fmaxf(ms[2], ms[3]));
-  float sum = 0.0f, x = 0.0f, y = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (ms[i] == -INF && ls[i] == 0.0f) continue;
-    const float by = __builtin_amdgcn_exp2f(ms[i] - top);
-    sum += by * ls[i], x += by * os[i][2 * threadIdx.x], y += by * os[i][2 * threadIdx.x + 1];
-  }
-  const float inv = sum > 0.0f ? 1.0f / sum : sum;
+  const float inv = L > 0.0f ? 1.0f / L : L;
   const int i = (int)fdiv((uint32_t)pair, a.drep), h = kvh * a.rep + pair - i * a.rep;
-  *(uint32_t *)(a.out + h * a.o_sh + (row0 + i) * a.o_sr + 2 * threadIdx.x) = pack_rne(x * inv, y * inv);
+  uint16_t *out = a.out + h * a.o_sh + (row0 + i) * a.o_sr + V * lane;
+  if constexpr (V == 2) *(uint32_t *)out = pack_rne(O[0] * inv, O[1] * inv);
+  else *out = (uint16_t)pack_rne(O[0] * inv, 0.0f);
 }
 
 // Many query pairs a request (a prompt's rows): a block of 4 waves takes 128 pairs of one key head, 32 a wave, so every
@@ -737,7 +769,7 @@ __global__ void __launch_bounds__(256, 2) pages_many_kernel(const AttendArgs a, 
     for (int i = 0; i < NU; i++) {
       const int u = tid + 256 * i;
       const int key = b * KB + u / UK, kid = max(__shfl(run.id, (key >> lg) - p0, 64), 0);
-      kr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)kid * (2 * a.c.kv) + kvh) * head + (key & mask) * HD + u % UK * 16));
+      kr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)kid * (2 * a.c.kv) + kvh) * head + (u % UK / 4 << (lg + 6)) + (key & mask) * 64 + u % 4 * 16));
       const int vkey = b * KB + 16 * (u & 3), vid = max(__shfl(run.id, (vkey >> lg) - p0, 64), 0);
       vr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)vid * (2 * a.c.kv) + a.c.kv + kvh) * head + (u / 4 << lg) + (vkey & mask)));
     }
@@ -796,23 +828,28 @@ static int check_pool(const bt_pages *c, PoolArgs *out) {
 
 constexpr int MOST_ROWS = 1 << 20;
 
+// The parts that a plan aims at, and a part's least blocks: all of a short table's keys (a part a request, and no join), else a
+// block for each of its 4 waves.
+static int parts_target(int kv) { return std::max(1, WAVES / (4 * kv)); }
+static int parts_least(int64_t keys) { return keys <= SHORT ? SHORT / KB : 4; }
+
 static int check_batch(const bt_batch *b, BatchArgs *out) {
   if (!b || !b->tables || !b->starts || !b->lengths || !b->parts) return fail(BT_EINVAL, "a batch needs its tables, starts, lengths and parts");
   if ((b->tables | b->starts | b->lengths | b->parts) % 4) return fail(BT_EINVAL, "a batch's tensors are int32-aligned");
-  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 || b->most < 1 ||
-      b->target < 1 || b->target > MOST_ROWS)
-    return fail(BT_EINVAL, "a batch of %d requests (1 to %d), %d rows (1 to %d), tables %d wide, %d rows a request at most, %d parts",
-                b->requests, MOST_REQUESTS, b->rows, MOST_ROWS, b->width, b->most, b->target);
+  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 || b->most < 1)
+    return fail(BT_EINVAL, "a batch of %d requests (1 to %d), %d rows (1 to %d), tables %d wide, %d rows a request at most",
+                b->requests, MOST_REQUESTS, b->rows, MOST_ROWS, b->width, b->most);
   if (out)
     *out = BatchArgs{(const int32_t *)(uintptr_t)b->tables, (const int32_t *)(uintptr_t)b->starts, (const int32_t *)(uintptr_t)b->lengths,
                      (const int32_t *)(uintptr_t)b->parts, b->tables_sr, b->requests, b->width, b->rows};
   return BT_OK;
 }
 
-// How a call is cut: `few`, the most pairs of a request whose keys are cut into parts, in `tiles` of 16; `many`, whether
-// requests may have more (their rows then share blocks of 128 pairs).
+// How a call is cut: `few`, the most pairs of a request whose keys are cut into parts, in tiles of 16 (`tiles` a wave); `many`,
+// whether requests may have more (their rows then share blocks of 128 pairs).
 struct AttendPlan {
-  int few, tiles, items;
+  int few, tiles, groups, items;
+  int waves;  // of a part's block
   bool many, join;
   uint64_t scratch;
 };
@@ -825,28 +862,30 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   const int64_t most = (int64_t)std::min(b->most, b->rows) * rep;
   p->many = most > 64;
   p->few = p->many ? 32 : (int)most;
-  p->tiles = p->few <= 16 ? 1 : p->few <= 32 ? 2 : 4;
-  p->items = b->target + b->requests;
+  p->tiles = p->few <= 16 ? 1 : 2;
+  p->groups = (p->few + 31) / 32;
+  p->items = parts_target(c->kv) + b->requests;
   const int64_t keys = (int64_t)b->width * c->page;
-  p->join = keys > KB;
-  const uint64_t bytes = (uint64_t)p->items * c->kv * (16 * p->tiles * (c->head_dim + 2)) * 4;
+  p->join = keys > SHORT;
+  p->waves = p->tiles == 1 && !p->join ? 8 : 4;
+  const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
-  if ((int64_t)p->items * c->kv > 0x3FFFFFFF) return fail(BT_EINVAL, "paged attention in %d parts of %d key heads", p->items, c->kv);
+  if ((int64_t)p->items * c->kv * p->groups > 0x3FFFFFFF || (int64_t)b->requests * heads * p->few > 0x7FFFFFFF) return fail(BT_EINVAL, "paged attention in %d parts of %d key heads", p->items, c->kv);
   return BT_OK;
 }
 
-template <int HD, int QT> static int launch_few(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+template <int HD, int QT, int NW> static int launch_few(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const int clear = (a.b.rows + 15) / 16;
-  pages_few_kernel<HD, QT><<<(unsigned)(p.items * a.c.kv + clear), 64, 0, s>>>(a);
+  pages_few_kernel<HD, QT, NW><<<(unsigned)(p.items * a.c.kv * p.groups + clear), 64 * NW, 0, s>>>(a);
   BT_LAUNCHED("paged attention");
   if (p.join) {
-    pages_join_kernel<HD, QT><<<(unsigned)(a.b.requests * a.c.kv * p.few), 256, 0, s>>>(a, p.few);
+    pages_join_kernel<HD><<<(unsigned)ceil_div((int64_t)a.b.requests * a.c.kv * p.few, 4), 256, 0, s>>>(a);
     BT_LAUNCHED("paged attention's join");
   }
   return BT_OK;
 }
 template <int HD> static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  const int status = p.tiles == 1 ? launch_few<HD, 1>(a, p, s) : p.tiles == 2 ? launch_few<HD, 2>(a, p, s) : launch_few<HD, 4>(a, p, s);
+  const int status = p.tiles == 2 ? launch_few<HD, 2, 4>(a, p, s) : p.waves == 8 ? launch_few<HD, 1, 8>(a, p, s) : launch_few<HD, 1, 4>(a, p, s);
   if (status || !p.many) return status;
   const int tiles = (int)((int64_t)a.b.rows * a.rep >> 7) + a.b.requests;
   pages_many_kernel<HD><<<(unsigned)(tiles * a.c.kv), 256, 0, s>>>(a, tiles);
@@ -873,13 +912,13 @@ int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
   while (lg < 9 && (1 << lg) != a->page) lg++;
   if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", a->page);
   if (a->requests < 1 || a->requests > MOST_REQUESTS || a->width < 1 || a->n_free < 1 || a->rows < 1 || a->rows > MOST_ROWS ||
-      a->most < 1 || a->target < 1 || a->pages < 1 || (int64_t)a->pages * a->page > 0x7FFFFFFFll)
+      a->most < 1 || a->kv < 1 || a->kv > 1024 || a->pages < 1 || (int64_t)a->pages * a->page > 0x7FFFFFFFll)
     return fail(BT_EINVAL, "a plan of %d requests (1 to %d), %d rows (1 to %d), %d a request at most, tables %d wide, %d free of %d pages",
                 a->requests, MOST_REQUESTS, a->rows, MOST_ROWS, a->most, a->width, a->n_free, a->pages);
   const auto at = [](uint64_t p) { return (int32_t *)(uintptr_t)p; };
   const PlanArgs k{at(a->tables), at(a->cached), at(a->fresh), at(a->free_pages), at(a->taken), at(a->starts), at(a->lengths),
                    at(a->places), at(a->slots), at(a->taken_out), at(a->parts), a->tables_sr, a->requests, a->width, a->n_free,
-                   a->rows, lg, a->pages, std::min(a->most, a->rows), a->target};
+                   a->rows, lg, a->pages, std::min(a->most, a->rows), parts_target(a->kv), parts_least((int64_t)a->width * a->page)};
   plan_kernel<<<1, PLAN_NT, 0, r->stream>>>(k);
   BT_LAUNCHED("a plan");
   if (a->rows > PLAN_ROWS) {
@@ -942,7 +981,7 @@ int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch,
     return fail(BT_EINVAL, "paged attention needs %llu bytes of 16-byte aligned scratch", (unsigned long long)p.scratch);
   a.q = (const uint16_t *)(uintptr_t)q, a.out = (uint16_t *)(uintptr_t)out, a.scratch = (float *)(uintptr_t)scratch;
   a.q_sh = q_sh, a.q_sr = q_sr, a.o_sh = o_sh, a.o_sr = o_sr;
-  a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few;
+  a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few, a.groups = p.groups;
   a.drep = make_fastdiv((uint32_t)a.rep);
   return pool->head_dim == 64 ? launch_attend<64>(a, p, r->stream) : launch_attend<128>(a, p, r->stream);
 }

@@ -41,12 +41,12 @@ class Batch:
   places: each row's place in its request, -1 behind the last request's rows; slots: the row of a flat cache of
   pages * page rows that the token takes, -1 where there is no page; taken: how many of the free list's pages are
   used so far (more than it has: that many less were missing)."""
-  def __init__(self, tables, starts, lengths, places, slots, taken, parts, rows, most, target, page, pages, kv):
+  def __init__(self, tables, starts, lengths, places, slots, taken, parts, rows, most, page, pages, kv):
     self.tables, self.starts, self.lengths, self.places, self.slots = tables, starts, lengths, places, slots
-    self.taken, self.parts, self.rows, self.most, self.target = taken, parts, rows, most, target
+    self.taken, self.parts, self.rows, self.most = taken, parts, rows, most
     self.page, self.pages, self.kv, self.requests = page, pages, kv, tables.rows
     self.args = _lib.BatchArgs(tables.addr, starts.addr, lengths.addr, parts.addr, tables.sr, tables.rows, tables.cols,
-                               rows, most, target, 0)
+                               rows, most)
 
 
 class Pages:
@@ -82,15 +82,14 @@ class Pages:
     cached, new, free = _row(cached, self.rt, "cached", n), _row(new, self.rt, "new", n), _row(free, self.rt, "free")
     if taken is not None: taken = _row(taken, self.rt, "taken", 1)
     most = min(most, rows)
-    target = max(1, 2048 // self.kv)
     made = lambda cols: Tensor(self.rt, 1, cols, dtype="int32")
     starts, lengths, places, slots, used, parts = (made(c) for c in (n + 1, n, rows, rows, 1, n + 2))
     _written(t.storage)
     args = _lib.PlanArgs(t.addr, cached.addr, new.addr, free.addr, taken.addr if taken is not None else 0, starts.addr,
                          lengths.addr, places.addr, slots.addr, used.addr, parts.addr, t.sr, n, t.cols, free.cols, rows,
-                         self.page, self.pages, most, target)
+                         self.page, self.pages, most, self.kv)
     self.rt.run("plan", "pages_plan", ctypes.byref(args))
-    return Batch(t, starts, lengths, places, slots, used, parts, rows, most, target, self.page, self.pages, self.kv)
+    return Batch(t, starts, lengths, places, slots, used, parts, rows, most, self.page, self.pages, self.kv)
 
   def _fits(self, batch):
     if not (isinstance(batch, Batch) and batch.tables.rt is self.rt and (batch.page, batch.pages, batch.kv) ==

@@ -347,8 +347,8 @@ int bt_put_bfp(bt_runtime *rt, int fmt, uint64_t exps, uint64_t vals, int64_t ba
  * lists a request's pages in order, so its token at place t lies in page tables[r, t / page], row t % page. An entry outside
  * [0, pages) holds no page: what would be put there is dropped, and attention doesn't see it.
  *
- * values: [pages][2 kv][page * head_dim] bytes, key heads then value heads; a key head's are [page][head_dim], a value
- * head's [head_dim][page]. A byte is an 8-bit float (sign, 4 exponent bits biased by 7, 3 mantissa bits; at most 448), and
+ * values: [pages][2 kv][page * head_dim] bytes, key heads then value heads; a key head's are [head_dim / 64][page][64], a
+ * value head's [head_dim][page]. A byte is an 8-bit float (sign, 4 exponent bits biased by 7, 3 mantissa bits; at most 448), and
  * stands for that times scales[id, head], fp32 [pages][2 kv], a power of two from 2^-100 to 2^119: exact in bf16. */
 typedef struct {
   uint64_t values, scales;
@@ -363,20 +363,22 @@ typedef struct {
  * the first page not begun, cached / page rounded up, to the last that the new length needs are kept up to the first
  * that holds no page; the others are taken from free_pages in order, after the first taken[0] (0 without taken), -1 where these run
  * out. taken_out[0] is taken[0] plus the entries so made: past n_free, so many pages were missing. Entries past the
- * tables' width are not made. parts[requests + 2] is bt_pages_attend's: about `target` runs of keys over all requests. */
+ * tables' width are not made. parts[requests + 2] is bt_pages_attend's, for caches of kv key
+ * heads: how it cuts the requests' keys. */
 typedef struct {
   uint64_t tables, cached, fresh, free_pages, taken;
   uint64_t starts, lengths, places, slots, taken_out, parts;
   int64_t tables_sr;
-  int32_t requests, width, n_free, rows, page, pages, most, target;
+  int32_t requests, width, n_free, rows, page, pages, most, kv;
 } bt_plan_args;
 int bt_pages_plan(bt_runtime *rt, const bt_plan_args *args);
 
-/* The plan's results that the calls below read; width, rows, most and target as they were planned with. */
+/* The plan's results that the calls below read; tables_sr, width, rows and most as they were planned with, for pools of its page, pages
+ * and kv. */
 typedef struct {
   uint64_t tables, starts, lengths, parts;
   int64_t tables_sr;
-  int32_t requests, width, rows, most, target, pad_;
+  int32_t requests, width, rows, most;
 } bt_batch;
 
 /* The batch's rows of 2 kv heads, x bf16 (element strides x_sb a head, x_sr a row), into their pages. A page's head takes the

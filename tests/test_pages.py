@@ -46,17 +46,17 @@ def test_structs_match_the_header(tmp_path):
 
 def need(pool=None, batch=None, heads=8, window=0):
   c = _lib.PagesArgs(**({"values": 4096, "scales": 4096, "pages": 10, "page": 64, "kv": 2, "head_dim": 64} | (pool or {})))
-  b = _lib.BatchArgs(**({"tables": 4096, "starts": 4096, "lengths": 4096, "parts": 4096, "tables_sr": 8, "requests": 3, "width": 8,
-                         "rows": 6, "most": 2, "target": 1024} | (batch or {})))
+  b = _lib.BatchArgs(**({"tables": 4096, "starts": 4096, "lengths": 4096, "parts": 4096, "tables_sr": 8, "requests": 3, "width": 20,
+                         "rows": 6, "most": 2} | (batch or {})))
   n = ctypes.c_uint64()
   _lib.call("pages_attend_scratch", ctypes.byref(c), ctypes.byref(b), heads, window, ctypes.byref(n))
   return n.value
 
 
 def test_attention_scratch():
-  # two heads, 1027 parts at most, 16 pairs (2 rows of 4 heads fill 8) of 64 dims, a maximum and a sum
-  assert need() == 1027 * 2 * 16 * 66 * 4
-  assert need(batch={"width": 1}) == 0  # one block of keys: nothing to join
+  # two heads, 256 + 3 parts at most, 8 pairs (2 rows of 4 heads) of 64 dims, a maximum and a sum in 4 words
+  assert need() == 259 * 2 * 8 * 68 * 4
+  assert need(batch={"width": 8}) == 0  # 512 keys at most: a part a request, nothing to join
 
 
 @pytest.mark.parametrize("bad, why", [
@@ -65,7 +65,7 @@ def test_attention_scratch():
   (dict(pool={"values": 0}), "values and scales"), (dict(pool={"values": 4104}), "aligned"),
   (dict(batch={"tables": 0}), "needs its tables"), (dict(batch={"starts": 4098}), "aligned"), (dict(batch={"requests": 0}), "a batch of"),
   (dict(batch={"requests": 2049}), "a batch of"), (dict(batch={"rows": (1 << 20) + 1}), "a batch of"), (dict(batch={"width": 0}), "a batch of"),
-  (dict(batch={"most": 0}), "a batch of"), (dict(batch={"target": 0}), "a batch of"), (dict(heads=7), "7 heads"), (dict(heads=0), "0 heads"),
+  (dict(batch={"most": 0}), "a batch of"), (dict(heads=7), "7 heads"), (dict(heads=0), "0 heads"),
   (dict(window=-1), "window")])
 def test_attention_refuses(bad, why):
   with pytest.raises(ValueError, match=why): need(**bad)
