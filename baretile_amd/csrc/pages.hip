@@ -4,8 +4,8 @@
 // A page holds `page` tokens of every key and value head under one id. A head's values are e4m3 codes (4 exponent and 3
 // mantissa bits, at most 448) times one power of two for the page and head, so each is exact in bf16 and the conversion
 // v_cvt_scalef32_pk_bf16_fp8 applies the scale: half an instruction a value, where a block float's decoding takes 2.5.
-// Keys are kept by row, 64 dims at a time, [head width / 64][page][64], and values by dimension, [head width][page], so that both
-// products of attention read their operands from memory as they lie, 16 bytes a lane, with no transposition and no trip
+// Keys are kept by row, 64 dims at a time, [head width / 64][page][64], and values by dimension, up to 64 tokens at a time,
+// [page / 64][head width][64], so that both products of attention read their operands from memory as they lie, 16 bytes a lane, with no transposition and no trip
 // through LDS, and each load of a wave covers whole lines (rows of 128 dims, of which a load takes half a line each: 8
 // requests of 8191 keys 20.8 us, by halves 19.5; 32 of 4096 47.5 and 45.4):
 //   S^T = K Q^T: lane (n, g) (n = l % 16, g = l / 16) holds for tile kt (of 4 in a block of 64 keys) the key
@@ -186,6 +186,11 @@ struct PoolArgs {
   float *scales;
   int32_t pages, page_log2, kv;
 };
+// Where a value head's code of dimension `dim` and row `row` of a page lies.
+template <int HD> __device__ __forceinline__ int value_at(int dim, int row, int lg) {
+  const int run = min(lg, 6);
+  return (row >> run) * (HD << run) + (dim << run) + (row & ((1 << run) - 1));
+}
 struct BatchArgs {
   const int32_t *tables, *starts, *lengths, *parts;
   int64_t tables_sr;
@@ -323,7 +328,7 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
     const int w0 = held && by != 1.0f ? 0 : held / 4, w1 = (held + count + 3) / 4, words = w1 - w0;
     for (int e = tid; e < words * HD; e += 256) {
       const int dim = e / words, w = w0 + e - dim * words;
-      uint32_t *word = (uint32_t *)(to + (dim << lg)) + w;
+      uint32_t *word = (uint32_t *)(to + value_at<HD>(dim, 4 * w, lg));
       const uint32_t now = *(const uint32_t *)(turned + dim * line + 4 * w);
       const int kept = min(max(held - 4 * w, 0), 4), end = min(held + count - 4 * w, 4);
       if (kept == 0 && end == 4) {
@@ -364,7 +369,7 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const PoolArgs c, uint1
   const int line = page + 4, wl = lg - 2;
   for (int e = tid; e < HD << wl; e += 256) {
     const int dim = e >> wl, w = e & ((1 << wl) - 1);
-    *(uint32_t *)(turned + dim * line + 4 * w) = gload((const uint32_t *)(from + (dim << lg)) + w);
+    *(uint32_t *)(turned + dim * line + 4 * w) = gload((const uint32_t *)(from + value_at<HD>(dim, 4 * w, lg)));
   }
   __syncthreads();
   for (int e = tid; e < page * HD / 8; e += 256) {
@@ -383,9 +388,9 @@ struct AttendArgs {
   BatchArgs b;
   const uint16_t *q;
   uint16_t *out;
-  float *scratch;
+  float *scratch, *split_scratch;
   int64_t q_sh, q_sr, o_sh, o_sr;
-  int32_t rep, window, items, few, groups;  // items: the most parts a plan makes; few: the most query pairs that parts
+  int32_t rep, window, splits, items, few, groups;  // items: the most parts a plan makes; few: the most query pairs that parts
                                              // are for, in `groups` that fold the keys apart
   FastDiv drep;
 };
@@ -415,6 +420,26 @@ __device__ __forceinline__ PageRun page_run(const AttendArgs &a, int r, int kvh,
   return w;
 }
 
+// Where key `key` lies: its page (0 where it is none, whose keys are hidden), its row there, the head's scales. ONE: blocks of 64
+// keys lie in one page (of 64 tokens or more), so `key` is the wave's and everything here is in scalar registers.
+struct PageAt {
+  int id, real, in;
+  float ks, vs;
+};
+template <bool ONE> __device__ __forceinline__ PageAt page_at(const PageRun &run, int p0, int key, int lg) {
+  PageAt p;
+  const int from = (key >> lg) - p0;
+  if constexpr (ONE) {
+    p.id = __builtin_amdgcn_readlane(run.id, from);
+    p.ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(run.ks), from));
+    p.vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(run.vs), from));
+  } else {
+    p.id = __shfl(run.id, from, 64), p.ks = __shfl(run.ks, from, 64), p.vs = __shfl(run.vs, from, 64);
+  }
+  p.real = p.id >= 0, p.id = max(p.id, 0), p.in = key & ((1 << lg) - 1);
+  return p;
+}
+
 __device__ __forceinline__ bf16x8 fp8_to_bf16(uint32_t lo, uint32_t hi, float s) {
   u32x4 w;
   w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s, false));
@@ -439,6 +464,11 @@ __device__ __forceinline__ float sum_groups(float x) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// l plus both bf16 values of w.
+__device__ __forceinline__ float sum_pair(uint32_t w, float l) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3F803F80u), l, false);
+}
+
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr float INF = __builtin_inff();
 
@@ -454,7 +484,8 @@ template <int HD> struct Running {
     for (int c = 0; c < HD / 16; c++) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   // s: the block's scores, hidden keys at -inf; p: the lane's 16 weights as bf16, the second operand of the two 32-key
-  // steps of O^T. They are rounded to nearest; l sums them unrounded, in 32 bits.
+  // steps of O^T. They are rounded to nearest (the operand's type); l sums them as
+  // rounded, in 32 bits.
   __device__ __forceinline__ void weigh(const f32x4 (&s)[4], bf16x8 (&p)[2]) {
     float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
@@ -475,8 +506,9 @@ template <int HD> struct Running {
       float e[4];
 #pragma unroll
       for (int i = 0; i < 4; i++) e[i] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], LOG2E, -ref));
-      l += (e[0] + e[1]) + (e[2] + e[3]);
-      w[kt / 2][kt % 2 * 2] = pack_rne(e[0], e[1]), w[kt / 2][kt % 2 * 2 + 1] = pack_rne(e[2], e[3]);
+      const uint32_t p0 = pack_rne(e[0], e[1]), p1 = pack_rne(e[2], e[3]);
+      l = sum_pair(p1, sum_pair(p0, l));
+      w[kt / 2][kt % 2 * 2] = p0, w[kt / 2][kt % 2 * 2 + 1] = p1;
     }
     p[0] = __builtin_bit_cast(bf16x8, w[0]), p[1] = __builtin_bit_cast(bf16x8, w[1]);
   }
@@ -504,26 +536,32 @@ __device__ __forceinline__ uint16_t *out_row(const AttendArgs &a, const Piece &p
 }
 
 // One block of 64 keys against QT tiles of pairs. key: the lane's first key (its 16 are in a row), seen: whether their page
-// is one; keys(kt, j) and values(c): the lane's 16 codes of each piece; between: run once the scores are made.
+// is one; keys(kt, j) and values(c): the lane's 16 codes of each piece; between: run once the scores are made. Matrix instructions on
+// one accumulator are kept 2 QT apart: one that follows its like at once waits for it.
 template <int HD, int QT, class Keys, class Values, class Between>
 __device__ __forceinline__ void fold_block(const Query<HD> (&q)[QT], Running<HD> (&st)[QT], int key, bool seen, float ks, float vs,
                                            Keys keys, Values values, Between between) {
-  constexpr int J = HD / 64;
+  constexpr int J = HD / 64, C = HD / 16;
   f32x4 s[QT][4];
 #pragma unroll
-  for (int kt = 0; kt < 4; kt++) {
-    bf16x8 kf[2 * J];
+  for (int kp = 0; kp < 4; kp += 2) {
+    bf16x8 kf[2][2 * J];
 #pragma unroll
-    for (int j = 0; j < J; j++) {
-      const u32x4 w = keys(kt, j);
-      kf[2 * j] = fp8_to_bf16(w[0], w[1], ks), kf[2 * j + 1] = fp8_to_bf16(w[2], w[3], ks);
-    }
+    for (int i = 0; i < 2; i++)
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-      s[t][kt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int j = 0; j < J; j++) {
+        const u32x4 w = keys(kp + i, j);
+        kf[i][2 * j] = fp8_to_bf16(w[0], w[1], ks), kf[i][2 * j + 1] = fp8_to_bf16(w[2], w[3], ks);
+      }
 #pragma unroll
-      for (int k = 0; k < 2 * J; k++) s[t][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[k], q[t].f[k], s[t][kt], 0, 0, 0);
-    }
+    for (int k = 0; k < 2 * J; k++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          if (k == 0) s[t][kp + i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          s[t][kp + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], q[t].f[k], s[t][kp + i], 0, 0, 0);
+        }
   }
   between();
   bf16x8 w[QT][2];
@@ -540,14 +578,20 @@ __device__ __forceinline__ void fold_block(const Query<HD> (&q)[QT], Running<HD>
     st[t].weigh(s[t], w[t]);
   }
 #pragma unroll
-  for (int c = 0; c < HD / 16; c++) {
-    const u32x4 x = values(c);
-    const bf16x8 v0 = fp8_to_bf16(x[0], x[1], vs), v1 = fp8_to_bf16(x[2], x[3], vs);
+  for (int cp = 0; cp < C; cp += 2) {
+    bf16x8 v[2][2];
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-      st[t].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, w[t][0], st[t].o[c], 0, 0, 0);
-      st[t].o[c] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, w[t][1], st[t].o[c], 0, 0, 0);
+    for (int i = 0; i < 2; i++) {
+      const u32x4 x = values(cp + i);
+      v[i][0] = fp8_to_bf16(x[0], x[1], vs), v[i][1] = fp8_to_bf16(x[2], x[3], vs);
     }
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+          st[t].o[cp + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i][h], w[t][h], st[t].o[cp + i], 0, 0, 0);
   }
 }
 // The finished rows of a tile: O / l in bf16, 4 dims a store. A row that sees no key is zeros; a NaN stays one.
@@ -567,12 +611,12 @@ template <int HD> __device__ __forceinline__ void store_rows(const AttendArgs &a
 // requested while the block before weighs its scores, its values while it multiplies, so 16 KB a wave (heads of 128) are always
 // in flight. Two waves a SIMD: held to their registers (the compiler's own choice put O into accumulation registers as
 // well, which left one of QT = 2: 16 requests of 5 rows of 4 heads over 2048 keys 20.1 us, 15.2 so).
-template <int HD, int QT, int NW>
+template <int HD, int QT, int NW, bool ONE>
 __global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs a) {
   constexpr int J = HD / 64, C = HD / 16;
   __shared__ __attribute__((aligned(16))) f32x4 joined[NW / 2][QT * C][64];
   __shared__ float joined_m[NW / 2][QT][64], joined_l[NW / 2][QT][64];
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = a.items * a.c.kv, group = blockIdx.x / units, unit = blockIdx.x - group * units;
   if (group >= a.groups) return clear_rows<HD>(a, blockIdx.x - a.groups * units, tid, 64 * NW);
@@ -603,29 +647,32 @@ __global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs 
     const auto turn = [&](int b) {  // the 64 pages that block b's keys lie in, if they are not there yet
       if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, run = page_run(a, p.r, kvh, p0, lane);
     };
+    const uint8_t *base = a.c.values + kvh * head;
+    const int run6 = min(lg, 6);
+    const uint32_t krow = ((ONE ? 16 * (n >> 2) : 0) + (n & 3)) * 64 + 16 * g, vrow = (n << run6) + (ONE ? 16 * g : 0);
     const auto fetch_keys = [&](int b, float &s) {
-      const int key = b * KB + 16 * (n >> 2), from = (key >> lg) - p0;
-      const int id = max(__shfl(run.id, from, 64), 0);
-      s = __shfl(run.ks, from, 64);
-      const uint8_t *k = a.c.values + ((int64_t)id * (2 * a.c.kv) + kvh) * head + ((key & mask) + (n & 3)) * 64 + 16 * g;
+      const PageAt at = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * (n >> 2)), lg);
+      s = at.ks;
+      const uint8_t *k = base + (int64_t)at.id * (2 * a.c.kv) * head + at.in * 64;
 #pragma unroll
-      for (int kt = 0; kt < 4; kt++)
+      for (int j = 0; j < J; j++) {
+        const uint8_t *kj = k + (j << (lg + 6));
 #pragma unroll
-        for (int j = 0; j < J; j++) kw[kt][j] = __builtin_nontemporal_load((const u32x4 *)(k + 4 * kt * 64 + (j << (lg + 6))));
+        for (int kt = 0; kt < 4; kt++) kw[kt][j] = __builtin_nontemporal_load((const u32x4 *)(kj + (krow + 4 * kt * 64)));
+      }
     };
     const auto fetch_values = [&](int b, float &s, int &valid) {
-      const int key = b * KB + 16 * g, from = (key >> lg) - p0;
-      valid = __shfl(run.id, from, 64);
-      s = __shfl(run.vs, from, 64);
-      const uint8_t *v = a.c.values + ((int64_t)max(valid, 0) * (2 * a.c.kv) + a.c.kv + kvh) * head + (n << lg) + (key & mask);
+      const PageAt at = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
+      valid = at.real, s = at.vs;
+      const uint8_t *v = base + ((int64_t)at.id * (2 * a.c.kv) + a.c.kv) * head + value_at<HD>(0, at.in, lg);
 #pragma unroll
-      for (int c = 0; c < C; c++) vw[c] = __builtin_nontemporal_load((const u32x4 *)(v + (c << (lg + 4))));
+      for (int c = 0; c < C; c++) vw[c] = __builtin_nontemporal_load((const u32x4 *)(v + (c << (run6 + 4)) + vrow));
     };
     fetch_keys(b0, ks);
     fetch_values(b0, vs, id_v);
     for (int b = b0; b < b1; b += NW) {
       const bool more = b + NW < b1;
-      fold_block<HD, QT>(q, st, b * KB + 16 * g, id_v >= 0, ks, vs, [&](int kt, int j) { return kw[kt][j]; },
+      fold_block<HD, QT>(q, st, b * KB + 16 * g, id_v, ks, vs, [&](int kt, int j) { return kw[kt][j]; },
                          [&](int c) { return vw[c]; }, [&] {
                            if (more) turn(b + NW), fetch_keys(b + NW, ks_next);
                          });
@@ -678,20 +725,10 @@ __global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs 
   }
 }
 
-// Joins a request's parts: a wave (request, key head, pair), 4 a block; M = max m, L = sum 2^(m - M) l, out = sum 2^(m - M) O / L.
-// 16 parts' sums are requested at once, so that the usual plan is one trip to memory.
-template <int HD>
-__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
+// A pair's output from `parts` parts' sums, `step` floats apart, by a wave: M = max m, L = sum 2^(m - M) l, out = sum
+// 2^(m - M) O / L. 16 parts' are requested at once, so that the usual plan is one trip to memory.
+template <int HD> __device__ __forceinline__ void join_parts(const float *from, int64_t step, int parts, uint16_t *out, int lane) {
   constexpr int V = HD / 64, TURN = 16;
-  const int lane = threadIdx.x & 63;
-  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = unit / a.few;
-  const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
-  if (r >= a.b.requests) return;
-  const int row0 = gload(a.b.starts + r), n = gload(a.b.starts + r + 1) - row0, first = gload(a.b.parts + r);
-  const int parts = gload(a.b.parts + r + 1) - first;
-  if (parts <= 1 || first + parts > a.items || pair >= n * a.rep || n * a.rep > a.few) return;
-  const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
-  const float *from = a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4);
   float M = -INF, L = 0.0f, O[V];
 #pragma unroll
   for (int i = 0; i < V; i++) O[i] = 0.0f;
@@ -726,52 +763,91 @@ __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
     M = top;
   }
   const float inv = L > 0.0f ? 1.0f / L : L;
-  const int i = (int)fdiv((uint32_t)pair, a.drep), h = kvh * a.rep + pair - i * a.rep;
-  uint16_t *out = a.out + h * a.o_sh + (row0 + i) * a.o_sr + V * lane;
-  if constexpr (V == 2) *(uint32_t *)out = pack_rne(O[0] * inv, O[1] * inv);
-  else *out = (uint16_t)pack_rne(O[0] * inv, 0.0f);
+  if constexpr (V == 2) *(uint32_t *)(out + 2 * lane) = pack_rne(O[0] * inv, O[1] * inv);
+  else out[lane] = (uint16_t)pack_rne(O[0] * inv, 0.0f);
 }
 
-// Many query pairs a request (a prompt's rows): a block of 4 waves takes 128 pairs of one key head, 32 a wave, so every
-// fragment that a wave converts feeds two matrix instructions. Blocks of 64 keys and values pass through LDS as codes, one
-// barrier a block, the next block's codes held in registers meanwhile. 16-byte units are placed so that the 16 lanes of a
-// read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2) (heads of 64: u ^ (r / 16)), values'
-// unit u of dim d at u ^ (d / 4) % 4.
+// Joins a request's parts: a wave (request, key head, pair), 4 a block.
 template <int HD>
-__global__ void __launch_bounds__(256, 2) pages_many_kernel(const AttendArgs a, int tiles) {
+__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = unit / a.few;
+  const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
+  if (r >= a.b.requests) return;
+  Piece p{r, 0, gload(a.b.starts + r), 0, 0};
+  p.n = gload(a.b.starts + r + 1) - p.row0;
+  const int first = gload(a.b.parts + r), parts = gload(a.b.parts + r + 1) - first;
+  if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
+  const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
+  join_parts<HD>(a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4), step, parts, out_row(a, p, kvh, pair), lane);
+}
+
+constexpr int TILE_LOG2 = 7, TILE = 1 << TILE_LOG2;  // pairs of a block
+// The tile that `slot` is: 128 pairs of request p->r from pair 128 p->k on. Request r owns tiles starts[r] * rep / 128 + r and on:
+// at least as many as its pairs fill. False where there are none, or few enough for pages_few_kernel.
+__device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lane, Piece *p) {
+  return find_piece(a.b, slot, lane, [&](int i, int s) { return (int)((uint32_t)s * (uint32_t)a.rep >> TILE_LOG2) + i; }, p) &&
+         p->n * a.rep > a.few && TILE * p->k < p->n * a.rep;
+}
+
+// Many query pairs a request (a prompt's rows): a block takes 128 pairs of one key head against a `splits`th of the blocks of
+// keys that they see. Its 8 waves are two halves of 4 that take every other block of keys, each wave 32 pairs, so
+// every fragment that a wave converts feeds two matrix instructions; the halves join through LDS at the end. Blocks of 64 keys
+// and values pass through LDS as codes, one barrier a step, the next step's codes held in registers meanwhile. 16-byte units are
+// placed so that the 16 lanes of a read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2)
+// (heads of 64: u ^ (r / 16)), values' unit u of dim d at u ^ (d / 4) % 4.
+template <int HD, bool ONE>
+__global__ void __launch_bounds__(512, 2) pages_many_kernel(const AttendArgs a, int tiles) {
   constexpr int C = HD / 16, UK = HD / 16, NU = HD * KB / 16 / 256;  // units of a key's row; units a thread
-  __shared__ __attribute__((aligned(16))) uint8_t kl[2][KB * HD], vl[2][KB * HD];
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int slot = tiles - 1 - blockIdx.x / a.c.kv, kvh = blockIdx.x % a.c.kv;  // the longest rows first
+  __shared__ __attribute__((aligned(16))) uint8_t kl[2][2][KB * HD], vl[2][2][KB * HD];  // [half][stage]
+  const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = blockIdx.x % a.c.kv, unit = blockIdx.x / a.c.kv, split = unit % a.splits;
+  const int slot = tiles - 1 - unit / a.splits;  // the longest rows first
   Piece p;
-  // request r owns tiles starts[r] * rep / 128 + r and on: at least as many as its pairs fill
-  if (!find_piece(a.b, slot, lane, [&](int i, int s) { return (int)((uint32_t)s * (uint32_t)a.rep >> 7) + i; }, &p)) return;
-  const int pairs = p.n * a.rep, pair0 = 128 * p.k;
-  if (pairs <= a.few || pair0 >= pairs) return;
+  if (!find_tile(a, slot, lane, &p)) return;
+  const int pairs = p.n * a.rep, pair0 = TILE * p.k, mine0 = pair0 + 32 * wave;
   Query<HD> q[2];
   Running<HD> st[2];
 #pragma unroll
-  for (int t = 0; t < 2; t++) q[t].load(a, p, kvh, pair0 + 32 * wave + 16 * t + n, g), st[t].clear();
+  for (int t = 0; t < 2; t++) q[t].load(a, p, kvh, mine0 + 16 * t + n, g), st[t].clear();
   const int cached = p.len - p.n, room = min(p.len, a.b.width << lg);
   const auto place = [&](int pair) { return cached + (int)fdiv((uint32_t)min(pair, pairs - 1), a.drep); };
   const auto low = [&](int at) { return a.window > 0 ? max(at - a.window + 1, 0) : 0; };
-  const int b0 = low(place(pair0)) / KB, b1 = min(place(pair0 + 127), room - 1) / KB + 1;
+  int b0 = low(place(pair0)) / KB, b1 = min(place(pair0 + TILE - 1), room - 1) / KB + 1;
+  if (a.splits > 1) {
+    const int each = (b1 - b0 + a.splits - 1) / a.splits;
+    b0 += split * each, b1 = min(b0 + each, b1);
+  }
   // the wave's own keys: blocks outside them it only helps to bring in
-  const int wlo = low(place(pair0 + 32 * wave)), whi = pair0 + 32 * wave < pairs ? place(pair0 + 32 * wave + 31) : -1;
+  const int wlo = low(place(mine0)), whi = mine0 < pairs ? place(mine0 + 32 - 1) : -1;
   const int64_t head = (int64_t)HD << lg;
   int p0 = b0 * KB >> lg;
   PageRun run = page_run(a, p.r, kvh, p0, lane);
   u32x4 kr[NU], vr[NU];
+  const uint8_t *base = a.c.values + kvh * head;
+  uint32_t kunit[NU], vunit[NU];  // the thread's units in a block of keys, and where each starts in it
+#pragma unroll
+  for (int i = 0; i < NU; i++) {
+    const int u = tid + 256 * i;
+    kunit[i] = (u % UK / 4 << (lg + 6)) + (ONE ? u / UK * 64 : u / UK % 16 * 64) + u % 4 * 16;
+    vunit[i] = (u / 4 << min(lg, 6)) + (ONE ? 16 * (u & 3) : 0);
+  }
   const auto fetch = [&](int b) {
     if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, run = page_run(a, p.r, kvh, p0, lane);
+    if constexpr (ONE) {
+      const PageAt at = page_at<true>(run, p0, b * KB, lg);
+      const uint8_t *k = base + (int64_t)at.id * (2 * a.c.kv) * head + at.in * 64, *v = base + ((int64_t)at.id * (2 * a.c.kv) + a.c.kv) * head + value_at<HD>(0, at.in, lg);
 #pragma unroll
-    for (int i = 0; i < NU; i++) {
-      const int u = tid + 256 * i;
-      const int key = b * KB + u / UK, kid = max(__shfl(run.id, (key >> lg) - p0, 64), 0);
-      kr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)kid * (2 * a.c.kv) + kvh) * head + (u % UK / 4 << (lg + 6)) + (key & mask) * 64 + u % 4 * 16));
-      const int vkey = b * KB + 16 * (u & 3), vid = max(__shfl(run.id, (vkey >> lg) - p0, 64), 0);
-      vr[i] = gload((const u32x4 *)(a.c.values + ((int64_t)vid * (2 * a.c.kv) + a.c.kv + kvh) * head + (u / 4 << lg) + (vkey & mask)));
+      for (int i = 0; i < NU; i++) kr[i] = gload((const u32x4 *)(k + kunit[i])), vr[i] = gload((const u32x4 *)(v + vunit[i]));
+    } else {
+#pragma unroll
+      for (int i = 0; i < NU; i++) {
+        const int u = tid + 256 * i;
+        const PageAt k = page_at<false>(run, p0, b * KB + (u / UK & ~15), lg), v = page_at<false>(run, p0, b * KB + 16 * (u & 3), lg);
+        kr[i] = gload((const u32x4 *)(base + (int64_t)k.id * (2 * a.c.kv) * head + k.in * 64 + kunit[i]));
+        vr[i] = gload((const u32x4 *)(base + ((int64_t)v.id * (2 * a.c.kv) + a.c.kv) * head + v.in + vunit[i]));
+      }
     }
   };
   const auto turned = [](int row) { return HD == 128 ? row >> 4 << 1 | (row >> 1 & 1) : row >> 4; };
@@ -779,36 +855,80 @@ __global__ void __launch_bounds__(256, 2) pages_many_kernel(const AttendArgs a, 
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       const int u = tid + 256 * i, row = u / UK, dim = u / 4;
-      *(u32x4 *)(kl[to] + row * HD + 16 * (u % UK ^ turned(row))) = kr[i];
-      *(u32x4 *)(vl[to] + dim * KB + 16 * ((u & 3) ^ (dim >> 2 & 3))) = vr[i];
+      *(u32x4 *)(kl[half][to] + row * HD + 16 * (u % UK ^ turned(row))) = kr[i];
+      *(u32x4 *)(vl[half][to] + dim * KB + 16 * ((u & 3) ^ (dim >> 2 & 3))) = vr[i];
     }
   };
-  if (b0 < b1) fetch(b0), store(0);
+  if (b0 + half < b1) fetch(b0 + half), store(0);
   __syncthreads();
-  for (int b = b0; b < b1; b++) {
-    const int now = (b - b0) & 1;
-    const int fk = ((b * KB + 16 * (n >> 2)) >> lg) - p0, fv = ((b * KB + 16 * g) >> lg) - p0;
-    const float ks = __shfl(run.ks, fk, 64), vs = __shfl(run.vs, fv, 64);
-    const bool seen = __shfl(run.id, fv, 64) >= 0;
-    if (b + 1 < b1) fetch(b + 1);
-    if (b * KB <= whi && b * KB + KB > wlo) {
-      const uint8_t *k = kl[now], *v = vl[now];
-      fold_block<HD, 2>(q, st, b * KB + 16 * g, seen, ks, vs,
+  for (int b = b0 + half, now = 0; b - half < b1; b += 2, now ^= 1) {
+    const PageAt ka = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * (n >> 2)), lg), va = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
+    if (b + 2 < b1) fetch(b + 2);
+    if (b < b1 && b * KB <= whi && b * KB + KB > wlo) {
+      const uint8_t *k = kl[half][now], *v = vl[half][now];
+      fold_block<HD, 2>(q, st, b * KB + 16 * g, va.real, ka.ks, va.vs,
                         [&](int kt, int j) {
                           const int row = 16 * (n >> 2) + 4 * kt + (n & 3);
                           return *(const u32x4 *)(k + row * HD + 16 * ((4 * j + g) ^ turned(row)));
                         },
                         [&](int c) { return *(const u32x4 *)(v + (16 * c + n) * KB + 16 * (g ^ (n >> 2))); }, [] {});
     }
-    if (b + 1 < b1) store(now ^ 1);
+    if (b + 2 < b1) store(now ^ 1);
     __syncthreads();
   }
+  f32x4 *joined = (f32x4 *)kl;  // a tile of pairs at a time: every wave of the second half's O^T, maxima and sums
+  float *sums = (float *)vl;
 #pragma unroll
   for (int t = 0; t < 2; t++) {
-    const int pair = pair0 + 32 * wave + 16 * t + n;
-    const float l = sum_groups(st[t].l);
-    if (pair < pairs) store_rows<HD>(a, p, kvh, pair, g, st[t], l);
+    if (half) {
+#pragma unroll
+      for (int c = 0; c < C; c++) joined[(wave * C + c) * 64 + lane] = st[t].o[c];
+      sums[(2 * wave) * 64 + lane] = st[t].m, sums[(2 * wave + 1) * 64 + lane] = st[t].l;
+    }
+    __syncthreads();
+    if (!half) {
+      const float m = sums[(2 * wave) * 64 + lane], top = fmaxf(st[t].m, m);
+      const float mine = st[t].m == -INF ? 0.0f : __builtin_amdgcn_exp2f(st[t].m - top);
+      const float other = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+      st[t].m = top, st[t].l = st[t].l * mine + sums[(2 * wave + 1) * 64 + lane] * other;
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        const f32x4 o = joined[(wave * C + c) * 64 + lane];
+#pragma unroll
+        for (int i = 0; i < 4; i++) st[t].o[c][i] = st[t].o[c][i] * mine + o[i] * other;
+      }
+    }
+    __syncthreads();
   }
+  if (half) return;
+#pragma unroll
+  for (int t = 0; t < 2; t++) {
+    const int pair = mine0 + 16 * t + n;
+    const float l = sum_groups(st[t].l);
+    if (pair >= pairs) continue;
+    if (a.splits == 1) {
+      store_rows<HD>(a, p, kvh, pair, g, st[t], l);
+    } else {
+      float *to = a.split_scratch + ((((int64_t)slot * a.c.kv + kvh) * a.splits + split) * TILE + pair - pair0) * (HD + 4);
+#pragma unroll
+      for (int c = 0; c < C; c++) *(f32x4 *)(to + 16 * c + 4 * g) = st[t].o[c];
+      if (g == 0) to[HD] = st[t].m, to[HD + 1] = l;
+    }
+  }
+}
+
+// Joins the splits of the tiles' keys: a wave (tile, key head, pair), 4 a block.
+template <int HD>
+__global__ void __launch_bounds__(256) pages_splits_kernel(const AttendArgs a, int tiles) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int at = unit & (TILE - 1), kvh = (unit >> TILE_LOG2) % a.c.kv, slot = (unit >> TILE_LOG2) / a.c.kv;
+  Piece p;
+  if (!find_tile(a, slot, lane, &p)) return;
+  const int pair = TILE * p.k + at;
+  if (pair >= p.n * a.rep) return;
+  join_parts<HD>(a.split_scratch + (((int64_t)slot * a.c.kv + kvh) * a.splits * TILE + at) * (HD + 4), TILE * (HD + 4), a.splits,
+                 out_row(a, p, kvh, pair), lane);
 }
 
 // ---- entry points ----------------------------------------------------------------------------------------------------
@@ -849,9 +969,10 @@ static int check_batch(const bt_batch *b, BatchArgs *out) {
 // whether requests may have more (their rows then share blocks of 128 pairs).
 struct AttendPlan {
   int few, tiles, groups, items;
-  int waves;  // of a part's block
+  int waves;             // of a part's block
+  int many_tiles, splits;  // tiles of 128 pairs, and the pieces that each one's keys are cut into
   bool many, join;
-  uint64_t scratch;
+  uint64_t scratch, split_scratch;
 };
 static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int window, AttendPlan *p) {
   if (int s = check_pool(c, nullptr)) return s;
@@ -870,13 +991,21 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   p->waves = p->tiles == 1 && !p->join ? 8 : 4;
   const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
+  // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least
+  p->many_tiles = (int)((int64_t)b->rows * rep >> TILE_LOG2) + b->requests, p->splits = 1, p->split_scratch = 0;
+  if (p->many) {
+    const int64_t blocks = (int64_t)p->many_tiles * c->kv;
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / (8 * KB), 16}));
+    if (blocks * p->splits > 0x3FFFFF) return fail(BT_EINVAL, "paged attention of %d rows of %d heads is too large", b->rows, heads);
+    if (p->splits > 1) p->split_scratch = (uint64_t)blocks * p->splits * TILE * (c->head_dim + 4) * 4;
+  }
   if ((int64_t)p->items * c->kv * p->groups > 0x3FFFFFFF || (int64_t)b->requests * heads * p->few > 0x7FFFFFFF) return fail(BT_EINVAL, "paged attention in %d parts of %d key heads", p->items, c->kv);
   return BT_OK;
 }
 
-template <int HD, int QT, int NW> static int launch_few(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+template <int HD, int QT, int NW, bool ONE> static int launch_few(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const int clear = (a.b.rows + 15) / 16;
-  pages_few_kernel<HD, QT, NW><<<(unsigned)(p.items * a.c.kv * p.groups + clear), 64 * NW, 0, s>>>(a);
+  pages_few_kernel<HD, QT, NW, ONE><<<(unsigned)(p.items * a.c.kv * p.groups + clear), 64 * NW, 0, s>>>(a);
   BT_LAUNCHED("paged attention");
   if (p.join) {
     pages_join_kernel<HD><<<(unsigned)ceil_div((int64_t)a.b.requests * a.c.kv * p.few, 4), 256, 0, s>>>(a);
@@ -884,12 +1013,17 @@ template <int HD, int QT, int NW> static int launch_few(const AttendArgs &a, con
   }
   return BT_OK;
 }
-template <int HD> static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  const int status = p.tiles == 2 ? launch_few<HD, 2, 4>(a, p, s) : p.waves == 8 ? launch_few<HD, 1, 8>(a, p, s) : launch_few<HD, 1, 4>(a, p, s);
+template <int HD, bool ONE> static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  const int status = p.tiles == 2    ? launch_few<HD, 2, 4, ONE>(a, p, s)
+                     : p.waves == 8 ? launch_few<HD, 1, 8, ONE>(a, p, s)
+                                    : launch_few<HD, 1, 4, ONE>(a, p, s);
   if (status || !p.many) return status;
-  const int tiles = (int)((int64_t)a.b.rows * a.rep >> 7) + a.b.requests;
-  pages_many_kernel<HD><<<(unsigned)(tiles * a.c.kv), 256, 0, s>>>(a, tiles);
+  pages_many_kernel<HD, ONE><<<(unsigned)(p.many_tiles * a.c.kv * p.splits), 512, 0, s>>>(a, p.many_tiles);
   BT_LAUNCHED("paged attention");
+  if (p.splits > 1) {
+    pages_splits_kernel<HD><<<(unsigned)(p.many_tiles * a.c.kv * (TILE / 4)), 256, 0, s>>>(a, p.many_tiles);
+    BT_LAUNCHED("paged attention's join");
+  }
   return BT_OK;
 }
 
@@ -963,7 +1097,7 @@ int bt_pages_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t
   if (!bytes) return fail(BT_EINVAL, "no result pointer");
   AttendPlan p;
   if (int s = plan_attend(pool, batch, heads, window, &p)) return s;
-  *bytes = p.scratch;
+  *bytes = p.scratch + p.split_scratch;
   return BT_OK;
 }
 
@@ -977,13 +1111,17 @@ int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch,
   check_pool(pool, &a.c), check_batch(batch, &a.b);
   if (!q || !out || q % 16 || q_sh % 8 || q_sr % 8 || out % 16 || o_sh % 8 || o_sr % 8)
     return fail(BT_EINVAL, "paged attention needs q and out rows on 16-byte boundaries");
-  if (p.scratch && (!scratch || scratch % 16 || scratch_bytes < p.scratch))
-    return fail(BT_EINVAL, "paged attention needs %llu bytes of 16-byte aligned scratch", (unsigned long long)p.scratch);
+  const uint64_t need = p.scratch + p.split_scratch;
+  if (need && (!scratch || scratch % 16 || scratch_bytes < need))
+    return fail(BT_EINVAL, "paged attention needs %llu bytes of 16-byte aligned scratch", (unsigned long long)need);
   a.q = (const uint16_t *)(uintptr_t)q, a.out = (uint16_t *)(uintptr_t)out, a.scratch = (float *)(uintptr_t)scratch;
+  a.split_scratch = (float *)(uintptr_t)(scratch + p.scratch), a.splits = p.splits;
   a.q_sh = q_sh, a.q_sr = q_sr, a.o_sh = o_sh, a.o_sr = o_sr;
   a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few, a.groups = p.groups;
   a.drep = make_fastdiv((uint32_t)a.rep);
-  return pool->head_dim == 64 ? launch_attend<64>(a, p, r->stream) : launch_attend<128>(a, p, r->stream);
+  const bool one = pool->page >= KB;
+  if (pool->head_dim == 64) return one ? launch_attend<64, true>(a, p, r->stream) : launch_attend<64, false>(a, p, r->stream);
+  return one ? launch_attend<128, true>(a, p, r->stream) : launch_attend<128, false>(a, p, r->stream);
 }
 
 }  // extern "C"

@@ -348,7 +348,7 @@ int bt_put_bfp(bt_runtime *rt, int fmt, uint64_t exps, uint64_t vals, int64_t ba
  * [0, pages) holds no page: what would be put there is dropped, and attention doesn't see it.
  *
  * values: [pages][2 kv][page * head_dim] bytes, key heads then value heads; a key head's are [head_dim / 64][page][64], a
- * value head's [head_dim][page]. A byte is an 8-bit float (sign, 4 exponent bits biased by 7, 3 mantissa bits; at most 448), and
+ * value head's [page / 64][head_dim][64] (pages of 16 or 32: [head_dim][page]). A byte is an 8-bit float (sign, 4 exponent bits biased by 7, 3 mantissa bits; at most 448), and
  * stands for that times scales[id, head], fp32 [pages][2 kv], a power of two from 2^-100 to 2^119: exact in bf16. */
 typedef struct {
   uint64_t values, scales;
