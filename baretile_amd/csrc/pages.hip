@@ -82,25 +82,24 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int j, int start, in
   a.slots[j] = real && id_or_free >= 0 ? (id_or_free << a.page_log2) + (place & mask) : -1;
 }
 
-// One block. Requests are scanned 1024 at a time: first their rows, cut to `most` each and to the rows there are, and the
+// One block, of 64, 256 or 1024 threads by the larger of its requests and the rows it writes. Requests are scanned a thread each: first their rows, cut to `most` each and to the rows there are, and the
 // pages they take; then, with the keys' blocks counted, the parts that attention cuts each request's keys into: as many
 // parts over all requests as `target`, of whole blocks of 64 keys and `least` of them, so that uneven lengths make parts of
 // even length.
 // Latency bounds it: three scans of about a microsecond and two trips to memory.
-constexpr int PLAN_NT = 1024;
 constexpr int PLAN_ROWS = 2048;  // rows that the plan's one block writes itself; more go to plan_rows_kernel's many
-__global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
+template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs a) {
   __shared__ int starts[MOST_REQUESTS + 1], first[MOST_REQUESTS], from[MOST_REQUESTS + 1], cache[MOST_REQUESTS];
-  __shared__ int sums[PLAN_NT / 64];
+  __shared__ int sums[NT / 64];
   const int lg = a.page_log2, room = (int)min((int64_t)a.width << lg, (int64_t)0x40000000);
   const int taken = a.taken ? gload(a.taken) : 0;
   int rows = 0, takes = 0, blocks = 0;
-  for (int base = 0; base < a.requests; base += PLAN_NT) {
+  for (int base = 0; base < a.requests; base += NT) {
     const int r = base + threadIdx.x;
     int c = 0, n = 0, total;
     if (r < a.requests) c = min(max(gload(a.cached + r), 0), room), n = min(max(gload(a.fresh + r), 0), a.most);
-    // at most 2^20 rows and 2^20 a request: a sum over 1024 requests keeps to 31 bits
-    const int s = rows + block_exclusive<PLAN_NT>(n, sums, &total);
+    // 2^20 rows at most, and so many a request: a sum over 1024 requests keeps to 31 bits
+    const int s = rows + block_exclusive<NT>(n, sums, &total);
     const int s0 = min(s, a.rows), s1 = min(s + n, a.rows);
     rows = min(rows + total, a.rows);
     n = s1 - s0;
@@ -114,10 +113,10 @@ __global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
       starts[r] = s0, first[r] = k, cache[r] = c;
       a.starts[r] = s0, a.lengths[r] = c + n;
     }
-    const int off = block_exclusive<PLAN_NT>(need, sums, &total);
+    const int off = block_exclusive<NT>(need, sums, &total);
     if (r < a.requests) from[r] = takes + off;
     takes += total;
-    block_exclusive<PLAN_NT>(n > 0 ? (min(c + n, room) + KB - 1) / KB : 0, sums, &total);
+    block_exclusive<NT>(n > 0 ? (min(c + n, room) + KB - 1) / KB : 0, sums, &total);
     blocks += total;
   }
   const int last = rows;
@@ -129,7 +128,7 @@ __global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
   const int per = max(a.least, ((blocks + a.target - 1) / a.target + 3) & ~3);
   int made = 0;
   __syncthreads();
-  for (int base = 0; base < a.requests; base += PLAN_NT) {
+  for (int base = 0; base < a.requests; base += NT) {
     const int r = base + threadIdx.x;
     int parts = 0, total;
     if (r < a.requests) {
@@ -137,7 +136,7 @@ __global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
       const int mine = max(per, (nb + MOST_PARTS - 1) / MOST_PARTS);
       parts = (nb + mine - 1) / mine;
     }
-    const int off = block_exclusive<PLAN_NT>(parts, sums, &total);
+    const int off = block_exclusive<NT>(parts, sums, &total);
     if (r < a.requests) a.parts[r] = made + off;
     made += total;
   }
@@ -147,12 +146,12 @@ __global__ void __launch_bounds__(PLAN_NT) plan_kernel(const PlanArgs a) {
     const int id = gload(a.free_pages + e);
     return (uint32_t)id < (uint32_t)a.pages ? id : -1;
   };
-  for (int e = threadIdx.x; e < takes; e += PLAN_NT) {
+  for (int e = threadIdx.x; e < takes; e += NT) {
     const int r = owner_of(from, a.requests, e);
     a.tables[r * a.tables_sr + first[r] + e - from[r]] = page_at(taken + e);
   }
   if (a.rows > PLAN_ROWS) return;
-  for (int j = threadIdx.x; j < a.rows; j += PLAN_NT) {
+  for (int j = threadIdx.x; j < a.rows; j += NT) {
     const bool real = j < last;
     const int r = real ? owner_of(starts, a.requests, j) : 0;
     const int on = (cache[r] + j - starts[r]) >> lg;
@@ -244,39 +243,39 @@ __device__ __forceinline__ float scale_of(float amax) {
   return __uint_as_float((uint32_t)min(max(e, 27), 246) << 23);
 }
 
-// A block: the rows that one request puts into one page of one head. Its rows are loaded once (up to 16 loads of 16 bytes
-// a thread, all at once), their largest finite size gives the scale, and a page that already holds rows and whose scale
+// A block: the rows that one request puts into one page of one head, PAGE of them at most. They are loaded once (up to 16 loads of
+// 16 bytes a thread, all at once), their largest finite size gives the scale, and a page that already holds rows and whose scale
 // grows has them rounded again. Values turn by dimension in LDS, so they are stored as whole words.
-template <int HD>
-__global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
+template <int HD, int NT, int PAGE>
+__global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
                                                         int64_t x_sr) {
-  constexpr int U = HD / 8, MOST = 256 * U / 256;  // 16-byte units of a row, loads a thread for the largest page
-  __shared__ float tops[4];
-  __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (256 + 4)];
+  constexpr int U = HD / 8, MOST = PAGE * U / NT;  // 16-byte units of a row, loads a thread for the most rows
+  __shared__ float tops[NT / 64];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (PAGE + 4)];  // by dimension, from the new rows' first word on
   const int tid = threadIdx.x, lane = tid & 63, lg = c.page_log2, page = 1 << lg, heads = 2 * c.kv;
   const int at = blockIdx.x / heads, h = blockIdx.x - at * heads;
   Piece p;
   // request r owns pieces starts[r] / page + 2 r and on: at least as many as the pages its rows touch
   if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> lg) + 2 * i; }, &p)) return;
   const int cached = p.len - p.n, on = (cached >> lg) + p.k;
-  const int from = max(cached, on << lg), count = min(p.len, (on + 1) << lg) - from;
+  const int from = max(cached, on << lg), count = min(min(p.len, (on + 1) << lg) - from, PAGE);
   if (count <= 0 || on >= b.width) return;
-  const int id = gload(b.tables + p.r * b.tables_sr + on);
-  if ((uint32_t)id >= (uint32_t)c.pages) return;
+  const int id = gload(b.tables + p.r * b.tables_sr + on);  // the rows are requested before it is looked at
   const int held = from & (page - 1), units = count * U;
   const uint16_t *src = x + h * x_sb + (int64_t)(p.row0 + from - cached) * x_sr;
-  float *scale_at = c.scales + (int64_t)id * heads + h;
-  const float old = held ? gload(scale_at) : 0.0f;
   u32x4 v[MOST];
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < MOST; i++) {
-    const int e = tid + 256 * i;
-    if (256 * i < units) v[i] = e < units ? gload((const u32x4 *)(src + e / U * x_sr + e % U * 8)) : u32x4{0, 0, 0, 0};
+    const int e = tid + NT * i;
+    if (NT * i < units) v[i] = e < units ? gload((const u32x4 *)(src + e / U * x_sr + e % U * 8)) : u32x4{0, 0, 0, 0};
   }
+  if ((uint32_t)id >= (uint32_t)c.pages) return;
+  float *scale_at = c.scales + (int64_t)id * heads + h;
+  const float old = held ? gload(scale_at) : 0.0f;
 #pragma unroll
   for (int i = 0; i < MOST; i++)
-    if (256 * i < units)
+    if (NT * i < units)
 #pragma unroll
       for (int k = 0; k < 4; k++) {
         const uint32_t lo = v[i][k] << 16 & 0x7FFFFFFFu, hi = v[i][k] & 0x7FFF0000u;
@@ -287,13 +286,14 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
   for (int d = 1; d < 64; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
   if (lane == 0) tops[tid >> 6] = top;
   __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+#pragma unroll
+  for (int i = 0; i < NT / 64; i++) top = fmaxf(top, tops[i]);
   const float s = fmaxf(scale_of(top), old), inv = __uint_as_float((254u << 23) - __float_as_uint(s));  // 1 / s, exact
   const float by = old * inv;
   uint8_t *to = c.values + (((int64_t)id * heads + h) << lg) * HD;
   if (h < c.kv) {  // keys: 64 dims of a row are 4 units of 16
     if (held && by != 1.0f)
-      for (int e = tid; e < held * HD / 16; e += 256) {
+      for (int e = tid; e < held * HD / 16; e += NT) {
         u32x4 *at = (u32x4 *)(to + (e / 4 / held << (lg + 6)) + e / 4 % held * 64 + e % 4 * 16), w = *at;
 #pragma unroll
         for (int k = 0; k < 4; k++) w[k] = rescaled4(w[k], by);
@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
       }
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-      const int e = tid + 256 * i;
-      if (256 * i < units && e < units) {
+      const int e = tid + NT * i;
+      if (NT * i < units && e < units) {
         uint2 w;
         const auto val = [&](int k) { return __uint_as_float(k & 1 ? v[i][k / 2] & 0xFFFF0000u : v[i][k / 2] << 16) * inv; };
         w.x = codes_of4(val(0), val(1), val(2), val(3)), w.y = codes_of4(val(4), val(5), val(6), val(7));
@@ -310,12 +310,13 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
       }
     }
   } else {  // values: each dimension's codes lie along the page
-    const int line = page + 4;
+    constexpr int line = PAGE + 4;
+    const int base = held & ~3;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-      const int e = tid + 256 * i;
-      if (256 * i < units && e < units) {
-        const int row = held + e / U, dim = e % U * 8;
+      const int e = tid + NT * i;
+      if (NT * i < units && e < units) {
+        const int row = held - base + e / U, dim = e % U * 8;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
           const uint32_t w = codes_of(__uint_as_float(v[i][k] << 16) * inv, __uint_as_float(v[i][k] & 0xFFFF0000u) * inv);
@@ -326,10 +327,10 @@ __global__ void __launch_bounds__(256) put_pages_kernel(const PoolArgs c, const 
     __syncthreads();
     // whole words of 4 rows: from the page's start where its rows are rounded again, else from the word with the first new row
     const int w0 = held && by != 1.0f ? 0 : held / 4, w1 = (held + count + 3) / 4, words = w1 - w0;
-    for (int e = tid; e < words * HD; e += 256) {
+    for (int e = tid; e < words * HD; e += NT) {
       const int dim = e / words, w = w0 + e - dim * words;
       uint32_t *word = (uint32_t *)(to + value_at<HD>(dim, 4 * w, lg));
-      const uint32_t now = *(const uint32_t *)(turned + dim * line + 4 * w);
+      const uint32_t now = 4 * w >= base ? *(const uint32_t *)(turned + dim * line + 4 * w - base) : 0;
       const int kept = min(max(held - 4 * w, 0), 4), end = min(held + count - 4 * w, 4);
       if (kept == 0 && end == 4) {
         *word = now;
@@ -372,12 +373,17 @@ __global__ void __launch_bounds__(256) read_pages_kernel(const PoolArgs c, uint1
     *(uint32_t *)(turned + dim * line + 4 * w) = gload((const uint32_t *)(from + value_at<HD>(dim, 4 * w, lg)));
   }
   __syncthreads();
-  for (int e = tid; e < page * HD / 8; e += 256) {
-    const int row = e / (HD / 8), dim = e % (HD / 8) * 8;
-    uint32_t w[2] = {0, 0};
+  for (int e = tid; e < page * HD / 16; e += 256) {  // 4 dims of 4 rows, turned by byte permutes
+    const int dim = e % (HD / 4) * 4, row = e / (HD / 4) * 4;
+    uint32_t w[4];
 #pragma unroll
-    for (int k = 0; k < 8; k++) w[k / 4] |= (uint32_t)turned[(dim + k) * line + row] << 8 * (k % 4);
-    *(uint4 *)(to + 8 * e) = make_uint4(pair(w[0], false), pair(w[0], true), pair(w[1], false), pair(w[1], true));
+    for (int k = 0; k < 4; k++) w[k] = *(const uint32_t *)(turned + (dim + k) * line + row);
+    const uint32_t a01 = __builtin_amdgcn_perm(w[1], w[0], 0x05010400), b01 = __builtin_amdgcn_perm(w[1], w[0], 0x07030602);
+    const uint32_t a23 = __builtin_amdgcn_perm(w[3], w[2], 0x05010400), b23 = __builtin_amdgcn_perm(w[3], w[2], 0x07030602);
+    const uint32_t r[4] = {__builtin_amdgcn_perm(a23, a01, 0x05040100), __builtin_amdgcn_perm(a23, a01, 0x07060302),
+                           __builtin_amdgcn_perm(b23, b01, 0x05040100), __builtin_amdgcn_perm(b23, b01, 0x07060302)};
+#pragma unroll
+    for (int k = 0; k < 4; k++) *(uint2 *)(to + (row + k) * HD + dim) = make_uint2(pair(r[k], false), pair(r[k], true));
   }
 }
 
@@ -1053,7 +1059,10 @@ int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
   const PlanArgs k{at(a->tables), at(a->cached), at(a->fresh), at(a->free_pages), at(a->taken), at(a->starts), at(a->lengths),
                    at(a->places), at(a->slots), at(a->taken_out), at(a->parts), a->tables_sr, a->requests, a->width, a->n_free,
                    a->rows, lg, a->pages, std::min(a->most, a->rows), parts_target(a->kv), parts_least((int64_t)a->width * a->page)};
-  plan_kernel<<<1, PLAN_NT, 0, r->stream>>>(k);
+  const int most = std::max(a->requests, a->rows > PLAN_ROWS ? 1 : a->rows);
+  if (most <= 64) plan_kernel<64><<<1, 64, 0, r->stream>>>(k);
+  else if (most <= 256) plan_kernel<256><<<1, 256, 0, r->stream>>>(k);
+  else plan_kernel<1024><<<1, 1024, 0, r->stream>>>(k);
   BT_LAUNCHED("a plan");
   if (a->rows > PLAN_ROWS) {
     plan_rows_kernel<<<(unsigned)ceil_div(a->rows, 256), 256, 0, r->stream>>>(k);
@@ -1073,8 +1082,18 @@ int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, ui
   const int64_t blocks = (int64_t)((b.rows >> c.page_log2) + 2 * b.requests) * 2 * c.kv;
   if (blocks > 0x7FFFFFFF) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, 2 * c.kv);
   const uint16_t *src = (const uint16_t *)(uintptr_t)x;
-  if (pool->head_dim == 64) put_pages_kernel<64><<<(unsigned)blocks, 256, 0, r->stream>>>(c, b, src, x_sb, x_sr);
-  else put_pages_kernel<128><<<(unsigned)blocks, 256, 0, r->stream>>>(c, b, src, x_sb, x_sr);
+  // the most rows of a request in one page: 16 at most are a wave's
+  const int most = std::min(std::min(batch->most, batch->rows), pool->page);
+  const auto launch = [&](auto kernel, int threads) { kernel<<<(unsigned)blocks, threads, 0, r->stream>>>(c, b, src, x_sb, x_sr); };
+  if (pool->head_dim == 64) {
+    if (most <= 16) launch(put_pages_kernel<64, 64, 16>, 64);
+    else if (most <= 64) launch(put_pages_kernel<64, 256, 64>, 256);
+    else launch(put_pages_kernel<64, 256, 256>, 256);
+  } else {
+    if (most <= 16) launch(put_pages_kernel<128, 64, 16>, 64);
+    else if (most <= 64) launch(put_pages_kernel<128, 256, 64>, 256);
+    else launch(put_pages_kernel<128, 256, 256>, 256);
+  }
   BT_LAUNCHED("a paged put");
   return BT_OK;
 }
