@@ -952,7 +952,10 @@ static int check_pool(const bt_pages *c, PoolArgs *out) {
   return BT_OK;
 }
 
-constexpr int MOST_ROWS = 1 << 20;
+constexpr int MOST_ROWS = 1 << 20, MOST_KEYS = 1 << 30;  // rows of a batch, tokens of a request's table
+
+// A launch of `blocks` of `threads` fits the 32 bits that a grid counts threads in.
+static bool grid_fits(int64_t blocks, int threads) { return blocks > 0 && blocks * threads <= 0xFFFFFFFFll; }
 
 // The parts that a plan aims at, and a part's least blocks: all of a short table's keys (a part a request, and no join), else a
 // block for each of its 4 waves.
@@ -962,7 +965,7 @@ static int parts_least(int64_t keys) { return keys <= SHORT ? SHORT / KB : 4; }
 static int check_batch(const bt_batch *b, BatchArgs *out) {
   if (!b || !b->tables || !b->starts || !b->lengths || !b->parts) return fail(BT_EINVAL, "a batch needs its tables, starts, lengths and parts");
   if ((b->tables | b->starts | b->lengths | b->parts) % 4) return fail(BT_EINVAL, "a batch's tensors are int32-aligned");
-  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 || b->most < 1)
+  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 || b->width > MOST_KEYS / 16 || b->most < 1)
     return fail(BT_EINVAL, "a batch of %d requests (1 to %d), %d rows (1 to %d), tables %d wide, %d rows a request at most",
                 b->requests, MOST_REQUESTS, b->rows, MOST_ROWS, b->width, b->most);
   if (out)
@@ -985,6 +988,7 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   if (int s = check_batch(b, nullptr)) return s;
   if (heads < 1 || heads % c->kv || window < 0 || (int64_t)heads * b->rows > 0x3FFFFFFF)
     return fail(BT_EINVAL, "paged attention of %d heads over %d key heads, %d rows, window %d", heads, c->kv, b->rows, window);
+  if ((int64_t)b->width * c->page > MOST_KEYS) return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b->width, c->page);
   const int rep = heads / c->kv;
   const int64_t most = (int64_t)std::min(b->most, b->rows) * rep;
   p->many = most > 64;
@@ -1002,10 +1006,11 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   if (p->many) {
     const int64_t blocks = (int64_t)p->many_tiles * c->kv;
     p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / (8 * KB), 16}));
-    if (blocks * p->splits > 0x3FFFFF) return fail(BT_EINVAL, "paged attention of %d rows of %d heads is too large", b->rows, heads);
     if (p->splits > 1) p->split_scratch = (uint64_t)blocks * p->splits * TILE * (c->head_dim + 4) * 4;
   }
-  if ((int64_t)p->items * c->kv * p->groups > 0x3FFFFFFF || (int64_t)b->requests * heads * p->few > 0x7FFFFFFF) return fail(BT_EINVAL, "paged attention in %d parts of %d key heads", p->items, c->kv);
+  if (!grid_fits((int64_t)p->items * c->kv * p->groups + (b->rows + 15) / 16, 64 * p->waves) ||
+      !grid_fits((int64_t)b->requests * c->kv * p->few, 64) || (p->many && !grid_fits((int64_t)p->many_tiles * c->kv * TILE, 64)))
+    return fail(BT_EINVAL, "paged attention of %d rows and %d requests over %d heads is too large", b->rows, b->requests, heads);
   return BT_OK;
 }
 
@@ -1052,7 +1057,7 @@ int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
   while (lg < 9 && (1 << lg) != a->page) lg++;
   if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", a->page);
   if (a->requests < 1 || a->requests > MOST_REQUESTS || a->width < 1 || a->n_free < 1 || a->rows < 1 || a->rows > MOST_ROWS ||
-      a->most < 1 || a->kv < 1 || a->kv > 1024 || a->pages < 1 || (int64_t)a->pages * a->page > 0x7FFFFFFFll)
+      (int64_t)a->width * a->page > MOST_KEYS || a->most < 1 || a->kv < 1 || a->kv > 1024 || a->pages < 1 || (int64_t)a->pages * a->page > 0x7FFFFFFFll)
     return fail(BT_EINVAL, "a plan of %d requests (1 to %d), %d rows (1 to %d), %d a request at most, tables %d wide, %d free of %d pages",
                 a->requests, MOST_REQUESTS, a->rows, MOST_ROWS, a->most, a->width, a->n_free, a->pages);
   const auto at = [](uint64_t p) { return (int32_t *)(uintptr_t)p; };
@@ -1080,7 +1085,8 @@ int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, ui
   if (int s = check_batch(batch, &b)) return s;
   if (!x || x % 16 || x_sb % 8 || x_sr % 8) return fail(BT_EINVAL, "a paged cache takes rows on 16-byte boundaries");
   const int64_t blocks = (int64_t)((b.rows >> c.page_log2) + 2 * b.requests) * 2 * c.kv;
-  if (blocks > 0x7FFFFFFF) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, 2 * c.kv);
+  if ((int64_t)b.width * pool->page > MOST_KEYS) return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b.width, pool->page);
+  if (!grid_fits(blocks, 256)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, 2 * c.kv);
   const uint16_t *src = (const uint16_t *)(uintptr_t)x;
   // the most rows of a request in one page: 16 at most are a wave's
   const int most = std::min(std::min(batch->most, batch->rows), pool->page);
@@ -1105,7 +1111,7 @@ int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out) {
   if (int s = check_pool(pool, &c)) return s;
   if (!out || out % 16) return fail(BT_EINVAL, "pages are read to a 16-byte aligned tensor");
   const int64_t blocks = (int64_t)c.pages * 2 * c.kv;
-  if (blocks > 0x7FFFFFFF) return fail(BT_EINVAL, "%d pages of %d heads are too many to read at once", c.pages, 2 * c.kv);
+  if (!grid_fits(blocks, 256)) return fail(BT_EINVAL, "%d pages of %d heads are too many to read at once", c.pages, 2 * c.kv);
   if (pool->head_dim == 64) read_pages_kernel<64><<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out);
   else read_pages_kernel<128><<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out);
   BT_LAUNCHED("reading pages");

@@ -379,6 +379,7 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
 // 49152 12.3 us), else 16, which spreads a chunk's maximum and sums over more of them (112 rows of 131072 in 32 requests: the three
 // launches 13.1, 8.5 and 5.9 us; with 32 a lane, whose draw is one wave's long run, 14.4, 10.4 and 9.3).
 static int verify_per(const bt_verify_args *a) { return (int64_t)a->rows * a->vocab <= 1 << 22 ? 8 : 16; }
+static int verify_chunks(const bt_verify_args *a) { return ceil_div(a->vocab, 64 * verify_per(a)); }
 static int check_verify(const bt_verify_args *a) {
   if (!a || !a->logits || !a->ids || !a->starts || !a->uniforms || !a->tokens || !a->counts)
     return fail(BT_EINVAL, "verifying drafts needs logits, ids, starts, uniforms and results");
@@ -386,9 +387,11 @@ static int check_verify(const bt_verify_args *a) {
     return fail(BT_EINVAL, "verifying drafts takes tensors on 4-byte boundaries");
   if (a->requests < 1 || a->rows < 1 || a->vocab < 1 || a->vocab > 1 << 20 || a->requests > 1 << 20 || a->rows > 1 << 20)
     return fail(BT_EINVAL, "verifying %d requests' %d rows of %d logits (each 1 to 2^20)", a->requests, a->rows, a->vocab);
+  // a grid counts its threads in 32 bits: a wave a chunk of every row, and of every request, a block of 4 at least
+  if ((int64_t)std::max(a->rows, a->requests) * (verify_chunks(a) + WAVES) * 64 > 0xFFFFFFFFll)
+    return fail(BT_EINVAL, "verifying %d requests' %d rows of %d logits is too large", a->requests, a->rows, a->vocab);
   return BT_OK;
 }
-static int verify_chunks(const bt_verify_args *a) { return ceil_div(a->vocab, 64 * verify_per(a)); }
 static uint64_t verify_bytes(const bt_verify_args *a) {
   return (uint64_t)a->rows * verify_chunks(a) * sizeof(ChunkStat) + (uint64_t)a->requests * (sizeof(Draw) + 8 * verify_chunks(a));
 }
@@ -432,8 +435,6 @@ int bt_verify(bt_runtime *rt, const bt_verify_args *a) {
   k.draws = (Draw *)(k.stats + (int64_t)a->rows * k.chunks), k.left = (double *)(k.draws + a->requests);
   k.logits_sr = a->logits_sr, k.probs_sr = a->probs_sr, k.t_sr = a->t_sr, k.uniforms_sr = a->uniforms_sr;
   k.requests = a->requests, k.rows = a->rows, k.vocab = a->vocab;
-  if ((int64_t)std::max(a->rows, a->requests) * k.chunks > 0x7FFFFFFF)
-    return fail(BT_EINVAL, "verifying %d rows of %d logits is too large", a->rows, a->vocab);
   const bool wide = a->logits % 16 == 0 && a->logits_sr % 4 == 0 && a->probs % 16 == 0 && a->probs_sr % 4 == 0 && a->vocab % 4 == 0;
   if (verify_per(a) == 8) return wide ? launch_verify<8, true>(k, r->stream) : launch_verify<8, false>(k, r->stream);
   return wide ? launch_verify<16, true>(k, r->stream) : launch_verify<16, false>(k, r->stream);

@@ -1,7 +1,7 @@
 """Llama-family decoders on baretile_amd tensors: the device side of baretile/models/llama.py.
 
 The functions keep the reference's names and meaning (llama.py:48-373): precision, rms, rope, rotary, fuse, layer,
-attention, mlp, forward, prefill, kv_cache, upload. They run on Tensor only. The NumPy twin that the reference keeps
+attention, mlp, forward, prefill, kv_cache, upload; paged_cache and paged_forward run over shared pages. They run on Tensor only. The NumPy twin that the reference keeps
 in the same functions is this repository's CPU oracle (oracle/llama_ref.py), which the tests compare against.
 
 The numbers follow the reference's device path (llama.py:88-183):
@@ -20,6 +20,7 @@ import operator
 import os
 from types import SimpleNamespace
 import numpy as np
+from baretile_amd.pages import Pages
 from baretile_amd.tensor import Tensor, jit
 
 
@@ -243,6 +244,12 @@ def kv_cache(rt, c, size):
   return [Tensor.zeros(rt, size, head(c), batch=2 * c.kv).cast(fmt).realize() for _ in range(c.layers)]
 
 
+def paged_cache(rt, c, pages, page=64):
+  """A pool of `pages` pages of `page` tokens per block (baretile_amd.pages): the cache of paged_forward, 8 bits a value.
+  Every block's pool is of one shape, so one plan serves them all."""
+  return [Pages(rt, pages, c.kv, head(c), page) for _ in range(c.layers)]
+
+
 _aranges = {}
 
 
@@ -255,12 +262,14 @@ def _arange(rt, n):  # an int32 row 0 .. n-1, made once per runtime (a recording
 def rope_into(qkv, cos, sin, cache, rows, c):
   """RoPE of each token's heads with the key and value heads put into the cache at rows (llama.py:132-160): one
   kernel for a bf16 cache (rope_put); a block-float cache takes the rows from a bf16 stage through put, which rounds
-  each run of 16 as a cast does (kernels.py:1083-1168). Returns the query heads, (tokens, heads * head)."""
-  if cache.dtype == "bf16": return qkv.rope_put(cos, sin, cache, rows, c.heads, c.kv)
+  each run of 16 as a cast does (kernels.py:1083-1168), and so does a paged one, whose rows are its pages.Batch. Returns
+  the query heads, (tokens, heads * head)."""
+  paged = isinstance(cache, Pages)
+  if not paged and cache.dtype == "bf16": return qkv.rope_put(cos, sin, cache, rows, c.heads, c.kv)
   n = qkv.rows
   stage = Tensor(qkv.rt, n, head(c), batch=2 * c.kv)
   q = qkv.rope_put(cos, sin, stage, _arange(qkv.rt, n), c.heads, c.kv)
-  cache.put(rows, stage)
+  cache.put(rows, stage)  # Tensor.put, or Pages.put
   return q
 
 
@@ -281,12 +290,14 @@ def rope(x, cos, sin, turn):
 def heads_out(h, p, c, rot, places, cache, rows, firsts=None, apart=False):
   """One block's attention over its cache, up to the o product (llama.py:132-170): qkv, then RoPE with the new keys and
   values put into the cache at rows in one kernel (x cos + (x @ turn) sin, worked out in fp32 from the turn's pairs),
-  then one attention kernel from each token's place (and, with slots, from its slot's first row; apart: a token a slot)."""
+  then one attention kernel from each token's place (and, with slots, from its slot's first row; apart: a token a slot).
+  A paged cache takes its step's pages.Batch for rows (and has the places from it)."""
   rep = c.heads // c.kv
   qkv = h.matmul(p["qkv_proj"])
   n = qkv.rows
   q = rope_into(qkv.reshape(n, qkv.cols), rot[0].reshape(n, rot[0].cols), rot[1].reshape(n, rot[1].cols), cache,
                 rows, c).split(c.heads)
+  if isinstance(cache, Pages): return cache.attend(q, rows, merged=True)
   k, v = cache[:c.kv, :, :], cache[c.kv:, :, :]
   return q.attend(k.repeat_interleave(rep), v.repeat_interleave(rep), places, firsts=firsts, merged=True,
                   apart=apart)
@@ -456,6 +467,26 @@ def forward(ids, places, w, c, caches, every=False, slots=None):
     for l in range(c.layers): x = layer(x, ps[l], c, rot, column, caches[l], rows, firsts, apart)
     h = rms(x, w["norm"], c)
   if not (every or slots) and n > 1: h = h[:, n - 1:n, :]  # the last token's row
+  return h.matmul(w["embed.T"], "fp32")
+
+
+def paged_forward(ids, batch, w, c, caches):
+  """Logits after every row of ids (an int32 row of batch.rows) in fp32, over a paged cache (paged_cache): batch is the
+  step's plan, made by one of the caches, and says which request and place each row is, so requests may bring a token
+  each, a token and its drafts (serve.verify takes the logits), or chunks of prompts, all in one step. Rows behind the last
+  request's (whose ids are anything) give logits of no meaning."""
+  if len(caches) != c.layers or ids.cols != batch.rows:
+    raise ValueError(f"paged_forward needs {c.layers} caches and ids for the batch's {batch.rows} rows: {len(caches)}, {ids.shape}")
+  x = w["embed"].gather(ids).float()
+  rot = (w["cos"].gather(batch.places), w["sin"].gather(batch.places), w["turn"])
+  ps = blocks(w, c.layers)
+  if batch.rows <= 32 and ps and chain_fits(x, w["norm"], c, ps):
+    norms = [p["input_layernorm"] for p in ps[1:]] + [w["norm"]]
+    h = rms(x, ps[0]["input_layernorm"], c)
+    for l in range(c.layers): x, h = chained_layer(x, h, ps[l], c, rot, None, caches[l], batch, None, norms[l])
+  else:
+    for l in range(c.layers): x = layer(x, ps[l], c, rot, None, caches[l], batch)
+    h = rms(x, w["norm"], c)
   return h.matmul(w["embed.T"], "fp32")
 
 

@@ -76,8 +76,9 @@ class Pages:
     rows, most = operator.index(rows), rows if most is None else operator.index(most)
     if not (1 <= rows <= ROWS and most >= 1): raise ValueError(f"a plan takes 1 to {ROWS} rows, and one a request at least: {rows}, {most}")
     t = _int32(tables, self.rt, "a plan's tables")
-    if not (t.rows <= REQUESTS and t.sc == 1 and t.rep == 1 and not t.cyc and t.op is None and (t.sr >= t.cols or t.rows == 1)):
-      raise ValueError(f"a plan's tables are at most {REQUESTS} rows, each contiguous and apart from the others: {t.shape}")
+    if not (t.rows <= REQUESTS and t.cols * self.page <= 1 << 30 and t.sc == 1 and t.rep == 1 and not t.cyc and t.op is None and (t.sr >= t.cols or t.rows == 1)):
+      raise ValueError(f"a plan's tables are at most {REQUESTS} rows of pages of 2^30 tokens in all, each contiguous and "
+                       f"apart from the others: {t.shape}")
     n = t.rows
     cached, new, free = _row(cached, self.rt, "cached", n), _row(new, self.rt, "new", n), _row(free, self.rt, "free")
     if taken is not None: taken = _row(taken, self.rt, "taken", 1)
@@ -108,6 +109,7 @@ class Pages:
                        f"{getattr(x, 'shape', '')}")
     x = x.realize()
     if x.sc != 1 or x.rep != 1 or x.cyc or x.sb % 8 or x.sr % 8 or x.addr % 16: x = x.contiguous()
+    _written(self.scales.storage)
     self.rt.run("pages_put", "pages_put", ctypes.byref(self.args), ctypes.byref(batch.args), x.addr, x.sb, x.sr,
                 reads=4 * self.kv * batch.rows * self.head)
 
@@ -117,7 +119,7 @@ class Pages:
     Rows behind the last request's come back as zeros. merged gives the result as merge() of it, (rows, heads * head)."""
     self._fits(batch)
     window = operator.index(window)
-    if window < 0: raise ValueError("attention needs a nonnegative window")
+    if not 0 <= window < 1 << 31: raise ValueError(f"attention needs a nonnegative window of less than 2^31, not {window}")
     if not (isinstance(q, Tensor) and q.rt is self.rt and q.dtype == "bf16" and q.batch % self.kv == 0 and len(q.shape) <= 3 and
             (q.rows, q.cols) == (batch.rows, self.head)):
       raise ValueError(f"attend needs bf16 queries of a multiple of {self.kv} heads, ({batch.rows}, {self.head}) each: "

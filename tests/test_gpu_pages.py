@@ -214,6 +214,13 @@ def test_attend_long(rt):
   attended(rt, np.random.default_rng(6), 4, 1, 64, 64, [40000, 100], [1, 2])
 
 
+@pytest.mark.parametrize("hd, page, window", [(64, 16, 0), (128, 32, 0), (64, 16, 1500), (128, 128, 700), (64, 256, 0)])
+@pytest.mark.parametrize("new", [[1, 2], [4, 70]])
+def test_attend_past_a_wave_of_pages(rt, hd, page, window, new):
+  # over 64 pages of 16 or 32 tokens, which a wave's lanes hold at a time, and prompts whose keys are cut into splits
+  attended(rt, np.random.default_rng(hd + page), 4, 2, hd, page, [3100, 2500], new, window, spare=5)
+
+
 def test_attend_a_row_that_is_not_a_number(rt):
   rng = np.random.default_rng(7)
   for new in ([2, 2], [40, 40]):
@@ -396,6 +403,55 @@ def test_a_recorded_step_follows_its_lengths(rt):
     vt, vc = P.verify(ls, ds, starts, us)
     assert np.array_equal(ints(tokens), vt) and np.array_equal(ints(counts), vc)
     want_cached = total
+
+
+def numpy_step(L, ids, w, c, caches, scales, plan, places):
+  """Logits of every row as paged_forward gives them, over NumPy pages (caches, scales: one of each a block)."""
+  tables, starts, lengths = plan
+  x = w["embed"][ids].astype(np.float32)
+  nh, hd = c.heads + 2 * c.kv, L.head(c)
+  at = np.maximum(places, 0)
+  rot = [L.split(w[t][at], nh) for t in ("cos", "sin")]
+  for l in range(c.layers):
+    p = L.block(w, l)
+    heads = L.rope(L.split(L.rms(x, p["input_layernorm"], c.eps) @ p["qkv_proj"], nh), *rot, w["turn"])
+    P.put(caches[l], scales[l], tables, starts, lengths, B.bf16(heads[c.heads:]))
+    o, _ = P.attend(heads[:c.heads], caches[l], tables, starts, lengths)
+    x = x + L.merge(o) @ p["o_proj"]
+    x = x + L.mlp(L.rms(x, p["post_attention_layernorm"], c.eps), p)
+  return L.rms(x, w["norm"], c.eps) @ w["embed.T"]
+
+
+@pytest.mark.parametrize("page, spare", [(16, 3), (64, 0)])
+def test_paged_llama_matches_numpy(rt, page, spare):
+  # prompts of three requests in one step, then a token and drafts each, one request's drafts given up in between and its
+  # places taken again, over pages: every row's logits within 3% of the largest (test_models.py:849), as for the other
+  # caches, and the picks that serve.verify makes of them the oracle's
+  from baretile_amd.models import llama
+  from oracle import llama_ref as L
+  rng = np.random.default_rng(41)
+  c, w = L.smol(rng, 2, vocab=256, places=96)
+  dc = llama.model(dim=576, heads=9, kv=3, layers=2, eps=1e-5, theta=10000.0, vocab=256, ffn=1536)
+  dw = llama.upload(rt, {k: v for k, v in w.items() if k not in ("cos", "sin", "turn", "embed.T")}, dc, places=96)
+  pages, width = 24, 96 // page
+  caches = llama.paged_cache(rt, dc, pages, page)
+  values, scales = ([np.zeros((pages, 6, page, 64)) for _ in range(2)], [np.full((pages, 6), 2.0 ** -100) for _ in range(2)])
+  tables, cached, taken, free = np.full((3, width), -1), np.zeros(3, int), 0, rng.permutation(pages)
+  for new, kept in (([20, 7, 33], [20, 7, 33]), ([1, 4, 3], [1, 2, 3]), ([5, 3, 0], [1, 3, 0]), ([1, 1, 1], [1, 1, 1])):
+    rows = sum(new) + spare
+    ids = rng.integers(0, 256, rows)
+    b, (tables, starts, lengths, places, _, taken) = planned(rt, caches[0], tables, cached, new, free, rows, taken)
+    logits = llama.paged_forward(row(rt, ids), b, dw, dc, caches).realize()
+    got = np.array(logits.tolist()).reshape(rows, -1)[:starts[-1]]
+    want = numpy_step(L, ids, w, c, values, scales, (tables, starts, lengths), places)[:starts[-1]]
+    assert np.abs(got - want).max() <= 0.03 * np.abs(want).max(), np.abs(got - want).max()
+    u = rng.random((2, rows)).astype(np.float32)
+    tokens, counts = serve.verify(logits.reshape(rows, 256), row(rt, ids), b.starts, Tensor.of(rt, u, "fp32"))
+    vt, vc = P.verify(np.array(logits.tolist(), np.float32).reshape(rows, -1), ids, starts, u)
+    assert np.array_equal(ints(tokens), vt) and np.array_equal(ints(counts), vc)
+    cached = cached + kept
+  with pytest.raises(ValueError, match="paged_forward"): llama.paged_forward(row(rt, [1]), b, dw, dc, caches)
+  with pytest.raises(ValueError, match="paged_forward"): llama.paged_forward(row(rt, [1] * rows), b, dw, dc, caches[:1])
 
 
 def test_refusals(rt):

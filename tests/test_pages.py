@@ -65,14 +65,17 @@ def test_attention_scratch():
   (dict(pool={"values": 0}), "values and scales"), (dict(pool={"values": 4104}), "aligned"),
   (dict(batch={"tables": 0}), "needs its tables"), (dict(batch={"starts": 4098}), "aligned"), (dict(batch={"requests": 0}), "a batch of"),
   (dict(batch={"requests": 2049}), "a batch of"), (dict(batch={"rows": (1 << 20) + 1}), "a batch of"), (dict(batch={"width": 0}), "a batch of"),
-  (dict(batch={"most": 0}), "a batch of"), (dict(heads=7), "7 heads"), (dict(heads=0), "0 heads"),
+  (dict(batch={"most": 0}), "a batch of"), (dict(batch={"width": 1 << 27}), "a batch of"),
+  (dict(batch={"width": 1 << 25}), "over 2"), (dict(batch={"requests": 2048, "most": 12, "rows": 12}, pool={"kv": 1024}, heads=4096), "too large"),
+  (dict(batch={"rows": 1 << 20, "most": 1 << 20}, heads=512), "too large"), (dict(heads=1 << 20, batch={"rows": 1 << 12}), "heads over"), (dict(heads=7), "7 heads"), (dict(heads=0), "0 heads"),
   (dict(window=-1), "window")])
 def test_attention_refuses(bad, why):
   with pytest.raises(ValueError, match=why): need(**bad)
 
 
 @pytest.mark.parametrize("bad", [{"logits": 0}, {"ids": 0}, {"uniforms": 0}, {"counts": 0}, {"logits": 4098}, {"vocab": 0},
-                                 {"vocab": (1 << 20) + 1}, {"rows": 0}, {"requests": 0}])
+                                 {"vocab": (1 << 20) + 1}, {"rows": 0}, {"requests": 0},
+                                 {"vocab": 1 << 20, "rows": 1 << 17}, {"requests": 1 << 20, "vocab": 1 << 17}])
 def test_verify_refuses(bad):
   fields = {"logits": 4096, "uniforms": 4096, "ids": 4096, "starts": 4096, "tokens": 4096, "counts": 4096, "rows": 5, "requests": 1,
             "vocab": 1000}
