@@ -396,8 +396,10 @@ struct AttendArgs {
   uint16_t *out;
   float *scratch, *split_scratch;
   int64_t q_sh, q_sr, o_sh, o_sr;
-  int32_t rep, window, splits, items, few, groups;  // items: the most parts a plan makes; few: the most query pairs that parts
-                                             // are for, in `groups` that fold the keys apart
+  int32_t rep, window;
+  int32_t items, few, groups;  // the most parts a plan makes, the most query pairs they are for, in `groups` that fold the keys apart
+  int32_t tiles, splits;       // tiles of 128 pairs, and the pieces that each one's keys are cut into
+  uint32_t joins;              // the waves that join parts
   FastDiv drep;
 };
 
@@ -617,15 +619,15 @@ template <int HD> __device__ __forceinline__ void store_rows(const AttendArgs &a
 // requested while the block before weighs its scores, its values while it multiplies, so 16 KB a wave (heads of 128) are always
 // in flight. Two waves a SIMD: held to their registers (the compiler's own choice put O into accumulation registers as
 // well, which left one of QT = 2: 16 requests of 5 rows of 4 heads over 2048 keys 20.1 us, 15.2 so).
-template <int HD, int QT, int NW, bool ONE>
-__global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs a) {
+template <int HD, int QT, int NW> constexpr int few_lds() { return NW / 2 * QT * (HD / 16 * 16 + 8) * 64; }
+template <int HD, int QT, int NW, bool ONE> __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, char *lds) {
   constexpr int J = HD / 64, C = HD / 16;
-  __shared__ __attribute__((aligned(16))) f32x4 joined[NW / 2][QT * C][64];
-  __shared__ float joined_m[NW / 2][QT][64], joined_l[NW / 2][QT][64];
+  f32x4 (*joined)[QT * C][64] = (f32x4(*)[QT * C][64])lds;
+  float (*joined_m)[QT][64] = (float (*)[QT][64])(joined + NW / 2), (*joined_l)[QT][64] = joined_m + NW / 2;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int units = a.items * a.c.kv, group = blockIdx.x / units, unit = blockIdx.x - group * units;
-  if (group >= a.groups) return clear_rows<HD>(a, blockIdx.x - a.groups * units, tid, 64 * NW);
+  const int units = a.items * a.c.kv, group = block / units, unit = block - group * units;
+  if (group >= a.groups) return clear_rows<HD>(a, block - a.groups * units, tid, 64 * NW);
   const int item = unit / a.c.kv, kvh = unit - item * a.c.kv, pair0 = 16 * QT * group;
   const int per = gload(a.b.parts + a.b.requests + 1);
   Piece p;
@@ -731,6 +733,12 @@ __global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs 
   }
 }
 
+template <int HD, int QT, int NW, bool ONE>
+__global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[few_lds<HD, QT, NW>()];
+  few_pairs<HD, QT, NW, ONE>(a, blockIdx.x, lds);
+}
+
 // A pair's output from `parts` parts' sums, `step` floats apart, by a wave: M = max m, L = sum 2^(m - M) l, out = sum
 // 2^(m - M) O / L. 16 parts' are requested at once, so that the usual plan is one trip to memory.
 template <int HD> __device__ __forceinline__ void join_parts(const float *from, int64_t step, int parts, uint16_t *out, int lane) {
@@ -773,21 +781,6 @@ template <int HD> __device__ __forceinline__ void join_parts(const float *from, 
   else out[lane] = (uint16_t)pack_rne(O[0] * inv, 0.0f);
 }
 
-// Joins a request's parts: a wave (request, key head, pair), 4 a block.
-template <int HD>
-__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
-  const int lane = threadIdx.x & 63;
-  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), heads = unit / a.few;
-  const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
-  if (r >= a.b.requests) return;
-  Piece p{r, 0, gload(a.b.starts + r), 0, 0};
-  p.n = gload(a.b.starts + r + 1) - p.row0;
-  const int first = gload(a.b.parts + r), parts = gload(a.b.parts + r + 1) - first;
-  if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
-  const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
-  join_parts<HD>(a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4), step, parts, out_row(a, p, kvh, pair), lane);
-}
-
 constexpr int TILE_LOG2 = 7, TILE = 1 << TILE_LOG2;  // pairs of a block
 // The tile that `slot` is: 128 pairs of request p->r from pair 128 p->k on. Request r owns tiles starts[r] * rep / 128 + r and on:
 // at least as many as its pairs fill. False where there are none, or few enough for pages_few_kernel.
@@ -802,14 +795,13 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 // and values pass through LDS as codes, one barrier a step, the next step's codes held in registers meanwhile. 16-byte units are
 // placed so that the 16 lanes of a read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2)
 // (heads of 64: u ^ (r / 16)), values' unit u of dim d at u ^ (d / 4) % 4.
-template <int HD, bool ONE>
-__global__ void __launch_bounds__(512, 2) pages_many_kernel(const AttendArgs a, int tiles) {
+template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const AttendArgs &a, const int block, char *lds) {
   constexpr int C = HD / 16, UK = HD / 16, NU = HD * KB / 16 / 256;  // units of a key's row; units a thread
-  __shared__ __attribute__((aligned(16))) uint8_t kl[2][2][KB * HD], vl[2][2][KB * HD];  // [half][stage]
+  uint8_t (*kl)[2][KB * HD] = (uint8_t(*)[2][KB * HD])lds, (*vl)[2][KB * HD] = kl + 2;  // [half][stage]
   const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int kvh = blockIdx.x % a.c.kv, unit = blockIdx.x / a.c.kv, split = unit % a.splits;
-  const int slot = tiles - 1 - unit / a.splits;  // the longest rows first
+  const int kvh = block % a.c.kv, unit = block / a.c.kv, split = unit % a.splits;
+  const int slot = a.tiles - 1 - unit / a.splits;  // the longest rows first
   Piece p;
   if (!find_tile(a, slot, lane, &p)) return;
   const int pairs = p.n * a.rep, pair0 = TILE * p.k, mine0 = pair0 + 32 * wave;
@@ -923,14 +915,36 @@ __global__ void __launch_bounds__(512, 2) pages_many_kernel(const AttendArgs a, 
   }
 }
 
-// Joins the splits of the tiles' keys: a wave (tile, key head, pair), 4 a block.
+// A batch that may hold both: the tiles of many pairs, then the parts of few, which fill the CUs that the tiles leave. In one
+// launch: 
+template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages_mixed_kernel(const AttendArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[std::max(4 * 2 * KB * HD, few_lds<HD, 2, 8>())];
+  const int tiles = a.tiles * a.c.kv * a.splits;
+  if ((int)blockIdx.x < tiles) many_pairs<HD, ONE>(a, blockIdx.x, lds);
+  else few_pairs<HD, 2, 8, ONE>(a, blockIdx.x - tiles, lds);
+}
+
+// Joins what attention cut, a wave a pair, 4 a block: the parts of a request's keys (request, key head, pair), then the splits of the
+// tiles' (tile, key head, pair).
 template <int HD>
-__global__ void __launch_bounds__(256) pages_splits_kernel(const AttendArgs a, int tiles) {
+__global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
   const int lane = threadIdx.x & 63;
-  const uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int at = unit & (TILE - 1), kvh = (unit >> TILE_LOG2) % a.c.kv, slot = (unit >> TILE_LOG2) / a.c.kv;
+  uint32_t unit = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   Piece p;
-  if (!find_tile(a, slot, lane, &p)) return;
+  if (unit < a.joins) {
+    const uint32_t heads = unit / a.few;
+    const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
+    p = Piece{r, 0, gload(a.b.starts + r), 0, 0};
+    p.n = gload(a.b.starts + r + 1) - p.row0;
+    const int first = gload(a.b.parts + r), parts = gload(a.b.parts + r + 1) - first;
+    if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
+    const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
+    join_parts<HD>(a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4), step, parts, out_row(a, p, kvh, pair), lane);
+    return;
+  }
+  unit -= a.joins;
+  const int at = unit & (TILE - 1), kvh = (unit >> TILE_LOG2) % a.c.kv, slot = (unit >> TILE_LOG2) / a.c.kv;
+  if (slot >= a.tiles || a.splits == 1 || !find_tile(a, slot, lane, &p)) return;
   const int pair = TILE * p.k + at;
   if (pair >= p.n * a.rep) return;
   join_parts<HD>(a.split_scratch + (((int64_t)slot * a.c.kv + kvh) * a.splits * TILE + at) * (HD + 4), TILE * (HD + 4), a.splits,
@@ -981,6 +995,7 @@ struct AttendPlan {
   int waves;             // of a part's block
   int many_tiles, splits;  // tiles of 128 pairs, and the pieces that each one's keys are cut into
   bool many, join;
+  int64_t joins;  // waves that join parts
   uint64_t scratch, split_scratch;
 };
 static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int window, AttendPlan *p) {
@@ -998,7 +1013,7 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   p->items = parts_target(c->kv) + b->requests;
   const int64_t keys = (int64_t)b->width * c->page;
   p->join = keys > SHORT;
-  p->waves = p->tiles == 1 && !p->join ? 8 : 4;
+  p->waves = p->many || (p->tiles == 1 && !p->join) ? 8 : 4;
   const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
   // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least
@@ -1008,31 +1023,24 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
     p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / (8 * KB), 16}));
     if (p->splits > 1) p->split_scratch = (uint64_t)blocks * p->splits * TILE * (c->head_dim + 4) * 4;
   }
-  if (!grid_fits((int64_t)p->items * c->kv * p->groups + (b->rows + 15) / 16, 64 * p->waves) ||
-      !grid_fits((int64_t)b->requests * c->kv * p->few, 64) || (p->many && !grid_fits((int64_t)p->many_tiles * c->kv * TILE, 64)))
+  p->joins = p->join ? (int64_t)b->requests * c->kv * p->few : 0;
+  if (!grid_fits((int64_t)p->items * c->kv * p->groups + (b->rows + 15) / 16 + (p->many ? (int64_t)p->many_tiles * c->kv * p->splits : 0),
+                 64 * p->waves) ||
+      !grid_fits(std::max<int64_t>(p->joins, 1) + (p->many ? (int64_t)p->many_tiles * c->kv * TILE : 0), 64))
     return fail(BT_EINVAL, "paged attention of %d rows and %d requests over %d heads is too large", b->rows, b->requests, heads);
   return BT_OK;
 }
 
-template <int HD, int QT, int NW, bool ONE> static int launch_few(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  const int clear = (a.b.rows + 15) / 16;
-  pages_few_kernel<HD, QT, NW, ONE><<<(unsigned)(p.items * a.c.kv * p.groups + clear), 64 * NW, 0, s>>>(a);
-  BT_LAUNCHED("paged attention");
-  if (p.join) {
-    pages_join_kernel<HD><<<(unsigned)ceil_div((int64_t)a.b.requests * a.c.kv * p.few, 4), 256, 0, s>>>(a);
-    BT_LAUNCHED("paged attention's join");
-  }
-  return BT_OK;
-}
 template <int HD, bool ONE> static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
-  const int status = p.tiles == 2    ? launch_few<HD, 2, 4, ONE>(a, p, s)
-                     : p.waves == 8 ? launch_few<HD, 1, 8, ONE>(a, p, s)
-                                    : launch_few<HD, 1, 4, ONE>(a, p, s);
-  if (status || !p.many) return status;
-  pages_many_kernel<HD, ONE><<<(unsigned)(p.many_tiles * a.c.kv * p.splits), 512, 0, s>>>(a, p.many_tiles);
+  const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;
+  if (p.many) pages_mixed_kernel<HD, ONE><<<tiles * p.splits + parts, 512, 0, s>>>(a);
+  else if (p.tiles == 2) pages_few_kernel<HD, 2, 4, ONE><<<parts, 256, 0, s>>>(a);
+  else if (p.waves == 8) pages_few_kernel<HD, 1, 8, ONE><<<parts, 512, 0, s>>>(a);
+  else pages_few_kernel<HD, 1, 4, ONE><<<parts, 256, 0, s>>>(a);
   BT_LAUNCHED("paged attention");
-  if (p.splits > 1) {
-    pages_splits_kernel<HD><<<(unsigned)(p.many_tiles * a.c.kv * (TILE / 4)), 256, 0, s>>>(a, p.many_tiles);
+  const int64_t joins = p.joins + (p.splits > 1 ? (int64_t)tiles * TILE : 0);
+  if (joins) {
+    pages_join_kernel<HD><<<(unsigned)ceil_div(joins, 4), 256, 0, s>>>(a);
     BT_LAUNCHED("paged attention's join");
   }
   return BT_OK;
@@ -1143,6 +1151,7 @@ int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch,
   a.split_scratch = (float *)(uintptr_t)(scratch + p.scratch), a.splits = p.splits;
   a.q_sh = q_sh, a.q_sr = q_sr, a.o_sh = o_sh, a.o_sr = o_sr;
   a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few, a.groups = p.groups;
+  a.tiles = p.many_tiles, a.joins = (uint32_t)p.joins;
   a.drep = make_fastdiv((uint32_t)a.rep);
   const bool one = pool->page >= KB;
   if (pool->head_dim == 64) return one ? launch_attend<64, true>(a, p, r->stream) : launch_attend<64, false>(a, p, r->stream);
