@@ -5,9 +5,9 @@
 // mantissa bits, at most 448) times one power of two for the page and head, so each is exact in bf16 and the conversion
 // v_cvt_scalef32_pk_bf16_fp8 applies the scale: half an instruction a value, where a block float's decoding takes 2.5.
 // Keys are kept by row, 64 dims at a time, [head width / 64][page][64], and values by dimension, up to 64 tokens at a time,
-// [page / 64][head width][64], so that both products of attention read their operands from memory as they lie, 16 bytes a lane, with no transposition and no trip
-// through LDS, and each load of a wave covers whole lines (rows of 128 dims, of which a load takes half a line each: 8
-// requests of 8191 keys 20.8 us, by halves 19.5; 32 of 4096 47.5 and 45.4):
+// [page / 64][head width][64], so that both products of attention read their operands from memory as they lie, 16 bytes a
+// lane, with no transposition and no trip through LDS, and each load of a wave covers whole lines (keys by rows of 128 dims,
+// of which a load takes half a line each: 8 requests of up to 8191 keys 20.8 us, by halves 19.5; 32 of 4096 47.5 and 45.4):
 //   S^T = K Q^T: lane (n, g) (n = l % 16, g = l / 16) holds for tile kt (of 4 in a block of 64 keys) the key
 //     16 (n / 4) + 4 kt + n % 4, dims 64 j + 16 g .. + 15 (the contraction takes dims in any order that both operands share);
 //   so in the result lane (n, g) holds keys 16 g + 4 kt + i, i < 4, against pair n: 16 keys in a row over the 4 tiles;
@@ -25,9 +25,11 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KB = 64;          // keys of a block
-constexpr int MOST_PARTS = 32;  // parts of one request
-constexpr int SHORT = 8 * KB;   // keys that tables of one part a request hold at most
-constexpr int WAVES = 2048;     // waves that attention's parts are for, over all key heads
+constexpr int MOST_PARTS = 32;  // parts of one request (with 64, one request of 65536 keys: 32.4 us against 27.1)
+constexpr int SHORT = 16 * KB;  // keys that tables of one part a request hold at most
+// Waves that attention's parts are for, over all key heads: 8 on each of the 256 CUs, which is what their registers allow at once
+// (8 requests of up to 8191 keys: 19.7 us; with 1024 23.4, with 3072 22.5).
+constexpr int WAVES = 2048;
 constexpr int MOST_REQUESTS = 2048;
 
 // ---- the plan ------------------------------------------------------------------------------------------------------
@@ -82,12 +84,15 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int j, int start, in
   a.slots[j] = real && id_or_free >= 0 ? (id_or_free << a.page_log2) + (place & mask) : -1;
 }
 
-// One block, of 64, 256 or 1024 threads by the larger of its requests and the rows it writes. Requests are scanned a thread each: first their rows, cut to `most` each and to the rows there are, and the
-// pages they take; then, with the keys' blocks counted, the parts that attention cuts each request's keys into: as many
-// parts over all requests as `target`, of whole blocks of 64 keys and `least` of them, so that uneven lengths make parts of
-// even length.
-// Latency bounds it: three scans of about a microsecond and two trips to memory.
-constexpr int PLAN_ROWS = 2048;  // rows that the plan's one block writes itself; more go to plan_rows_kernel's many
+// One block, of 64, 256 or 1024 threads by the larger of its requests and the rows it writes. Requests are scanned a thread
+// each: first their rows, cut to `most` each and to the rows there are, and the pages they take; then, with the keys' blocks
+// counted, the parts that attention cuts each request's keys into: as many parts over all requests as `target`, of whole blocks
+// of 64 keys and `least` of them, so that uneven lengths make parts of even length.
+// Latency bounds it: three scans of about a microsecond and two trips to memory. 32 requests of a row: 4.3 us (5.7 by 1024
+// threads, whose scans pass 16 sums through LDS); 512 with 8500 rows: 6.2 and 4.1 us for the rows.
+// The block writes up to PLAN_ROWS rows itself, past that many blocks of plan_rows_kernel do: 2048 rows 6.8 us here, 3.5 + 3.2 us
+// and a launch more there; 8192 12.4 us and 4.5 + 4.0.
+constexpr int PLAN_ROWS = 2048;
 template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs a) {
   __shared__ int starts[MOST_REQUESTS + 1], first[MOST_REQUESTS], from[MOST_REQUESTS + 1], cache[MOST_REQUESTS];
   __shared__ int sums[NT / 64];
@@ -244,8 +249,13 @@ __device__ __forceinline__ float scale_of(float amax) {
 }
 
 // A block: the rows that one request puts into one page of one head, PAGE of them at most. They are loaded once (up to 16 loads of
-// 16 bytes a thread, all at once), their largest finite size gives the scale, and a page that already holds rows and whose scale
-// grows has them rounded again. Values turn by dimension in LDS, so they are stored as whole words.
+// 16 bytes a thread, all at once and before the page's id is there), their largest finite size gives the scale, and a page that
+// already holds rows and whose scale grows has them rounded again. Values turn by dimension in LDS, so they are stored as
+// whole words.
+// Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 190 us, 4.2 TB/s; a decode step's 32 rows are
+// latency, 5.1 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
+// by one wave (512 requests of one row 29.6 us, by four waves 56; of 8 rows 36 and 58), up to 64 by four waves with loads for 64
+// (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
 template <int HD, int NT, int PAGE>
 __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
                                                         int64_t x_sr) {
@@ -345,7 +355,8 @@ __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const B
   if (tid == 0) *scale_at = s;
 }
 
-// A block: one page of one head as bf16 rows.
+// A block: one page of one head as bf16 rows. Values turn back through LDS, 4 x 4 codes a thread by byte permutes. 12.6 million
+// values (38 MB read and written): 9.6 us, 3.9 TB/s.
 template <int HD>
 __global__ void __launch_bounds__(256) read_pages_kernel(const PoolArgs c, uint16_t *out) {
   __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (256 + 4)];
@@ -397,7 +408,7 @@ struct AttendArgs {
   float *scratch, *split_scratch;
   int64_t q_sh, q_sr, o_sh, o_sr;
   int32_t rep, window;
-  int32_t items, few, groups;  // the most parts a plan makes, the most query pairs they are for, in `groups` that fold the keys apart
+  int32_t items, few, groups;  // the most parts a plan makes, the most query pairs they are for, in groups of 32
   int32_t tiles, splits;       // tiles of 128 pairs, and the pieces that each one's keys are cut into
   uint32_t joins;              // the waves that join parts
   FastDiv drep;
@@ -428,8 +439,9 @@ __device__ __forceinline__ PageRun page_run(const AttendArgs &a, int r, int kvh,
   return w;
 }
 
-// Where key `key` lies: its page (0 where it is none, whose keys are hidden), its row there, the head's scales. ONE: blocks of 64
-// keys lie in one page (of 64 tokens or more), so `key` is the wave's and everything here is in scalar registers.
+// Where key `key` lies: its page (0 where it is none, whose keys are hidden), its row there, the head's scales. ONE: blocks of
+// 64 keys lie in one page (of 64 tokens or more), so `key` is the wave's and everything here is in scalar registers (a 2048-row
+// prompt 64.3 us, without 68.3; decoding alike).
 struct PageAt {
   int id, real, in;
   float ks, vs;
@@ -492,8 +504,8 @@ template <int HD> struct Running {
     for (int c = 0; c < HD / 16; c++) o[c] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   }
   // s: the block's scores, hidden keys at -inf; p: the lane's 16 weights as bf16, the second operand of the two 32-key
-  // steps of O^T. They are rounded to nearest (the operand's type); l sums them as
-  // rounded, in 32 bits.
+  // steps of O^T. They are rounded to nearest, since the operand is bf16; l sums them as rounded, in 32 bits, so that a row's
+  // weights still add up to 1.
   __device__ __forceinline__ void weigh(const f32x4 (&s)[4], bf16x8 (&p)[2]) {
     float top = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3]));
 #pragma unroll
@@ -544,8 +556,8 @@ __device__ __forceinline__ uint16_t *out_row(const AttendArgs &a, const Piece &p
 }
 
 // One block of 64 keys against QT tiles of pairs. key: the lane's first key (its 16 are in a row), seen: whether their page
-// is one; keys(kt, j) and values(c): the lane's 16 codes of each piece; between: run once the scores are made. Matrix instructions on
-// one accumulator are kept 2 QT apart: one that follows its like at once waits for it.
+// is one; keys(kt, j) and values(c): the lane's 16 codes of each piece; between: run once the scores are made. Matrix
+// instructions on one accumulator are kept 2 QT apart: one that follows its like at once waits for it.
 template <int HD, int QT, class Keys, class Values, class Between>
 __device__ __forceinline__ void fold_block(const Query<HD> (&q)[QT], Running<HD> (&st)[QT], int key, bool seen, float ks, float vs,
                                            Keys keys, Values values, Between between) {
@@ -615,12 +627,18 @@ template <int HD> __device__ __forceinline__ void store_rows(const AttendArgs &a
 
 // Few query pairs a request: a block of NW waves a part. A part is a run of whole blocks of 64 keys of one request, against QT
 // tiles of 16 of its pairs, so every key and value is read and converted once for all of them; the waves take its
-// blocks in turn and join by halves through LDS, lane by lane, since every wave's state lies in the same lanes. A block's keys are
-// requested while the block before weighs its scores, its values while it multiplies, so 16 KB a wave (heads of 128) are always
-// in flight. Two waves a SIMD: held to their registers (the compiler's own choice put O into accumulation registers as
+// blocks in turn and join by halves through LDS, lane by lane, since every wave's state lies in the same lanes. A block's keys
+// are requested while the block before weighs its scores, its values while it multiplies, so 16 KB a wave (heads of 128) are
+// always in flight. Two waves a SIMD: held to their registers (the compiler's own choice put O into accumulation registers as
 // well, which left one of QT = 2: 16 requests of 5 rows of 4 heads over 2048 keys 20.1 us, 15.2 so).
+// Memory bounds it once every CU has its waves: 32 requests of 4096 keys of 8 heads of 128 (269 MB) 44.8 us, 6.0 TB/s; one of
+// 65536 23.1 us, 5.8. 8 requests of up to 8191 (101 MB) 19.7 us and 16 of 2048 in drafts (51 MB) 15 us are two or three blocks a
+// wave, so the trips to memory before the first and the join in LDS are a third of it. Loads past the caches, since no key is
+// read twice (through them, with caches of three steps in turn: 51.5 us for the 44.8). One tile of pairs where 16 will do: 8
+// requests of 8191 keys 23.7, with a second one empty 25.9.
 template <int HD, int QT, int NW> constexpr int few_lds() { return NW / 2 * QT * (HD / 16 * 16 + 8) * 64; }
-template <int HD, int QT, int NW, bool ONE> __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, char *lds) {
+template <int HD, int QT, int NW, bool ONE>
+__device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, char *lds) {
   constexpr int J = HD / 64, C = HD / 16;
   f32x4 (*joined)[QT * C][64] = (f32x4(*)[QT * C][64])lds;
   float (*joined_m)[QT][64] = (float (*)[QT][64])(joined + NW / 2), (*joined_l)[QT][64] = joined_m + NW / 2;
@@ -795,6 +813,11 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 // and values pass through LDS as codes, one barrier a step, the next step's codes held in registers meanwhile. 16-byte units are
 // placed so that the 16 lanes of a read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2)
 // (heads of 64: u ^ (r / 16)), values' unit u of dim d at u ^ (d / 4) % 4.
+// The instructions beside the matrix ones bound it: a prompt of 2048 rows of 32 heads of 128 (34.4 GF) 62 us, 555 TFLOP/s; 4096
+// rows 213 us, 645. Vector instructions run 58 % of the time and matrix ones 28 %, hardly ever together, since the waves of a
+// block keep step. Dropped: 4 waves of 64 pairs (118 us for the 62) and 4 of 32 with no halves (78); codes converted once, into
+// bf16 in LDS (63.5 and 226 us for the 62 and 213: twice the LDS traffic); scores from 8-bit products with q in two parts (no
+// faster); fences that interleave the two kinds, wave priorities and loads from LDS a tile ahead (no change).
 template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const AttendArgs &a, const int block, char *lds) {
   constexpr int C = HD / 16, UK = HD / 16, NU = HD * KB / 16 / 256;  // units of a key's row; units a thread
   uint8_t (*kl)[2][KB * HD] = (uint8_t(*)[2][KB * HD])lds, (*vl)[2][KB * HD] = kl + 2;  // [half][stage]
@@ -835,14 +858,16 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
     if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, run = page_run(a, p.r, kvh, p0, lane);
     if constexpr (ONE) {
       const PageAt at = page_at<true>(run, p0, b * KB, lg);
-      const uint8_t *k = base + (int64_t)at.id * (2 * a.c.kv) * head + at.in * 64, *v = base + ((int64_t)at.id * (2 * a.c.kv) + a.c.kv) * head + value_at<HD>(0, at.in, lg);
+      const uint8_t *k = base + (int64_t)at.id * (2 * a.c.kv) * head + at.in * 64;
+      const uint8_t *v = base + ((int64_t)at.id * (2 * a.c.kv) + a.c.kv) * head + value_at<HD>(0, at.in, lg);
 #pragma unroll
       for (int i = 0; i < NU; i++) kr[i] = gload((const u32x4 *)(k + kunit[i])), vr[i] = gload((const u32x4 *)(v + vunit[i]));
     } else {
 #pragma unroll
       for (int i = 0; i < NU; i++) {
         const int u = tid + 256 * i;
-        const PageAt k = page_at<false>(run, p0, b * KB + (u / UK & ~15), lg), v = page_at<false>(run, p0, b * KB + 16 * (u & 3), lg);
+        const PageAt k = page_at<false>(run, p0, b * KB + (u / UK & ~15), lg);
+        const PageAt v = page_at<false>(run, p0, b * KB + 16 * (u & 3), lg);
         kr[i] = gload((const u32x4 *)(base + (int64_t)k.id * (2 * a.c.kv) * head + k.in * 64 + kunit[i]));
         vr[i] = gload((const u32x4 *)(base + ((int64_t)v.id * (2 * a.c.kv) + a.c.kv) * head + v.in + vunit[i]));
       }
@@ -860,7 +885,8 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
   if (b0 + half < b1) fetch(b0 + half), store(0);
   __syncthreads();
   for (int b = b0 + half, now = 0; b - half < b1; b += 2, now ^= 1) {
-    const PageAt ka = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * (n >> 2)), lg), va = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
+    const PageAt ka = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * (n >> 2)), lg);
+    const PageAt va = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
     if (b + 2 < b1) fetch(b + 2);
     if (b < b1 && b * KB <= whi && b * KB + KB > wlo) {
       const uint8_t *k = kl[half][now], *v = vl[half][now];
@@ -915,8 +941,8 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
   }
 }
 
-// A batch that may hold both: the tiles of many pairs, then the parts of few, which fill the CUs that the tiles leave. In one
-// launch: 
+// A batch that may hold both: the tiles of many pairs, then the parts of few, which fill the CUs that the tiles leave. As two
+// launches the parts cost 4.5 to 6 us even where every request has many pairs.
 template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages_mixed_kernel(const AttendArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[std::max(4 * 2 * KB * HD, few_lds<HD, 2, 8>())];
   const int tiles = a.tiles * a.c.kv * a.splits;
@@ -924,8 +950,8 @@ template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages_mixe
   else few_pairs<HD, 2, 8, ONE>(a, blockIdx.x - tiles, lds);
 }
 
-// Joins what attention cut, a wave a pair, 4 a block: the parts of a request's keys (request, key head, pair), then the splits of the
-// tiles' (tile, key head, pair).
+// Joins what attention cut, a wave a pair, 4 a block: the parts of a request's keys (request, key head, pair), then the splits of
+// the tiles' (tile, key head, pair). Latency: 4.0 to 4.6 us from one part a request to 32.
 template <int HD>
 __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
   const int lane = threadIdx.x & 63;
@@ -939,7 +965,8 @@ __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
     const int first = gload(a.b.parts + r), parts = gload(a.b.parts + r + 1) - first;
     if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
     const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
-    join_parts<HD>(a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4), step, parts, out_row(a, p, kvh, pair), lane);
+    const float *from = a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4);
+    join_parts<HD>(from, step, parts, out_row(a, p, kvh, pair), lane);
     return;
   }
   unit -= a.joins;
@@ -955,7 +982,8 @@ __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
 
 static int check_pool(const bt_pages *c, PoolArgs *out) {
   if (!c || !c->values || !c->scales) return fail(BT_EINVAL, "a paged cache needs its values and scales");
-  if (c->head_dim != 64 && c->head_dim != 128) return fail(BT_EINVAL, "a paged cache's heads are 64 or 128 wide, not %d", c->head_dim);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(BT_EINVAL, "a paged cache's heads are 64 or 128 wide, not %d", c->head_dim);
   int lg = 0;
   while (lg < 9 && (1 << lg) != c->page) lg++;
   if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", c->page);
@@ -972,24 +1000,31 @@ constexpr int MOST_ROWS = 1 << 20, MOST_KEYS = 1 << 30;  // rows of a batch, tok
 static bool grid_fits(int64_t blocks, int threads) { return blocks > 0 && blocks * threads <= 0xFFFFFFFFll; }
 
 // The parts that a plan aims at, and a part's least blocks: all of a short table's keys (a part a request, and no join), else a
-// block for each of its 4 waves.
+// block for each of its 4 waves. 1000 keys in one part and in parts with their join: one request of 3 heads of 64 6.2 us and 4.4
+// + 3.1, 32 of 8 heads of 128 14.6 and 14.2 + 4.2, drafts' 5 rows of 16 14.2 and 12.6 + 4.5; 2000 keys: 9.8 us and 4.7 + 3.8,
+// 8 requests of 8 heads of 128 15.4 and 9.9 + 4.0.
 static int parts_target(int kv) { return std::max(1, WAVES / (4 * kv)); }
 static int parts_least(int64_t keys) { return keys <= SHORT ? SHORT / KB : 4; }
 
 static int check_batch(const bt_batch *b, BatchArgs *out) {
-  if (!b || !b->tables || !b->starts || !b->lengths || !b->parts) return fail(BT_EINVAL, "a batch needs its tables, starts, lengths and parts");
+  if (!b || !b->tables || !b->starts || !b->lengths || !b->parts)
+    return fail(BT_EINVAL, "a batch needs its tables, starts, lengths and parts");
   if ((b->tables | b->starts | b->lengths | b->parts) % 4) return fail(BT_EINVAL, "a batch's tensors are int32-aligned");
-  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 || b->width > MOST_KEYS / 16 || b->most < 1)
+  if (b->requests < 1 || b->requests > MOST_REQUESTS || b->rows < 1 || b->rows > MOST_ROWS || b->width < 1 ||
+      b->width > MOST_KEYS / 16 || b->most < 1)
     return fail(BT_EINVAL, "a batch of %d requests (1 to %d), %d rows (1 to %d), tables %d wide, %d rows a request at most",
                 b->requests, MOST_REQUESTS, b->rows, MOST_ROWS, b->width, b->most);
   if (out)
-    *out = BatchArgs{(const int32_t *)(uintptr_t)b->tables, (const int32_t *)(uintptr_t)b->starts, (const int32_t *)(uintptr_t)b->lengths,
-                     (const int32_t *)(uintptr_t)b->parts, b->tables_sr, b->requests, b->width, b->rows};
+    *out = BatchArgs{(const int32_t *)(uintptr_t)b->tables,  (const int32_t *)(uintptr_t)b->starts,
+                     (const int32_t *)(uintptr_t)b->lengths, (const int32_t *)(uintptr_t)b->parts,
+                     b->tables_sr, b->requests, b->width, b->rows};
   return BT_OK;
 }
 
 // How a call is cut: `few`, the most pairs of a request whose keys are cut into parts, in tiles of 16 (`tiles` a wave); `many`,
-// whether requests may have more (their rows then share blocks of 128 pairs).
+// whether requests may have more, whose rows then share blocks of 128 pairs, and then parts are for up to 32 pairs. Where no
+// request can have more than 64 all go to parts, 32 pairs at a time, which reads keys twice but spreads them further: 48 pairs of
+// one request over 65536 keys 46.9 + 4.9 us in parts, 85.3 + 4.0 in tiles; 64 pairs of 16 over 2048 34.4 + 8.5 and 30.2 + 11.2.
 struct AttendPlan {
   int few, tiles, groups, items;
   int waves;             // of a part's block
@@ -1003,7 +1038,8 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   if (int s = check_batch(b, nullptr)) return s;
   if (heads < 1 || heads % c->kv || window < 0 || (int64_t)heads * b->rows > 0x3FFFFFFF)
     return fail(BT_EINVAL, "paged attention of %d heads over %d key heads, %d rows, window %d", heads, c->kv, b->rows, window);
-  if ((int64_t)b->width * c->page > MOST_KEYS) return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b->width, c->page);
+  if ((int64_t)b->width * c->page > MOST_KEYS)
+    return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b->width, c->page);
   const int rep = heads / c->kv;
   const int64_t most = (int64_t)std::min(b->most, b->rows) * rep;
   p->many = most > 64;
@@ -1016,17 +1052,18 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   p->waves = p->many || (p->tiles == 1 && !p->join) ? 8 : 4;
   const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
-  // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least
+  // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least: 100 rows of 32 heads over 8192 keys
+  // 235 us whole, 38 + 6.8 in 16 splits; 32 rows over 65536 85.6 + 4.1 in 16, 60.2 + 5.2 in 32
   p->many_tiles = (int)((int64_t)b->rows * rep >> TILE_LOG2) + b->requests, p->splits = 1, p->split_scratch = 0;
   if (p->many) {
     const int64_t blocks = (int64_t)p->many_tiles * c->kv;
-    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / (8 * KB), 16}));
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / (8 * KB), 64}));
     if (p->splits > 1) p->split_scratch = (uint64_t)blocks * p->splits * TILE * (c->head_dim + 4) * 4;
   }
   p->joins = p->join ? (int64_t)b->requests * c->kv * p->few : 0;
-  if (!grid_fits((int64_t)p->items * c->kv * p->groups + (b->rows + 15) / 16 + (p->many ? (int64_t)p->many_tiles * c->kv * p->splits : 0),
-                 64 * p->waves) ||
-      !grid_fits(std::max<int64_t>(p->joins, 1) + (p->many ? (int64_t)p->many_tiles * c->kv * TILE : 0), 64))
+  const int64_t tiles = p->many ? (int64_t)p->many_tiles * c->kv : 0;
+  if (!grid_fits((int64_t)p->items * c->kv * p->groups + (b->rows + 15) / 16 + tiles * p->splits, 64 * p->waves) ||
+      !grid_fits(std::max<int64_t>(p->joins, 1) + tiles * TILE, 64))
     return fail(BT_EINVAL, "paged attention of %d rows and %d requests over %d heads is too large", b->rows, b->requests, heads);
   return BT_OK;
 }
@@ -1065,13 +1102,16 @@ int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
   while (lg < 9 && (1 << lg) != a->page) lg++;
   if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", a->page);
   if (a->requests < 1 || a->requests > MOST_REQUESTS || a->width < 1 || a->n_free < 1 || a->rows < 1 || a->rows > MOST_ROWS ||
-      (int64_t)a->width * a->page > MOST_KEYS || a->most < 1 || a->kv < 1 || a->kv > 1024 || a->pages < 1 || (int64_t)a->pages * a->page > 0x7FFFFFFFll)
-    return fail(BT_EINVAL, "a plan of %d requests (1 to %d), %d rows (1 to %d), %d a request at most, tables %d wide, %d free of %d pages",
+      (int64_t)a->width * a->page > MOST_KEYS || a->most < 1 || a->kv < 1 || a->kv > 1024 || a->pages < 1 ||
+      (int64_t)a->pages * a->page > 0x7FFFFFFFll)
+    return fail(BT_EINVAL,
+                "a plan of %d requests (1 to %d), %d rows (1 to %d), %d a request at most, tables %d wide, %d free of %d pages",
                 a->requests, MOST_REQUESTS, a->rows, MOST_ROWS, a->most, a->width, a->n_free, a->pages);
   const auto at = [](uint64_t p) { return (int32_t *)(uintptr_t)p; };
   const PlanArgs k{at(a->tables), at(a->cached), at(a->fresh), at(a->free_pages), at(a->taken), at(a->starts), at(a->lengths),
                    at(a->places), at(a->slots), at(a->taken_out), at(a->parts), a->tables_sr, a->requests, a->width, a->n_free,
-                   a->rows, lg, a->pages, std::min(a->most, a->rows), parts_target(a->kv), parts_least((int64_t)a->width * a->page)};
+                   a->rows, lg, a->pages, std::min(a->most, a->rows), parts_target(a->kv),
+                   parts_least((int64_t)a->width * a->page)};
   const int most = std::max(a->requests, a->rows > PLAN_ROWS ? 1 : a->rows);
   if (most <= 64) plan_kernel<64><<<1, 64, 0, r->stream>>>(k);
   else if (most <= 256) plan_kernel<256><<<1, 256, 0, r->stream>>>(k);
@@ -1093,10 +1133,11 @@ int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, ui
   if (int s = check_batch(batch, &b)) return s;
   if (!x || x % 16 || x_sb % 8 || x_sr % 8) return fail(BT_EINVAL, "a paged cache takes rows on 16-byte boundaries");
   const int64_t blocks = (int64_t)((b.rows >> c.page_log2) + 2 * b.requests) * 2 * c.kv;
-  if ((int64_t)b.width * pool->page > MOST_KEYS) return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b.width, pool->page);
+  if ((int64_t)b.width * pool->page > MOST_KEYS)
+    return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b.width, pool->page);
   if (!grid_fits(blocks, 256)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, 2 * c.kv);
   const uint16_t *src = (const uint16_t *)(uintptr_t)x;
-  // the most rows of a request in one page: 16 at most are a wave's
+  // the most rows of a request in one page
   const int most = std::min(std::min(batch->most, batch->rows), pool->page);
   const auto launch = [&](auto kernel, int threads) { kernel<<<(unsigned)blocks, threads, 0, r->stream>>>(c, b, src, x_sb, x_sr); };
   if (pool->head_dim == 64) {
@@ -1134,8 +1175,9 @@ int bt_pages_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t
   return BT_OK;
 }
 
-int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr, uint64_t out,
-                    int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch, uint64_t scratch_bytes) {
+int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr,
+                    uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,
+                    uint64_t scratch_bytes) {
   Runtime *r;
   if (int s = enter(rt, &r)) return s;
   AttendPlan p;

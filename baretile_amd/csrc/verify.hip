@@ -57,10 +57,10 @@ __device__ __forceinline__ bool greedy(float t) { return t > 3.4028234663852886e
 // t log2(e), as weight() takes it.
 __device__ __forceinline__ double in_log2(float t) { return (double)t * 1.4426950408889634074; }
 
-// exp(t (x - m)) as 2^(x - m) t2, t2 = t log2(e): 2^n by the exponent and 2^f, |f| <= 1/2, by the polynomial of degree 9 through
-// it at the Chebyshev points, its constant set to 1 so that the largest weigh exactly that (3.3e-14 relative; a draw over 2^17
-// tokens falls on the other side of a border less than once in 10^8). 16 64-bit instructions, where exp() takes about 40 and bounded the first launch. -inf and what is below
-// 2^-1074 give 0.
+// exp(t (x - m)) as 2^((x - m) t2), t2 = t log2(e): 2^n by the exponent and 2^f, |f| <= 1/2, by the polynomial of degree 9
+// through it at the Chebyshev points, its constant set to 1 so that the largest weigh exactly that (3.3e-14 relative; a draw over
+// 2^17 tokens falls on the other side of a border less than once in 10^8). 16 64-bit instructions, where exp() takes about 40
+// and bounded the first launch. -inf and what is below 2^-1074 give 0.
 __device__ __forceinline__ double weight(float x, float m, double t2) {
   const double y = fmax(((double)x - (double)m) * t2, -2000.0), n = rint(y), f = y - n;
   double p = 0x1.b6571e229927fp-24;
@@ -220,7 +220,8 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs &a, int row, float 
 }
 
 // What chunk c's tokens may still be drawn with, times z: p, or where a draft was refused what p has over q.
-template <int PER, bool WIDE> __device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int c, int lane, double (&out)[PER]) {
+template <int PER, bool WIDE>
+__device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int c, int lane, double (&out)[PER]) {
   float x[PER], q[PER];
   const int v0 = c * 64 * PER;
   const bool drawn = f.refused && a.probs;

@@ -1,8 +1,9 @@
 """Llama-family decoders on baretile_amd tensors: the device side of baretile/models/llama.py.
 
 The functions keep the reference's names and meaning (llama.py:48-373): precision, rms, rope, rotary, fuse, layer,
-attention, mlp, forward, prefill, kv_cache, upload; paged_cache and paged_forward run over shared pages. They run on Tensor only. The NumPy twin that the reference keeps
-in the same functions is this repository's CPU oracle (oracle/llama_ref.py), which the tests compare against.
+attention, mlp, forward, prefill, kv_cache, upload; paged_cache and paged_forward, which it lacks, run over shared pages. They
+run on Tensor only. The NumPy twin that the reference keeps in the same functions is this repository's CPU oracle
+(oracle/llama_ref.py), which the tests compare against.
 
 The numbers follow the reference's device path (llama.py:88-183):
   - the residual stream is fp32 and each half of a block adds onto it in its last matmul's kernel;

@@ -46,12 +46,13 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None):
   ids[j]]. tokens, an int32 row, has for each row the token that follows it: accepted drafts, then at the first refusal a token
   drawn with uniforms[1] from what p has over probs, or after the last draft one from p, -1 behind that. counts, an int32 row,
   has each request's new tokens."""
-  rt = logits.rt
+  rt = getattr(logits, "rt", None)
   for x, dtype in ((logits, "fp32"), (ids, "int32"), (starts, "int32"), (uniforms, "fp32"), (probs, "fp32"), (t, "fp32")):
     if x is not None and not (isinstance(x, Tensor) and x.rt is rt and x.batch == 1 and x.dtype == dtype):
       raise ValueError(f"verify needs {dtype} matrices on one runtime: {getattr(x, 'dtype', type(x))} {getattr(x, 'shape', '')}")
   rows, vocab = logits.rows, logits.cols
-  if not ((ids.rows, ids.cols) == (1, rows) and starts.rows == 1 and starts.cols >= 2 and (uniforms.rows, uniforms.cols) == (2, rows) and
+  if not ((ids.rows, ids.cols) == (1, rows) and starts.rows == 1 and starts.cols >= 2 and
+          (uniforms.rows, uniforms.cols) == (2, rows) and
           (probs is None or (probs.rows, probs.cols) == (rows, vocab)) and (t is None or (t.rows, t.cols) == (rows, 1))):
     raise ValueError(f"verify needs ids (1, {rows}), starts (1, requests + 1), uniforms (2, {rows}), probs ({rows}, {vocab}) and t "
                      f"({rows}, 1): {ids.shape} {starts.shape} {uniforms.shape} "
@@ -63,8 +64,8 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None):
   probs, t = (whole(x) if x is not None else None for x in (probs, t))
   requests = starts.cols - 1
   tokens, counts = Tensor(rt, 1, rows, dtype="int32"), Tensor(rt, 1, requests, dtype="int32")
-  args = _lib.VerifyArgs(logits.addr, probs.addr if probs is not None else 0, t.addr if t is not None else 0, uniforms.addr, ids.addr,
-                         starts.addr, tokens.addr, counts.addr, 0, 0, logits.sr, probs.sr if probs is not None else 0,
+  args = _lib.VerifyArgs(logits.addr, probs.addr if probs is not None else 0, t.addr if t is not None else 0, uniforms.addr,
+                         ids.addr, starts.addr, tokens.addr, counts.addr, 0, 0, logits.sr, probs.sr if probs is not None else 0,
                          t.sr if t is not None else 0, uniforms.sr, requests, rows, vocab, 0)
   need = ctypes.c_uint64()
   _lib.call("verify_scratch", ctypes.byref(args), ctypes.byref(need))

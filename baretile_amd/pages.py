@@ -74,9 +74,11 @@ class Pages:
     empty entry, so that drafts that were refused leave theirs to the next step; the pages it needs from there on go into
     `tables`."""
     rows, most = operator.index(rows), rows if most is None else operator.index(most)
-    if not (1 <= rows <= ROWS and most >= 1): raise ValueError(f"a plan takes 1 to {ROWS} rows, and one a request at least: {rows}, {most}")
+    if not (1 <= rows <= ROWS and most >= 1):
+      raise ValueError(f"a plan takes 1 to {ROWS} rows, and one a request at least: {rows}, {most}")
     t = _int32(tables, self.rt, "a plan's tables")
-    if not (t.rows <= REQUESTS and t.cols * self.page <= 1 << 30 and t.sc == 1 and t.rep == 1 and not t.cyc and t.op is None and (t.sr >= t.cols or t.rows == 1)):
+    if not (t.rows <= REQUESTS and t.cols * self.page <= 1 << 30 and t.sc == 1 and t.rep == 1 and not t.cyc and t.op is None and
+            (t.sr >= t.cols or t.rows == 1)):
       raise ValueError(f"a plan's tables are at most {REQUESTS} rows of pages of 2^30 tokens in all, each contiguous and "
                        f"apart from the others: {t.shape}")
     n = t.rows

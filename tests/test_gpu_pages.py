@@ -214,6 +214,19 @@ def test_attend_long(rt):
   attended(rt, np.random.default_rng(6), 4, 1, 64, 64, [40000, 100], [1, 2])
 
 
+@pytest.mark.parametrize("new", [[40, 2], [17, 30]])
+def test_attend_long_behind_a_prompt(rt, new):
+  attended(rt, np.random.default_rng(11), 4, 1, 64, 64, [40000, 100], new)  # keys cut into as many splits as there are
+
+
+@pytest.mark.parametrize("hd, page", [(64, 16), (128, 64), (128, 256)])
+@pytest.mark.parametrize("lengths", [[1024, 3], [1025, 1024], [1008, 961]])
+@pytest.mark.parametrize("new", [[1, 1], [6, 2]])
+def test_attend_at_a_short_tables_end(rt, hd, page, lengths, new):
+  # tables of 1024 keys are one part a request; of one page more, several and a join
+  attended(rt, np.random.default_rng(hd + page), 8, 2, hd, page, lengths, new, spare=1)
+
+
 @pytest.mark.parametrize("hd, page, window", [(64, 16, 0), (128, 32, 0), (64, 16, 1500), (128, 128, 700), (64, 256, 0)])
 @pytest.mark.parametrize("new", [[1, 2], [4, 70]])
 def test_attend_past_a_wave_of_pages(rt, hd, page, window, new):
