@@ -636,12 +636,13 @@ template <int HD> __device__ __forceinline__ void store_rows(const AttendArgs &a
 // wave, so the trips to memory before the first and the join in LDS are a third of it. Loads past the caches, since no key is
 // read twice (through them, with caches of three steps in turn: 51.5 us for the 44.8). One tile of pairs where 16 will do: 8
 // requests of 8191 keys 23.7, with a second one empty 25.9.
-template <int HD, int QT, int NW> constexpr int few_lds() { return NW / 2 * QT * (HD / 16 * 16 + 8) * 64; }
+template <int HD, int QT, int NW> struct FewLds {
+  f32x4 o[NW / 2][QT * (HD / 16)][64];
+  float m[NW / 2][QT][64], l[NW / 2][QT][64];
+};
 template <int HD, int QT, int NW, bool ONE>
-__device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, char *lds) {
+__device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, FewLds<HD, QT, NW> &lds) {
   constexpr int J = HD / 64, C = HD / 16;
-  f32x4 (*joined)[QT * C][64] = (f32x4(*)[QT * C][64])lds;
-  float (*joined_m)[QT][64] = (float (*)[QT][64])(joined + NW / 2), (*joined_l)[QT][64] = joined_m + NW / 2;
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = a.items * a.c.kv, group = block / units, unit = block - group * units;
@@ -711,22 +712,22 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
     if (wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int t = 0; t < QT; t++) {
-        joined_m[wave - half][t][lane] = st[t].m, joined_l[wave - half][t][lane] = st[t].l;
+        lds.m[wave - half][t][lane] = st[t].m, lds.l[wave - half][t][lane] = st[t].l;
 #pragma unroll
-        for (int c = 0; c < C; c++) joined[wave - half][t * C + c][lane] = st[t].o[c];
+        for (int c = 0; c < C; c++) lds.o[wave - half][t * C + c][lane] = st[t].o[c];
       }
     }
     __syncthreads();
     if (wave < half) {
 #pragma unroll
       for (int t = 0; t < QT; t++) {
-        const float m = joined_m[wave][t][lane], top = fmaxf(st[t].m, m);
+        const float m = lds.m[wave][t][lane], top = fmaxf(st[t].m, m);
         const float mine = st[t].m == -INF ? 0.0f : __builtin_amdgcn_exp2f(st[t].m - top);
         const float other = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-        st[t].m = top, st[t].l = st[t].l * mine + joined_l[wave][t][lane] * other;
+        st[t].m = top, st[t].l = st[t].l * mine + lds.l[wave][t][lane] * other;
 #pragma unroll
         for (int c = 0; c < C; c++) {
-          const f32x4 o = joined[wave][t * C + c][lane];
+          const f32x4 o = lds.o[wave][t * C + c][lane];
 #pragma unroll
           for (int i = 0; i < 4; i++) st[t].o[c][i] = st[t].o[c][i] * mine + o[i] * other;
         }
@@ -753,7 +754,7 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
 
 template <int HD, int QT, int NW, bool ONE>
 __global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[few_lds<HD, QT, NW>()];
+  __shared__ FewLds<HD, QT, NW> lds;
   few_pairs<HD, QT, NW, ONE>(a, blockIdx.x, lds);
 }
 
@@ -818,9 +819,11 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 // block keep step. Dropped: 4 waves of 64 pairs (118 us for the 62) and 4 of 32 with no halves (78); codes converted once, into
 // bf16 in LDS (63.5 and 226 us for the 62 and 213: twice the LDS traffic); scores from 8-bit products with q in two parts (no
 // faster); fences that interleave the two kinds, wave priorities and loads from LDS a tile ahead (no change).
-template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const AttendArgs &a, const int block, char *lds) {
+template <int HD> struct ManyLds {
+  __attribute__((aligned(16))) uint8_t k[2][2][KB * HD], v[2][2][KB * HD];  // [half][stage]
+};
+template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const AttendArgs &a, const int block, ManyLds<HD> &lds) {
   constexpr int C = HD / 16, UK = HD / 16, NU = HD * KB / 16 / 256;  // units of a key's row; units a thread
-  uint8_t (*kl)[2][KB * HD] = (uint8_t(*)[2][KB * HD])lds, (*vl)[2][KB * HD] = kl + 2;  // [half][stage]
   const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = block % a.c.kv, unit = block / a.c.kv, split = unit % a.splits;
@@ -878,8 +881,8 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
 #pragma unroll
     for (int i = 0; i < NU; i++) {
       const int u = tid + 256 * i, row = u / UK, dim = u / 4;
-      *(u32x4 *)(kl[half][to] + row * HD + 16 * (u % UK ^ turned(row))) = kr[i];
-      *(u32x4 *)(vl[half][to] + dim * KB + 16 * ((u & 3) ^ (dim >> 2 & 3))) = vr[i];
+      *(u32x4 *)(lds.k[half][to] + row * HD + 16 * (u % UK ^ turned(row))) = kr[i];
+      *(u32x4 *)(lds.v[half][to] + dim * KB + 16 * ((u & 3) ^ (dim >> 2 & 3))) = vr[i];
     }
   };
   if (b0 + half < b1) fetch(b0 + half), store(0);
@@ -889,7 +892,7 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
     const PageAt va = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
     if (b + 2 < b1) fetch(b + 2);
     if (b < b1 && b * KB <= whi && b * KB + KB > wlo) {
-      const uint8_t *k = kl[half][now], *v = vl[half][now];
+      const uint8_t *k = lds.k[half][now], *v = lds.v[half][now];
       fold_block<HD, 2>(q, st, b * KB + 16 * g, va.real, ka.ks, va.vs,
                         [&](int kt, int j) {
                           const int row = 16 * (n >> 2) + 4 * kt + (n & 3);
@@ -900,8 +903,8 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
     if (b + 2 < b1) store(now ^ 1);
     __syncthreads();
   }
-  f32x4 *joined = (f32x4 *)kl;  // a tile of pairs at a time: every wave of the second half's O^T, maxima and sums
-  float *sums = (float *)vl;
+  f32x4 *joined = (f32x4 *)lds.k;  // a tile of pairs at a time: every wave of the second half's O^T, maxima and sums
+  float *sums = (float *)lds.v;
 #pragma unroll
   for (int t = 0; t < 2; t++) {
     if (half) {
@@ -944,10 +947,13 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
 // A batch that may hold both: the tiles of many pairs, then the parts of few, which fill the CUs that the tiles leave. As two
 // launches the parts cost 4.5 to 6 us even where every request has many pairs.
 template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages_mixed_kernel(const AttendArgs a) {
-  __shared__ __attribute__((aligned(16))) char lds[std::max(4 * 2 * KB * HD, few_lds<HD, 2, 8>())];
+  __shared__ union {
+    ManyLds<HD> many;
+    FewLds<HD, 2, 8> few;
+  } lds;
   const int tiles = a.tiles * a.c.kv * a.splits;
-  if ((int)blockIdx.x < tiles) many_pairs<HD, ONE>(a, blockIdx.x, lds);
-  else few_pairs<HD, 2, 8, ONE>(a, blockIdx.x - tiles, lds);
+  if ((int)blockIdx.x < tiles) many_pairs<HD, ONE>(a, blockIdx.x, lds.many);
+  else few_pairs<HD, 2, 8, ONE>(a, blockIdx.x - tiles, lds.few);
 }
 
 // Joins what attention cut, a wave a pair, 4 a block: the parts of a request's keys (request, key head, pair), then the splits of
