@@ -206,24 +206,29 @@ struct Piece {
   int r, k, row0, n, len;
 };
 // The request whose pieces `before(i, starts[i])` .. `before(i + 1, ..)` hold piece `at`, found by the wave's lanes
-// together, 64 requests a trip to memory (a search by halves would be a trip a step).
+// together: of more than 64 requests first which of 64 equal runs, then which of the run's, a trip to memory each (64 at a time
+// from the first on, a put of 2048 requests' rows 135 us, so 90; a search by halves would be a trip a step). Starts count within
+// the rows there are and lengths hold their rows, whatever they say.
 template <class F> __device__ __forceinline__ bool find_piece(const BatchArgs &b, int at, int lane, F before, Piece *p) {
-  for (int base = 0; base < b.requests; base += 64) {
-    const int i = min(base + lane, b.requests - 1);
-    const int s0 = gload(b.starts + i), s1 = gload(b.starts + i + 1), len = gload(b.lengths + i);
-    const int lo = before(i, s0), hi = before(i + 1, s1);
-    const uint64_t hit = __ballot(base + lane < b.requests && lo <= at && at < hi);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      p->r = base + l;
-      p->k = at - __builtin_amdgcn_readlane(lo, l);
-      p->row0 = __builtin_amdgcn_readlane(s0, l);
-      p->n = __builtin_amdgcn_readlane(s1, l) - p->row0;
-      p->len = __builtin_amdgcn_readlane(len, l);
-      return true;
-    }
+  const auto start = [&](int i) { return min(max(gload(b.starts + i), 0), b.rows); };
+  int base = 0;
+  if (b.requests > 64) {
+    const int run = (b.requests + 63) >> 6, i = min(lane * run, b.requests - 1);  // at most 32 of MOST_REQUESTS
+    const uint64_t from = __ballot(before(i, start(i)) <= at);
+    base = from ? min((63 - __builtin_clzll(from)) * run, b.requests - 1) : 0;
   }
-  return false;
+  const int i = min(base + lane, b.requests - 1);
+  const int s0 = start(i), s1 = max(start(i + 1), s0), len = gload(b.lengths + i);
+  const int lo = before(i, s0), hi = before(i + 1, s1);
+  const uint64_t hit = __ballot(base + lane < b.requests && lo <= at && at < hi);
+  if (!hit) return false;
+  const int l = __builtin_ctzll(hit);
+  p->r = base + l;
+  p->k = at - __builtin_amdgcn_readlane(lo, l);
+  p->row0 = __builtin_amdgcn_readlane(s0, l);
+  p->n = __builtin_amdgcn_readlane(s1, l) - p->row0;
+  p->len = max(__builtin_amdgcn_readlane(len, l), p->n);
+  return true;
 }
 
 // Two codes of x0, x1 in the low half: nearest even, at most 448 in size (a NaN, which no code stands for in a cache, 448).
@@ -254,7 +259,7 @@ __device__ __forceinline__ float scale_of(float amax) {
 // whole words.
 // Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 190 us, 4.2 TB/s; a decode step's 32 rows are
 // latency, 5.1 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
-// by one wave (512 requests of one row 29.6 us, by four waves 56; of 8 rows 36 and 58), up to 64 by four waves with loads for 64
+// by one wave (512 requests of one row 25.8 us, by four waves 48.4; of 8 rows 31.0 and 49.8), up to 64 by four waves with loads for 64
 // (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
 template <int HD, int NT, int PAGE>
 __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
@@ -966,8 +971,8 @@ __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
   if (unit < a.joins) {
     const uint32_t heads = unit / a.few;
     const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
-    p = Piece{r, 0, gload(a.b.starts + r), 0, 0};
-    p.n = gload(a.b.starts + r + 1) - p.row0;
+    p = Piece{r, 0, min(max(gload(a.b.starts + r), 0), a.b.rows), 0, 0};
+    p.n = min(gload(a.b.starts + r + 1), a.b.rows) - p.row0;
     const int first = gload(a.b.parts + r), parts = gload(a.b.parts + r + 1) - first;
     if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
     const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
@@ -1055,7 +1060,9 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   p->items = parts_target(c->kv) + b->requests;
   const int64_t keys = (int64_t)b->width * c->page;
   p->join = keys > SHORT;
-  p->waves = p->many || (p->tiles == 1 && !p->join) ? 8 : 4;
+  // a block of 8 waves where a part a request leaves most CUs idle: one request of 3 heads of 64 and 1000 keys 6.4 us, with 4 waves
+  // 6.8; 512 of 8 heads and 500 keys 121.4 and 88.7
+  p->waves = p->many || (p->tiles == 1 && !p->join && (int64_t)b->requests * c->kv < 64) ? 8 : 4;
   const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
   // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least: 100 rows of 32 heads over 8192 keys

@@ -194,6 +194,22 @@ def test_attend_many_rows(rt, heads, kv, hd, page, lengths, new):
   attended(rt, np.random.default_rng(heads + page + sum(lengths)), heads, kv, hd, page, lengths, new, spare=17)
 
 
+@pytest.mark.parametrize("new", [[1, 1, 0], [2, 1, 40]])
+def test_attend_many_heads_to_one(rt, new):
+  attended(rt, np.random.default_rng(12), 130, 1, 64, 32, [700, 90, 50], new)  # a token's pairs pass a tile
+
+
+@pytest.mark.parametrize("requests", [64, 65, 300, 2048])
+def test_many_requests(rt, requests):
+  # some without rows or tokens; decoding steps, drafts and a prompt among them
+  rng = np.random.default_rng(requests)
+  lengths = rng.integers(0, 40, requests)
+  new = np.minimum(lengths, rng.choice([0, 1, 3], requests))
+  attended(rt, rng, 4, 2, 64, 16, lengths.tolist(), new.tolist(), spare=3, most=3)
+  lengths[requests // 2], new[requests // 2] = 100, 50
+  attended(rt, rng, 4, 2, 64, 16, lengths.tolist(), new.tolist())
+
+
 @pytest.mark.parametrize("window", [1, 7, 64, 100, 1000])
 @pytest.mark.parametrize("lengths, new", [([300, 40], [1, 3]), ([400, 150], [100, 70])])
 def test_attend_window(rt, window, lengths, new):
@@ -365,6 +381,17 @@ def test_verify_reads_starts_within_its_rows(rt):
   for starts in ([0, 9], [-5, 2], [3, 1], [2 ** 31 - 1, -2 ** 31]):
     tokens, counts = serve.verify(logits, row(rt, [1, 2, 3, 4]), row(rt, starts), u)
     assert len(ints(tokens)) == 4 and len(ints(counts)) == 1  # (starts that no plan makes: any tokens, but nothing outside)
+
+
+def test_a_batch_reads_starts_within_its_rows(rt):
+  rng = np.random.default_rng(13)
+  pool, values, tables, _ = filled(rt, rng, 4, 2, 64, 16, [30, 50])
+  b, _ = planned(rt, pool, tables, [20, 10], [10, 40], [-1], 50)
+  x, q = Tensor.of(rt, bf16_rows(rng, 4, 50, 64)), Tensor.of(rt, B.bf16(rng.normal(0, 0.2, (4, 50, 64))))
+  for starts in ([0, 10, 9000], [-5, 20, 30], [40, 3, 50], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1]):
+    b.starts.assign(row(rt, starts))  # (starts that no plan makes: any rows, but nothing outside)
+    pool.put(b, x)
+    assert np.array(pool.attend(q, b).tolist()).shape == (4, 50, 64)
 
 
 # ---- together
