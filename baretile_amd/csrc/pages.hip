@@ -645,30 +645,34 @@ template <int HD, int QT, int NW> struct FewLds {
   f32x4 o[NW / 2][QT * (HD / 16)][64];
   float m[NW / 2][QT][64], l[NW / 2][QT][64];
 };
+// tid: the thread among the part's, which pass every barrier, as other parts of their block may be at work.
 template <int HD, int QT, int NW, bool ONE>
-__device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, FewLds<HD, QT, NW> &lds) {
+__device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, const int tid, FewLds<HD, QT, NW> &lds) {
   constexpr int J = HD / 64, C = HD / 16;
-  const int tid = threadIdx.x, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
+  const int lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int units = a.items * a.c.kv, group = block / units, unit = block - group * units;
-  if (group >= a.groups) return clear_rows<HD>(a, block - a.groups * units, tid, 64 * NW);
   const int item = unit / a.c.kv, kvh = unit - item * a.c.kv, pair0 = 16 * QT * group;
   const int per = gload(a.b.parts + a.b.requests + 1);
-  Piece p;
+  Piece p{0, 0, 0, 0, 0};
   const int32_t *at = a.b.parts;
-  if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p)) return;
+  if (group >= a.groups) clear_rows<HD>(a, block - a.groups * units, tid, 64 * NW);
+  else if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p) || p.n * a.rep > a.few) p.n = 0;
   const int pairs = p.n * a.rep;
-  if (pairs > a.few || pair0 >= pairs) return;
+  const bool real = pair0 < pairs;
   const int room = min(p.len, a.b.width << lg), nb = (room + KB - 1) / KB;
   const int mine = max(per, (nb + MOST_PARTS - 1) / MOST_PARTS), parts = (nb + mine - 1) / mine;
   int b0 = p.k * mine;
-  const int b1 = min(b0 + mine, nb);
+  const int b1 = real ? min(b0 + mine, nb) : 0;
   if (a.window > 0) b0 = max(b0, max(p.len - p.n - a.window + 1, 0) / KB);
   b0 += wave;
   Query<HD> q[QT];
   Running<HD> st[QT];
 #pragma unroll
-  for (int t = 0; t < QT; t++) q[t].load(a, p, kvh, pair0 + 16 * t + n, g), st[t].clear();
+  for (int t = 0; t < QT; t++) {
+    if (real) q[t].load(a, p, kvh, pair0 + 16 * t + n, g);
+    st[t].clear();
+  }
   if (b0 < b1) {
     const int64_t head = (int64_t)HD << lg;  // codes of one page of one head
     int p0 = b0 * KB >> lg;
@@ -714,7 +718,7 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
   }
 #pragma unroll
   for (int half = NW / 2; half; half /= 2) {
-    if (wave >= half && wave < 2 * half) {
+    if (real && wave >= half && wave < 2 * half) {
 #pragma unroll
       for (int t = 0; t < QT; t++) {
         lds.m[wave - half][t][lane] = st[t].m, lds.l[wave - half][t][lane] = st[t].l;
@@ -723,7 +727,7 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
       }
     }
     __syncthreads();
-    if (wave < half) {
+    if (real && wave < half) {
 #pragma unroll
       for (int t = 0; t < QT; t++) {
         const float m = lds.m[wave][t][lane], top = fmaxf(st[t].m, m);
@@ -740,7 +744,7 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
     }
     __syncthreads();
   }
-  if (wave) return;
+  if (wave || !real) return;
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     const int pair = pair0 + 16 * t + n;
@@ -760,7 +764,7 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
 template <int HD, int QT, int NW, bool ONE>
 __global__ void __launch_bounds__(64 * NW, 2) pages_few_kernel(const AttendArgs a) {
   __shared__ FewLds<HD, QT, NW> lds;
-  few_pairs<HD, QT, NW, ONE>(a, blockIdx.x, lds);
+  few_pairs<HD, QT, NW, ONE>(a, blockIdx.x, threadIdx.x, lds);
 }
 
 // A pair's output from `parts` parts' sums, `step` floats apart, by a wave: M = max m, L = sum 2^(m - M) l, out = sum
@@ -819,8 +823,8 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 // and values pass through LDS as codes, one barrier a step, the next step's codes held in registers meanwhile. 16-byte units are
 // placed so that the 16 lanes of a read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2)
 // (heads of 64: u ^ (r / 16)), values' unit u of dim d at u ^ (d / 4) % 4.
-// The instructions beside the matrix ones bound it: a prompt of 2048 rows of 32 heads of 128 (34.4 GF) 62 us, 555 TFLOP/s; 4096
-// rows 213 us, 645. Vector instructions run 58 % of the time and matrix ones 28 %, hardly ever together, since the waves of a
+// The instructions beside the matrix ones bound it: a prompt of 2048 rows of 32 heads of 128 (34.4 GF) 65 us, 529 TFLOP/s; 4096
+// rows 217 us, 633 (62 and 213 in a launch without parts, as which the steps below were timed). Vector instructions run 58 % of the time and matrix ones 28 %, hardly ever together, since the waves of a
 // block keep step. Dropped: 4 waves of 64 pairs (118 us for the 62) and 4 of 32 with no halves (78); codes converted once, into
 // bf16 in LDS (63.5 and 226 us for the 62 and 213: twice the LDS traffic); scores from 8-bit products with q in two parts (no
 // faster); fences that interleave the two kinds, wave priorities and loads from LDS a tile ahead (no change).
@@ -949,16 +953,20 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs(const Att
   }
 }
 
-// A batch that may hold both: the tiles of many pairs, then the parts of few, which fill the CUs that the tiles leave. As two
-// launches the parts cost 4.5 to 6 us even where every request has many pairs.
+// A batch that may hold both: the tiles of many pairs, then the parts of few, two a block, which fill the CUs that the tiles
+// leave. As two launches the parts cost 4.5 to 6 us even where every request has many pairs; 16 requests of 5 rows over 4096 keys
+// beside one of 256 over 2048: 70.1 us as four launches, 60.0; 60 of a row over 2000 beside 2 of 512 over 1000: 81.3 and 86.3.
+// Dropped: tiles and parts by eights in turn, 78.4 us for those 86.3, but a 2048-row prompt 105 for its 64.9 (idle parts shift
+// the tiles); a part to a block of 8 waves, 200 requests of 500 keys beside 8 of 300 rows 101.5 us for 93.1.
 template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages_mixed_kernel(const AttendArgs a) {
   __shared__ union {
     ManyLds<HD> many;
-    FewLds<HD, 2, 8> few;
+    FewLds<HD, 2, 4> few[2];
   } lds;
   const int tiles = a.tiles * a.c.kv * a.splits;
-  if ((int)blockIdx.x < tiles) many_pairs<HD, ONE>(a, blockIdx.x, lds.many);
-  else few_pairs<HD, 2, 8, ONE>(a, blockIdx.x - tiles, lds.few);
+  if ((int)blockIdx.x < tiles) return many_pairs<HD, ONE>(a, blockIdx.x, lds.many);
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  few_pairs<HD, 2, 4, ONE>(a, 2 * (blockIdx.x - tiles) + half, threadIdx.x & 255, lds.few[half]);
 }
 
 // Joins what attention cut, a wave a pair, 4 a block: the parts of a request's keys (request, key head, pair), then the splits of
@@ -1066,7 +1074,7 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
   // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least: 100 rows of 32 heads over 8192 keys
-  // 235 us whole, 38 + 6.8 in 16 splits; 32 rows over 65536 85.6 + 4.1 in 16, 60.2 + 5.2 in 32
+  // 235 us whole, 40 + 6.8 in 16 splits; 32 rows over 65536 85.6 + 4.1 in 16, 60.2 + 5.2 in 32
   p->many_tiles = (int)((int64_t)b->rows * rep >> TILE_LOG2) + b->requests, p->splits = 1, p->split_scratch = 0;
   if (p->many) {
     const int64_t blocks = (int64_t)p->many_tiles * c->kv;
@@ -1083,7 +1091,7 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
 
 template <int HD, bool ONE> static int launch_attend(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;
-  if (p.many) pages_mixed_kernel<HD, ONE><<<tiles * p.splits + parts, 512, 0, s>>>(a);
+  if (p.many) pages_mixed_kernel<HD, ONE><<<tiles * p.splits + (parts + 1) / 2, 512, 0, s>>>(a);
   else if (p.tiles == 2) pages_few_kernel<HD, 2, 4, ONE><<<parts, 256, 0, s>>>(a);
   else if (p.waves == 8) pages_few_kernel<HD, 1, 8, ONE><<<parts, 512, 0, s>>>(a);
   else pages_few_kernel<HD, 1, 4, ONE><<<parts, 256, 0, s>>>(a);
