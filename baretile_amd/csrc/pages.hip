@@ -360,11 +360,12 @@ __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const B
   if (tid == 0) *scale_at = s;
 }
 
-// A block: one page of one head as bf16 rows. Values turn back through LDS, 4 x 4 codes a thread by byte permutes. 12.6 million
-// values (38 MB read and written): 9.6 us, 3.9 TB/s.
-template <int HD>
+// A block: one page of one head as bf16 rows. Values turn back through LDS, 4 x 4 codes a thread by byte permutes. PAGE: the
+// longest page that LDS holds. 12.6 million values of pages of 64 (38 MB read and written): 7.7 us, 4.9 TB/s, and 9.9 with LDS for
+// 256 (4 blocks a CU).
+template <int HD, int PAGE>
 __global__ void __launch_bounds__(256) read_pages_kernel(const PoolArgs c, uint16_t *out) {
-  __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (256 + 4)];
+  __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (PAGE + 4)];
   const int tid = threadIdx.x, lg = c.page_log2, page = 1 << lg, heads = 2 * c.kv;
   const int64_t unit = blockIdx.x;
   const int h = (int)(unit % heads);
@@ -824,10 +825,11 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 // placed so that the 16 lanes of a read meet distinct banks: keys' unit u of row r at u ^ (2 (r / 16) + (r / 2) % 2)
 // (heads of 64: u ^ (r / 16)), values' unit u of dim d at u ^ (d / 4) % 4.
 // The instructions beside the matrix ones bound it: a prompt of 2048 rows of 32 heads of 128 (34.4 GF) 65 us, 529 TFLOP/s; 4096
-// rows 217 us, 633 (62 and 213 in a launch without parts, as which the steps below were timed). Vector instructions run 58 % of the time and matrix ones 28 %, hardly ever together, since the waves of a
-// block keep step. Dropped: 4 waves of 64 pairs (118 us for the 62) and 4 of 32 with no halves (78); codes converted once, into
-// bf16 in LDS (63.5 and 226 us for the 62 and 213: twice the LDS traffic); scores from 8-bit products with q in two parts (no
-// faster); fences that interleave the two kinds, wave priorities and loads from LDS a tile ahead (no change).
+// rows 217 us, 633 (62 and 213 in a launch without parts, as which the steps below were timed). Vector instructions run 58 % of
+// the time and matrix ones 28 %, hardly ever together, since the waves of a block keep step. Dropped: 4 waves of 64 pairs (118
+// us for the 62) and 4 of 32 with no halves (78); codes converted once, into bf16 in LDS (63.5 and 226 us for the 62 and 213:
+// twice the LDS traffic); scores from 8-bit products with q in two parts (no faster); fences that interleave the two kinds,
+// wave priorities and loads from LDS a tile ahead (no change).
 template <int HD> struct ManyLds {
   __attribute__((aligned(16))) uint8_t k[2][2][KB * HD], v[2][2][KB * HD];  // [half][stage]
 };
@@ -1182,8 +1184,9 @@ int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out) {
   if (!out || out % 16) return fail(BT_EINVAL, "pages are read to a 16-byte aligned tensor");
   const int64_t blocks = (int64_t)c.pages * 2 * c.kv;
   if (!grid_fits(blocks, 256)) return fail(BT_EINVAL, "%d pages of %d heads are too many to read at once", c.pages, 2 * c.kv);
-  if (pool->head_dim == 64) read_pages_kernel<64><<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out);
-  else read_pages_kernel<128><<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out);
+  const auto launch = [&](auto kernel) { kernel<<<(unsigned)blocks, 256, 0, r->stream>>>(c, (uint16_t *)(uintptr_t)out); };
+  if (pool->head_dim == 64) pool->page <= 64 ? launch(read_pages_kernel<64, 64>) : launch(read_pages_kernel<64, 256>);
+  else pool->page <= 64 ? launch(read_pages_kernel<128, 64>) : launch(read_pages_kernel<128, 256>);
   BT_LAUNCHED("reading pages");
   return BT_OK;
 }
