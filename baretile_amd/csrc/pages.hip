@@ -210,16 +210,18 @@ struct Piece {
 // from the first on, a put of 2048 requests' rows 135 us, so 90; a search by halves would be a trip a step). Starts count within
 // the rows there are and lengths hold their rows, whatever they say.
 template <class F> __device__ __forceinline__ bool find_piece(const BatchArgs &b, int at, int lane, F before, Piece *p) {
-  const auto start = [&](int i) { return min(max(gload(b.starts + i), 0), b.rows); };
+  const auto held = [&](int s) { return min(max(s, 0), b.rows); };
   int base = 0;
   if (b.requests > 64) {
     const int run = (b.requests + 63) >> 6, i = min(lane * run, b.requests - 1);  // at most 32 of MOST_REQUESTS
-    const uint64_t from = __ballot(before(i, start(i)) <= at);
+    const uint64_t from = __ballot(before(i, held(gload(b.starts + i))) <= at);
     base = from ? min((63 - __builtin_clzll(from)) * run, b.requests - 1) : 0;
   }
   const int i = min(base + lane, b.requests - 1);
-  const int s0 = start(i), s1 = max(start(i + 1), s0), len = gload(b.lengths + i);
-  const int lo = before(i, s0), hi = before(i + 1, s1);
+  int f0 = gload(b.starts + i), f1 = gload(b.starts + i + 1), len = gload(b.lengths + i);
+  int lo = before(i, held(f0)), hi = before(i + 1, held(f1));
+  asm volatile("" : "+v"(f0), "+v"(f1), "+v"(len), "+v"(lo), "+v"(hi));  // all requested at once, not once the piece is found
+  const int s0 = held(f0), s1 = max(held(f1), s0);
   const uint64_t hit = __ballot(base + lane < b.requests && lo <= at && at < hi);
   if (!hit) return false;
   const int l = __builtin_ctzll(hit);
@@ -259,7 +261,7 @@ __device__ __forceinline__ float scale_of(float amax) {
 // whole words.
 // Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 190 us, 4.2 TB/s; a decode step's 32 rows are
 // latency, 5.1 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
-// by one wave (512 requests of one row 25.8 us, by four waves 48.4; of 8 rows 31.0 and 49.8), up to 64 by four waves with loads for 64
+// by one wave (512 requests of one row 25.8 us, by four waves 48.4; of 8 rows 31.0 and 49.8), up to 64 with loads for 64
 // (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
 template <int HD, int NT, int PAGE>
 __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
@@ -411,13 +413,15 @@ struct AttendArgs {
   BatchArgs b;
   const uint16_t *q;
   uint16_t *out;
-  float *scratch, *split_scratch;
+  float *scratch;
   int64_t q_sh, q_sr, o_sh, o_sr;
+  FastDiv drep;
   int32_t rep, window;
   int32_t items, few, groups;  // the most parts a plan makes, the most query pairs they are for, in groups of 32
-  int32_t tiles, splits;       // tiles of 128 pairs, and the pieces that each one's keys are cut into
-  uint32_t joins;              // the waves that join parts
-  FastDiv drep;
+  // from here on, past the three cache lines that pages_few_kernel reads (a fourth: 16 requests of 5 rows 15.2 us, so 14.7):
+  uint32_t joins;         // the waves that join parts
+  int32_t tiles, splits;  // tiles of 128 pairs, and the pieces that each one's keys are cut into
+  float *split_scratch;
 };
 
 // Rows behind the last request's are zeros: block `at` clears 16 of them, every head.
@@ -679,17 +683,14 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
     int p0 = b0 * KB >> lg;
     PageRun run = page_run(a, p.r, kvh, p0, lane);
     u32x4 kw[4][J], vw[C];
-    float ks, vs, ks_next = 0, vs_next = 0;
-    int id_v, id_v_next = 0;
     const auto turn = [&](int b) {  // the 64 pages that block b's keys lie in, if they are not there yet
       if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, run = page_run(a, p.r, kvh, p0, lane);
     };
     const uint8_t *base = a.c.values + kvh * head;
     const int run6 = min(lg, 6);
     const uint32_t krow = ((ONE ? 16 * (n >> 2) : 0) + (n & 3)) * 64 + 16 * g, vrow = (n << run6) + (ONE ? 16 * g : 0);
-    const auto fetch_keys = [&](int b, float &s) {
+    const auto fetch_keys = [&](int b) {
       const PageAt at = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * (n >> 2)), lg);
-      s = at.ks;
       const uint8_t *k = base + (int64_t)at.id * (2 * a.c.kv) * head + at.in * 64;
 #pragma unroll
       for (int j = 0; j < J; j++) {
@@ -698,23 +699,23 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
         for (int kt = 0; kt < 4; kt++) kw[kt][j] = __builtin_nontemporal_load((const u32x4 *)(kj + (krow + 4 * kt * 64)));
       }
     };
-    const auto fetch_values = [&](int b, float &s, int &valid) {
+    const auto fetch_values = [&](int b) {
       const PageAt at = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
-      valid = at.real, s = at.vs;
       const uint8_t *v = base + ((int64_t)at.id * (2 * a.c.kv) + a.c.kv) * head + value_at<HD>(0, at.in, lg);
 #pragma unroll
       for (int c = 0; c < C; c++) vw[c] = __builtin_nontemporal_load((const u32x4 *)(v + (c << (run6 + 4)) + vrow));
     };
-    fetch_keys(b0, ks);
-    fetch_values(b0, vs, id_v);
+    fetch_keys(b0), fetch_values(b0);
     for (int b = b0; b < b1; b += NW) {
       const bool more = b + NW < b1;
-      fold_block<HD, QT>(q, st, b * KB + 16 * g, id_v, ks, vs, [&](int kt, int j) { return kw[kt][j]; },
+      // the scales once the codes are requested, so that these don't wait for them
+      const PageAt ka = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * (n >> 2)), lg);
+      const PageAt va = page_at<ONE>(run, p0, b * KB + (ONE ? 0 : 16 * g), lg);
+      fold_block<HD, QT>(q, st, b * KB + 16 * g, va.real, ka.ks, va.vs, [&](int kt, int j) { return kw[kt][j]; },
                          [&](int c) { return vw[c]; }, [&] {
-                           if (more) turn(b + NW), fetch_keys(b + NW, ks_next);
+                           if (more) turn(b + NW), fetch_keys(b + NW);
                          });
-      if (more) fetch_values(b + NW, vs_next, id_v_next);
-      ks = ks_next, vs = vs_next, id_v = id_v_next;
+      if (more) fetch_values(b + NW);
     }
   }
 #pragma unroll
