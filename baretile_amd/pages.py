@@ -103,7 +103,8 @@ class Pages:
   def put(self, batch, x):
     """Puts the batch's rows into their pages (bt_pages_put): x (2 kv, rows, head) bf16, key heads then value heads, as rope_put
     gives them. Each page and head takes the smallest power of two under which its largest value is at most 448; where a
-    page that holds rows needs a larger one, those are rounded again under it. Rows without a page are dropped."""
+    page that holds rows needs a larger one, those are rounded again under it. Rows without a page are dropped. Requests may
+    share pages that they only read; a page that takes rows is one request's."""
     self._fits(batch)
     if not (isinstance(x, Tensor) and x.rt is self.rt and x.dtype == "bf16" and
             (x.batch, x.rows, x.cols) == (2 * self.kv, batch.rows, self.head)):

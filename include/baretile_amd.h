@@ -385,7 +385,8 @@ typedef struct {
 /* The batch's rows of 2 kv heads, x bf16 (element strides x_sb a head, x_sr a row), into their pages. A page's head takes the
  * smallest power of two s with every finite value at most 448 s in size; a page that holds rows keeps the larger of its own and the
  * new rows', and where that grows its rows are rounded again. Values round to nearest even; infinities and NaNs are stored as the
- * largest value of their sign. Two requests must not put rows into one page. */
+ * largest value of their sign. No page may take rows twice in one put: two requests, or two entries of one, that name the
+ * same page to put rows into give either's. */
 int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t x, int64_t x_sb, int64_t x_sr);
 /* Every page as bf16, [pages][2 kv][page][head_dim]. */
 int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out);
