@@ -357,15 +357,15 @@ typedef struct {
 } bt_pages;
 
 /* A step's plan from its requests' lengths, all int32. Request r (of `requests`, up to 2048) holds cached[r] tokens and brings
- * n = fresh[r] more (0 if negative), at most `most`, and as many as fit in the `rows` rows (up to 2^20) behind those of the
- * requests before it. Written: starts[requests + 1], each one's first row and the end of the last's; lengths[r] = cached[r] + n; for every
- * row, places[rows] (its token's place) and slots[rows] (table entry * page + place % page, where a flat cache of
- * pages * page rows would hold it), -1 behind the last request's rows, and slots also where there is no page. Table entries from
- * the first page not begun, cached / page rounded up, to the last that the new length needs are kept up to the first
- * that holds no page; the others are taken from free_pages in order, after the first taken[0] (0 without taken), -1 where these
- * run out. taken_out[0] is taken[0] plus the entries so made: past n_free, so many pages were missing. Entries past the
- * tables' width are not made. parts[requests + 2] is bt_pages_attend's, for caches of kv key heads: how it cuts the requests'
- * keys. */
+ * n = fresh[r] more (0 if negative), at most `most`, and as many as fit in the `rows` rows (up to 2^20) behind those of
+ * the requests before it. Written: starts[requests + 1], each one's first row and the end of the last's; lengths[r] =
+ * cached[r] + n; for every row, places[rows] (its token's place) and slots[rows] (table entry * page + place % page, where
+ * a flat cache of pages * page rows would hold it), -1 behind the last request's rows, and slots also where there is no
+ * page. Table entries from the first page not begun, cached / page rounded up, to the last that the new length needs are
+ * kept up to the first that holds no page; the others are taken from free_pages in order, after the first taken[0] (0
+ * without taken), -1 where these run out. taken_out[0] is taken[0] plus the entries so made: past n_free, so many pages
+ * were missing. Entries past the tables' width are not made. parts[requests + 2] is bt_pages_attend's, for caches of kv
+ * key heads: how it cuts the requests' keys. */
 typedef struct {
   uint64_t tables, cached, fresh, free_pages, taken;
   uint64_t starts, lengths, places, slots, taken_out, parts;
@@ -391,10 +391,10 @@ int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, ui
 /* Every page as bf16, [pages][2 kv][page][head_dim]. */
 int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out);
 /* out[e, j, :] = softmax(q[e, j, :] . k + mask) @ v for the batch's rows j and heads e, over the pages of j's request and
- * key head e / (heads / kv): keys at places up to j's own and, with window > 0, after its place - window. bf16 with element strides;
- * scores, maxima and sums in fp32, the weights rounded to bf16 before they meet v; no scale is applied. Rows behind the last
- * request's are zeros, and so is a row that sees no key. bt_pages_attend_scratch gives the bytes of scratch (16-byte aligned);
- * calls that share one scratch buffer must not overlap. */
+ * key head e / (heads / kv): keys at places up to j's own and, with window > 0, after its place - window. bf16 with
+ * element strides; scores, maxima and sums in fp32, the weights rounded to bf16 before they meet v; no scale is applied.
+ * Rows behind the last request's are zeros, and so is a row that sees no key. bt_pages_attend_scratch gives the bytes of
+ * scratch (16-byte aligned); calls that share one scratch buffer must not overlap. */
 int bt_pages_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t heads, int32_t window, uint64_t *bytes);
 int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr,
                     uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,
@@ -410,15 +410,15 @@ int bt_topk(bt_runtime *rt, int dtype, uint64_t x, int64_t batch, int64_t rows, 
 
 /* ---- drafted tokens verified: no counterpart in the reference's greedy heads (serve.py:43-63) --------------------------
  *
- * Rows starts[r] .. starts[r + 1] - 1 (int32, requests + 1) are request r's: its last token, then its drafts, ids[rows] the
- * tokens fed there. logits (fp32 rows of vocab, row stride in elements) are the target's after each row, t (0: all 1) each
- * row's inverse temperature (below 0 or NaN: 0; infinite: the first largest alone), p_j = softmax(t_j logits_j); probs (0:
- * drafts were certain) the distributions that the drafts were drawn from, row j's that of ids[j]. uniforms are two rows of
- * numbers in [0, 1). Draft ids[j] is accepted where uniforms[0, j] * probs[j, ids[j]] < p_{j-1}(ids[j]). tokens[rows], the token after
- * each row: the accepted drafts up to the first refused, then one drawn from max(p - probs, 0) at the refusal or from p
- * after the last, the first whose running sum passes uniforms[1, j] times the whole; -1 behind it and behind the last
- * request. counts[requests]: each one's new tokens. A logit of NaN counts as -inf; a row of nothing else accepts
- * and draws nothing. All in 64 bits. */
+ * Rows starts[r] .. starts[r + 1] - 1 (int32, requests + 1) are request r's: its last token, then its drafts, ids[rows]
+ * the tokens fed there. logits (fp32 rows of vocab, row stride in elements) are the target's after each row, t (0: all 1)
+ * each row's inverse temperature (below 0 or NaN: 0; infinite: the first largest alone), p_j = softmax(t_j logits_j);
+ * probs (0: drafts were certain) the distributions that the drafts were drawn from, row j's that of ids[j]. uniforms are
+ * two rows of numbers in [0, 1). Draft ids[j] is accepted where uniforms[0, j] * probs[j, ids[j]] < p_{j-1}(ids[j]).
+ * tokens[rows], the token after each row: the accepted drafts up to the first refused, then one drawn from max(p - probs,
+ * 0) at the refusal or from p after the last, the first whose running sum passes uniforms[1, j] times the whole; -1 behind
+ * it and behind the last request. counts[requests]: each one's new tokens. A logit of NaN counts as -inf; a row of nothing
+ * else accepts and draws nothing. All in 64 bits. */
 typedef struct {
   uint64_t logits, probs, t, uniforms, ids, starts, tokens, counts, scratch, scratch_bytes;
   int64_t logits_sr, probs_sr, t_sr, uniforms_sr;
