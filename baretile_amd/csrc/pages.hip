@@ -259,8 +259,8 @@ __device__ __forceinline__ float scale_of(float amax) {
 // 16 bytes a thread, all at once and before the page's id is there), their largest finite size gives the scale, and a page that
 // already holds rows and whose scale grows has them rounded again. Values turn by dimension in LDS, so they are stored as
 // whole words.
-// Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 190 us, 4.2 TB/s; a decode step's 32 rows are
-// latency, 5.1 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
+// Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 181 us, 4.4 TB/s; a decode step's 32 rows are
+// latency, 5.3 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
 // by one wave (512 requests of one row 25.8 us, by four waves 48.4; of 8 rows 31.0 and 49.8), up to 64 with loads for 64
 // (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
 template <int HD, int NT, int PAGE>
@@ -285,7 +285,8 @@ __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const B
 #pragma unroll
   for (int i = 0; i < MOST; i++) {
     const int e = tid + NT * i;
-    if (NT * i < units) v[i] = e < units ? gload((const u32x4 *)(src + e / U * x_sr + e % U * 8)) : u32x4{0, 0, 0, 0};
+    // (past the last row it is read again, so that no load waits behind a lane's branch)
+    if (NT * i < units) v[i] = gload((const u32x4 *)(src + min(e / U, count - 1) * x_sr + e % U * 8));
   }
   if ((uint32_t)id >= (uint32_t)c.pages) return;
   float *scale_at = c.scales + (int64_t)id * heads + h;
