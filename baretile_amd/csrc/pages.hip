@@ -830,8 +830,9 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 // rows 217 us, 633 (62 and 213 in a launch without parts, as which the steps below were timed). Vector instructions run 58 % of
 // the time and matrix ones 28 %, hardly ever together, since the waves of a block keep step. Dropped: 4 waves of 64 pairs (118
 // us for the 62) and 4 of 32 with no halves (78); codes converted once, into bf16 in LDS (63.5 and 226 us for the 62 and 213:
-// twice the LDS traffic); scores from 8-bit products with q in two parts (no faster); fences that interleave the two kinds,
-// wave priorities and loads from LDS a tile ahead (no change).
+// twice the LDS traffic); scores from 8-bit products with q in two parts (no faster); the halves half a step apart, one at its
+// products while the other weighs (68.5 us for the 65), with a barrier between the two as well (72); fences that interleave
+// the two kinds, wave priorities and loads from LDS a tile ahead (no change).
 template <int HD> struct ManyLds {
   __attribute__((aligned(16))) uint8_t k[2][2][KB * HD], v[2][2][KB * HD];  // [half][stage]
 };
