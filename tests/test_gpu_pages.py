@@ -445,6 +445,93 @@ def test_a_recorded_step_follows_its_lengths(rt):
     want_cached = total
 
 
+def test_a_jit_step_takes_its_tables_and_rows(rt):
+  # plan, put and attention under jit: its inputs are copied in, and the tables that the plan fills come back
+  rng = np.random.default_rng(14)
+  pool = Pages(rt, 12, 2, 64, 16)
+  free = rng.permutation(12)
+  fr = row(rt, free)
+  def step(tables, cached, new, taken, x, q):
+    b = pool.plan(tables, cached, new, fr, 30, taken)
+    pool.put(b, x)
+    return pool.attend(q, b)
+  f = jit(step)
+  values, s = np.zeros((12, 4, 16, 64)), np.full((12, 4), 2.0 ** -100)
+  tables, want_tables, cached, used = Tensor.of(rt, np.full((2, 6), -1), "int32"), np.full((2, 6), -1), np.zeros(2, int), 0
+  for new in ([20, 3], [1, 4], [0, 12], [5, 1]):
+    x, q = bf16_rows(rng, 4, 30, 64), B.bf16(rng.normal(0, 0.2, (8, 30, 64)))
+    got = np.array(f(tables, row(rt, cached), row(rt, new), row(rt, [used]), Tensor.of(rt, x), Tensor.of(rt, q)).tolist())
+    want_tables, starts, total, _, _, used = P.plan(want_tables, cached, new, free, 30, 16, 12, used)
+    P.put(values, s, want_tables, starts, total, x)
+    want, weighed = P.attend(q, values, want_tables, starts, total)
+    assert np.array_equal(np.array(tables.tolist()), want_tables) and np.array_equal(whole(pool), values)
+    assert np.all(np.abs(got - want) <= bound(q, values, weighed, want))
+    cached = total
+
+
+def test_tables_and_rows_that_are_views(rt):
+  rng = np.random.default_rng(15)
+  pool = Pages(rt, 20, 2, 64, 16)
+  all_tables = np.full((5, 9), 7)
+  all_tables[1:4, 2:8] = -1
+  t = Tensor.of(rt, all_tables, "int32")
+  lengths, rows = [40, 0, 17], 60
+  wide = Tensor.of(rt, np.stack([np.arange(20), rng.permutation(20)]), "int32")
+  free = np.array(wide.tolist(), int)[1]
+  x, q = bf16_rows(rng, 4, 2 * rows, 64), B.bf16(rng.normal(0, 0.2, (8, 2 * rows, 64)))
+  b = pool.plan(t[1:4, 2:8], row(rt, [0, 0, 0]), row(rt, [9, *lengths, 9])[:, 1:4], wide[1:2, :], rows)
+  want_tables, starts, total, *_ = P.plan(all_tables[1:4, 2:8], [0, 0, 0], lengths, free, rows, 16, 20)
+  all_tables[1:4, 2:8] = want_tables
+  assert np.array_equal(np.array(t.tolist()), all_tables)
+  pool.put(b, Tensor.of(rt, x)[:, rows // 2:rows // 2 + rows, :])
+  values, s = np.zeros((20, 4, 16, 64)), np.full((20, 4), 2.0 ** -100)
+  P.put(values, s, want_tables, starts, total, x[:, rows // 2:rows // 2 + rows])
+  assert np.array_equal(whole(pool), values)
+  q = q[:, 5:5 + rows]
+  got = np.array(pool.attend(Tensor.of(rt, np.concatenate([q[:, :3], q], 1))[:, 3:, :], b).tolist())
+  want, weighed = P.attend(q, values, want_tables, starts, total)
+  assert np.all(np.abs(got - want) <= bound(q, values, weighed, want))
+
+
+def test_pages_past_32_bits(rt):
+  # the last pages of a pool of 5 GB hold what the first of a small one do, bit for bit
+  rng = np.random.default_rng(16)
+  kv, hd, page, n = 2, 128, 256, 40000
+  lengths = [700, 300]
+  x, q = Tensor.of(rt, bf16_rows(rng, 2 * kv, 1000, hd)), Tensor.of(rt, B.bf16(rng.normal(0, 0.2, (8, 1000, hd))))
+  outs = []
+  for pages in (5, n):
+    pool = Pages(rt, pages, kv, hd, page)
+    b = pool.plan(Tensor.of(rt, np.full((2, 3), -1), "int32"), row(rt, [0, 0]), row(rt, lengths), row(rt, range(pages - 5, pages)), 1000)
+    pool.put(b, x)
+    step = pool.plan(b.tables, row(rt, [699, 298]), row(rt, [1, 2]), row(rt, [-1]), 3)
+    outs.append([pool.attend(q, b).tobytes(), pool.attend(q[:, :3, :], step).tobytes(),
+                 pool.values()[(pages - 5) * 2 * kv:, :, :].contiguous().tobytes()])
+    del pool, b, step
+  assert outs[0] == outs[1]
+
+
+def test_a_long_cache(rt):
+  # 300000 tokens, over 1172 pages that 19 loads of a wave's page table bring in
+  attended(rt, np.random.default_rng(17), 4, 1, 64, 256, [300000, 5], [1, 1], most=1)
+  attended(rt, np.random.default_rng(18), 4, 1, 64, 256, [300000, 5], [2, 1], window=100000)
+
+
+def test_a_closed_runtime(chip):
+  from baretile_amd.runtime import Runtime
+  first = Runtime(chip)
+  pool = Pages(first, 4, 2, 64, 16)
+  b = pool.plan(Tensor.of(first, [[-1]], "int32"), row(first, [0]), row(first, [1]), row(first, [0]), 1)
+  x, q = Tensor.zeros(first, 1, 64, 4), Tensor.zeros(first, 1, 64, 4)
+  second = Runtime(chip)
+  try:
+    for f in (lambda: pool.put(b, x), lambda: pool.attend(q, b), pool.values, lambda: Pages(first, 4, 2, 64, 16)):
+      with pytest.raises(RuntimeError): f()
+    other = Pages(second, 4, 2, 64, 16)
+    with pytest.raises(ValueError, match="batch must be planned"): other.put(b, Tensor.zeros(second, 1, 64, 4))
+  finally: second.close()
+
+
 def numpy_step(L, ids, w, c, caches, scales, plan, places):
   """Logits of every row as paged_forward gives them, over NumPy pages (caches, scales: one of each a block)."""
   tables, starts, lengths = plan
@@ -489,6 +576,8 @@ def test_paged_llama_matches_numpy(rt, page, spare):
     tokens, counts = serve.verify(logits.reshape(rows, 256), row(rt, ids), b.starts, Tensor.of(rt, u, "fp32"))
     vt, vc = P.verify(np.array(logits.tolist(), np.float32).reshape(rows, -1), ids, starts, u)
     assert np.array_equal(ints(tokens), vt) and np.array_equal(ints(counts), vc)
+    again, _ = serve.verify(llama.paged_forward(row(rt, ids), b, dw, dc, caches), row(rt, ids), b.starts, Tensor.of(rt, u, "fp32"))
+    assert np.array_equal(ints(again), vt)  # the step again, its rows put over themselves, its logits taken as they come
     cached = cached + kept
   with pytest.raises(ValueError, match="paged_forward"): llama.paged_forward(row(rt, [1]), b, dw, dc, caches)
   with pytest.raises(ValueError, match="paged_forward"): llama.paged_forward(row(rt, [1] * rows), b, dw, dc, caches[:1])
