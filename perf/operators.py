@@ -389,8 +389,9 @@ def _prepare_own(s):
   pools = [Pages(rt, s["pages"], case["kv"], case["head"], page) for _ in s["old"]]
   table = _tensor(torch.full_like(s["base"], -1).to(torch.int32))
   filled = int(s["filled"].sum())
-  first = pools[0].plan(table, row(torch.zeros_like(s["cached"])), row(s["filled"]), free, filled)
-  for pool, x in zip(pools, s["old"]): pool.put(first, _tensor(x))
+  if filled:  # (a plan takes a row at least)
+    first = pools[0].plan(table, row(torch.zeros_like(s["cached"])), row(s["filled"]), free, filled)
+    for pool, x in zip(pools, s["old"]): pool.put(first, _tensor(x))
   batch = pools[0].plan(table, cached, new, free, rows, taken=taken, most=case["new"])
   if kind == "put":
     x = _tensor(s["x"])
