@@ -419,8 +419,9 @@ struct AttendArgs {
   FastDiv drep;
   int32_t rep, window;
   int32_t items, few, groups;  // the most parts a plan makes, the most query pairs they are for, in groups of 32
+  int32_t least;               // a part's least blocks of keys, beside the plan's
   // from here on, past the three cache lines that pages_few_kernel reads (a fourth: 16 requests of 5 rows 15.2 us, so 14.7):
-  uint32_t joins;         // the waves that join parts
+  uint32_t joins;         // waves that join parts
   int32_t tiles, splits;  // tiles of 128 pairs, and the pieces that each one's keys are cut into
   float *split_scratch;
 };
@@ -665,9 +666,9 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
   if (group >= a.groups) clear_rows<HD>(a, block - a.groups * units, tid, 64 * NW);
   else if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p) || p.n * a.rep > a.few) p.n = 0;
   const int pairs = p.n * a.rep;
-  const bool real = pair0 < pairs;
   const int room = min(p.len, a.b.width << lg), nb = (room + KB - 1) / KB;
-  const int mine = max(per, (nb + MOST_PARTS - 1) / MOST_PARTS), parts = (nb + mine - 1) / mine;
+  const int mine = max(max(per, a.least), (nb + MOST_PARTS - 1) / MOST_PARTS), parts = (nb + mine - 1) / mine;
+  const bool real = pair0 < pairs && p.k < parts;
   int b0 = p.k * mine;
   const int b1 = real ? min(b0 + mine, nb) : 0;
   if (a.window > 0) b0 = max(b0, max(p.len - p.n - a.window + 1, 0) / KB);
@@ -1054,6 +1055,7 @@ struct AttendPlan {
   int waves;             // of a part's block
   int many_tiles, splits;  // tiles of 128 pairs, and the pieces that each one's keys are cut into
   bool many, join;
+  int least;
   int64_t joins;  // waves that join parts
   uint64_t scratch, split_scratch;
 };
@@ -1071,19 +1073,24 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   p->tiles = p->few <= 16 ? 1 : 2;
   p->groups = (p->few + 31) / 32;
   p->items = parts_target(c->kv) + b->requests;
-  const int64_t keys = (int64_t)b->width * c->page;
-  p->join = keys > SHORT;
+  // keys: what a request's rows see between them. Where a window leaves few of a long table's, one part has them: 32 requests
+  // of 8192 keys in a window of 128 6.8 us and a launch less, in the plan's parts 6.7 + 3.5; of 1000 17.8, 18.8 + 4.0
+  const int64_t held = (int64_t)b->width * c->page, keys = window ? std::min<int64_t>(held, (int64_t)window + b->most) : held;
+  p->join = keys > SHORT, p->least = !p->join ? MOST_KEYS / KB : 1;
   // a block of 8 waves where a part a request leaves most CUs idle: one request of 3 heads of 64 and 1000 keys 6.4 us, with 4 waves
   // 6.8; 512 of 8 heads and 500 keys 121.4 and 88.7
   p->waves = p->many || (p->tiles == 1 && !p->join && (int64_t)b->requests * c->kv < 64) ? 8 : 4;
   const uint64_t bytes = (uint64_t)p->items * c->kv * p->few * (c->head_dim + 4) * 4;
   p->scratch = p->join ? bytes : 0;
-  // tiles that leave CUs idle have their keys cut, while a cut keeps 8 blocks of keys at least: 100 rows of 32 heads over 8192 keys
-  // 235 us whole, 40 + 6.8 in 16 splits; 32 rows over 65536 85.6 + 4.1 in 16, 60.2 + 5.2 in 32
+  // tiles that leave CUs idle (of 256, a block each at a time) have their keys cut, while a cut keeps 8 blocks of keys at least:
+  // 100 rows of 32 heads over 8192 keys 235 us whole, 32.4 + 5.0 in 8 splits, 38.5 + 7.1 in 16; 512 rows 161 whole, 95 + 11.7 in
+  // 2 and 119.5 + 12.0 in 3; 32 rows over 65536 86.1 + 4.0 in 16, 62.8 + 5.7 in 32, 72.6 + 7.6 in 48. A request's last tile
+  // counts by half, but for the first's.
   p->many_tiles = (int)((int64_t)b->rows * rep >> TILE_LOG2) + b->requests, p->splits = 1, p->split_scratch = 0;
   if (p->many) {
     const int64_t blocks = (int64_t)p->many_tiles * c->kv;
-    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({512 / blocks, keys / (8 * KB), 64}));
+    const int64_t full = (ceil_div((int64_t)b->rows * rep, TILE) + (b->requests - 1) / 2) * c->kv;
+    p->splits = (int)std::max<int64_t>(1, std::min<int64_t>({256 / full, keys / (8 * KB), 64}));
     if (p->splits > 1) p->split_scratch = (uint64_t)blocks * p->splits * TILE * (c->head_dim + 4) * 4;
   }
   p->joins = p->join ? (int64_t)b->requests * c->kv * p->few : 0;
@@ -1219,7 +1226,7 @@ int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch,
   a.q = (const uint16_t *)(uintptr_t)q, a.out = (uint16_t *)(uintptr_t)out, a.scratch = (float *)(uintptr_t)scratch;
   a.split_scratch = (float *)(uintptr_t)(scratch + p.scratch), a.splits = p.splits;
   a.q_sh = q_sh, a.q_sr = q_sr, a.o_sh = o_sh, a.o_sr = o_sr;
-  a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few, a.groups = p.groups;
+  a.rep = heads / a.c.kv, a.window = window, a.items = p.items, a.few = p.few, a.groups = p.groups, a.least = p.least;
   a.tiles = p.many_tiles, a.joins = (uint32_t)p.joins;
   a.drep = make_fastdiv((uint32_t)a.rep);
   const bool one = pool->page >= KB;

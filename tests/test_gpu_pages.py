@@ -216,6 +216,13 @@ def test_attend_window(rt, window, lengths, new):
   attended(rt, np.random.default_rng(window), 8, 2, 64, 16, lengths, new, window)
 
 
+@pytest.mark.parametrize("window", [1, 40, 1000, 1019, 1020, 1100])
+@pytest.mark.parametrize("new", [[1, 1, 5], [4, 0, 1], [3, 1, 70]])
+def test_attend_window_over_long_tables(rt, window, new):
+  # windows that leave a part's keys of tables that hold many more, and one key too many for that
+  attended(rt, np.random.default_rng(window), 8, 2, 64, 32, [5000, 90, 2001], new, window, most=max(new))
+
+
 @pytest.mark.parametrize("new", [[1, 3, 1], [90, 80, 1]])
 def test_attend_hides_pages_that_are_none(rt, new):
   def holes(t):
