@@ -24,10 +24,10 @@ struct ChunkStat {
   float m;
   int32_t at;
 };
-// Where a request draws: after `accepted` drafts, from `row`, with the row's maximum and sum.
+// Where a request draws: after `accepted` drafts, from `row`, with the row's maximum and sum and its number in [0, 1).
 struct Draw {
   double z, t2;
-  float m;
+  float m, u;
   int32_t accepted, row, refused, without, token;  // without: the token that a certain draft takes out, or -1; token:
 };                                                 // where there is nothing to draw, the one to take (-1: none)
 struct VerifyArgs {
@@ -189,13 +189,13 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
 // A row's maximum, its first place (greedy rows) and its sum, by a wave from the row's chunks.
 struct RowStat {
   double z;
-  float m;
+  float m, t;
   int at;
 };
 __device__ __forceinline__ RowStat row_stat(const VerifyArgs &a, int row, float t, int lane) {
   const ChunkStat *stats = a.stats + (int64_t)row * a.chunks;
   constexpr int G = 4;  // chunks a lane loads at once: all of up to 256
-  RowStat r{0.0, NONE, NOWHERE};
+  RowStat r{0.0, NONE, t, NOWHERE};
   ChunkStat s[G];
 #pragma unroll
   for (int i = 0; i < G; i++) {
@@ -274,8 +274,9 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
   __syncthreads();
   Draw f;
   f.accepted = refusal - 1, f.row = start + f.accepted, f.refused = refusal < n;
-  const float t = inverse(a, f.row);
-  const RowStat s = refusal <= KEPT ? kept[refusal - 1] : row_stat(a, f.row, t, lane);
+  const RowStat s = refusal <= KEPT ? kept[refusal - 1] : row_stat(a, f.row, inverse(a, f.row), lane);
+  const float t = s.t;
+  f.u = c == 0 ? gload(a.uniforms + a.uniforms_sr + f.row) : 0.0f;
   f.z = s.z, f.m = s.m, f.t2 = in_log2(t), f.without = f.refused && !a.probs ? gload(a.ids + f.row + 1) : -1;
   const bool known = s.m == NONE || greedy(t);
   f.token = s.m == NONE ? -1 : greedy(t) ? s.at : NOWHERE;
@@ -302,39 +303,49 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
     for (int j = max(0, gload(a.starts + a.requests)) + lane; j < a.rows; j += 64) a.tokens[j] = -1;
     return;
   }
+  constexpr int KEEP = 4;  // sums a lane keeps: of up to 256 chunks all
+  const double *left = a.left + (int64_t)r * a.chunks;
+  const int each = (a.chunks + 63) / 64, c0 = lane * each, c1 = min(c0 + each, a.chunks);  // the lane's chunks
+  Draw f = a.draws[r];
+  double kept[KEEP];
+#pragma unroll
+  for (int i = 0; i < KEEP; i++) kept[i] = gload(left + min(c0 + i, a.chunks - 1));  // requested with the rest, used or not
   int n;
   const int start = request_rows(a, r, &n);
   if (n == 0) {
     if (lane == 0) a.counts[r] = 0;
     return;
   }
-  Draw f = a.draws[r];
   if (f.token == NOWHERE) {
-    const double *left = a.left + (int64_t)r * a.chunks;
-    const float u = gload(a.uniforms + a.uniforms_sr + f.row);
-    const int each = (a.chunks + 63) / 64, c0 = lane * each, c1 = min(c0 + each, a.chunks);  // the lane's chunks
+    const float u = f.u;
+    const auto each_of = [&](auto value, auto step) {  // step(c, value(c, its kept sum)) for the lane's chunks in order
+#pragma unroll
+      for (int i = 0; i < KEEP; i++)
+        if (c0 + i < c1) step(c0 + i, value(c0 + i, kept[i]));
+      for (int c = c0 + KEEP; c < c1; c++) step(c, value(c, gload(left + c)));
+    };
     double s = 0.0;
-#pragma unroll 4
-    for (int c = c0; c < c1; c++) s += gload(left + c);
+    const auto as_left = [](int, double l) { return l; };
+    each_of(as_left, [&](int, double l) { s += l; });
     double all = wave_sum64(s);
     const bool none = !(all > 0.0);  // p nowhere over q, yet a draft refused (by rounding): all of p is drawn from
     const ChunkStat *stats = a.stats + (int64_t)f.row * a.chunks;
-    const auto chunk = [&](int c) { return none ? stats[c].s * weight(stats[c].m, f.m, f.t2) : gload(left + c); };
+    const auto as_weighed = [&](int c, double) { return stats[c].s * weight(stats[c].m, f.m, f.t2); };
     if (none) {
       f.refused = 0, f.without = -1, s = 0.0;
-      for (int c = c0; c < c1; c++) s += chunk(c);
+      each_of(as_weighed, [&](int, double l) { s += l; });
       all = wave_sum64(s);
     }
     double goal = (double)u * all, upto = wave_before(s), from = 0.0;
     // the first chunk whose running sum passes the goal; by rounding none may, then the last with any weight
     int pick = NOWHERE, last = -1;
-#pragma unroll 4
-    for (int c = c0; c < c1; c++) {
-      const double l = chunk(c);
+    const auto look = [&](int c, double l) {
       if (l > 0.0) last = c;
       if (pick == NOWHERE && l > 0.0 && upto + l > goal) pick = c, from = upto;
       upto += l;
-    }
+    };
+    if (none) each_of(as_weighed, look);
+    else each_of(as_left, look);
     uint64_t who = __ballot(pick != NOWHERE);
     if (who) {
       const int l = __builtin_ctzll(who);
@@ -378,7 +389,7 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
 
 // Logits a lane of a chunk's 64: 8 up to 2^22 logits, where larger chunks would leave waves too few to fill the card (5 rows of
 // 49152 12.3 us), else 16, which spreads a chunk's maximum and sums over more of them (112 rows of 131072 in 32 requests: the three
-// launches 13.1, 8.5 and 5.9 us; with 32 a lane, whose draw is one wave's long run, 14.4, 10.4 and 9.3).
+// launches 13.1, 8.5 and 5.6 us; with 32 a lane, whose draw is one wave's long run, 14.4, 10.4 and 9.3).
 static int verify_per(const bt_verify_args *a) { return (int64_t)a->rows * a->vocab <= 1 << 22 ? 8 : 16; }
 static int verify_chunks(const bt_verify_args *a) { return ceil_div(a->vocab, 64 * verify_per(a)); }
 static int check_verify(const bt_verify_args *a) {
