@@ -985,9 +985,13 @@ __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
   if (unit < a.joins) {
     const uint32_t heads = unit / a.few;
     const int pair = unit - heads * a.few, r = heads / a.c.kv, kvh = heads - r * a.c.kv;
-    p = Piece{r, 0, min(max(gload(a.b.starts + r), 0), a.b.rows), 0, 0};
-    p.n = min(gload(a.b.starts + r + 1), a.b.rows) - p.row0;
-    const int first = gload(a.b.parts + r), parts = gload(a.b.parts + r + 1) - first;
+    int f0 = gload(a.b.starts + r), f1 = gload(a.b.starts + r + 1);
+    int first = gload(a.b.parts + r), last = gload(a.b.parts + r + 1);
+    asm volatile("" : "+v"(f0), "+v"(f1), "+v"(first), "+v"(last));  // all requested at once
+    first = __builtin_amdgcn_readfirstlane(first);
+    const int parts = __builtin_amdgcn_readfirstlane(last) - first;
+    p = Piece{r, 0, __builtin_amdgcn_readfirstlane(min(max(f0, 0), a.b.rows)), 0, 0};
+    p.n = __builtin_amdgcn_readfirstlane(min(f1, a.b.rows)) - p.row0;
     if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
     const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
     const float *from = a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4);
