@@ -223,6 +223,13 @@ def test_attend_window_over_long_tables(rt, window, new):
   attended(rt, np.random.default_rng(window), 8, 2, 64, 32, [5000, 90, 2001], new, window, most=max(new))
 
 
+@pytest.mark.parametrize("hd, page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("lengths, window", [([1024, 3], 0), ([5000, 300], 954), ([5000, 300], 955)])
+def test_attend_prompts_keys_in_splits_and_one_part(rt, hd, page, lengths, window):
+  # 1024 keys to see: a prompt's are cut in two, and joined, while the other request's are one part; of one more both join
+  attended(rt, np.random.default_rng(hd + window), 4, 2, hd, page, lengths, [70, 3], window, most=70)
+
+
 @pytest.mark.parametrize("new", [[1, 3, 1], [90, 80, 1]])
 def test_attend_hides_pages_that_are_none(rt, new):
   def holes(t):
