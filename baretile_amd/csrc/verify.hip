@@ -24,12 +24,12 @@ struct ChunkStat {
   float m;
   int32_t at;
 };
-// Where a request draws: after `accepted` drafts, from `row`, with the row's maximum and sum and its number in [0, 1).
+// Where a request draws: after `accepted` drafts, from that row, with its maximum and sum and its number in [0, 1).
 struct Draw {
   double z, t2;
   float m, u;
-  int32_t accepted, row, refused, without, token;  // without: the token that a certain draft takes out, or -1; token:
-};                                                 // where there is nothing to draw, the one to take (-1: none)
+  int32_t accepted, refused, without, token;  // without: the token that a certain draft takes out, or -1; token: where there
+};                                            // is nothing to draw, the one to take (-1: none)
 struct VerifyArgs {
   const float *logits, *probs, *t, *uniforms;
   const int32_t *ids, *starts;
@@ -221,12 +221,12 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs &a, int row, float 
 
 // What chunk c's tokens may still be drawn with, times z: p, or where a draft was refused what p has over q.
 template <int PER, bool WIDE>
-__device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int c, int lane, double (&out)[PER]) {
+__device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int row, int c, int lane, double (&out)[PER]) {
   float x[PER], q[PER];
   const int v0 = c * 64 * PER;
   const bool drawn = f.refused && a.probs;
-  Chunk<PER, WIDE>::load(x, a.logits + f.row * a.logits_sr, v0, a.vocab, lane, NONE);
-  if (drawn) Chunk<PER, WIDE>::load(q, a.probs + (f.row + 1) * a.probs_sr, v0, a.vocab, lane, 0.0f);
+  Chunk<PER, WIDE>::load(x, a.logits + row * a.logits_sr, v0, a.vocab, lane, NONE);
+  if (drawn) Chunk<PER, WIDE>::load(q, a.probs + (row + 1) * a.probs_sr, v0, a.vocab, lane, 0.0f);
 #pragma unroll
   for (int i = 0; i < PER; i++) {
     const double p = weight(logit(x[i]), f.m, f.t2);
@@ -273,11 +273,12 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
   }
   __syncthreads();
   Draw f;
-  f.accepted = refusal - 1, f.row = start + f.accepted, f.refused = refusal < n;
-  const RowStat s = refusal <= KEPT ? kept[refusal - 1] : row_stat(a, f.row, inverse(a, f.row), lane);
+  f.accepted = refusal - 1, f.refused = refusal < n;
+  const int from = start + f.accepted;
+  const RowStat s = refusal <= KEPT ? kept[refusal - 1] : row_stat(a, from, inverse(a, from), lane);
   const float t = s.t;
-  f.u = c == 0 ? gload(a.uniforms + a.uniforms_sr + f.row) : 0.0f;
-  f.z = s.z, f.m = s.m, f.t2 = in_log2(t), f.without = f.refused && !a.probs ? gload(a.ids + f.row + 1) : -1;
+  f.u = c == 0 ? gload(a.uniforms + a.uniforms_sr + from) : 0.0f;
+  f.z = s.z, f.m = s.m, f.t2 = in_log2(t), f.without = f.refused && !a.probs ? gload(a.ids + from + 1) : -1;
   const bool known = s.m == NONE || greedy(t);
   f.token = s.m == NONE ? -1 : greedy(t) ? s.at : NOWHERE;
   if (c == 0 && lane == 0) a.draws[r] = f;
@@ -285,12 +286,12 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
   double sum = 0.0;
   if ((f.refused && a.probs) || (f.without >= 0 && f.without / (64 * PER) == c)) {
     double v[PER];
-    left_of<PER, WIDE>(a, f, c, lane, v);
+    left_of<PER, WIDE>(a, f, from, c, lane, v);
 #pragma unroll
     for (int i = 0; i < PER; i++) sum += v[i];
     sum = wave_sum64(sum);
   } else {  // p's share of the chunk is known
-    const ChunkStat k = a.stats[(int64_t)f.row * a.chunks + c];
+    const ChunkStat k = a.stats[(int64_t)from * a.chunks + c];
     sum = k.s * weight(k.m, f.m, f.t2);
   }
   if (lane == 0) a.left[(int64_t)r * a.chunks + c] = sum;
@@ -317,7 +318,7 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
     return;
   }
   if (f.token == NOWHERE) {
-    const float u = f.u;
+    const int row = start + f.accepted;
     const auto each_of = [&](auto value, auto step) {  // step(c, value(c, its kept sum)) for the lane's chunks in order
 #pragma unroll
       for (int i = 0; i < KEEP; i++)
@@ -329,14 +330,14 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
     each_of(as_left, [&](int, double l) { s += l; });
     double all = wave_sum64(s);
     const bool none = !(all > 0.0);  // p nowhere over q, yet a draft refused (by rounding): all of p is drawn from
-    const ChunkStat *stats = a.stats + (int64_t)f.row * a.chunks;
+    const ChunkStat *stats = a.stats + (int64_t)row * a.chunks;
     const auto as_weighed = [&](int c, double) { return stats[c].s * weight(stats[c].m, f.m, f.t2); };
     if (none) {
       f.refused = 0, f.without = -1, s = 0.0;
       each_of(as_weighed, [&](int, double l) { s += l; });
       all = wave_sum64(s);
     }
-    double goal = (double)u * all, upto = wave_before(s), from = 0.0;
+    double goal = (double)f.u * all, upto = wave_before(s), from = 0.0;
     // the first chunk whose running sum passes the goal; by rounding none may, then the last with any weight
     int pick = NOWHERE, last = -1;
     const auto look = [&](int c, double l) {
@@ -358,7 +359,7 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
     // the chunk's tokens in order: RUN in a row a lane, 64 RUN a turn
     constexpr int RUN = WIDE ? 4 : 1, TURNS = PER / RUN;
     double v[PER], before[TURNS], carry = 0.0;
-    left_of<PER, WIDE>(a, f, pick, lane, v);
+    left_of<PER, WIDE>(a, f, row, pick, lane, v);
 #pragma unroll
     for (int i = 0; i < TURNS; i++) {
       double mine = 0.0;
