@@ -233,6 +233,16 @@ template <class F> __device__ __forceinline__ bool find_piece(const BatchArgs &b
   return true;
 }
 
+// Request r whole, as one piece.
+__device__ __forceinline__ Piece whole_piece(const BatchArgs &b, int r) {
+  int f0 = gload(b.starts + r), f1 = gload(b.starts + r + 1), len = gload(b.lengths + r);
+  asm volatile("" : "+v"(f0), "+v"(f1), "+v"(len));  // all requested at once
+  Piece p{r, 0, __builtin_amdgcn_readfirstlane(min(max(f0, 0), b.rows)), 0, 0};
+  p.n = max(__builtin_amdgcn_readfirstlane(min(f1, b.rows)) - p.row0, 0);
+  p.len = max(__builtin_amdgcn_readfirstlane(len), p.n);
+  return p;
+}
+
 // Two codes of x0, x1 in the low half: nearest even, at most 448 in size (a NaN, which no code stands for in a cache, 448).
 __device__ __forceinline__ uint32_t codes_of(float x0, float x1) {
   x0 = __builtin_copysignf(fminf(fabsf(x0), 448.0f), x0), x1 = __builtin_copysignf(fminf(fabsf(x1), 448.0f), x1);
@@ -418,8 +428,8 @@ struct AttendArgs {
   int64_t q_sh, q_sr, o_sh, o_sr;
   FastDiv drep;
   int32_t rep, window;
-  int32_t items, few, groups;  // the most parts a plan makes, the most query pairs they are for, in groups of 32
-  int32_t least;               // a part's least blocks of keys, beside the plan's
+  int32_t items, few, groups;  // the most parts there are, the most query pairs they are for, in groups of 32
+  int32_t least;               // a part's least blocks of keys, beside the plan's; over 1: a part a request
   // from here on, past the three cache lines that pages_few_kernel reads (a fourth: 16 requests of 5 rows 15.2 us, so 14.7):
   uint32_t joins;         // waves that join parts
   int32_t tiles, splits;  // tiles of 128 pairs, and the pieces that each one's keys are cut into
@@ -664,7 +674,9 @@ __device__ __forceinline__ void few_pairs(const AttendArgs &a, const int block, 
   Piece p{0, 0, 0, 0, 0};
   const int32_t *at = a.b.parts;
   if (group >= a.groups) clear_rows<HD>(a, block - a.groups * units, tid, 64 * NW);
-  else if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p) || p.n * a.rep > a.few) p.n = 0;
+  else if (a.least > 1) p = whole_piece(a.b, item);
+  else if (!find_piece(a.b, item, lane, [&](int i, int) { return gload(at + i); }, &p)) p.n = 0;
+  if (p.n * a.rep > a.few) p.n = 0;
   const int pairs = p.n * a.rep;
   const int room = min(p.len, a.b.width << lg), nb = (room + KB - 1) / KB;
   const int mine = max(max(per, a.least), (nb + MOST_PARTS - 1) / MOST_PARTS), parts = (nb + mine - 1) / mine;
@@ -1076,11 +1088,11 @@ static int plan_attend(const bt_pages *c, const bt_batch *b, int heads, int wind
   p->few = p->many ? 32 : (int)most;
   p->tiles = p->few <= 16 ? 1 : 2;
   p->groups = (p->few + 31) / 32;
-  p->items = parts_target(c->kv) + b->requests;
   // keys: what a request's rows see between them. Where a window leaves few of a long table's, one part has them: 32 requests
-  // of 8192 keys in a window of 128 6.8 us and a launch less, in the plan's parts 6.7 + 3.5; of 1000 17.8, 18.8 + 4.0
+  // of 8192 keys in a window of 128 5.7 us and a launch less, in the plan's parts 6.7 + 3.5; of 1000 17.8, 18.8 + 4.0
   const int64_t held = (int64_t)b->width * c->page, keys = window ? std::min<int64_t>(held, (int64_t)window + b->most) : held;
   p->join = keys > SHORT, p->least = !p->join ? MOST_KEYS / KB : 1;
+  p->items = p->join ? parts_target(c->kv) + b->requests : b->requests;  // (least > 1: the requests themselves)
   // a block of 8 waves where a part a request leaves most CUs idle: one request of 3 heads of 64 and 1000 keys 6.4 us, with 4 waves
   // 6.8; 512 of 8 heads and 500 keys 121.4 and 88.7
   p->waves = p->many || (p->tiles == 1 && !p->join && (int64_t)b->requests * c->kv < 64) ? 8 : 4;
