@@ -207,7 +207,7 @@ struct Piece {
 };
 // The request whose pieces `before(i, starts[i])` .. `before(i + 1, ..)` hold piece `at`, found by the wave's lanes
 // together: of more than 64 requests first which of 64 equal runs, then which of the run's, a trip to memory each (64 at a time
-// from the first on, a put of 2048 requests' rows 135 us, so 90; a search by halves would be a trip a step). Starts count within
+// from the first on, a put over 2048 requests 135 us, so 90; a search by halves would be a trip a step). Starts count within
 // the rows there are and lengths hold their rows, whatever they say.
 template <class F> __device__ __forceinline__ bool find_piece(const BatchArgs &b, int at, int lane, F before, Piece *p) {
   const auto held = [&](int s) { return min(max(s, 0), b.rows); };
@@ -271,19 +271,23 @@ __device__ __forceinline__ float scale_of(float amax) {
 // whole words.
 // Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 181 us, 4.4 TB/s; a decode step's 32 rows are
 // latency, 5.3 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
-// by one wave (512 requests of one row 25.8 us, by four waves 48.4; of 8 rows 31.0 and 49.8), up to 64 with loads for 64
-// (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
+// by one wave (512 requests of one row 25.8 us, by four waves 48.4, of 8 rows 31.0 and 49.8, all with a search for the request),
+// up to 64 with loads for 64 (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
 template <int HD, int NT, int PAGE>
 __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
-                                                        int64_t x_sr) {
+                                                        int64_t x_sr, int each) {
   constexpr int U = HD / 8, MOST = PAGE * U / NT;  // 16-byte units of a row, loads a thread for the most rows
   __shared__ float tops[NT / 64];
   __shared__ __attribute__((aligned(16))) uint8_t turned[HD * (PAGE + 4)];  // by dimension, from the new rows' first word on
   const int tid = threadIdx.x, lane = tid & 63, lg = c.page_log2, page = 1 << lg, heads = 2 * c.kv;
   const int at = blockIdx.x / heads, h = blockIdx.x - at * heads;
   Piece p;
-  // request r owns pieces starts[r] / page + 2 r and on: at least as many as the pages its rows touch
-  if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> lg) + 2 * i; }, &p)) return;
+  if (each) {  // pieces of every request
+    p = whole_piece(b, at / each);
+    p.k = at - p.r * each;
+  } else if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> lg) + 2 * i; }, &p)) {
+    return;  // request r owns pieces starts[r] / page + 2 r and on: at least as many as the pages its rows touch
+  }
   const int cached = p.len - p.n, on = (cached >> lg) + p.k;
   const int from = max(cached, on << lg), count = min(min(p.len, (on + 1) << lg) - from, PAGE);
   if (count <= 0 || on >= b.width) return;
@@ -1181,21 +1185,26 @@ int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, ui
   if (int s = check_pool(pool, &c)) return s;
   if (int s = check_batch(batch, &b)) return s;
   if (!x || x % 16 || x_sb % 8 || x_sr % 8) return fail(BT_EINVAL, "a paged cache takes rows on 16-byte boundaries");
-  const int64_t blocks = (int64_t)((b.rows >> c.page_log2) + 2 * b.requests) * 2 * c.kv;
+  const int most = std::min(batch->most, batch->rows);
+  // the pages that a request's rows can touch, where they are few; else pieces go by the rows there are, which takes a search
+  // (2048 requests of a row: 73.5 us, by a search 89; 32 alike)
+  const int each = most == 1 ? 1 : most <= pool->page ? 2 : 0;
+  const int64_t blocks = (each ? (int64_t)each * b.requests : (b.rows >> c.page_log2) + 2 * b.requests) * 2 * c.kv;
   if ((int64_t)b.width * pool->page > MOST_KEYS)
     return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b.width, pool->page);
   if (!grid_fits(blocks, 256)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, 2 * c.kv);
   const uint16_t *src = (const uint16_t *)(uintptr_t)x;
-  // the most rows of a request in one page
-  const int most = std::min(std::min(batch->most, batch->rows), pool->page);
-  const auto launch = [&](auto kernel, int threads) { kernel<<<(unsigned)blocks, threads, 0, r->stream>>>(c, b, src, x_sb, x_sr); };
+  const int top = std::min(most, pool->page);  // the most rows of a request in one page
+  const auto launch = [&](auto kernel, int threads) {
+    kernel<<<(unsigned)blocks, threads, 0, r->stream>>>(c, b, src, x_sb, x_sr, each);
+  };
   if (pool->head_dim == 64) {
-    if (most <= 16) launch(put_pages_kernel<64, 64, 16>, 64);
-    else if (most <= 64) launch(put_pages_kernel<64, 256, 64>, 256);
+    if (top <= 16) launch(put_pages_kernel<64, 64, 16>, 64);
+    else if (top <= 64) launch(put_pages_kernel<64, 256, 64>, 256);
     else launch(put_pages_kernel<64, 256, 256>, 256);
   } else {
-    if (most <= 16) launch(put_pages_kernel<128, 64, 16>, 64);
-    else if (most <= 64) launch(put_pages_kernel<128, 256, 64>, 256);
+    if (top <= 16) launch(put_pages_kernel<128, 64, 16>, 64);
+    else if (top <= 64) launch(put_pages_kernel<128, 256, 64>, 256);
     else launch(put_pages_kernel<128, 256, 256>, 256);
   }
   BT_LAUNCHED("a paged put");
