@@ -28,7 +28,7 @@ constexpr int KB = 64;          // keys of a block
 constexpr int MOST_PARTS = 32;  // parts of one request (with 64, one request of 65536 keys: 32.4 us against 27.1)
 constexpr int SHORT = 16 * KB;  // keys that tables of one part a request hold at most
 // Waves that attention's parts are for, over all key heads: 8 on each of the 256 CUs, which is what their registers allow at once
-// (8 requests of up to 8191 keys: 19.7 us; with 1024 23.4, with 3072 22.5).
+// (8 requests of up to 8191 keys: 19.7 us; with half as many 23.4, with half as many again 22.5).
 constexpr int WAVES = 2048;
 constexpr int MOST_REQUESTS = 2048;
 
