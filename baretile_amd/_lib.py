@@ -90,7 +90,7 @@ class VerifyArgs(ctypes.Structure):  # bt_verify_args
               ("starts", c_uint64), ("tokens", c_uint64), ("counts", c_uint64), ("scratch", c_uint64),
               ("scratch_bytes", c_uint64), ("logits_sr", c_int64), ("probs_sr", c_int64), ("t_sr", c_int64),
               ("uniforms_sr", c_int64), ("requests", c_int32), ("rows", c_int32), ("vocab", c_int32),
-              ("pad_", c_int32)]
+              ("pad_", c_int32), ("drafts", c_uint64)]
 
 
 RT = c_void_p

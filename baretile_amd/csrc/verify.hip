@@ -1,6 +1,6 @@
 // Drafted tokens checked against the target's probabilities, from random numbers that the caller draws.
 //
-// For a request whose rows bring a token and then its drafts, p_j = softmax(t_j x_j) of row j's logits is the target's choice
+// For a request whose rows bring a token and then its drafts (behind a prompt's other rows, where `drafts` counts them), p_j = softmax(t_j x_j) of row j's logits is the target's choice
 // of the token after row j, and q_j the distribution that the draft fed at row j was drawn from. Row j's draft d is
 // accepted where u0_j q_j(d) < p_{j-1}(d). The first refusal, after row j, draws from max(p_j - q_{j+1}, 0); where every
 // draft was accepted the last row draws from p: the first token whose running sum passes u1_j times the whole. Tokens
@@ -32,7 +32,7 @@ struct Draw {
 };                                            // is nothing to draw, the one to take (-1: none)
 struct VerifyArgs {
   const float *logits, *probs, *t, *uniforms;
-  const int32_t *ids, *starts;
+  const int32_t *ids, *starts, *drafts;
   int32_t *tokens, *counts;
   ChunkStat *stats;  // [rows][chunks]
   Draw *draws;       // [requests]
@@ -234,11 +234,14 @@ __device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int 
     else out[i] = v0 + Chunk<PER, WIDE>::place(lane, i) == f.without ? 0.0 : p;
   }
 }
-// The first row of request r, and its rows: within those there are, whatever starts holds.
-__device__ __forceinline__ int request_rows(const VerifyArgs &a, int r, int *n) {
-  const int s0 = gload(a.starts + r), s1 = gload(a.starts + r + 1), start = min(max(s0, 0), a.rows);
-  *n = min(max(s1, start), a.rows) - start;
-  return start;
+// The first row of request r that is verified, and how many are: all of its rows, or with drafts its last token's and that many
+// drafts'. `ahead` rows of it lie before them. Within the rows there are, whatever starts and drafts hold.
+__device__ __forceinline__ int request_rows(const VerifyArgs &a, int r, int *n, int *ahead) {
+  const int s0 = gload(a.starts + r), s1 = gload(a.starts + r + 1), d = a.drafts ? gload(a.drafts + r) : NOWHERE;
+  const int start = min(max(s0, 0), a.rows), rows = min(max(s1, start), a.rows) - start;
+  *n = min(max(d, -1), rows - 1) + 1;
+  *ahead = rows - *n;
+  return start + *ahead;
 }
 
 // Block (request, 4 chunks): the first refused draft, found by every block for itself, then what is left of a chunk a wave.
@@ -247,8 +250,8 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
   __shared__ int refusal;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int blocks = (a.chunks + WAVES - 1) / WAVES, r = blockIdx.x / blocks, c = (blockIdx.x - r * blocks) * WAVES + w;
-  int n;
-  const int start = request_rows(a, r, &n);
+  int n, ahead;
+  const int start = request_rows(a, r, &n, &ahead);
   if (n == 0) return;
   if (tid == 0) refusal = n;
   __syncthreads();
@@ -311,8 +314,9 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
   double kept[KEEP];
 #pragma unroll
   for (int i = 0; i < KEEP; i++) kept[i] = gload(left + min(c0 + i, a.chunks - 1));  // requested with the rest, used or not
-  int n;
-  const int start = request_rows(a, r, &n);
+  int n, ahead;
+  const int start = request_rows(a, r, &n, &ahead);
+  for (int i = lane; i < ahead; i += 64) a.tokens[start - ahead + i] = -1;
   if (n == 0) {
     if (lane == 0) a.counts[r] = 0;
     return;
@@ -396,7 +400,7 @@ static int verify_chunks(const bt_verify_args *a) { return ceil_div(a->vocab, 64
 static int check_verify(const bt_verify_args *a) {
   if (!a || !a->logits || !a->ids || !a->starts || !a->uniforms || !a->tokens || !a->counts)
     return fail(BT_EINVAL, "verifying drafts needs logits, ids, starts, uniforms and results");
-  if ((a->logits | a->probs | a->t | a->uniforms | a->ids | a->starts | a->tokens | a->counts) % 4)
+  if ((a->logits | a->probs | a->t | a->uniforms | a->ids | a->starts | a->tokens | a->counts | a->drafts) % 4)
     return fail(BT_EINVAL, "verifying drafts takes tensors on 4-byte boundaries");
   if (a->requests < 1 || a->rows < 1 || a->vocab < 1 || a->vocab > 1 << 20 || a->requests > 1 << 20 || a->rows > 1 << 20)
     return fail(BT_EINVAL, "verifying %d requests' %d rows of %d logits (each 1 to 2^20)", a->requests, a->rows, a->vocab);
@@ -442,6 +446,7 @@ int bt_verify(bt_runtime *rt, const bt_verify_args *a) {
   const auto f = [](uint64_t p) { return (const float *)(uintptr_t)p; };
   k.logits = f(a->logits), k.probs = f(a->probs), k.t = f(a->t), k.uniforms = f(a->uniforms);
   k.ids = (const int32_t *)(uintptr_t)a->ids, k.starts = (const int32_t *)(uintptr_t)a->starts;
+  k.drafts = (const int32_t *)(uintptr_t)a->drafts;
   k.tokens = (int32_t *)(uintptr_t)a->tokens, k.counts = (int32_t *)(uintptr_t)a->counts;
   k.chunks = verify_chunks(a);
   k.stats = (ChunkStat *)(uintptr_t)a->scratch;

@@ -474,9 +474,9 @@ def forward(ids, places, w, c, caches, every=False, slots=None):
 def paged_forward(ids, batch, w, c, caches):
   """Logits after every row of ids (an int32 row of batch.rows) in fp32, over a paged cache (paged_cache): batch is the
   step's plan, made by one of the caches, and says which request and place each row is, so requests may bring a token
-  each, a token and its drafts (serve.verify takes the logits), or chunks of prompts, all in one step. Requests are at most
-  as long as the weights' places (upload). Rows behind the last request's (whose ids are anything) give logits of no
-  meaning."""
+  each, a token and its drafts, or chunks of prompts, all in one step (serve.verify takes the logits, and how many of each
+  request's rows are drafts). Requests are at most as long as the weights' places (upload). Rows behind the last request's (whose
+  ids are anything) give logits of no meaning."""
   if len(caches) != c.layers or ids.cols != batch.rows:
     raise ValueError(f"paged_forward needs {c.layers} caches and ids for the batch's {batch.rows} rows: {len(caches)}, {ids.shape}")
   x = w["embed"].gather(ids).float()

@@ -35,38 +35,45 @@ def heads(logits, t=None, k=64):
   return values, ids, lse.realize()
 
 
-def verify(logits, ids, starts, uniforms, probs=None, t=None):
+def verify(logits, ids, starts, uniforms, probs=None, t=None, drafts=None):
   """Drafted tokens against the target's probabilities, on the device (bt_verify): (tokens, counts). Row j of logits (rows,
   vocab) fp32 follows token ids[j] (an int32 row); request r's rows starts[r] .. starts[r + 1] - 1 (an int32 row of requests + 1, as
-  pages.Batch has it) are its last token, then its drafts. uniforms (2, rows) fp32 are numbers in [0, 1); probs (rows, vocab) fp32
-  the distributions that each row's ids was drawn from (None: the drafts were certain, as greedy ones are); t, a column with
-  each row's inverse temperature (None: 1; infinity: the first largest alone, as greedy picks are).
+  pages.Batch has it) are its last token, then its drafts. drafts (an int32 row) says how many of each request's rows are drafts,
+  its last ones, where rows of a prompt may lie ahead: 0 for a prompt's last chunk, whose token is then the one after its last row;
+  below 0 for one that is to have no token yet, or brings no row (None: every row after a request's first is a draft). uniforms (2,
+  rows) fp32 are numbers in [0, 1); probs (rows, vocab) fp32 the distributions that each row's ids was drawn from (None: the drafts
+  were certain, as greedy ones are); t, a column with each row's inverse temperature (None: 1; infinity: the first largest alone,
+  as greedy picks are).
 
   With p = softmax(t * logits) in 64 bits, the draft at row j is accepted where uniforms[0, j] * probs[j, ids[j]] < p[j - 1,
   ids[j]]. tokens, an int32 row, has for each row the token that follows it: accepted drafts, then at the first refusal a token
-  drawn with uniforms[1] from what p has over probs, or after the last draft one from p, -1 behind that. counts, an int32 row,
-  has each request's new tokens."""
+  drawn with uniforms[1] from what p has over probs, or after the last draft one from p, -1 behind that and ahead of the last
+  token's row. counts, an int32 row, has each request's new tokens. (So a request's cache holds lengths - drafts - 1 + counts
+  tokens that stand, lengths being its Batch's.)"""
   rt = getattr(logits, "rt", None)
-  for x, dtype in ((logits, "fp32"), (ids, "int32"), (starts, "int32"), (uniforms, "fp32"), (probs, "fp32"), (t, "fp32")):
+  for x, dtype in ((logits, "fp32"), (ids, "int32"), (starts, "int32"), (uniforms, "fp32"), (probs, "fp32"), (t, "fp32"),
+                   (drafts, "int32")):
     if x is not None and not (isinstance(x, Tensor) and x.rt is rt and x.batch == 1 and x.dtype == dtype):
       raise ValueError(f"verify needs {dtype} matrices on one runtime: {getattr(x, 'dtype', type(x))} {getattr(x, 'shape', '')}")
   rows, vocab = logits.rows, logits.cols
   if not ((ids.rows, ids.cols) == (1, rows) and starts.rows == 1 and starts.cols >= 2 and
           (uniforms.rows, uniforms.cols) == (2, rows) and
-          (probs is None or (probs.rows, probs.cols) == (rows, vocab)) and (t is None or (t.rows, t.cols) == (rows, 1))):
-    raise ValueError(f"verify needs ids (1, {rows}), starts (1, requests + 1), uniforms (2, {rows}), probs ({rows}, {vocab}) and t "
-                     f"({rows}, 1): {ids.shape} {starts.shape} {uniforms.shape} "
-                     f"{getattr(probs, 'shape', None)} {getattr(t, 'shape', None)}")
+          (probs is None or (probs.rows, probs.cols) == (rows, vocab)) and (t is None or (t.rows, t.cols) == (rows, 1)) and
+          (drafts is None or (drafts.rows, drafts.cols) == (1, starts.cols - 1))):
+    raise ValueError(f"verify needs ids (1, {rows}), starts (1, requests + 1), uniforms (2, {rows}), probs ({rows}, {vocab}), t "
+                     f"({rows}, 1) and drafts (1, requests): {ids.shape} {starts.shape} {uniforms.shape} "
+                     f"{getattr(probs, 'shape', None)} {getattr(t, 'shape', None)} {getattr(drafts, 'shape', None)}")
   def whole(x):  # rows of contiguous values
     x = x.realize()
     return x if x.sc == 1 and x.rep == 1 and not x.cyc else x.contiguous()
   logits, ids, starts, uniforms = (whole(x) for x in (logits, ids, starts, uniforms))
-  probs, t = (whole(x) if x is not None else None for x in (probs, t))
+  probs, t, drafts = (whole(x) if x is not None else None for x in (probs, t, drafts))
   requests = starts.cols - 1
   tokens, counts = Tensor(rt, 1, rows, dtype="int32"), Tensor(rt, 1, requests, dtype="int32")
   args = _lib.VerifyArgs(logits.addr, probs.addr if probs is not None else 0, t.addr if t is not None else 0, uniforms.addr,
                          ids.addr, starts.addr, tokens.addr, counts.addr, 0, 0, logits.sr, probs.sr if probs is not None else 0,
-                         t.sr if t is not None else 0, uniforms.sr, requests, rows, vocab, 0)
+                         t.sr if t is not None else 0, uniforms.sr, requests, rows, vocab, 0,
+                         drafts.addr if drafts is not None else 0)
   need = ctypes.c_uint64()
   _lib.call("verify_scratch", ctypes.byref(args), ctypes.byref(need))
   scratch = Storage(rt, need.value)

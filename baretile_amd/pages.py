@@ -6,12 +6,14 @@ its tokens fill. A page holds the tokens of every key and value head, a head's a
 under one power of two, which makes each value exact in bf16: half of a bf16 cache's memory, and decoded in one
 instruction for two values where a bfp8 cache takes five.
 
-A step over several requests, each with any number of new tokens (a token, a token and its drafts, a prompt's chunk):
+A step over several requests, each with any number of new tokens (a token, a token and its drafts, a prompt's chunk), of which
+the last drafts[r] of request r are drafts (0: none; -1: no token follows
+yet, as behind a chunk that does not end its prompt, or the request brings no row):
 
   batch = pool.plan(tables, cached, new, free, rows)   # once a step; every block's pool of the same shape shares it
   pool.put(batch, x)                                   # each block's keys and values
   o = pool.attend(q, batch)                            # and its attention
-  tokens, counts = serve.verify(logits, ids, batch.starts, uniforms)
+  tokens, counts = serve.verify(logits, ids, batch.starts, uniforms, drafts=drafts)
 """
 import ctypes, operator
 from baretile_amd import _lib

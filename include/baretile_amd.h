@@ -411,18 +411,20 @@ int bt_topk(bt_runtime *rt, int dtype, uint64_t x, int64_t batch, int64_t rows, 
 /* ---- drafted tokens verified: no counterpart in the reference's greedy heads (serve.py:43-63) --------------------------
  *
  * Rows starts[r] .. starts[r + 1] - 1 (int32, requests + 1) are request r's: its last token, then its drafts, ids[rows]
- * the tokens fed there. logits (fp32 rows of vocab, row stride in elements) are the target's after each row, t (0: all 1)
+ * the tokens fed there. drafts (0: every row after a request's first is one) counts each request's drafts, its last rows; the
+ * rows ahead of its last token's, as a prompt's are, are not looked at, and with drafts[r] below 0 none of its rows is. logits (fp32 rows of vocab, row stride in elements) are the target's after each row, t (0: all 1)
  * each row's inverse temperature (below 0 or NaN: 0; infinite: the first largest alone), p_j = softmax(t_j logits_j);
  * probs (0: drafts were certain) the distributions that the drafts were drawn from, row j's that of ids[j]. uniforms are
  * two rows of numbers in [0, 1). Draft ids[j] is accepted where uniforms[0, j] * probs[j, ids[j]] < p_{j-1}(ids[j]).
  * tokens[rows], the token after each row: the accepted drafts up to the first refused, then one drawn from max(p - probs,
  * 0) at the refusal or from p after the last, the first whose running sum passes uniforms[1, j] times the whole; -1 behind
- * it and behind the last request. counts[requests]: each one's new tokens. A logit of NaN counts as -inf; a row of nothing
+ * it, ahead of its last token's row and behind the last request. counts[requests]: each one's new tokens. A logit of NaN counts as -inf; a row of nothing
  * else accepts and draws nothing. All in 64 bits. */
 typedef struct {
   uint64_t logits, probs, t, uniforms, ids, starts, tokens, counts, scratch, scratch_bytes;
   int64_t logits_sr, probs_sr, t_sr, uniforms_sr;
   int32_t requests, rows, vocab, pad_;
+  uint64_t drafts;
 } bt_verify_args;
 int bt_verify_scratch(const bt_verify_args *args, uint64_t *bytes);
 int bt_verify(bt_runtime *rt, const bt_verify_args *args);

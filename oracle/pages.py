@@ -94,7 +94,7 @@ def attend(q, values, tables, starts, lengths, window=0):
   return out, weighed
 
 
-def verify(logits, ids, starts, uniforms, probs=None, t=None):
+def verify(logits, ids, starts, uniforms, probs=None, t=None, drafts=None):
   """(tokens, counts) as serve.verify gives them. What is drawn from is not normalized, in extended precision, so that equal weights
   add exactly and a number on the border between two falls where it should."""
   rows, vocab = logits.shape
@@ -114,7 +114,8 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None):
     upto = np.cumsum(w)
     past = np.flatnonzero((upto > u * upto[-1]) & (w > 0))
     return past[0] if len(past) else np.flatnonzero(w > 0)[-1]
-  for s, e in zip(starts[:-1], starts[1:]):
+  for r, (s, e) in enumerate(zip(starts[:-1], starts[1:])):
+    if drafts is not None: s = max(s, e - max(int(drafts[r]) + 1, 0))  # what lies ahead is not looked at
     a, n, made = 0, e - s, -1
     while n > 0:
       p, z = choice(s + a)

@@ -622,3 +622,61 @@ def test_refusals(rt):
   for args in ((Tensor.zeros(rt, 4, 50), ids, starts, u), (logits, r(1), starts, u), (logits, ids, r(0), u), (logits, ids, starts, logits),
                (logits, ids, starts, u, u), (logits, ids, starts, u, None, u), (logits, ids, None, u)):
     with pytest.raises((ValueError, AttributeError)): serve.verify(*args)
+
+
+def verified_behind(rt, logits, ids, starts, uniforms, drafts, probs=None, t=None):
+  """verified() with a count of drafts a request: the rows ahead are not looked at."""
+  of = lambda a: Tensor.of(rt, np.asarray(a, np.float32), "fp32")
+  tokens, counts = serve.verify(of(logits), row(rt, ids), row(rt, starts), of(uniforms), of(probs) if probs is not None else None,
+                                of(np.reshape(t, (-1, 1))) if t is not None else None, row(rt, drafts))
+  want = P.verify(logits, ids, starts, uniforms, probs, None if t is None else np.asarray(t, np.float32), drafts)
+  assert np.array_equal(ints(tokens), want[0]) and np.array_equal(ints(counts), want[1]), (ints(tokens), ints(counts), want)
+
+
+@pytest.mark.parametrize("vocab", [300, 3001])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_behind_a_prompts_rows(rt, vocab, drawn):
+  rng = np.random.default_rng(vocab)
+  starts = [0, 90, 91, 91, 96, 170, 180]
+  rows = 183
+  logits = 3 * rng.normal(0, 1, (rows, vocab)).astype(np.float32)
+  probs = near(rng, logits) if drawn else None
+  ids = np.roll(logits, 1, 0).argmax(1)
+  ids[::7] = rng.integers(0, vocab, len(ids[::7]))
+  for drafts in ([0] * 6, [0, 0, -1, 4, -1, 3], [-1] * 6, [89, 90, 0, 2, 73, 2 ** 31 - 1], [-2 ** 31, 5, 5, 5, 70, 1]):
+    u = rng.random((2, rows)).astype(np.float32)
+    verified_behind(rt, logits, ids, starts, u, drafts, probs)
+    verified_behind(rt, logits, ids, starts, u, drafts, probs, [np.inf] * rows)
+    verified_behind(rt, logits, ids, starts, u, drafts, probs, rng.uniform(0.5, 2, rows))
+
+
+def test_a_prompts_next_token_follows_its_last_row(rt):
+  # one step with a prompt's last chunk, a chunk that does not end its prompt, a token and its drafts, and a request without
+  # rows: greedily, the prompt's token is what its last row's logits give, and as good as llama.forward's over a bf16 cache
+  # (whose logits the paged ones keep to within 3% of the largest, on either side)
+  from baretile_amd.models import llama
+  from oracle import llama_ref as L
+  rng = np.random.default_rng(43)
+  c, w = L.smol(rng, 2, vocab=256, places=96)
+  dc = llama.model(dim=576, heads=9, kv=3, layers=2, eps=1e-5, theta=10000.0, vocab=256, ffn=1536)
+  dw = llama.upload(rt, {k: v for k, v in w.items() if k not in ("cos", "sin", "turn", "embed.T")}, dc, places=96)
+  caches = llama.paged_cache(rt, dc, 30, 16)
+  prompts = [rng.integers(0, 256, n) for n in (37, 20, 9)]
+  b, (tables, *_, taken) = planned(rt, caches[0], np.full((4, 6), -1), [0] * 4, [0, 0, 9, 0], rng.permutation(30), 9)
+  llama.paged_forward(row(rt, prompts[2]), b, dw, dc, caches).realize()
+  ids, drafts = np.concatenate([prompts[0], prompts[1], [5, 6, 7], [0]]), [0, -1, 2, -1]
+  b, (_, starts, *_) = planned(rt, caches[0], tables, [0, 0, 9, 0], [37, 20, 3, 0], rng.permutation(30), 61, taken)
+  logits = llama.paged_forward(row(rt, ids), b, dw, dc, caches).realize()
+  u, t = rng.random((2, 61)).astype(np.float32), np.full((61, 1), np.inf)
+  tokens, counts = serve.verify(logits.reshape(61, 256), row(rt, ids), b.starts, Tensor.of(rt, u, "fp32"), t=Tensor.of(rt, t, "fp32"),
+                                drafts=row(rt, drafts))
+  got = np.array(logits.tolist(), np.float32).reshape(61, 256)
+  want = P.verify(got, ids, starts, u, t=t, drafts=drafts)
+  assert np.array_equal(ints(tokens), want[0]) and np.array_equal(ints(counts), want[1])
+  token = ints(tokens)[36]
+  assert token == got[36].argmax() and (ints(tokens)[:36] == -1).all() and ints(counts)[:2].tolist() == [1, 0]
+  plain = llama.forward(row(rt, prompts[0]), row(rt, range(37)), dw, dc, llama.kv_cache(rt, dc, 96))
+  plain = np.array(plain.tolist()).reshape(-1)
+  assert plain[token] >= plain.max() - 0.06 * np.abs(plain).max()
+  with pytest.raises(ValueError, match="drafts"): serve.verify(logits.reshape(61, 256), row(rt, ids), b.starts, Tensor.of(rt, u, "fp32"),
+                                                               drafts=row(rt, drafts[:3]))

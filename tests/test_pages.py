@@ -86,6 +86,30 @@ def test_verify_refuses(bad):
     _lib.call("verify_scratch", ctypes.byref(_lib.VerifyArgs(**(fields | bad))), ctypes.byref(n))
 
 
+def test_a_prompts_rows_are_no_drafts():
+  # with drafts, each request is verified as if its last rows were all it had
+  rng = np.random.default_rng(1)
+  logits, ids = rng.normal(0, 2, (40, 500)).astype(np.float32), rng.integers(0, 500, 40)
+  ids[31:40] = logits[30:39].argmax(1)  # drafts that greedy rows take
+  u, greedy = rng.random((2, 40)).astype(np.float32), np.full(40, np.inf)
+  tokens, counts = P.verify(logits, ids, [0, 25, 30, 30, 40], u, t=greedy, drafts=[0, -1, 0, 4])
+  assert counts.tolist() == [1, 0, 0, 5]
+  assert tokens[24] == logits[24].argmax() and (tokens[:24] == -1).all() and (tokens[25:35] == -1).all()
+  assert np.array_equal(tokens[35:], logits[35:].argmax(1))
+  for t in (None, greedy):
+    tokens, counts = P.verify(logits, ids, [0, 40], u, t=t, drafts=[6])
+    alone = P.verify(logits[33:], ids[33:], [0, 7], u[:, 33:], t=None if t is None else t[33:])
+    assert np.array_equal(tokens[33:], alone[0]) and np.array_equal(counts, alone[1]) and (tokens[:33] == -1).all()
+
+
+def test_verify_refuses_drafts_off_their_boundary():
+  fields = {"logits": 4096, "uniforms": 4096, "ids": 4096, "starts": 4096, "tokens": 4096, "counts": 4096, "rows": 5, "requests": 1,
+            "vocab": 1000}
+  n = ctypes.c_uint64()
+  _lib.call("verify_scratch", ctypes.byref(_lib.VerifyArgs(**fields, drafts=4096)), ctypes.byref(n))
+  with pytest.raises(ValueError, match="4-byte"): _lib.call("verify_scratch", ctypes.byref(_lib.VerifyArgs(**fields, drafts=4098)), ctypes.byref(n))
+
+
 def test_no_runtime():
   for name, args in (("pages_plan", (None,)), ("pages_put", (None, None, 0, 0, 0)), ("pages_read", (None, 0)), ("verify", (None,)),
                      ("pages_attend", (None, None, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0))):
