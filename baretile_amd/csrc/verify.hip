@@ -303,8 +303,10 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
 // Wave (request): the chunk, the token, and the request's rows of the result.
 template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_kernel(const VerifyArgs a) {
   const int r = blockIdx.x, lane = threadIdx.x;
-  if (r == a.requests) {  // rows behind the last request's
-    for (int j = max(0, gload(a.starts + a.requests)) + lane; j < a.rows; j += 64) a.tokens[j] = -1;
+  if (r == a.requests) {  // rows of no request: ahead of the first's and behind the last's
+    const int first = min(gload(a.starts), a.rows), last = max(0, gload(a.starts + a.requests));
+    for (int j = lane; j < first; j += 64) a.tokens[j] = -1;
+    for (int j = last + lane; j < a.rows; j += 64) a.tokens[j] = -1;
     return;
   }
   constexpr int KEEP = 4;  // sums a lane keeps: of up to 256 chunks all

@@ -418,8 +418,8 @@ int bt_topk(bt_runtime *rt, int dtype, uint64_t x, int64_t batch, int64_t rows, 
  * two rows of numbers in [0, 1). Draft ids[j] is accepted where uniforms[0, j] * probs[j, ids[j]] < p_{j-1}(ids[j]).
  * tokens[rows], the token after each row: the accepted drafts up to the first refused, then one drawn from max(p - probs,
  * 0) at the refusal or from p after the last, the first whose running sum passes uniforms[1, j] times the whole; -1 behind
- * it, ahead of its last token's row and behind the last request. counts[requests]: each one's new tokens. A logit of NaN counts as -inf; a row of nothing
- * else accepts and draws nothing. All in 64 bits. */
+ * it, ahead of its last token's row, and for rows of no request. counts[requests]: each one's new tokens. A logit of NaN
+ * counts as -inf; a row of nothing else accepts and draws nothing. All in 64 bits. */
 typedef struct {
   uint64_t logits, probs, t, uniforms, ids, starts, tokens, counts, scratch, scratch_bytes;
   int64_t logits_sr, probs_sr, t_sr, uniforms_sr;

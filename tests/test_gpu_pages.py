@@ -680,3 +680,15 @@ def test_a_prompts_next_token_follows_its_last_row(rt):
   assert plain[token] >= plain.max() - 0.06 * np.abs(plain).max()
   with pytest.raises(ValueError, match="drafts"): serve.verify(logits.reshape(61, 256), row(rt, ids), b.starts, Tensor.of(rt, u, "fp32"),
                                                                drafts=row(rt, drafts[:3]))
+
+
+def test_verify_writes_the_rows_ahead_of_its_first_request(rt):
+  # a run of a longer batch's requests: the rows of the requests before it have no token either
+  rng = np.random.default_rng(44)
+  logits, u = rng.normal(0, 2, (70, 100)).astype(np.float32), rng.random((2, 70)).astype(np.float32)
+  ids, starts = logits.argmax(1), Tensor.of(rt, [[0, 4, 66, 68, 69]], "int32")
+  old = Tensor.of(rt, np.full((1, 70), 7), "int32")  # what the result's memory may hold
+  del old
+  tokens, counts = serve.verify(Tensor.of(rt, logits, "fp32"), row(rt, ids), starts[:, 2:], Tensor.of(rt, u, "fp32"))
+  want = P.verify(logits, ids, [66, 68, 69], u)
+  assert np.array_equal(ints(tokens), want[0]) and np.array_equal(ints(counts), want[1])
