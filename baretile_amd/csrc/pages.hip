@@ -98,7 +98,11 @@ template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanAr
   __shared__ int sums[NT / 64];
   const int lg = a.page_log2, room = (int)min((int64_t)a.width << lg, (int64_t)0x40000000);
   const int taken = a.taken ? gload(a.taken) : 0;
-  int rows = 0, takes = 0, blocks = 0;
+  // blocks of keys may pass 32 bits (2048 requests of 2^24): where they could pass 2^30 they are summed by their lower 12 bits and
+  // the rest
+  const bool large = (int64_t)a.requests * ((room + KB - 1) / KB) > 1 << 30;
+  int rows = 0, takes = 0;
+  int64_t blocks = 0;
   for (int base = 0; base < a.requests; base += NT) {
     const int r = base + threadIdx.x;
     int c = 0, n = 0, total;
@@ -121,8 +125,10 @@ template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanAr
     const int off = block_exclusive<NT>(need, sums, &total);
     if (r < a.requests) from[r] = takes + off;
     takes += total;
-    block_exclusive<NT>(n > 0 ? (min(c + n, room) + KB - 1) / KB : 0, sums, &total);
+    const int nb = n > 0 ? (min(c + n, room) + KB - 1) / KB : 0;
+    block_exclusive<NT>(large ? nb & 4095 : nb, sums, &total);
     blocks += total;
+    if (large) block_exclusive<NT>(nb >> 12, sums, &total), blocks += (int64_t)total << 12;
   }
   const int last = rows;
   if (threadIdx.x == 0) {
@@ -130,7 +136,10 @@ template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanAr
     a.starts[a.requests] = last;
     a.taken_out[0] = taken + takes;
   }
-  const int per = max(a.least, ((blocks + a.target - 1) / a.target + 3) & ~3);
+  int each;  // (a part holds one request's blocks, 2^24 at most, however few parts there are for them)
+  if (large) each = (int)min((blocks + a.target - 1) / a.target, (int64_t)(0x40000000 / KB));
+  else each = ((int)blocks + a.target - 1) / a.target;
+  const int per = max(a.least, (each + 3) & ~3);
   int made = 0;
   __syncthreads();
   for (int base = 0; base < a.requests; base += NT) {

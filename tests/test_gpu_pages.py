@@ -692,3 +692,17 @@ def test_verify_writes_the_rows_ahead_of_its_first_request(rt):
   tokens, counts = serve.verify(Tensor.of(rt, logits, "fp32"), row(rt, ids), starts[:, 2:], Tensor.of(rt, u, "fp32"))
   want = P.verify(logits, ids, [66, 68, 69], u)
   assert np.array_equal(ints(tokens), want[0]) and np.array_equal(ints(counts), want[1])
+
+
+def test_plan_counts_blocks_past_32_bits(rt):
+  # 160 requests of 2^30 tokens: 2^24 blocks of keys each, 2.7 billion in all. As many parts as attention launches, 512 and one
+  # a request for one key head, and a run of at most 2^24 blocks to each.
+  pool, requests = Pages(rt, 4, 1, 64, 256), 160
+  tables = Tensor(rt, requests, 1 << 22, dtype="int32")
+  rt.fill32(tables.addr, -1, requests << 22)
+  b = pool.plan(tables, row(rt, [2 ** 30 - 1] * requests), row(rt, [1] * requests), row(rt, [0]), requests)
+  *parts, per = ints(b.parts).tolist()
+  blocks = 1 << 24
+  assert per == (-(-requests * blocks // 512) + 3) // 4 * 4 <= blocks
+  assert parts == [i * -(-blocks // per) for i in range(requests + 1)] and parts[-1] <= 512 + requests
+  assert ints(b.lengths).tolist() == [2 ** 30] * requests and ints(b.starts).tolist() == list(range(requests + 1))
