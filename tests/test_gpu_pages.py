@@ -1,8 +1,10 @@
 """The paged 8-bit cache and the verification of drafts on the GPU, against oracle/pages.py in 64 bits: plans, puts and tokens
 exactly, attention within what its roundings allow. Needs a GPU."""
+import ctypes
 import numpy as np
 import pytest
 
+from baretile_amd import _lib
 from baretile_amd.models import serve
 from baretile_amd.pages import Pages
 from baretile_amd.tensor import Recording, Tensor, jit
@@ -706,3 +708,119 @@ def test_plan_counts_blocks_past_32_bits(rt):
   assert per == (-(-requests * blocks // 512) + 3) // 4 * 4 <= blocks
   assert parts == [i * -(-blocks // per) for i in range(requests + 1)] and parts[-1] <= 512 + requests
   assert ints(b.lengths).tolist() == [2 ** 30] * requests and ints(b.starts).tolist() == list(range(requests + 1))
+
+
+# ---- attention past the 64 pages of a request that a wave's lanes hold at a time. Every row's head has one key, at a place of its
+# own, that outweighs all others (score 24; the others', of rows of hd unit normals, keep within 6 24 / hd^0.5, at most 18, and mostly
+# within half of that), so a page that is read in another's place is another result altogether.
+
+def shared(rt, rng, kv, hd, page, tokens):
+  """A pool of one request's tokens: (pool, values, its pages). Requests that only read may share them."""
+  pages = tokens // page
+  pool, values, s = Pages(rt, pages, kv, hd, page), np.zeros((pages, 2 * kv, page, hd)), np.full((pages, 2 * kv), 2.0 ** -100)
+  x = B.bf16(rng.normal(0, 1, (2 * kv, tokens, hd)))
+  b, (tables, starts, lengths, *_) = planned(rt, pool, np.full((1, pages), -1), [0], [tokens], rng.permutation(pages), tokens)
+  pool.put(b, Tensor.of(rt, x))
+  P.put(values, s, tables, starts, lengths, x)
+  return pool, values, tables[0]
+
+
+def pointed(rng, heads, values, tables, starts, lengths, window=0):
+  """Queries that each point at one of the keys that their row sees, one row's heads at places all over: (q, the places)."""
+  pages, kv2, page, hd = values.shape
+  q, at = np.zeros((heads, starts[-1], hd)), np.zeros((heads, starts[-1]), int)
+  for r, length in enumerate(lengths):
+    for i in range(starts[r], starts[r + 1]):
+      place = length - starts[r + 1] + i
+      for h in range(heads):
+        at[h, i] = t = rng.integers(max(0, place + 1 - window) if window else 0, place + 1)
+        k = values[tables[r, t // page], h // (heads // (kv2 // 2)), t % page]
+        q[h, i] = 24 * k / (k @ k)
+  return B.bf16(q), at
+
+
+def attend_by_head(q, values, tables, starts, lengths, window=0):
+  """oracle.pages.attend, a request's head at a time."""
+  pages, kv2, page, hd = values.shape
+  rep = q.shape[0] // (kv2 // 2)
+  out, weighed = np.zeros(q.shape), np.zeros(q.shape)
+  for r, length in enumerate(lengths):
+    rows = slice(starts[r], starts[r + 1])
+    place = np.arange(length - (starts[r + 1] - starts[r]), length)[:, None]
+    held = values[tables[r, :-(-length // page)]]
+    key = np.arange(held.shape[0] * page)
+    hidden = (key > place) | ((key <= place - window) if window else False)
+    for h in range(q.shape[0]):
+      k, v = (held[:, i].reshape(-1, hd) for i in (h // rep, kv2 // 2 + h // rep))
+      s = np.where(hidden, -np.inf, q[h, rows].astype(np.float64) @ k.T)
+      p = np.exp(s - s.max(1, keepdims=True))
+      p /= p.sum(1, keepdims=True)
+      out[h, rows], weighed[h, rows] = p @ v, p @ np.abs(v)
+  return out, weighed
+
+
+def points_found(rt, rng, pool, values, heads, tables, lengths, new, window=0, most=None):
+  """Attention with pointed queries against the 64-bit form, and the batch: what it found is near the value pointed at."""
+  rows, kv, rep = sum(new), pool.kv, heads // pool.kv
+  b, (made, starts, total, *_) = planned(rt, pool, tables, [n - m for n, m in zip(lengths, new)], new, [-1], rows, most=most)
+  q, at = pointed(rng, heads, values, made, starts, total, window)
+  got = np.array(pool.attend(Tensor.of(rt, q), b, window).tolist()).reshape(q.shape)
+  want, weighed = attend_by_head(q, values, made, starts, total, window)
+  owner = np.repeat(np.arange(len(new)), new)
+  v = np.stack([values[made[owner, at[h] // pool.page], kv + h // rep, at[h] % pool.page] for h in range(heads)])
+  assert (np.abs(want - v).max(-1) < 0.1).mean() > 0.95  # (the queries do point)
+  assert np.all(np.abs(got - want) <= bound(q, values, weighed, want)), np.abs(got - want).max()
+  return b
+
+
+def pages_of_a_part(b, lengths):
+  """The most pages of a part of the batch's, from the plan's least blocks of keys a part."""
+  per, blocks = int(ints(b.parts)[-1]), -(-max(lengths) // 64)
+  return max(per, -(-blocks // 32)) * 64 // b.page
+
+
+@pytest.mark.parametrize("hd, page, requests, new", [(64, 16, 32, 1), (128, 16, 32, 1), (64, 32, 48, 1), (64, 16, 32, 5), (64, 16, 32, 17)])
+def test_attend_parts_of_more_pages_than_a_wave_holds(rt, hd, page, requests, new):
+  rng = np.random.default_rng(hd + page + new)
+  pool, values, pages = shared(rt, rng, 8, hd, page, 4000)
+  tables = np.stack([rng.permutation(pages) for _ in range(requests)])
+  lengths = rng.integers(3900, 4001, requests).tolist()
+  b = points_found(rt, rng, pool, values, 16, tables, lengths, [new] * requests, most=new)
+  assert pages_of_a_part(b, lengths) > 64
+  # with a window that leaves a part's first blocks out, and a part's last
+  points_found(rt, rng, pool, values, 16, tables, lengths, [new] * requests, window=3333, most=new)
+
+
+@pytest.mark.parametrize("new", [1, 6])
+def test_attend_a_long_cache_of_short_pages(rt, new):
+  # one request of 65536 keys is cut into 32 parts of 128 pages of 16; of 2^18 keys, of 256 pages of 32
+  rng = np.random.default_rng(new)
+  for page, tokens in ((16, 1 << 16), (32, 1 << 18)):
+    pool, values, pages = shared(rt, rng, 1, 64, page, tokens)
+    b = points_found(rt, rng, pool, values, 8, pages[None], [tokens], [new], most=new)
+    assert pages_of_a_part(b, [tokens]) > 64
+  pool, values, pages = shared(rt, rng, 1, 64, 256, 300032)  # and one whose parts' pages are loaded once each, 38 at most
+  assert pages_of_a_part(points_found(rt, rng, pool, values, 8, pages[None], [300000], [new], most=new), [300000]) <= 64
+
+
+@pytest.mark.parametrize("hd, page, tokens, window", [(64, 16, 2608, 0), (128, 16, 1600, 0), (64, 32, 3008, 0), (64, 64, 4608, 0),
+                                                      (64, 16, 2608, 1500)])
+def test_attend_tiles_of_more_pages_than_a_wave_holds(rt, hd, page, tokens, window):
+  # a prompt of 520 rows of 32 heads over 8, which are tiles enough that none has its keys cut
+  rng = np.random.default_rng(hd + page + window)
+  pool, values, pages = shared(rt, rng, 8, hd, page, tokens)
+  b = points_found(rt, rng, pool, values, 32, pages[None], [tokens - 3], [520], window)
+  need = ctypes.c_uint64()
+  _lib.call("pages_attend_scratch", ctypes.byref(pool.args), ctypes.byref(b.args), 32, window, ctypes.byref(need))
+  items = 2048 // (4 * 8) + 1
+  assert need.value == items * 8 * 32 * (hd + 4) * 4  # the parts' alone: no splits
+  assert min(tokens, window + 520 if window else tokens) > 64 * page
+
+
+def test_attend_parts_of_many_pages_beside_tiles(rt):
+  rng = np.random.default_rng(45)
+  pool, values, pages = shared(rt, rng, 8, 64, 16, 4000)
+  tables = np.stack([rng.permutation(pages) for _ in range(33)])
+  lengths = [4000] * 16 + [2100] + [3990] * 16
+  b = points_found(rt, rng, pool, values, 16, tables, lengths, [1] * 16 + [300] + [2] * 16)
+  assert pages_of_a_part(b, lengths) > 64
