@@ -824,3 +824,47 @@ def test_attend_parts_of_many_pages_beside_tiles(rt):
   lengths = [4000] * 16 + [2100] + [3990] * 16
   b = points_found(rt, rng, pool, values, 16, tables, lengths, [1] * 16 + [300] + [2] * 16)
   assert pages_of_a_part(b, lengths) > 64
+
+
+# ---- verification, 16 logits a lane (past 2^22 logits) and requests of more rows than a block keeps sums of (64)
+
+@pytest.mark.parametrize("rows, vocab", [(40, 131072), (40, 131073), (23, 200001), (15, 300004), (15, 300001), (4200, 1000), (66000, 64)])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_of_more_logits(rt, rows, vocab, drawn):
+  assert rows * vocab > 1 << 22
+  rng = np.random.default_rng(vocab)
+  lengths = rng.integers(0, 8, 2 * rows)
+  starts = np.concatenate([[0], np.cumsum(lengths)])
+  starts = starts[starts <= rows - 2].tolist()
+  logits = 3 * rng.normal(0, 1, (rows, vocab)).astype(np.float32)
+  logits[rng.random((rows, vocab)) < 0.1] = -np.inf
+  logits[:, 0] = 0  # (a weight in every row)
+  p = soft(logits)
+  probs = soft(np.roll(np.where(np.isfinite(logits), logits, -9), 1, 0) + 0.7 * rng.normal(0, 1, logits.shape)).astype(np.float32)
+  upto = np.cumsum(probs, 1, dtype=np.float64)
+  ids = np.minimum((upto < rng.random((rows, 1)) * 0.999).sum(1), vocab - 1) if drawn else np.roll(p, 1, 0).argmax(1)
+  t = rng.uniform(0.5, 2, rows)
+  t[::9] = np.inf
+  for i in range(2):
+    verified(rt, logits, ids, starts, rng.random((2, rows)).astype(np.float32), probs if drawn else None, t.astype(np.float32) if i else None)
+
+
+@pytest.mark.parametrize("vocab", [1000, 1001, 20000])
+@pytest.mark.parametrize("drawn", [True, False])
+def test_verify_of_long_runs_of_drafts(rt, vocab, drawn):
+  # refused at their first draft, the last whose sums are kept, the first whose are not, far behind, or not at all
+  rng = np.random.default_rng(vocab)
+  starts, at = list(range(0, 1051, 150)), (1, 63, 64, 65, 149, None, 100)
+  rows = starts[-1] + 3
+  logits = 3 * rng.normal(0, 1, (rows, vocab)).astype(np.float32)
+  probs = near(rng, logits) if drawn else None
+  ids = np.roll(logits, 1, 0).argmax(1)
+  for t in (None, np.full(rows, np.inf, np.float32), rng.uniform(0.5, 2, rows).astype(np.float32)):
+    u = rng.random((2, rows)).astype(np.float32)
+    u[0] = 0  # any draft that has a weight is accepted
+    refused = ids.copy()
+    odd = logits.copy()
+    for s, k in zip(starts, at):
+      if k is not None: odd[s + k - 1, refused[s + k]] = -np.inf  # the draft at row s + k has none
+    got = verified(rt, odd, refused, starts, u, probs, t)
+    for s, k, n in zip(starts, at, got[1]): assert n == (150 if k is None else k)
