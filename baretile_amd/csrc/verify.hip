@@ -304,7 +304,7 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) veri
 template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_kernel(const VerifyArgs a) {
   const int r = blockIdx.x, lane = threadIdx.x;
   if (r == a.requests) {  // rows of no request: ahead of the first's and behind the last's
-    const int first = min(gload(a.starts), a.rows), last = max(0, gload(a.starts + a.requests));
+    const int first = min(gload(a.starts), a.rows), last = min(max(gload(a.starts + a.requests), 0), a.rows);
     for (int j = lane; j < first; j += 64) a.tokens[j] = -1;
     for (int j = last + lane; j < a.rows; j += 64) a.tokens[j] = -1;
     return;

@@ -7,7 +7,7 @@ import pytest
 from baretile_amd import _lib
 from baretile_amd.models import serve
 from baretile_amd.pages import Pages
-from baretile_amd.tensor import Recording, Tensor, jit
+from baretile_amd.tensor import Recording, Storage, Tensor, jit
 from oracle import bfp as B, pages as P
 
 pytestmark = pytest.mark.gpu
@@ -868,3 +868,53 @@ def test_verify_of_long_runs_of_drafts(rt, vocab, drawn):
       if k is not None: odd[s + k - 1, refused[s + k]] = -np.inf  # the draft at row s + k has none
     got = verified(rt, odd, refused, starts, u, probs, t)
     for s, k, n in zip(starts, at, got[1]): assert n == (150 if k is None else k)
+
+
+# ---- nothing outside: results and scratch between guards, pages of no request
+
+class Guarded:
+  """Device memory of exactly nbytes between guards, all of it a pattern at first."""
+  AHEAD, FILL = 1024, 0x5A5A5A5A
+
+  def __init__(self, rt, nbytes):
+    self.rt, self.nbytes, self.storage = rt, nbytes, Storage(rt, nbytes + 2 * self.AHEAD)
+    assert nbytes % 4 == 0
+    rt.fill32(self.storage.addr, self.FILL, (nbytes + 2 * self.AHEAD) // 4)
+    self.addr = self.storage.addr + self.AHEAD
+
+  def values(self, dtype):
+    """What lies between the guards, which have to be as they were."""
+    a = np.frombuffer(bytes(self.rt.download(self.storage.addr, self.nbytes + 2 * self.AHEAD)), np.uint32)
+    ahead = self.AHEAD // 4
+    assert (a[:ahead] == self.FILL).all() and (a[ahead + self.nbytes // 4:] == self.FILL).all()
+    return a[ahead:ahead + self.nbytes // 4].view(dtype)
+
+
+STRAY = ([0, 10, 9000], [-5, 20, 30], [40, 3, 50], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1], [50, 50, 50], [-1, -1, -1], [0, 50, 0])
+
+
+@pytest.mark.parametrize("vocab, probs", [(1000, True), (1001, False), (100000, True)])
+def test_verify_stays_within_its_memory(rt, vocab, probs):
+  rng = np.random.default_rng(vocab)
+  rows, R = 50, 2
+  logits, ids, u = rng.normal(0, 2, (rows, vocab)).astype(np.float32), rng.integers(-3, vocab + 3, rows), rng.random((2, rows)).astype(np.float32)
+  p = near(rng, logits) if probs else None
+  of = lambda a: Tensor.of(rt, a, "fp32")
+  held = [of(logits), row(rt, ids), of(u), of(p) if probs else None]
+  for starts, drafts in ([([0, 20, 47], None), ([0, 20, 47], [3, 0])] + [(s, None) for s in STRAY] +
+                         [(s, [2 ** 31 - 1, -2 ** 31]) for s in STRAY] + [(s, [7, 1]) for s in STRAY]):
+    s, d = row(rt, starts), row(rt, drafts) if drafts else None
+    tokens, counts = Guarded(rt, 4 * rows), Guarded(rt, 4 * R)
+    args = _lib.VerifyArgs(logits=held[0].addr, probs=held[3].addr if probs else 0, uniforms=held[2].addr, ids=held[1].addr, starts=s.addr,
+                           tokens=tokens.addr, counts=counts.addr, logits_sr=vocab, probs_sr=vocab, uniforms_sr=rows, requests=R, rows=rows,
+                           vocab=vocab, drafts=d.addr if drafts else 0)
+    need = ctypes.c_uint64()
+    _lib.call("verify_scratch", ctypes.byref(args), ctypes.byref(need))
+    scratch = Guarded(rt, need.value)
+    args.scratch, args.scratch_bytes = scratch.addr, need.value
+    rt.run("verify", "verify", ctypes.byref(args))
+    scratch.values(np.uint32)
+    got = tokens.values(np.int32), counts.values(np.int32)
+    if starts == [0, 20, 47]:
+      want = P.verify(logits, ids, starts, u, p, drafts=drafts)
+      assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
