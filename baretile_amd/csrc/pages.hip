@@ -247,7 +247,7 @@ __device__ __forceinline__ Piece whole_piece(const BatchArgs &b, int r) {
   int f0 = gload(b.starts + r), f1 = gload(b.starts + r + 1), len = gload(b.lengths + r);
   asm volatile("" : "+v"(f0), "+v"(f1), "+v"(len));  // all requested at once
   Piece p{r, 0, __builtin_amdgcn_readfirstlane(min(max(f0, 0), b.rows)), 0, 0};
-  p.n = max(__builtin_amdgcn_readfirstlane(min(f1, b.rows)) - p.row0, 0);
+  p.n = __builtin_amdgcn_readfirstlane(min(max(f1, p.row0), b.rows)) - p.row0;
   p.len = max(__builtin_amdgcn_readfirstlane(len), p.n);
   return p;
 }
@@ -1016,7 +1016,7 @@ __global__ void __launch_bounds__(256) pages_join_kernel(const AttendArgs a) {
     first = __builtin_amdgcn_readfirstlane(first);
     const int parts = __builtin_amdgcn_readfirstlane(last) - first;
     p = Piece{r, 0, __builtin_amdgcn_readfirstlane(min(max(f0, 0), a.b.rows)), 0, 0};
-    p.n = __builtin_amdgcn_readfirstlane(min(f1, a.b.rows)) - p.row0;
+    p.n = __builtin_amdgcn_readfirstlane(min(max(f1, p.row0), a.b.rows)) - p.row0;
     if (parts <= 1 || first + parts > a.items || pair >= p.n * a.rep || p.n * a.rep > a.few) return;
     const int64_t step = (int64_t)a.c.kv * a.few * (HD + 4);
     const float *from = a.scratch + first * step + ((int64_t)kvh * a.few + pair) * (HD + 4);

@@ -890,6 +890,19 @@ class Guarded:
     return a[ahead:ahead + self.nbytes // 4].view(dtype)
 
 
+def attend_guarded(rt, pool, b, q, window=0):
+  """Pages.attend's call with its result and exactly the scratch that it asks for between guards: the result's bits."""
+  heads, rows, hd = q.batch, q.rows, q.cols
+  need = ctypes.c_uint64()
+  pair = ctypes.byref(pool.args), ctypes.byref(b.args)
+  _lib.call("pages_attend_scratch", *pair, heads, window, ctypes.byref(need))
+  out, scratch = Guarded(rt, 2 * heads * rows * hd), Guarded(rt, need.value)
+  rt.run("pages_attend", "pages_attend", *pair, q.addr, q.sb, q.sr, out.addr, rows * hd, hd, heads, window, scratch.addr if need.value else 0,
+         need.value)
+  scratch.values(np.uint32)
+  return out.values(np.uint16)
+
+
 STRAY = ([0, 10, 9000], [-5, 20, 30], [40, 3, 50], [2 ** 31 - 1, -2 ** 31, 2 ** 31 - 1], [50, 50, 50], [-1, -1, -1], [0, 50, 0])
 
 
@@ -918,3 +931,22 @@ def test_verify_stays_within_its_memory(rt, vocab, probs):
     if starts == [0, 20, 47]:
       want = P.verify(logits, ids, starts, u, p, drafts=drafts)
       assert np.array_equal(got[0], want[0]) and np.array_equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("new, most, width", [([10, 40], None, 5), ([3, 2], 3, 5), ([3, 2], 1, 5), ([3, 2], 3, 80)])
+def test_stray_starts_touch_nothing_else(rt, new, most, width):
+  # starts that no plan makes: any rows of the batch's own, but no page of another request or of one that is left without rows, no
+  # guard, and no row past the last
+  rng = np.random.default_rng(13)
+  pool, _, tables, _ = filled(rt, rng, 4, 2, 64, 16, [60, 80, 50], width, spare=4)
+  own = np.array(tables)[:2]
+  b, _ = planned(rt, pool, own, [60 - max(new), 80 - max(new)], new, [-1], 50, most=most)
+  x, q = Tensor.of(rt, bf16_rows(rng, 4, 50, 64)), Tensor.of(rt, B.bf16(rng.normal(0, 0.2, (4, 50, 64))))
+  for starts in STRAY:
+    first, last = (np.clip(v, 0, 50) for v in (starts[:-1], starts[1:]))
+    others = np.setdiff1d(np.arange(pool.pages), own[last > first])
+    before = whole(pool)[others], scales(pool)[others]
+    b.starts.assign(row(rt, starts))
+    pool.put(b, x)
+    attend_guarded(rt, pool, b, q)
+    assert np.array_equal(whole(pool)[others], before[0]) and np.array_equal(scales(pool)[others], before[1])
