@@ -950,3 +950,51 @@ def test_stray_starts_touch_nothing_else(rt, new, most, width):
     pool.put(b, x)
     attend_guarded(rt, pool, b, q)
     assert np.array_equal(whole(pool)[others], before[0]) and np.array_equal(scales(pool)[others], before[1])
+
+
+@pytest.mark.parametrize("hd, page, lengths, new, window", [
+  (64, 16, [300, 40, 0, 77], [1, 3, 0, 2], 0), (64, 16, [3000, 40, 2000], [1, 3, 5], 0), (128, 64, [3000, 40, 2000], [5, 1, 9], 0),
+  (64, 32, [3000, 400, 2000], [1, 90, 5], 0), (128, 16, [700, 400], [333, 40], 0), (64, 16, [3000, 2000], [2, 70], 300), (64, 256, [5000, 9], [16, 9], 0)])
+def test_attend_stays_within_its_memory(rt, hd, page, lengths, new, window):
+  rng = np.random.default_rng(hd + page + sum(new))
+  pool, _, tables, _ = filled(rt, rng, 8, 2, hd, page, lengths)
+  rows = sum(new) + 5
+  b, _ = planned(rt, pool, tables, [n - m for n, m in zip(lengths, new)], new, [-1], rows)
+  q = Tensor.of(rt, B.bf16(rng.normal(0, 0.2, (8, rows, hd))))
+  assert attend_guarded(rt, pool, b, q, window).tobytes() == pool.attend(q, b, window).tobytes()
+
+
+@pytest.mark.parametrize("requests, rows", [(1, 1), (5, 33), (300, 900), (3, 2500)])
+def test_plan_stays_within_its_memory(rt, requests, rows):
+  rng = np.random.default_rng(requests)
+  page, width, pages = 16, 40, 3000
+  tables = np.full((requests, width), -1)
+  cached, new, free = rng.integers(0, 300, requests), rng.integers(0, 2 * rows // requests + 2, requests), rng.permutation(pages)
+  t = Guarded(rt, 4 * tables.size)
+  rt.upload(t.addr, tables.astype(np.int32).tobytes())
+  given = [row(rt, v) for v in (cached, new, free)]
+  made = [Guarded(rt, 4 * n) for n in (requests + 1, requests, rows, rows, 1, requests + 2)]  # starts, lengths, places, slots, taken, parts
+  args = _lib.PlanArgs(t.addr, *(g.addr for g in given), 0, *(m.addr for m in made), width, requests, width, pages, rows, page, pages, rows, 2)
+  rt.run("plan", "pages_plan", ctypes.byref(args))
+  want = P.plan(tables, cached, new, free, rows, page, pages)
+  assert np.array_equal(t.values(np.int32).reshape(tables.shape), want[0])
+  got = [m.values(np.int32) for m in made]
+  for g, w in zip(got, want[1:5]): assert np.array_equal(g, w)
+  assert got[4][0] == want[5]
+
+
+def test_plan_counts_blocks_of_many_requests(rt):
+  # 1100 requests of up to 2^28 tokens, over 2 billion blocks of keys in all, scanned in two turns; some bring no row
+  rng = np.random.default_rng(46)
+  pool, requests = Pages(rt, 4, 8, 64, 256), 1100
+  tables = Tensor(rt, requests, 1 << 20, dtype="int32")
+  rt.fill32(tables.addr, -1, requests << 20)
+  cached, new = rng.integers(2 ** 27, 2 ** 28 - 3, requests), rng.integers(0, 3, requests)
+  cached[5], new[5] = 0, 2
+  b = pool.plan(tables, row(rt, cached), row(rt, new), row(rt, [0]), 2200)
+  *parts, per = ints(b.parts).tolist()
+  blocks = np.where(new > 0, -(-(cached + new) // 64), 0)
+  assert blocks.sum() > 1 << 31
+  assert per == min((-(-int(blocks.sum()) // 64) + 3) // 4 * 4, 1 << 24)  # (a part holds one request's, so never more than 2^24)
+  assert parts == [0, *np.cumsum(-(-blocks // np.maximum(per, -(-blocks // 32)))).tolist()] and parts[-1] <= 64 + requests
+  assert np.array_equal(ints(b.lengths), cached + new) and np.array_equal(ints(b.starts), [0, *np.cumsum(new)])
