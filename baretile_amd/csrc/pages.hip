@@ -15,6 +15,7 @@
 // O^T's column is the lane's pair as well, so the running maximum rescales it with no move between lanes.
 #include "common.h"
 #include <algorithm>
+#include <type_traits>
 
 namespace bt {
 
@@ -90,19 +91,18 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int j, int start, in
 // of 64 keys and `least` of them, so that uneven lengths make parts of even length.
 // Latency bounds it: three scans of about a microsecond and two trips to memory. 32 requests of a row: 4.3 us (5.7 by 1024
 // threads, whose scans pass 16 sums through LDS); 512 with 8500 rows: 6.2 and 4.1 us for the rows.
+// LARGE: requests' blocks of keys may pass 2^30 in all (2048 of 2^24 would pass 32 bits), and are summed by their lower 12 bits
+// and the rest. A kernel of its own: decided on the device, every plan took 0.1 us more (32 requests 4.2 us for 4.1).
 // The block writes up to PLAN_ROWS rows itself, past that many blocks of plan_rows_kernel do: 2048 rows 6.8 us here, 3.5 + 3.2 us
 // and a launch more there; 8192 12.4 us and 4.5 + 4.0.
 constexpr int PLAN_ROWS = 2048;
-template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs a) {
+template <int NT, bool LARGE> __global__ void __launch_bounds__(NT) plan_kernel(const PlanArgs a) {
   __shared__ int starts[MOST_REQUESTS + 1], first[MOST_REQUESTS], from[MOST_REQUESTS + 1], cache[MOST_REQUESTS];
   __shared__ int sums[NT / 64];
   const int lg = a.page_log2, room = (int)min((int64_t)a.width << lg, (int64_t)0x40000000);
   const int taken = a.taken ? gload(a.taken) : 0;
-  // blocks of keys may pass 32 bits (2048 requests of 2^24): where they could pass 2^30 they are summed by their lower 12 bits and
-  // the rest
-  const bool large = (int64_t)a.requests * ((room + KB - 1) / KB) > 1 << 30;
   int rows = 0, takes = 0;
-  int64_t blocks = 0;
+  std::conditional_t<LARGE, int64_t, int> blocks = 0;
   for (int base = 0; base < a.requests; base += NT) {
     const int r = base + threadIdx.x;
     int c = 0, n = 0, total;
@@ -126,9 +126,9 @@ template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanAr
     if (r < a.requests) from[r] = takes + off;
     takes += total;
     const int nb = n > 0 ? (min(c + n, room) + KB - 1) / KB : 0;
-    block_exclusive<NT>(large ? nb & 4095 : nb, sums, &total);
+    block_exclusive<NT>(LARGE ? nb & 4095 : nb, sums, &total);
     blocks += total;
-    if (large) block_exclusive<NT>(nb >> 12, sums, &total), blocks += (int64_t)total << 12;
+    if constexpr (LARGE) block_exclusive<NT>(nb >> 12, sums, &total), blocks += (int64_t)total << 12;
   }
   const int last = rows;
   if (threadIdx.x == 0) {
@@ -136,10 +136,9 @@ template <int NT> __global__ void __launch_bounds__(NT) plan_kernel(const PlanAr
     a.starts[a.requests] = last;
     a.taken_out[0] = taken + takes;
   }
-  int each;  // (a part holds one request's blocks, 2^24 at most, however few parts there are for them)
-  if (large) each = (int)min((blocks + a.target - 1) / a.target, (int64_t)(0x40000000 / KB));
-  else each = ((int)blocks + a.target - 1) / a.target;
-  const int per = max(a.least, (each + 3) & ~3);
+  auto each = (blocks + a.target - 1) / a.target;
+  if constexpr (LARGE) each = min(each, (int64_t)(0x40000000 / KB));  // a part holds one request's blocks, 2^24 at most
+  const int per = max(a.least, ((int)each + 3) & ~3);
   int made = 0;
   __syncthreads();
   for (int base = 0; base < a.requests; base += NT) {
@@ -1175,9 +1174,10 @@ int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
                    a->rows, lg, a->pages, std::min(a->most, a->rows), parts_target(a->kv),
                    parts_least((int64_t)a->width * a->page)};
   const int most = std::max(a->requests, a->rows > PLAN_ROWS ? 1 : a->rows);
-  if (most <= 64) plan_kernel<64><<<1, 64, 0, r->stream>>>(k);
-  else if (most <= 256) plan_kernel<256><<<1, 256, 0, r->stream>>>(k);
-  else plan_kernel<1024><<<1, 1024, 0, r->stream>>>(k);
+  if ((int64_t)a->requests * ceil_div((int64_t)a->width * a->page, KB) > 1ll << 30) plan_kernel<1024, true><<<1, 1024, 0, r->stream>>>(k);
+  else if (most <= 64) plan_kernel<64, false><<<1, 64, 0, r->stream>>>(k);
+  else if (most <= 256) plan_kernel<256, false><<<1, 256, 0, r->stream>>>(k);
+  else plan_kernel<1024, false><<<1, 1024, 0, r->stream>>>(k);
   BT_LAUNCHED("a plan");
   if (a->rows > PLAN_ROWS) {
     plan_rows_kernel<<<(unsigned)ceil_div(a->rows, 256), 256, 0, r->stream>>>(k);
