@@ -21,7 +21,7 @@ import operator
 import os
 from types import SimpleNamespace
 import numpy as np
-from baretile_amd.pages import Pages
+from baretile_amd.pages import Batch, Pages
 from baretile_amd.tensor import Tensor, jit
 
 
@@ -477,8 +477,9 @@ def paged_forward(ids, batch, w, c, caches):
   each, a token and its drafts, or chunks of prompts, all in one step (serve.verify takes the logits, and how many of each
   request's rows are drafts). Requests are at most as long as the weights' places (upload). Rows behind the last request's (whose
   ids are anything) give logits of no meaning."""
-  if len(caches) != c.layers or ids.cols != batch.rows:
-    raise ValueError(f"paged_forward needs {c.layers} caches and ids for the batch's {batch.rows} rows: {len(caches)}, {ids.shape}")
+  if not (isinstance(batch, Batch) and isinstance(ids, Tensor) and len(caches) == c.layers and ids.cols == batch.rows):
+    raise ValueError(f"paged_forward needs {c.layers} caches and ids for the batch's {getattr(batch, 'rows', '')} rows: {len(caches)}, "
+                     f"{getattr(ids, 'shape', type(ids))} {type(batch)}")
   x = w["embed"].gather(ids).float()
   rot = (w["cos"].gather(batch.places), w["sin"].gather(batch.places), w["turn"])
   ps = blocks(w, c.layers)

@@ -48,12 +48,12 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None, drafts=None):
   With p = softmax(t * logits) in 64 bits, the draft at row j is accepted where uniforms[0, j] * probs[j, ids[j]] < p[j - 1,
   ids[j]]. tokens, an int32 row, has for each row the token that follows it: accepted drafts, then at the first refusal a token
   drawn with uniforms[1] from what p has over probs, or after the last draft one from p, -1 behind that, ahead of the last
-  token's row and for rows of no request. counts, an int32 row, has each request's new tokens. (So a request's cache holds lengths - drafts - 1 + counts
-  tokens that stand, lengths being its Batch's.)"""
+  token's row and for rows of no request. counts, an int32 row, has each request's new tokens. (So a request's cache holds lengths -
+  drafts - 1 + counts tokens that stand, lengths being its Batch's.)"""
   rt = getattr(logits, "rt", None)
-  for x, dtype in ((logits, "fp32"), (ids, "int32"), (starts, "int32"), (uniforms, "fp32"), (probs, "fp32"), (t, "fp32"),
-                   (drafts, "int32")):
-    if x is not None and not (isinstance(x, Tensor) and x.rt is rt and x.batch == 1 and x.dtype == dtype):
+  given = [(x, dtype) for x, dtype in ((probs, "fp32"), (t, "fp32"), (drafts, "int32")) if x is not None]
+  for x, dtype in [(logits, "fp32"), (ids, "int32"), (starts, "int32"), (uniforms, "fp32"), *given]:
+    if not (isinstance(x, Tensor) and x.rt is rt and x.batch == 1 and x.dtype == dtype):
       raise ValueError(f"verify needs {dtype} matrices on one runtime: {getattr(x, 'dtype', type(x))} {getattr(x, 'shape', '')}")
   rows, vocab = logits.rows, logits.cols
   if not ((ids.rows, ids.cols) == (1, rows) and starts.rows == 1 and starts.cols >= 2 and

@@ -998,3 +998,17 @@ def test_plan_counts_blocks_of_many_requests(rt):
   assert per == min((-(-int(blocks.sum()) // 64) + 3) // 4 * 4, 1 << 24)  # (a part holds one request's, so never more than 2^24)
   assert parts == [0, *np.cumsum(-(-blocks // np.maximum(per, -(-blocks // 32)))).tolist()] and parts[-1] <= 64 + requests
   assert np.array_equal(ints(b.lengths), cached + new) and np.array_equal(ints(b.starts), [0, *np.cumsum(new)])
+
+
+def test_missing_tensors_are_refused(rt):
+  from baretile_amd.models import llama
+  r = lambda *v: row(rt, v)
+  logits, ids, starts, u = Tensor.zeros(rt, 4, 50, dtype="fp32"), r(1, 2, 3, 4), r(0, 4), Tensor.zeros(rt, 2, 4, dtype="fp32")
+  for i in range(4):
+    args = [logits, ids, starts, u]
+    args[i] = None
+    with pytest.raises(ValueError, match="verify needs"): serve.verify(*args)
+  with pytest.raises(ValueError, match="verify needs"): serve.verify(logits, ids, starts, u, drafts=u)
+  dc = llama.smol(layers=1)
+  for bad in ((ids, None), (ids, starts), ([1, 2], None)):
+    with pytest.raises(ValueError, match="paged_forward needs"): llama.paged_forward(*bad, {}, dc, [None])
