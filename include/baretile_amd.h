@@ -393,8 +393,8 @@ int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out);
 /* out[e, j, :] = softmax(q[e, j, :] . k + mask) @ v for the batch's rows j and heads e, over the pages of j's request and
  * key head e / (heads / kv): keys at places up to j's own and, with window > 0, after its place - window. bf16 with
  * element strides; scores, maxima and sums in fp32, the weights rounded to bf16 before they meet v; no scale is applied.
- * Rows behind the last request's are zeros, and so is a row that sees no key. bt_pages_attend_scratch gives the bytes of
- * scratch (16-byte aligned); calls that share one scratch buffer must not overlap. */
+ * Rows behind the last request's are zeros, and so is a row that sees no key, or none that it scores above -inf; a score that is
+ * no number makes its row none. bt_pages_attend_scratch gives the bytes of scratch (16-byte aligned); calls that share one scratch buffer must not overlap. */
 int bt_pages_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t heads, int32_t window, uint64_t *bytes);
 int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr,
                     uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,

@@ -1012,3 +1012,51 @@ def test_missing_tensors_are_refused(rt):
   dc = llama.smol(layers=1)
   for bad in ((ids, None), (ids, starts), ([1, 2], None)):
     with pytest.raises(ValueError, match="paged_forward needs"): llama.paged_forward(*bad, {}, dc, [None])
+
+
+
+def test_attend_scores_below_every_number(rt):
+  # a row that sees only scores of -inf is zeros, as one that sees no key; beside keys with others they weigh nothing
+  rng = np.random.default_rng(47)
+  for lengths, new in (([90, 40], [2, 1]), ([90, 40], [2, 40]), ([2000, 40], [2, 1]), ([2000, 200], [2, 90])):
+    rows = sum(new)
+    pool = Pages(rt, 200, 2, 64, 16)
+    x = np.abs(bf16_rows(rng, 4, sum(lengths), 64)) + 0.5
+    x[0, lengths[0] - 5, 1] = x[1, lengths[0] - 5, 1] = 0  # one key of the first request scores 0 * -inf at dim 1: not a number
+    b, (tables, *_, taken) = planned(rt, pool, np.full((2, 130), -1), [0, 0], lengths, rng.permutation(200), sum(lengths))
+    pool.put(b, Tensor.of(rt, B.bf16(x)))
+    values, s = np.zeros((200, 4, 16, 64)), np.full((200, 4), 2.0 ** -100)
+    P.put(values, s, tables, [0, lengths[0], sum(lengths)], lengths, B.bf16(x))
+    q = np.abs(B.bf16(rng.normal(0, 0.02, (4, rows, 64))))
+    q[0, 0, 0] = q[2, rows - 1, 0] = -np.inf
+    q[3, 1, 1] = -np.inf  # with a key that this row's head scores NaN
+    b, (tables, starts, total, *_) = planned(rt, pool, tables, [n - m for n, m in zip(lengths, new)], new, [-1], rows, taken)
+    got = np.array(pool.attend(Tensor.of(rt, q), b).tolist())
+    odd = np.zeros((4, rows), bool)
+    odd[0, 0] = odd[2, rows - 1] = odd[3, 1] = True
+    assert (got[0, 0] == 0).all() and (got[2, rows - 1] == 0).all() and np.isnan(got[3, 1]).all()
+    q[odd] = 0
+    want, weighed = P.attend(q, values, tables, starts, total)
+    assert np.all(np.abs(got - want)[~odd] <= bound(q, values, weighed, want)[~odd])
+
+
+def test_a_recorded_verification_follows_its_drafts(rt):
+  rng = np.random.default_rng(48)
+  rows, R, vocab = 40, 4, 700
+  logits, ids, starts = Tensor.zeros(rt, rows, vocab, dtype="fp32"), row(rt, [0] * rows), row(rt, [0] * (R + 1))
+  u, drafts = Tensor.zeros(rt, 2, rows, dtype="fp32"), row(rt, [0] * R)
+  step = lambda: serve.verify(logits, ids, starts, u, drafts=drafts)
+  step()
+  rt.wait()
+  rec = Recording(rt)
+  with rec: tokens, counts = step()
+  for i in range(5):
+    ls, us = rng.normal(0, 3, (rows, vocab)).astype(np.float32), rng.random((2, rows)).astype(np.float32)
+    ds = np.roll(ls, 1, 0).argmax(1)
+    at, n = np.sort(rng.choice(rows + 1, R + 1)), rng.integers(-1, 9, R)
+    for t, v, kind in ((logits, ls, "fp32"), (ids, ds[None], "int32"), (starts, at[None], "int32"), (u, us, "fp32"), (drafts, n[None], "int32")):
+      t.assign(Tensor.of(rt, v, kind))
+    rec.send()
+    rt.wait()
+    want = P.verify(ls, ds, at, us, drafts=n)
+    assert np.array_equal(ints(tokens), want[0]) and np.array_equal(ints(counts), want[1]), i
