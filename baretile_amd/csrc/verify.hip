@@ -32,13 +32,14 @@ struct Draw {
 };                                            // is nothing to draw, the one to take (-1: none)
 struct VerifyArgs {
   const float *logits, *probs, *t, *uniforms;
-  const int32_t *ids, *starts, *drafts;
+  const int32_t *ids, *starts;
   int32_t *tokens, *counts;
   ChunkStat *stats;  // [rows][chunks]
   Draw *draws;       // [requests]
   double *left;      // [requests][chunks]: what is left to draw from
   int64_t logits_sr, probs_sr, t_sr, uniforms_sr;
   int32_t requests, rows, vocab, chunks;
+  const int32_t *drafts;  // or null: all of a request's rows but its first
 };
 
 constexpr int WAVES = 4;   // of a block; a chunk each
@@ -58,7 +59,7 @@ __device__ __forceinline__ bool greedy(float t) { return t > 3.4028234663852886e
 __device__ __forceinline__ double in_log2(float t) { return (double)t * 1.4426950408889634074; }
 
 // exp(t (x - m)) as 2^((x - m) t2), t2 = t log2(e): 2^n by the exponent and 2^f, |f| <= 1/2, by the polynomial of degree 9
-// through it at the Chebyshev points, its constant set to 1 so that the largest weigh exactly that (3.3e-14 relative; a draw over
+// through it at the Chebyshev points, its constant set to 1 so that the largest weigh exactly that (3.8e-14 relative; a draw over
 // 2^17 tokens falls on the other side of a border less than once in 10^8). 16 64-bit instructions, where exp() takes about 40
 // and bounded the first launch. -inf and what is below 2^-1074 give 0.
 __device__ __forceinline__ double weight(float x, float m, double t2) {
@@ -237,14 +238,16 @@ __device__ __forceinline__ void left_of(const VerifyArgs &a, const Draw &f, int 
 // The first row of request r that is verified, and how many are: all of its rows, or with drafts its last token's and that many
 // drafts'. `ahead` rows of it lie before them. Within the rows there are, whatever starts and drafts hold.
 __device__ __forceinline__ int request_rows(const VerifyArgs &a, int r, int *n, int *ahead) {
-  const int s0 = gload(a.starts + r), s1 = gload(a.starts + r + 1), d = a.drafts ? gload(a.drafts + r) : NOWHERE;
+  const int s0 = gload(a.starts + r), s1 = gload(a.starts + r + 1), given = gload((a.drafts ? a.drafts : a.starts) + r);
+  const int d = a.drafts ? given : NOWHERE;  // (a load either way: with a branch verify_draw_kernel took 5.7 us for 5.5)
   const int start = min(max(s0, 0), a.rows), rows = min(max(s1, start), a.rows) - start;
   *n = min(max(d, -1), rows - 1) + 1;
   *ahead = rows - *n;
   return start + *ahead;
 }
 
-// Block (request, 4 chunks): the first refused draft, found by every block for itself, then what is left of a chunk a wave.
+// Block (request, 4 chunks): the first refused draft, found by every block for itself (so a request's drafts cost its chunks' number
+// of searches, each as long as the drafts accepted), then what is left of a chunk a wave.
 template <int PER, bool WIDE> __global__ void __launch_bounds__(64 * WAVES) verify_left_kernel(const VerifyArgs a) {
   __shared__ RowStat kept[KEPT];
   __shared__ int refusal;
@@ -396,7 +399,7 @@ template <int PER, bool WIDE> __global__ void __launch_bounds__(64) verify_draw_
 
 // Logits a lane of a chunk's 64: 8 up to 2^22 logits, where larger chunks would leave waves too few to fill the card (5 rows of
 // 49152 12.3 us), else 16, which spreads a chunk's maximum and sums over more of them (112 rows of 131072 in 32 requests: the three
-// launches 13.1, 8.5 and 5.6 us; with 32 a lane, whose draw is one wave's long run, 14.4, 10.4 and 9.3).
+// launches 15.8, 9.3 and 5.5 us; with 32 a lane, whose draw is one wave's long run, 16.7, 10.6 and 8.8).
 static int verify_per(const bt_verify_args *a) { return (int64_t)a->rows * a->vocab <= 1 << 22 ? 8 : 16; }
 static int verify_chunks(const bt_verify_args *a) { return ceil_div(a->vocab, 64 * verify_per(a)); }
 static int check_verify(const bt_verify_args *a) {
