@@ -26,7 +26,7 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 constexpr int KB = 64;          // keys of a block
-constexpr int MOST_PARTS = 32;  // parts of one request (with 64, one request of 65536 keys: 32.4 us against 27.1)
+constexpr int MOST_PARTS = 32;  // parts of one request (64: of 65536 keys 23.0 us and a join of 7.6, for 23.0 + 4.6)
 constexpr int SHORT = 16 * KB;  // keys that tables of one part a request hold at most
 // Waves that attention's parts are for, over all key heads: 8 on each of the 256 CUs, which is what their registers allow at once
 // (8 requests of up to 8191 keys: 19.7 us; with half as many 23.4, with half as many again 22.5).
@@ -89,7 +89,7 @@ __device__ __forceinline__ void plan_row(const PlanArgs &a, int j, int start, in
 // each: first their rows, cut to `most` each and to the rows there are, and the pages they take; then, with the keys' blocks
 // counted, the parts that attention cuts each request's keys into: as many parts over all requests as `target`, of whole blocks
 // of 64 keys and `least` of them, so that uneven lengths make parts of even length.
-// Latency bounds it: three scans of about a microsecond and two trips to memory. 32 requests of a row: 4.3 us (5.7 by 1024
+// Latency bounds it: three scans of about a microsecond and two trips to memory. 32 requests of a row: 4.1 us (5.7 by 1024
 // threads, whose scans pass 16 sums through LDS); 512 with 8500 rows: 6.2 and 4.1 us for the rows.
 // LARGE: requests' blocks of keys may pass 2^30 in all (2048 of 2^24 would pass 32 bits), and are summed by their lower 12 bits
 // and the rest. A kernel of its own: decided on the device, every plan took 0.1 us more (32 requests 4.2 us for 4.1).
@@ -278,9 +278,12 @@ __device__ __forceinline__ float scale_of(float amax) {
 // already holds rows and whose scale grows has them rounded again. Values turn by dimension in LDS, so they are stored as
 // whole words.
 // Memory bounds it where there are many rows: 131072 of 16 heads of 128 (800 MB) 181 us, 4.4 TB/s; a decode step's 32 rows are
-// latency, 5.3 us. Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16
-// by one wave (512 requests of one row 25.8 us, by four waves 48.4, of 8 rows 31.0 and 49.8, all with a search for the request),
-// up to 64 with loads for 64 (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
+// latency, 5.3 us, and so are a few prompts' chunks: 3 requests' 1500 rows of 16 heads of 128 9.1 us for 9.2 MB, in 832 blocks,
+// three or four a CU, whose waves wait 64% of their cycles (for a chain of trips to memory and two barriers; vector instructions
+// are 16%, and of the LDS's 0.32 million cycles 0.19 are bank conflicts).
+// Rows by the most that a request can put into one page, so that registers, LDS and threads fit them: up to 16 by one wave (512
+// requests of one row 25.8 us, by four waves 48.4, of 8 rows 31.0 and 49.8, all with a search for the request), up to 64 with
+// loads for 64 (32 requests of 48 rows 10.2 us, with loads for 256 11.1).
 template <int HD, int NT, int PAGE>
 __global__ void __launch_bounds__(NT) put_pages_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
                                                         int64_t x_sr, int each) {

@@ -6,8 +6,10 @@ forward over every slot recorded once and replayed each step. Around them sits t
 slots that each own a region of every block's KV cache, prompts prefilled in chunks into their slot, a prompt's shared
 prefix reused from a free slot's cache rows, and one replayed decode step for all slots.
 
-Out of scope: sampling (temperature, top-k/top-p/min-p draws), the HTTP server, chat templates, tokenizers and text,
-stop strings, saved sessions, speculative decoding and Qwen's recurrent state. Streams speak token ids.
+Beside it, for callers with steps of their own (llama.paged_forward): `verify`, which checks drafted tokens and draws the next.
+
+Out of scope: sampling loops (top-k/top-p/min-p draws), the draft model and loop of speculative decoding, the HTTP server, chat
+templates, tokenizers and text, stop strings, saved sessions and Qwen's recurrent state. Streams speak token ids.
 """
 import ctypes, queue, threading
 import numpy as np

@@ -7,8 +7,8 @@ under one power of two, which makes each value exact in bf16: half of a bf16 cac
 instruction for two values where a bfp8 cache takes five.
 
 A step over several requests, each with any number of new tokens (a token, a token and its drafts, a prompt's chunk), of which
-the last drafts[r] of request r are drafts (0: none; -1: no token follows
-yet, as behind a chunk that does not end its prompt, or the request brings no row):
+the last drafts[r] of request r are drafts (0: none; -1: no token follows yet, as behind a chunk that does not end its prompt,
+or the request brings no row):
 
   batch = pool.plan(tables, cached, new, free, rows)   # once a step; every block's pool of the same shape shares it
   pool.put(batch, x)                                   # each block's keys and values
@@ -105,8 +105,9 @@ class Pages:
   def put(self, batch, x):
     """Puts the batch's rows into their pages (bt_pages_put): x (2 kv, rows, head) bf16, key heads then value heads, as rope_put
     gives them. Each page and head takes the smallest power of two under which its largest value is at most 448; where a
-    page that holds rows needs a larger one, those are rounded again under it. Rows without a page are dropped. Requests may
-    share pages that they only read; a page that takes rows is one request's."""
+    page that holds rows needs a larger one, those are rounded again under it. It stays so until the page is begun again, also
+    where it was a refused draft's value that needed it. Rows without a page are dropped. Requests may share pages that they
+    only read; a page that takes rows is one request's."""
     self._fits(batch)
     if not (isinstance(x, Tensor) and x.rt is self.rt and x.dtype == "bf16" and
             (x.batch, x.rows, x.cols) == (2 * self.kv, batch.rows, self.head)):

@@ -356,16 +356,16 @@ typedef struct {
   int32_t pages, page, kv, head_dim;
 } bt_pages;
 
-/* A step's plan from its requests' lengths, all int32. Request r (of `requests`, up to 2048) holds cached[r] tokens and brings
- * n = fresh[r] more (0 if negative), at most `most`, and as many as fit in the `rows` rows (up to 2^20) behind those of
- * the requests before it. Written: starts[requests + 1], each one's first row and the end of the last's; lengths[r] =
- * cached[r] + n; for every row, places[rows] (its token's place) and slots[rows] (table entry * page + place % page, where
- * a flat cache of pages * page rows would hold it), -1 behind the last request's rows, and slots also where there is no
- * page. Table entries from the first page not begun, cached / page rounded up, to the last that the new length needs are
- * kept up to the first that holds no page; the others are taken from free_pages in order, after the first taken[0] (0
- * without taken), -1 where these run out. taken_out[0] is taken[0] plus the entries so made: past n_free, so many pages
- * were missing. Entries past the tables' width are not made. parts[requests + 2] is bt_pages_attend's, for caches of kv
- * key heads: how it cuts the requests' keys. */
+/* A step's plan from its requests' lengths, all int32. Request r (of `requests`, up to 2048) holds cached[r] tokens
+ * (held to 0 .. width * page) and brings n = fresh[r] more (0 if negative), at most `most`, and as many as fit in the
+ * `rows` rows (up to 2^20) behind those of the requests before it. Written: starts[requests + 1], each one's first row
+ * and the end of the last's; lengths[r] = cached[r] + n; for every row, places[rows] (its token's place) and
+ * slots[rows] (table entry * page + place % page, where a flat cache of pages * page rows would hold it), -1 behind the
+ * last request's rows, and slots also where there is no page. Table entries from the first page not begun, cached /
+ * page rounded up, to the last that the new length needs are kept up to the first that holds no page; the others are
+ * taken from free_pages in order, after the first taken[0] (0 without taken), -1 where these run out. taken_out[0] is
+ * taken[0] plus the entries so made: past n_free, so many pages were missing. Entries past the tables' width are not
+ * made. parts[requests + 2] is bt_pages_attend's, for caches of kv key heads: how it cuts the requests' keys. */
 typedef struct {
   uint64_t tables, cached, fresh, free_pages, taken;
   uint64_t starts, lengths, places, slots, taken_out, parts;
@@ -382,19 +382,21 @@ typedef struct {
   int32_t requests, width, rows, most;
 } bt_batch;
 
-/* The batch's rows of 2 kv heads, x bf16 (element strides x_sb a head, x_sr a row), into their pages. A page's head takes the
- * smallest power of two s with every finite value at most 448 s in size; a page that holds rows keeps the larger of its own and the
- * new rows', and where that grows its rows are rounded again. Values round to nearest even; infinities and NaNs are stored as the
- * largest value of their sign. No page may take rows twice in one put: two requests, or two entries of one, that name the
- * same page to put rows into give either's. */
+/* The batch's rows of 2 kv heads, x bf16 (element strides x_sb a head, x_sr a row), into their pages. A page's head
+ * takes the smallest power of two s with every finite value at most 448 s in size; a page that holds rows keeps the
+ * larger of its own and the new rows', and where that grows its rows are rounded again. It stays so until the page is
+ * begun again, also where it was a refused draft's value that needed it. Values round to nearest even; infinities and
+ * NaNs are stored as the largest value of their sign. No page may take rows twice in one put: two requests, or two
+ * entries of one, that name the same page to put rows into give either's. */
 int bt_pages_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t x, int64_t x_sb, int64_t x_sr);
 /* Every page as bf16, [pages][2 kv][page][head_dim]. */
 int bt_pages_read(bt_runtime *rt, const bt_pages *pool, uint64_t out);
-/* out[e, j, :] = softmax(q[e, j, :] . k + mask) @ v for the batch's rows j and heads e, over the pages of j's request and
- * key head e / (heads / kv): keys at places up to j's own and, with window > 0, after its place - window. bf16 with
- * element strides; scores, maxima and sums in fp32, the weights rounded to bf16 before they meet v; no scale is applied.
- * Rows behind the last request's are zeros, and so is a row that sees no key, or none that it scores above -inf; a score that is
- * no number makes its row none. bt_pages_attend_scratch gives the bytes of scratch (16-byte aligned); calls that share one scratch buffer must not overlap. */
+/* out[e, j, :] = softmax(q[e, j, :] . k + mask) @ v for the batch's rows j and heads e, over the pages of j's request
+ * and key head e / (heads / kv): keys at places up to j's own and, with window > 0, after its place - window. bf16 with
+ * element strides; scores, maxima and sums in fp32, the weights rounded to bf16 before they meet v; no scale is
+ * applied. Rows behind the last request's are zeros, and so is a row that sees no key, or none that it scores above
+ * -inf; a score of NaN makes its row NaN. bt_pages_attend_scratch gives the bytes of scratch (16-byte aligned); calls
+ * that share one scratch buffer must not overlap. */
 int bt_pages_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t heads, int32_t window, uint64_t *bytes);
 int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr,
                     uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,
