@@ -1177,7 +1177,8 @@ int bt_pages_plan(bt_runtime *rt, const bt_plan_args *a) {
                    a->rows, lg, a->pages, std::min(a->most, a->rows), parts_target(a->kv),
                    parts_least((int64_t)a->width * a->page)};
   const int most = std::max(a->requests, a->rows > PLAN_ROWS ? 1 : a->rows);
-  if ((int64_t)a->requests * ceil_div((int64_t)a->width * a->page, KB) > 1ll << 30) plan_kernel<1024, true><<<1, 1024, 0, r->stream>>>(k);
+  const int64_t blocks = (int64_t)a->requests * ceil_div((int64_t)a->width * a->page, KB);  // of keys, at most
+  if (blocks > 1 << 30) plan_kernel<1024, true><<<1, 1024, 0, r->stream>>>(k);
   else if (most <= 64) plan_kernel<64, false><<<1, 64, 0, r->stream>>>(k);
   else if (most <= 256) plan_kernel<256, false><<<1, 256, 0, r->stream>>>(k);
   else plan_kernel<1024, false><<<1, 1024, 0, r->stream>>>(k);

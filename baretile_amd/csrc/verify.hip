@@ -1,7 +1,7 @@
 // Drafted tokens checked against the target's probabilities, from random numbers that the caller draws.
 //
-// For a request whose rows bring a token and then its drafts (behind a prompt's other rows, where `drafts` counts them), p_j = softmax(t_j x_j) of row j's logits is the target's choice
-// of the token after row j, and q_j the distribution that the draft fed at row j was drawn from. Row j's draft d is
+// For a request whose rows bring a token and then its drafts (behind a prompt's other rows, where `drafts` counts them), p_j =
+// softmax(t_j x_j) of row j's logits is the target's choice of the token after row j, and q_j the distribution that the draft fed at row j was drawn from. Row j's draft d is
 // accepted where u0_j q_j(d) < p_{j-1}(d). The first refusal, after row j, draws from max(p_j - q_{j+1}, 0); where every
 // draft was accepted the last row draws from p: the first token whose running sum passes u1_j times the whole. Tokens
 // so drawn are distributed as the target's own (speculative sampling: Leviathan, Kalman and Matias, 2023).
