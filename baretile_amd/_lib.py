@@ -132,6 +132,11 @@ SIGNATURES = {
   "bt_pages_read": [RT, POINTER(PagesArgs), U64],
   "bt_pages_attend_scratch": [POINTER(PagesArgs), POINTER(BatchArgs), c_int32, c_int32, POINTER(c_uint64)],
   "bt_pages_attend": [RT, POINTER(PagesArgs), POINTER(BatchArgs), U64, I64, I64, U64, I64, I64, c_int32, c_int32, U64, U64],
+  "bt_pages4_bytes": [POINTER(PagesArgs), POINTER(c_uint64)],
+  "bt_pages4_put": [RT, POINTER(PagesArgs), POINTER(BatchArgs), U64, I64, I64],
+  "bt_pages4_read": [RT, POINTER(PagesArgs), U64],
+  "bt_pages4_attend_scratch": [POINTER(PagesArgs), POINTER(BatchArgs), c_int32, c_int32, POINTER(c_uint64)],
+  "bt_pages4_attend": [RT, POINTER(PagesArgs), POINTER(BatchArgs), U64, I64, I64, U64, I64, I64, c_int32, c_int32, U64, U64],
   "bt_verify_scratch": [POINTER(VerifyArgs), POINTER(c_uint64)], "bt_verify": [RT, POINTER(VerifyArgs)],
 }
 

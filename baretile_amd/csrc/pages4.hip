@@ -1,0 +1,588 @@
+// The paged KV cache in 4 bits a value: rows put into their pages, attention over the pages, and the pages read back. Plans,
+// batches, parts, tiles and joins are the 8-bit cache's (pages.h, pages.hip).
+//
+// A value is a code of one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign (e2m1) times a scale. v_cvt_scalef32_pk_bf16_fp4 turns a byte
+// into two bf16 values times a power of two, so a key's scale, a power of two for 32 of its dims, costs nothing there. A value
+// row has one scale for all of its dims, which the weights of its key are multiplied by before they meet it: O = sum (p_t s_t) c_t.
+// That scale has two bits behind its leading one, since it costs the same (rows of uneven channels: their rounding's error 0.126 of
+// their size for 0.150 under powers of two; 0.126 and 0.127 are a key's under one scale of full precision and under a power of
+// two for each 32 dims). Every scale belongs to one row, so a row's codes are final when it is put: no page is rounded again as it
+// fills, and what it holds doesn't depend on how its rows came.
+//
+// A page is one run of bytes, for every key head (`kv` of them) a record of
+//   keys' codes    [page][HD / 2]              a row's dims in order, the even one in a byte's low half;
+//   keys' scales   [page / 16][HD / 32][4][4]  the exponent (biased by 127) of token 16 a + 4 j + i at [a][dims][i][j];
+//   values' codes  [page / 16][HD / 32][16][2][8]  16 tokens of dim 32 c + 16 j + n at [a][c][n][j], the even one in the low half;
+//   values' scales [page]                      bf16.
+// so that attention's operands lie as its lanes take them (pages.hip has the two products): lane (n, g) of a wave holds for tile
+// kt of a block of 64 keys the key 16 (n / 4) + 4 kt + n % 4, dims HD / 4 g and on, which are the codes of all four contraction
+// steps, in one load (the contraction takes dims in any order that both operands share), with the four tiles' exponents in a word; and
+// for dims 32 c .. + 31 the codes of its keys 16 g .. + 15 for dims 32 c + n and 32 c + 16 + n in another.
+#include "pages.h"
+
+namespace bt {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// Where the parts of a key head's record of a page start.
+template <int HD> struct Record {
+  static constexpr int ROW = HD / 2;  // bytes of a row's codes
+  static __host__ __device__ constexpr int key_scales(int lg) { return ROW << lg; }
+  static __host__ __device__ constexpr int values(int lg) { return (ROW + HD / 32) << lg; }
+  static __host__ __device__ constexpr int value_scales(int lg) { return (HD + HD / 32) << lg; }
+  static __host__ __device__ constexpr int bytes(int lg) { return (HD + HD / 32 + 2) << lg; }
+};
+template <int HD> __device__ __forceinline__ uint8_t *record_of(const PoolArgs &c, int id, int kvh) {
+  return c.values + ((int64_t)id * c.kv + kvh) * Record<HD>::bytes(c.page_log2);
+}
+
+template <int SEL> __device__ __forceinline__ uint32_t fp4_pair(uint32_t w, float s) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, SEL));
+}
+__device__ __forceinline__ bf16x8 fp4_to_bf16(uint32_t w, float s) {
+  return __builtin_bit_cast(bf16x8, u32x4{fp4_pair<0>(w, s), fp4_pair<1>(w, s), fp4_pair<2>(w, s), fp4_pair<3>(w, s)});
+}
+// 8 values of at most 6 in size after their rounding as codes, nearest, ties to even.
+__device__ __forceinline__ uint32_t fp4_codes(const float (&x)[8], float s) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[0], x[1], s, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[2], x[3], s, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[4], x[5], s, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[6], x[7], s, 3);
+}
+__device__ __forceinline__ float two(int e) { return __uint_as_float((uint32_t)e << 23); }  // 2^(e - 127)
+
+constexpr int LEAST_E = 27, MOST_E = 227;  // the scales' exponents, biased: 2^-100 to 2^100
+
+// The smallest power of two s with amax <= 7 s, so that no value is off by more than half the largest step, 2 s: its exponent.
+__device__ __forceinline__ int key_exponent(float amax) {
+  const uint32_t b = __float_as_uint(amax);  // 7 = 1.75 * 2^2
+  return min(max((int)(b >> 23) - ((b & 0x7FFFFFu) > 0x600000u ? 1 : 2), LEAST_E), MOST_E);
+}
+// The smallest s = k / 4 * 2^e, k = 4 .. 7, with amax <= 7 s.
+__device__ __forceinline__ float value_scale(float amax) {
+  const float half = two(key_exponent(amax) - 1);
+  float s = 2.0f * half;
+#pragma unroll
+  for (int k = 7; k >= 4; k--) s = amax <= 7.0f * (half * (0.25f * k)) ? half * (0.25f * k) : s;
+  return fmaxf(s, two(LEAST_E));
+}
+
+// ---- rows into pages ------------------------------------------------------------------------------------------------
+
+// A wave: the rows that one request puts into 16 tokens of one head. Rows are loaded once, all at once, and each one's scale is
+// made by its own lanes. Values turn by dimension in the wave's own LDS; tokens of the 16 that take no row keep their codes.
+template <int HD, int W>
+__global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
+                                                             int64_t x_sr, int each, int groups) {
+  constexpr int U = HD / 8, RP = 64 / U, TURNS = 16 / RP;  // 16-byte units of a row, rows of a turn
+  constexpr int LINE = 20;                                 // bytes of a dim in LDS: 16 tokens, and 4 so that dims fall in distinct banks
+  __shared__ __attribute__((aligned(16))) uint8_t turned[W][HD * LINE];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = c.page_log2;
+  const int at = blockIdx.x / groups, h = (blockIdx.x - at * groups) * W + w;
+  if (h >= 2 * c.kv) return;
+  Piece p;
+  if (each) {  // pieces of every request
+    p = whole_piece(b, at / each);
+    p.k = at - p.r * each;
+  } else if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> 4) + 2 * i; }, &p)) {
+    return;  // request r owns pieces starts[r] / 16 + 2 r and on: at least as many as the 16 tokens its rows touch
+  }
+  const int cached = p.len - p.n, token0 = ((cached >> 4) + p.k) << 4;
+  const int from = max(cached, token0), count = min(p.len, token0 + 16) - from, held = from - token0;
+  const int on = token0 >> lg, in = token0 & ((1 << lg) - 1);
+  if (count <= 0 || on >= b.width) return;
+  const int id = gload(b.tables + p.r * b.tables_sr + on);  // the rows are requested before it is looked at
+  const int unit = lane % U, row0 = lane / U;
+  const uint16_t *src = x + h * x_sb + (int64_t)(p.row0 + from - cached) * x_sr + 8 * unit;
+  u32x4 v[TURNS];
+#pragma unroll
+  for (int i = 0; i < TURNS; i++)  // (past the last row it is read again, so that no load waits behind a lane's branch)
+    if (RP * i < count) v[i] = gload((const u32x4 *)(src + min(row0 + RP * i, count - 1) * x_sr));
+  if ((uint32_t)id >= (uint32_t)c.pages) return;
+  const bool value = h >= c.kv;
+  uint8_t *rec = record_of<HD>(c, id, value ? h - c.kv : h);
+#pragma unroll
+  for (int i = 0; i < TURNS; i++) {
+    if (RP * i >= count) break;
+    const int row = row0 + RP * i, token = held + row;
+    float f[8], top = 0.0f;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      f[k] = __uint_as_float(k & 1 ? v[i][k / 2] & 0xFFFF0000u : v[i][k / 2] << 16);
+      top = fmaxf(top, (__float_as_uint(f[k]) & 0x7FFFFFFFu) < 0x7F800000u ? fabsf(f[k]) : 0.0f);
+    }
+    top = fmaxf(top, __shfl_xor(top, 1, 64)), top = fmaxf(top, __shfl_xor(top, 2, 64));  // 32 dims
+    if (!value) {
+      const int e = key_exponent(top);
+      const float s = two(e), most = 7.0f * s;
+#pragma unroll
+      for (int k = 0; k < 8; k++) f[k] = __builtin_copysignf(fminf(fabsf(f[k]), most), f[k]);  // (NaN: the most)
+      if (row < count) {
+        *(uint32_t *)(rec + (in + token) * Record<HD>::ROW + 4 * unit) = fp4_codes(f, s);
+        if (unit % 4 == 0) rec[Record<HD>::key_scales(lg) + in * (HD / 32) + 4 * unit + 4 * (token & 3) + (token >> 2)] = (uint8_t)e;
+      }
+    } else {
+#pragma unroll
+      for (int d = 4; d < U; d *= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
+      const float s = value_scale(top), inv = 1.0f / s;
+#pragma unroll
+      for (int k = 0; k < 8; k++) {
+        // x / s to 16 bits of precision: a quotient on the border between two codes comes out exactly there, and any other is
+        // 1 / 255 of it away at least (x has 8 bits, s times a border 6)
+        const float q = __uint_as_float((__float_as_uint(fminf(fabsf(f[k] * inv), 7.0f)) + 0x80u) & ~0xFFu);
+        f[k] = __builtin_copysignf(q, f[k]);
+      }
+      if (row < count) {
+        const uint32_t codes = fp4_codes(f, 1.0f);
+        uint8_t *to = turned[w] + 8 * unit * LINE + token;
+#pragma unroll
+        for (int k = 0; k < 8; k++) to[k * LINE] = (uint8_t)(codes >> 4 * k & 15);
+        if (unit == 0) ((uint16_t *)(rec + Record<HD>::value_scales(lg)))[in + token] = (uint16_t)(__float_as_uint(s) >> 16);
+      }
+    }
+  }
+  if (!value) return;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  uint64_t *to = (uint64_t *)(rec + Record<HD>::values(lg) + in * Record<HD>::ROW);
+  const uint64_t upto = held + count == 16 ? ~0ull : (1ull << 4 * (held + count)) - 1, fresh = upto & ~((1ull << 4 * held) - 1);
+#pragma unroll
+  for (int i = 0; i < HD / 64; i++) {
+    const int e = (HD / 64) * lane + i, dim = e >> 5 << 5 | (e & 1) << 4 | (e >> 1 & 15);
+    const uint32_t *line = (const uint32_t *)(turned[w] + dim * LINE);
+    uint32_t half[2];
+#pragma unroll
+    for (int k = 0; k < 2; k++) {  // a byte a token to half a byte
+      const uint32_t lo = line[2 * k] & 0x0F0F0F0Fu, hi = line[2 * k + 1] & 0x0F0F0F0Fu;  // (anything where no row is)
+      half[k] = __builtin_amdgcn_perm(hi | hi >> 4, lo | lo >> 4, 0x06040200);
+    }
+    const uint64_t now = (uint64_t)half[1] << 32 | half[0];
+    to[e] = fresh == ~0ull ? now : (now & fresh) | (to[e] & ~fresh);
+  }
+}
+
+// A block: 64 tokens of a page (or all of a shorter one), keys' or values', of one key head as bf16 rows, 16 tokens a wave. Values
+// turn back through the wave's LDS.
+template <int HD>
+__global__ void __launch_bounds__(256) read_pages4_kernel(const PoolArgs c, uint16_t *out, int runs) {
+  constexpr int U = HD / 8, RP = 64 / U, LINE = HD + 8;  // (rows of LDS 16 bytes apart from a power of two)
+  __shared__ __attribute__((aligned(16))) uint16_t turned[4][16 * LINE];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = c.page_log2, heads = 2 * c.kv;
+  const int64_t unit = blockIdx.x / runs;
+  const int in = 64 * (int)(blockIdx.x - unit * runs) + 16 * w, h = (int)(unit % heads);
+  if (in >> lg) return;
+  const bool value = h >= c.kv;
+  const uint8_t *rec = record_of<HD>(c, (int)(unit / heads), value ? h - c.kv : h);
+  uint16_t *to = out + ((unit << lg) + in) * HD;
+  if (!value) {
+#pragma unroll
+    for (int i = 0; i < 16 / RP; i++) {
+      const int row = lane / U + RP * i, u = lane % U;
+      const uint32_t codes = gload((const uint32_t *)(rec + (in + row) * Record<HD>::ROW + 4 * u));
+      const float s = two(gload(rec + Record<HD>::key_scales(lg) + in * (HD / 32) + 4 * (u & ~3) + 4 * (row & 3) + (row >> 2)));
+      *(uint4 *)(to + row * HD + 8 * u) = __builtin_bit_cast(uint4, fp4_to_bf16(codes, s));
+    }
+    return;
+  }
+  const u32x2 *codes = (const u32x2 *)(rec + Record<HD>::values(lg) + in * Record<HD>::ROW);
+  const uint16_t *scales = (const uint16_t *)(rec + Record<HD>::value_scales(lg)) + in;
+  float s[16];
+#pragma unroll
+  for (int t = 0; t < 16; t++) s[t] = __uint_as_float((uint32_t)gload(scales + t) << 16);
+#pragma unroll
+  for (int i = 0; i < HD / 64; i++) {
+    const int e = 64 * i + lane, dim = e >> 5 << 5 | (e & 1) << 4 | (e >> 1 & 15);
+    const u32x2 x = gload(codes + e);
+#pragma unroll
+    for (int k = 0; k < 2; k++) {
+      const u32x4 v = __builtin_bit_cast(u32x4, fp4_to_bf16(x[k], 1.0f));
+#pragma unroll
+      for (int t = 0; t < 8; t++) {  // times its row's scale: 5 bits, exact
+        const float f = __uint_as_float(t & 1 ? v[t / 2] & 0xFFFF0000u : v[t / 2] << 16) * s[8 * k + t];
+        turned[w][(8 * k + t) * LINE + dim] = (uint16_t)(__float_as_uint(f) >> 16);
+      }
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int i = 0; i < 16 / RP; i++) {
+    const int row = lane / U + RP * i, u = lane % U;
+    *(uint4 *)(to + row * HD + 8 * u) = *(const uint4 *)(turned[w] + row * LINE + 8 * u);
+  }
+}
+
+// ---- attention over pages --------------------------------------------------------------------------------------------
+
+// 64 of a request's pages from page `p0` on, one a lane (-1: none, whose keys are hidden).
+__device__ __forceinline__ int page_ids(const AttendArgs &a, int r, int p0, int lane) {
+  const int p = p0 + lane, id = p < a.b.width ? gload(a.b.tables + r * a.b.tables_sr + p) : -1;
+  return (uint32_t)id < (uint32_t)a.c.pages ? id : -1;
+}
+// The page that key `key` lies in. ONE: blocks of 64 keys lie in one page (of 64 tokens or more), so `key` is the wave's.
+template <bool ONE> __device__ __forceinline__ int page_of(int ids, int p0, int key, int lg) {
+  if constexpr (ONE) return __builtin_amdgcn_readlane(ids, (key >> lg) - p0);
+  else return __shfl(ids, (key >> lg) - p0, 64);
+}
+
+// What a lane holds of a block of 64 keys: its codes, its keys' exponents for the four tiles, its 16 values' scales.
+template <int HD> struct Block4 {
+  static constexpr int KW = HD / 32;  // words of a key's codes
+  uint32_t k[4][KW];
+  uint32_t ks;
+  u32x4 v[HD / 32], vs[2];
+};
+// The weights of a block's 16 pairs, times the values' scales, as bf16: rounded to nearest, since the second product's operand is
+// bf16. l sums them in 32 bits before either, so that a row's weights add up to 1 but for that rounding.
+template <int HD>
+__device__ __forceinline__ void weigh4(Running<HD> &st, const f32x4 (&s)[4], const u32x4 (&vs)[2], bf16x8 (&p)[2]) {
+  const float ref = st.reference(s);
+  u32x4 w[2];
+#pragma unroll
+  for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+    for (int i = 0; i < 4; i += 2) {
+      const uint32_t both = vs[kt / 2][kt % 2 * 2 + i / 2];
+      const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i], LOG2E, -ref));
+      const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kt][i + 1], LOG2E, -ref));
+      st.l += e0 + e1;
+      w[kt / 2][kt % 2 * 2 + i / 2] = pack_rne(e0 * __uint_as_float(both << 16), e1 * __uint_as_float(both & 0xFFFF0000u));
+    }
+  p[0] = __builtin_bit_cast(bf16x8, w[0]), p[1] = __builtin_bit_cast(bf16x8, w[1]);
+}
+
+// One block of 64 keys against QT tiles of pairs, as fold_block in pages.hip. key: the lane's first key, seen: whether their page is
+// one; values(c): the lane's codes of dims 32 c ..; between: run once the scores are made.
+template <int HD, int QT, class Keys, class Values, class Between>
+__device__ __forceinline__ void fold4(const Query<HD, HD / 4> (&q)[QT], Running<HD> (&st)[QT], int key, bool seen, uint32_t ks,
+                                      const u32x4 (&vs)[2], Keys keys, Values values, Between between) {
+  constexpr int KW = HD / 32;
+  f32x4 s[QT][4];
+#pragma unroll
+  for (int kp = 0; kp < 4; kp += 2) {
+    bf16x8 kf[2][KW];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+      const float scale = two(ks >> 8 * (kp + i) & 255);
+#pragma unroll
+      for (int j = 0; j < KW; j++) kf[i][j] = fp4_to_bf16(keys(kp + i, j), scale);
+    }
+#pragma unroll
+    for (int k = 0; k < KW; k++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          if (k == 0) s[t][kp + i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+          s[t][kp + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf[i][k], q[t].f[k], s[t][kp + i], 0, 0, 0);
+        }
+  }
+  between();
+  bf16x8 w[QT][2];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int lo = q[t].lo - key, hi = seen ? q[t].hi - key : -1;
+    if (!__all(lo <= 0 && hi >= 15)) {
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++)
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+          if (4 * kt + i < lo || 4 * kt + i > hi) s[t][kt][i] = -INF;
+    }
+    weigh4<HD>(st[t], s[t], vs, w[t]);
+  }
+#pragma unroll
+  for (int c = 0; c < HD / 32; c++) {
+    const u32x4 x = values(c);
+    bf16x8 v[2][2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) v[i][0] = fp4_to_bf16(x[2 * i], 1.0f), v[i][1] = fp4_to_bf16(x[2 * i + 1], 1.0f);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+          st[t].o[2 * c + i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v[i][h], w[t][h], st[t].o[2 * c + i], 0, 0, 0);
+  }
+}
+
+// Few query pairs a request, a part a block of NW waves, as few_pairs in pages.hip.
+template <int HD, int QT, int NW, bool ONE>
+__device__ __forceinline__ void few_pairs4(const AttendArgs &a, const int block, const int tid, FewLds<HD, QT, NW> &lds) {
+  constexpr int KW = HD / 32, V = HD / 32;
+  using R = Record<HD>;
+  const int lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  Part p;
+  take_part<HD, QT, NW>(a, block, tid, &p);
+  const int kvh = p.kvh, b0 = p.b0, b1 = p.b1;
+  Query<HD, HD / 4> q[QT];
+  Running<HD> st[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    if (p.real) q[t].load(a, p, kvh, p.pair0 + 16 * t + n, g);
+    st[t].clear();
+  }
+  if (b0 < b1) {
+    int p0 = b0 * KB >> lg;
+    int ids = page_ids(a, p.r, p0, lane);
+    Block4<HD> x;
+    const auto turn = [&](int b) {  // the 64 pages that block b's keys lie in, if they are not there yet
+      if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, ids = page_ids(a, p.r, p0, lane);
+    };
+    const uint32_t krow = ((ONE ? 16 * (n >> 2) : 0) + (n & 3)) * R::ROW + R::ROW / 4 * g;
+    const uint32_t kscale = (ONE ? (n >> 2) * (HD / 2) : 0) + (HD == 128 ? g : g >> 1) * 16 + (n & 3) * 4;
+    const uint32_t vrow = (ONE ? g * 16 * R::ROW : 0) + 16 * n, vscale = ONE ? 32 * g : 0;
+    const auto fetch_keys = [&](int b) {
+      const int key = b * KB + (ONE ? 0 : 16 * (n >> 2)), in = key & mask;
+      const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh), *k = rec + in * R::ROW;
+#pragma unroll
+      for (int kt = 0; kt < 4; kt++) {
+        if constexpr (HD == 128) {
+          const u32x4 w = __builtin_nontemporal_load((const u32x4 *)(k + (krow + 4 * kt * R::ROW)));
+#pragma unroll
+          for (int j = 0; j < KW; j++) x.k[kt][j] = w[j];
+        } else {
+          const u32x2 w = __builtin_nontemporal_load((const u32x2 *)(k + (krow + 4 * kt * R::ROW)));
+#pragma unroll
+          for (int j = 0; j < KW; j++) x.k[kt][j] = w[j];
+        }
+      }
+      x.ks = __builtin_nontemporal_load((const uint32_t *)(rec + R::key_scales(lg) + in * (HD / 32) + kscale));
+    };
+    const auto fetch_values = [&](int b) {
+      const int key = b * KB + (ONE ? 0 : 16 * g), in = key & mask;
+      const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh), *v = rec + R::values(lg) + in * R::ROW;
+      const u32x4 *vs = (const u32x4 *)(rec + R::value_scales(lg) + 2 * in + vscale);
+#pragma unroll
+      for (int i = 0; i < 2; i++) x.vs[i] = __builtin_nontemporal_load(vs + i);
+#pragma unroll
+      for (int c = 0; c < V; c++) x.v[c] = __builtin_nontemporal_load((const u32x4 *)(v + 256 * c + vrow));
+    };
+    fetch_keys(b0), fetch_values(b0);
+    for (int b = b0; b < b1; b += NW) {
+      const bool more = b + NW < b1;
+      const bool seen = page_of<ONE>(ids, p0, b * KB + (ONE ? 0 : 16 * g), lg) >= 0;
+      fold4<HD, QT>(q, st, b * KB + 16 * g, seen, x.ks, x.vs, [&](int kt, int j) { return x.k[kt][j]; },
+                    [&](int c) { return x.v[c]; }, [&] {
+                      if (more) turn(b + NW), fetch_keys(b + NW);
+                    });
+      if (more) fetch_values(b + NW);
+    }
+  }
+  finish_part<HD, QT, NW>(a, p, tid, st, lds);
+}
+
+template <int HD, int QT, int NW, bool ONE>
+__global__ void __launch_bounds__(64 * NW, 2) pages4_few_kernel(const AttendArgs a) {
+  __shared__ FewLds<HD, QT, NW> lds;
+  few_pairs4<HD, QT, NW, ONE>(a, blockIdx.x, threadIdx.x, lds);
+}
+
+// Many query pairs a request, 128 of one key head a block, as many_pairs in pages.hip: blocks of keys pass through LDS as codes
+// (8 KB a block of 64 keys and heads of 128), their scales straight into registers. Keys' 16-byte units are placed so that the 16
+// lanes of a read meet distinct banks: unit u of row r at u ^ r / 16 (heads of 64: 8-byte units); values' lie as they are read.
+template <int HD> struct Many4Lds {
+  __attribute__((aligned(16))) uint8_t k[2][2][KB * HD / 2], v[2][2][KB * HD / 2];  // [half][stage]
+  float sums[8 * 64];
+};
+template <int HD, bool ONE> __device__ __forceinline__ void many_pairs4(const AttendArgs &a, const int block, Many4Lds<HD> &lds) {
+  using R = Record<HD>;
+  constexpr int UNITS = 2 * HD, NU = 2 * UNITS / 256;  // 16-byte units of a block's keys (its values as many), of both a thread
+  const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int kvh = block % a.c.kv, unit = block / a.c.kv, split = unit % a.splits;
+  const int slot = a.tiles - 1 - unit / a.splits;  // the longest rows first
+  Piece p;
+  if (!find_tile(a, slot, lane, &p)) return;
+  const int pairs = p.n * a.rep, pair0 = TILE * p.k, mine0 = pair0 + 32 * wave;
+  Query<HD, HD / 4> q[2];
+  Running<HD> st[2];
+#pragma unroll
+  for (int t = 0; t < 2; t++) q[t].load(a, p, kvh, mine0 + 16 * t + n, g), st[t].clear();
+  const int cached = p.len - p.n, room = min(p.len, a.b.width << lg);
+  const auto place = [&](int pair) { return cached + (int)fdiv((uint32_t)min(pair, pairs - 1), a.drep); };
+  const auto low = [&](int at) { return a.window > 0 ? max(at - a.window + 1, 0) : 0; };
+  int b0 = low(place(pair0)) / KB, b1 = min(place(pair0 + TILE - 1), room - 1) / KB + 1;
+  if (a.splits > 1) {
+    const int each = (b1 - b0 + a.splits - 1) / a.splits;
+    b0 += split * each, b1 = min(b0 + each, b1);
+  }
+  // the wave's own keys: blocks outside them it only helps to bring in
+  const int wlo = low(place(mine0)), whi = mine0 < pairs ? place(mine0 + 32 - 1) : -1;
+  int p0 = b0 * KB >> lg;
+  int ids = page_ids(a, p.r, p0, lane);
+  u32x4 r[NU], vs[2];
+  uint32_t ks = 0;
+  const uint32_t kscale = (ONE ? (n >> 2) * (HD / 2) : 0) + (HD == 128 ? g : g >> 1) * 16 + (n & 3) * 4, vscale = ONE ? 32 * g : 0;
+  const auto fetch = [&](int b) {  // the block's codes, the thread's units
+    if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, ids = page_ids(a, p.r, p0, lane);
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+      const int u = tid + 256 * i, e = u % UNITS, token = ONE ? 0 : e / (HD / 2) * 16;
+      const int key = b * KB + token, in = key & mask;
+      const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh) + (u < UNITS ? 0 : R::values(lg));
+      r[i] = gload((const u32x4 *)(rec + (in - token) * R::ROW + 16 * e));
+    }
+  };
+  const auto fetch_scales = [&](int b) {
+    const int key = b * KB + (ONE ? 0 : 16 * (n >> 2)), value = b * KB + (ONE ? 0 : 16 * g);
+    const uint8_t *kr = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh);
+    const uint8_t *vr = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, value, lg), 0), kvh);
+    ks = gload((const uint32_t *)(kr + R::key_scales(lg) + (key & mask) * (HD / 32) + kscale));
+    const u32x4 *v = (const u32x4 *)(vr + R::value_scales(lg) + 2 * (value & mask) + vscale);
+    vs[0] = gload(v), vs[1] = gload(v + 1);
+  };
+  const auto store = [&](int to) {
+#pragma unroll
+    for (int i = 0; i < NU; i++) {
+      const int u = tid + 256 * i, e = u % UNITS;
+      if (u >= UNITS) {
+        *(u32x4 *)(lds.v[half][to] + 16 * e) = r[i];
+      } else if constexpr (HD == 128) {
+        *(u32x4 *)(lds.k[half][to] + e / 4 * R::ROW + 16 * (e % 4 ^ e >> 6)) = r[i];
+      } else {  // two units of 8 bytes
+        const int row = e / 2, at = row >> 4;
+        const u32x4 x = at & 1 ? u32x4{r[i][2], r[i][3], r[i][0], r[i][1]} : r[i];
+        *(u32x4 *)(lds.k[half][to] + row * R::ROW + 16 * (e % 2 ^ at >> 1)) = x;
+      }
+    }
+  };
+  if (b0 + half < b1) fetch(b0 + half), store(0);
+  __syncthreads();
+  for (int b = b0 + half, now = 0; b - half < b1; b += 2, now ^= 1) {
+    const bool mine = b < b1 && b * KB <= whi && b * KB + KB > wlo;
+    bool seen = false;
+    if (mine) fetch_scales(b), seen = page_of<ONE>(ids, p0, b * KB + (ONE ? 0 : 16 * g), lg) >= 0;
+    if (b + 2 < b1) fetch(b + 2);
+    if (mine) {
+      const uint8_t *k = lds.k[half][now], *v = lds.v[half][now];
+      u32x4 row;
+      fold4<HD, 2>(q, st, b * KB + 16 * g, seen, ks, vs,
+                   [&](int kt, int j) {
+                     if (j == 0) {
+                       const uint8_t *at = k + (16 * (n >> 2) + 4 * kt + (n & 3)) * R::ROW;
+                       if constexpr (HD == 128) {
+                         row = *(const u32x4 *)(at + 16 * (g ^ n >> 2));
+                       } else {
+                         const u32x2 w = *(const u32x2 *)(at + 8 * (g ^ n >> 2));
+                         row[0] = w[0], row[1] = w[1];
+                       }
+                     }
+                     return row[j];
+                   },
+                   [&](int c) { return *(const u32x4 *)(v + g * 16 * R::ROW + 256 * c + 16 * n); }, [] {});
+    }
+    if (b + 2 < b1) store(now ^ 1);
+    __syncthreads();
+  }
+  finish_tile<HD>(a, p, {slot, kvh, split}, half, wave, lane, st, (f32x4 *)lds.k, lds.sums);
+}
+
+// A batch that may hold both, as pages_mixed_kernel in pages.hip.
+template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages4_mixed_kernel(const AttendArgs a) {
+  __shared__ union {
+    Many4Lds<HD> many;
+    FewLds<HD, 2, 4> few[2];
+  } lds;
+  const int tiles = a.tiles * a.c.kv * a.splits;
+  if ((int)blockIdx.x < tiles) return many_pairs4<HD, ONE>(a, blockIdx.x, lds.many);
+  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  few_pairs4<HD, 2, 4, ONE>(a, 2 * (blockIdx.x - tiles) + half, threadIdx.x & 255, lds.few[half]);
+}
+
+// ---- entry points ----------------------------------------------------------------------------------------------------
+
+template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
+  const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;
+  if (p.many) pages4_mixed_kernel<HD, ONE><<<tiles * p.splits + (parts + 1) / 2, 512, 0, s>>>(a);
+  else if (p.tiles == 2) pages4_few_kernel<HD, 2, 4, ONE><<<parts, 256, 0, s>>>(a);
+  else if (p.waves == 8) pages4_few_kernel<HD, 1, 8, ONE><<<parts, 512, 0, s>>>(a);
+  else pages4_few_kernel<HD, 1, 4, ONE><<<parts, 256, 0, s>>>(a);
+  BT_LAUNCHED("paged attention");
+  return launch_pages_join(a, p, HD, s);
+}
+
+template <int HD> static int launch_put4(const PoolArgs &c, const BatchArgs &b, const uint16_t *x, int64_t x_sb, int64_t x_sr, int most,
+                                         hipStream_t s) {
+  const int heads = 2 * c.kv, each = most == 1 ? 1 : most <= 16 ? 2 : 0;
+  const int64_t pieces = each ? (int64_t)each * b.requests : (b.rows >> 4) + 2 * b.requests;
+  const int waves = pieces * heads <= 2048 ? 1 : 4, groups = (heads + waves - 1) / waves;
+  if (!grid_fits(pieces * groups, 64 * waves)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, heads);
+  if (waves == 1) put_pages4_kernel<HD, 1><<<(unsigned)(pieces * groups), 64, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
+  else put_pages4_kernel<HD, 4><<<(unsigned)(pieces * groups), 256, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
+  BT_LAUNCHED("a paged put");
+  return BT_OK;
+}
+
+}  // namespace bt
+
+using namespace bt;
+
+extern "C" {
+
+int bt_pages4_bytes(const bt_pages *pool, uint64_t *bytes) {
+  if (!bytes) return fail(BT_EINVAL, "no result pointer");
+  bt_pages c = pool ? *pool : bt_pages{};
+  c.values = 16;  // the shape alone counts
+  PoolArgs a;
+  if (int s = check_pool(&c, 4, &a)) return s;
+  *bytes = (uint64_t)c.pages * c.kv * (c.head_dim == 64 ? Record<64>::bytes(a.page_log2) : Record<128>::bytes(a.page_log2));
+  return BT_OK;
+}
+
+int bt_pages4_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t x, int64_t x_sb, int64_t x_sr) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  PoolArgs c;
+  BatchArgs b;
+  if (int s = check_pool(pool, 4, &c)) return s;
+  if (int s = check_batch(batch, &b)) return s;
+  if (!x || x % 16 || x_sb % 8 || x_sr % 8) return fail(BT_EINVAL, "a paged cache takes rows on 16-byte boundaries");
+  if ((int64_t)b.width * pool->page > MOST_KEYS)
+    return fail(BT_EINVAL, "tables %d wide of pages of %d tokens hold over 2^30", b.width, pool->page);
+  const uint16_t *src = (const uint16_t *)(uintptr_t)x;
+  const int most = std::min(batch->most, batch->rows);
+  if (pool->head_dim == 64) return launch_put4<64>(c, b, src, x_sb, x_sr, most, r->stream);
+  return launch_put4<128>(c, b, src, x_sb, x_sr, most, r->stream);
+}
+
+int bt_pages4_read(bt_runtime *rt, const bt_pages *pool, uint64_t out) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  PoolArgs c;
+  if (int s = check_pool(pool, 4, &c)) return s;
+  if (!out || out % 16) return fail(BT_EINVAL, "pages are read to a 16-byte aligned tensor");
+  const int runs = (pool->page + 63) / 64;
+  const int64_t blocks = (int64_t)c.pages * 2 * c.kv * runs;
+  if (!grid_fits(blocks, 256)) return fail(BT_EINVAL, "%d pages of %d heads are too many to read at once", c.pages, 2 * c.kv);
+  uint16_t *to = (uint16_t *)(uintptr_t)out;
+  if (pool->head_dim == 64) read_pages4_kernel<64><<<(unsigned)blocks, 256, 0, r->stream>>>(c, to, runs);
+  else read_pages4_kernel<128><<<(unsigned)blocks, 256, 0, r->stream>>>(c, to, runs);
+  BT_LAUNCHED("reading pages");
+  return BT_OK;
+}
+
+int bt_pages4_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t heads, int32_t window, uint64_t *bytes) {
+  if (!bytes) return fail(BT_EINVAL, "no result pointer");
+  AttendPlan p;
+  if (int s = plan_attend(pool, 4, batch, heads, window, &p)) return s;
+  *bytes = p.scratch + p.split_scratch;
+  return BT_OK;
+}
+
+int bt_pages4_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr,
+                     uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,
+                     uint64_t scratch_bytes) {
+  Runtime *r;
+  if (int s = enter(rt, &r)) return s;
+  AttendPlan p;
+  AttendArgs a;
+  if (int s = attend_args(pool, 4, batch, q, q_sh, q_sr, out, o_sh, o_sr, heads, window, scratch, scratch_bytes, &p, &a)) return s;
+  const bool one = pool->page >= KB;
+  if (pool->head_dim == 64) return one ? launch_attend4<64, true>(a, p, r->stream) : launch_attend4<64, false>(a, p, r->stream);
+  return one ? launch_attend4<128, true>(a, p, r->stream) : launch_attend4<128, false>(a, p, r->stream);
+}
+
+}  // extern "C"

@@ -245,10 +245,10 @@ def kv_cache(rt, c, size):
   return [Tensor.zeros(rt, size, head(c), batch=2 * c.kv).cast(fmt).realize() for _ in range(c.layers)]
 
 
-def paged_cache(rt, c, pages, page=64):
-  """A pool of `pages` pages of `page` tokens per block (baretile_amd.pages): the cache of paged_forward, 8 bits a value.
+def paged_cache(rt, c, pages, page=64, bits=8):
+  """A pool of `pages` pages of `page` tokens per block (baretile_amd.pages): the cache of paged_forward, 8 or 4 bits a value.
   Every block's pool is of one shape, so one plan serves them all."""
-  return [Pages(rt, pages, c.kv, head(c), page) for _ in range(c.layers)]
+  return [Pages(rt, pages, c.kv, head(c), page, bits) for _ in range(c.layers)]
 
 
 _aranges = {}

@@ -1,10 +1,11 @@
-"""A paged 8-bit KV cache: requests share a pool of pages through block tables, and a step's tables, row starts, places and
+"""A paged KV cache of 8 or 4 bits a value: requests share a pool of pages through block tables, and a step's tables, row starts, places and
 slots are made on the device from request lengths, so the whole step can be recorded and replayed.
 
 The reference keeps a fixed region a slot (llama.py:293-373), as models.serve.Engine does; here a request holds the pages
 its tokens fill. A page holds the tokens of every key and value head, a head's as 8-bit floats (4 exponent and 3 mantissa bits)
 under one power of two, which makes each value exact in bf16: half of a bf16 cache's memory, and decoded in one
-instruction for two values where a bfp8 cache takes five.
+instruction for two values where a bfp8 cache takes five. A pool of 4 bits halves that again: 4-bit floats (2 exponent bits and 1
+mantissa bit) under scales of each token's own, a power of two for 32 dims of a key, one for a value's whole row.
 
 A step over several requests, each with any number of new tokens (a token, a token and its drafts, a prompt's chunk), of which
 the last drafts[r] of request r are drafts (0: none; -1: no token follows yet, as behind a chunk that does not end its prompt,
@@ -52,21 +53,31 @@ class Batch:
 
 
 class Pages:
-  """A pool of `pages` pages of `page` tokens (16, 32, 64, 128 or 256) for kv key heads, 64 or 128 wide: one block's cache.
-  Pages start as zeros. Which pages are free, and which a request gives back, is the caller's to keep."""
-  def __init__(self, rt, pages, kv, head, page=64):
-    pages, kv, head, page = (operator.index(v) for v in (pages, kv, head, page))
+  """A pool of `pages` pages of `page` tokens (16, 32, 64, 128 or 256) for kv key heads, 64 or 128 wide: one block's cache, of 8 or
+  4 bits a value. Pages start as zeros. Which pages are free, and which a request gives back, is the caller's to keep."""
+  def __init__(self, rt, pages, kv, head, page=64, bits=8):
+    pages, kv, head, page, bits = (operator.index(v) for v in (pages, kv, head, page, bits))
+    if bits not in (4, 8): raise ValueError(f"a paged cache has 8 or 4 bits a value, not {bits}")
     if page not in PAGES: raise ValueError(f"a page holds {', '.join(map(str, PAGES))} tokens, not {page}")
     if head not in (64, 128): raise ValueError(f"a paged cache's heads are 64 or 128 wide, not {head}")
     if not (0 < kv <= 1024 and pages > 0 and pages * page < 1 << 31):
       raise ValueError(f"a paged cache of {pages} pages of {page} tokens and {kv} key heads")
     rt.check()
-    self.rt, self.pages, self.kv, self.head, self.page = rt, pages, kv, head, page
-    self.storage = Storage(rt, pages * 2 * kv * page * head)
+    self.rt, self.pages, self.kv, self.head, self.page, self.bits = rt, pages, kv, head, page, bits
+    if bits == 4:
+      self.scales, need = None, ctypes.c_uint64()  # (they lie among the codes)
+      self.args = _lib.PagesArgs(0, 0, pages, page, kv, head)
+      _lib.call("pages4_bytes", ctypes.byref(self.args), ctypes.byref(need))
+      self.storage = Storage(rt, need.value)
+      self.args.values = self.storage.addr
+    else:
+      self.storage = Storage(rt, pages * 2 * kv * page * head)
+      self.scales = Tensor(rt, pages, 2 * kv, dtype="fp32")
+      rt.fill32(self.scales.addr, 127 - 100 << 23, pages * 2 * kv)  # 2^-100, the smallest scale
+      self.args = _lib.PagesArgs(self.storage.addr, self.scales.addr, pages, page, kv, head)
     rt.fill32(self.storage.addr, 0, self.storage.nbytes // 4)
-    self.scales = Tensor(rt, pages, 2 * kv, dtype="fp32")
-    rt.fill32(self.scales.addr, 127 - 100 << 23, pages * 2 * kv)  # 2^-100, the smallest scale
-    self.args = _lib.PagesArgs(self.storage.addr, self.scales.addr, pages, page, kv, head)
+
+  def _call(self, name): return f"pages{'4' if self.bits == 4 else ''}_{name}"
 
   def plan(self, tables, cached, new, free, rows, taken=None, most=None):
     """The Batch of a step, made on the device (bt_pages_plan). tables (requests, width) int32: each request's pages in order,
@@ -103,10 +114,12 @@ class Pages:
                        f"heads on this runtime")
 
   def put(self, batch, x):
-    """Puts the batch's rows into their pages (bt_pages_put): x (2 kv, rows, head) bf16, key heads then value heads, as rope_put
-    gives them. Each page and head takes the smallest power of two under which its largest value is at most 448; where a
-    page that holds rows needs a larger one, those are rounded again under it. It stays so until the page is begun again, also
-    where it was a refused draft's value that needed it. Rows without a page are dropped. Requests may share pages that they
+    """Puts the batch's rows into their pages (bt_pages_put, bt_pages4_put): x (2 kv, rows, head) bf16, key heads then value heads,
+    as rope_put gives them. In 8 bits each page and head takes the smallest power of two under which its largest value is at most
+    448; where a page that holds rows needs a larger one, those are rounded again under it. It stays so until the page is begun
+    again, also where it was a refused draft's value that needed it. In 4 bits each row has scales of its own, the smallest under
+    which its largest value is at most 7 (a power of two for 32 dims of a key, one of 4 to 7 quarters of one for a value), and
+    what a page holds doesn't depend on the puts that its rows came in. Rows without a page are dropped. Requests may share pages that they
     only read; a page that takes rows is one request's."""
     self._fits(batch)
     if not (isinstance(x, Tensor) and x.rt is self.rt and x.dtype == "bf16" and
@@ -115,13 +128,14 @@ class Pages:
                        f"{getattr(x, 'shape', '')}")
     x = x.realize()
     if x.sc != 1 or x.rep != 1 or x.cyc or x.sb % 8 or x.sr % 8 or x.addr % 16: x = x.contiguous()
-    _written(self.scales.storage)
-    self.rt.run("pages_put", "pages_put", ctypes.byref(self.args), ctypes.byref(batch.args), x.addr, x.sb, x.sr,
+    if self.scales is not None: _written(self.scales.storage)
+    name = self._call("put")
+    self.rt.run(name, name, ctypes.byref(self.args), ctypes.byref(batch.args), x.addr, x.sb, x.sr,
                 reads=4 * self.kv * batch.rows * self.head)
 
   def attend(self, q, batch, window=0, merged=False):
-    """softmax(q @ k^T + mask) @ v over each row's request (bt_pages_attend): q (heads, rows, head) bf16, heads a multiple of kv;
-    a row sees its request's keys up to its own place and, with window, the last `window` of them. RoPE scales q beforehand.
+    """softmax(q @ k^T + mask) @ v over each row's request (bt_pages_attend, bt_pages4_attend): q (heads, rows, head) bf16, heads a
+    multiple of kv; a row sees its request's keys up to its own place and, with window, the last `window` of them. RoPE scales q beforehand.
     Rows behind the last request's come back as zeros. merged gives the result as merge() of it, (rows, heads * head)."""
     self._fits(batch)
     window = operator.index(window)
@@ -139,9 +153,10 @@ class Pages:
       out = Tensor(self.rt, q.rows, q.cols, batch=q.batch)
       osh, osr = out.sb, out.sr
     need, scratch = ctypes.c_uint64(), None
-    _lib.call("pages_attend_scratch", ctypes.byref(self.args), ctypes.byref(batch.args), q.batch, window, ctypes.byref(need))
+    name = self._call("attend")
+    _lib.call(name + "_scratch", ctypes.byref(self.args), ctypes.byref(batch.args), q.batch, window, ctypes.byref(need))
     if need.value: scratch = Storage(self.rt, need.value)  # freed (stream-ordered) once the launches that use it are queued
-    self.rt.run("pages_attend", "pages_attend", ctypes.byref(self.args), ctypes.byref(batch.args), q.addr, q.sb, q.sr, out.addr,
+    self.rt.run(name, name, ctypes.byref(self.args), ctypes.byref(batch.args), q.addr, q.sb, q.sr, out.addr,
                 osh, osr, q.batch, window, scratch.addr if scratch else 0, need.value)
     del scratch
     return out
@@ -149,5 +164,6 @@ class Pages:
   def values(self):
     """Every page's values as bf16, exactly: (pages * 2 kv, page, head), key heads then value heads of each page."""
     out = Tensor(self.rt, self.page, self.head, batch=self.pages * 2 * self.kv)
-    self.rt.run("pages_read", "pages_read", ctypes.byref(self.args), out.addr, reads=self.storage.nbytes)
+    name = self._call("read")
+    self.rt.run(name, name, ctypes.byref(self.args), out.addr, reads=self.storage.nbytes)
     return out

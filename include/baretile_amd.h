@@ -402,6 +402,28 @@ int bt_pages_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch,
                     uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,
                     uint64_t scratch_bytes);
 
+/* ---- the same cache in 4 bits a value -------------------------------------------------------------------------------
+ *
+ * Plans and batches are the 8-bit cache's, and one plan serves pools of both. In its bt_pages `scales` is not used: `values` holds
+ * bt_pages4_bytes of both, 16-byte aligned, zeros at first. A value is a 4-bit float (sign, 2 exponent bits biased by 1, 1 mantissa
+ * bit: 0, 1/2, 1, 3/2, 2, 3, 4, 6) times its row's scale: for a key a power of two for each 32 of its dims, for a value
+ * k / 4 * 2^e (k = 4 .. 7) for the row, both from 2^-100 to 2^100; exact in bf16. A page holds for every key head in turn
+ *   keys' codes [page][head_dim / 2], the even dim in a byte's low half; their scales' exponents, biased by 127, of token
+ *   16 a + 4 j + i at [page / 16 (a)][head_dim / 32][4 (i)][4 (j)]; values' codes of token 16 a + 2 t (low half) and the next for
+ *   dim 32 c + 16 j + n at [page / 16 (a)][head_dim / 32 (c)][16 (n)][2 (j)][8 (t)]; their scales, bf16 [page]. */
+int bt_pages4_bytes(const bt_pages *pool, uint64_t *bytes);
+/* bt_pages_put: each row takes the smallest scales s with every finite value at most 7 s in size, and rounds to the nearest code,
+ * ties to even, those over 6 s to 6 s; infinities and NaNs are stored as the largest value of their sign. Rows don't depend on one
+ * another, so pages hold the same however their rows came. */
+int bt_pages4_put(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t x, int64_t x_sb, int64_t x_sr);
+/* bt_pages_read. */
+int bt_pages4_read(bt_runtime *rt, const bt_pages *pool, uint64_t out);
+/* bt_pages_attend, but that weights are rounded to bf16 times their value's scale. */
+int bt_pages4_attend_scratch(const bt_pages *pool, const bt_batch *batch, int32_t heads, int32_t window, uint64_t *bytes);
+int bt_pages4_attend(bt_runtime *rt, const bt_pages *pool, const bt_batch *batch, uint64_t q, int64_t q_sh, int64_t q_sr,
+                     uint64_t out, int64_t o_sh, int64_t o_sr, int32_t heads, int32_t window, uint64_t scratch,
+                     uint64_t scratch_bytes);
+
 /* ---- top-k: replaces topk_kernel (Tensor.topk, tensor.py:685-706) ----------------------------------------------
  * values[b, r, p * k + j] and ids[b, r, p * k + j]: the k largest of part p of row r (parts equal parts of cols), in
  * descending order with equal values in column order (numpy's stable argsort of -x), -0 equal to 0. ids are columns of

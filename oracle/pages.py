@@ -1,5 +1,5 @@
-"""A paged 8-bit cache and drafted tokens' verification in NumPy, in 64 bits and whole numbers, request by request: what
-bt_pages_plan, bt_pages_put, bt_pages_attend and bt_verify (include/baretile_amd.h) define."""
+"""Paged caches of 8 and 4 bits and drafted tokens' verification in NumPy, in 64 bits and whole numbers, request by request: what
+bt_pages_plan, bt_pages_put, bt_pages4_put, bt_pages_attend and bt_verify (include/baretile_amd.h) define."""
 import numpy as np
 
 LEAST, LARGEST = -100, 119  # exponents of the scales
@@ -67,6 +67,45 @@ def put(values, scales, tables, starts, lengths, x):
         values[id, :, held:held + count] = grid(part / s[:, None, None]) * s[:, None, None]
         scales[id] = s
       at += count
+
+
+GRID4 = np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+LEAST4, LARGEST4 = -100, 100  # exponents of the 4-bit cache's scales
+
+
+def grid4(x):
+  """The nearest 4-bit floats (2 exponent bits, 1 mantissa bit), of two as near the one with the even code, at most 6 in size."""
+  x = np.asarray(x, np.float64)
+  with np.errstate(invalid="ignore"): a = np.minimum(np.where(np.isfinite(x), np.abs(x), 7.0), 7.0)
+  far = np.abs(a[..., None] - GRID4)
+  near = far == far.min(-1, keepdims=True)
+  pick = np.where(near & (np.arange(8) % 2 == 0), np.arange(8), -1).max(-1)  # the even code, where it is among the nearest
+  pick = np.where(pick >= 0, pick, np.argmax(near, -1))
+  return np.copysign(GRID4[pick], x) + 0.0
+
+
+def held4(x, value):
+  """Rows x (.., n, head) as the 4-bit cache holds them, the smallest scales s with every finite |x| <= 7 s: for a key (value
+  false) a power of two for each 32 dims, for a value k / 4 of one (k = 4 .. 7) for the row."""
+  x = np.asarray(x, np.float64)
+  scales = np.exp2(np.arange(LEAST4, LARGEST4 + 1, dtype=np.float64))
+  if value: scales = np.append(np.outer(scales[:-1], [1, 1.25, 1.5, 1.75]), scales[-1])
+  groups = x if value else x.reshape(*x.shape[:-1], -1, 32)
+  top = np.where(np.isfinite(groups), np.abs(groups), 0).max(-1)
+  s = scales[np.minimum(np.searchsorted(7 * scales, top), len(scales) - 1)][..., None]
+  return (grid4(groups / s) * s).reshape(x.shape)
+
+
+def put4(values, tables, starts, lengths, x):
+  """x (2 kv, rows, head) into values (pages, 2 kv, page, head) of the 4-bit cache, in place."""
+  pages, kv2, page, _ = values.shape
+  held = np.concatenate([held4(x[:kv2 // 2], False), held4(x[kv2 // 2:], True)])
+  for r, length in enumerate(lengths):
+    n = starts[r + 1] - starts[r]
+    for i in range(n):
+      k, at = divmod(length - n + i, page)
+      id = tables[r, k] if k < tables.shape[1] else -1
+      if 0 <= id < pages: values[id, :, at] = held[:, starts[r] + i]
 
 
 def attend(q, values, tables, starts, lengths, window=0):
