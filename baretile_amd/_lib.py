@@ -93,6 +93,13 @@ class VerifyArgs(ctypes.Structure):  # bt_verify_args
               ("pad_", c_int32), ("drafts", c_uint64)]
 
 
+class LogprobsArgs(ctypes.Structure):  # bt_logprobs_args
+  _fields_ = [("logits", c_uint64), ("ids", c_uint64), ("t", c_uint64), ("logprobs", c_uint64), ("entropy", c_uint64),
+              ("values", c_uint64), ("labels", c_uint64), ("scratch", c_uint64), ("scratch_bytes", c_uint64),
+              ("logits_sr", c_int64), ("t_sr", c_int64), ("rows", c_int32), ("vocab", c_int32), ("k", c_int32),
+              ("pad_", c_int32)]
+
+
 RT = c_void_p
 U64, I64 = c_uint64, c_int64
 # name: argument types. Every function returns an int status.
@@ -138,6 +145,8 @@ SIGNATURES = {
   "bt_pages4_attend_scratch": [POINTER(PagesArgs), POINTER(BatchArgs), c_int32, c_int32, POINTER(c_uint64)],
   "bt_pages4_attend": [RT, POINTER(PagesArgs), POINTER(BatchArgs), U64, I64, I64, U64, I64, I64, c_int32, c_int32, U64, U64],
   "bt_verify_scratch": [POINTER(VerifyArgs), POINTER(c_uint64)], "bt_verify": [RT, POINTER(VerifyArgs)],
+  "bt_logprobs_scratch": [POINTER(LogprobsArgs), POINTER(c_uint64)],
+  "bt_logprobs": [RT, POINTER(LogprobsArgs)],
 }
 
 _lib = None

@@ -6,12 +6,13 @@ forward over every slot recorded once and replayed each step. Around them sits t
 slots that each own a region of every block's KV cache, prompts prefilled in chunks into their slot, a prompt's shared
 prefix reused from a free slot's cache rows, and one replayed decode step for all slots.
 
-Beside it, for callers with steps of their own (llama.paged_forward): `verify`, which checks drafted tokens and draws the next.
+Beside it, for callers with steps of their own (llama.paged_forward): `verify`, which checks drafted tokens and draws the next, and
+`logprobs`, the log probabilities of given tokens with each row's entropy and likeliest tokens.
 
 Out of scope: sampling loops (top-k/top-p/min-p draws), the draft model and loop of speculative decoding, the HTTP server, chat
 templates, tokenizers and text, stop strings, saved sessions and Qwen's recurrent state. Streams speak token ids.
 """
-import ctypes, queue, threading
+import ctypes, operator, queue, threading
 import numpy as np
 from baretile_amd import _lib
 from baretile_amd.tensor import Storage, Tensor, jit
@@ -35,6 +36,12 @@ def heads(logits, t=None, k=64):
   m = values[:, :, 0:1]  # the row's largest: the first of its head
   lse = ((logits - m) * t).exp().sum(2).log()
   return values, ids, lse.realize()
+
+
+def _whole(x):
+  """x realized, as rows of contiguous values."""
+  x = x.realize()
+  return x if x.sc == 1 and x.rep == 1 and not x.cyc else x.contiguous()
 
 
 def verify(logits, ids, starts, uniforms, probs=None, t=None, drafts=None):
@@ -65,11 +72,8 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None, drafts=None):
     raise ValueError(f"verify needs ids (1, {rows}), starts (1, requests + 1), uniforms (2, {rows}), probs ({rows}, {vocab}), t "
                      f"({rows}, 1) and drafts (1, requests): {ids.shape} {starts.shape} {uniforms.shape} "
                      f"{getattr(probs, 'shape', None)} {getattr(t, 'shape', None)} {getattr(drafts, 'shape', None)}")
-  def whole(x):  # rows of contiguous values
-    x = x.realize()
-    return x if x.sc == 1 and x.rep == 1 and not x.cyc else x.contiguous()
-  logits, ids, starts, uniforms = (whole(x) for x in (logits, ids, starts, uniforms))
-  probs, t, drafts = (whole(x) if x is not None else None for x in (probs, t, drafts))
+  logits, ids, starts, uniforms = (_whole(x) for x in (logits, ids, starts, uniforms))
+  probs, t, drafts = (_whole(x) if x is not None else None for x in (probs, t, drafts))
   requests = starts.cols - 1
   tokens, counts = Tensor(rt, 1, rows, dtype="int32"), Tensor(rt, 1, requests, dtype="int32")
   args = _lib.VerifyArgs(logits.addr, probs.addr if probs is not None else 0, t.addr if t is not None else 0, uniforms.addr,
@@ -83,6 +87,37 @@ def verify(logits, ids, starts, uniforms, probs=None, t=None, drafts=None):
   rt.run("verify", "verify", ctypes.byref(args), reads=4 * vocab * (rows + (requests if probs is not None else 0)))
   del scratch
   return tokens, counts
+
+
+def logprobs(logits, ids, k=0, t=None):
+  """What rows of logits (rows, vocab) fp32 say of given tokens, on the device (bt_logprobs): (logprobs, entropy), and with k (up to
+  64) the row's likeliest tokens too, (logprobs, entropy, values, labels). ids, an int32 row, has each row's token; t, a column, each
+  row's inverse temperature (None: 1; infinity: the first largest alone). With p = softmax(t * logits), logprobs and entropy are fp32
+  rows, log p of each row's token (0 for an id that is none, as -1, so that a sum passes it by) and -sum p log p; values (rows, k)
+  fp32 are log p of its k largest logits, largest first, equal ones in column order, and labels (rows, k) int32 their columns,
+  -inf and -1 where fewer are over -inf."""
+  rt, k = getattr(logits, "rt", None), operator.index(k)
+  for x, dtype in [(logits, "fp32"), (ids, "int32"), *([(t, "fp32")] if t is not None else [])]:
+    if not (isinstance(x, Tensor) and x.rt is rt and x.batch == 1 and x.dtype == dtype):
+      raise ValueError(f"logprobs needs {dtype} matrices on one runtime: {getattr(x, 'dtype', type(x))} {getattr(x, 'shape', '')}")
+  rows, vocab = logits.rows, logits.cols
+  if not ((ids.rows, ids.cols) == (1, rows) and (t is None or (t.rows, t.cols) == (rows, 1)) and 0 <= k <= 64):
+    raise ValueError(f"logprobs needs ids (1, {rows}), t ({rows}, 1) and at most 64 alternatives: {ids.shape} "
+                     f"{getattr(t, 'shape', None)} {k}")
+  logits, ids = _whole(logits), _whole(ids)
+  t = _whole(t) if t is not None else None
+  made = [Tensor(rt, 1, rows, dtype="fp32"), Tensor(rt, 1, rows, dtype="fp32")]
+  if k: made += [Tensor(rt, rows, k, dtype="fp32"), Tensor(rt, rows, k, dtype="int32")]
+  args = _lib.LogprobsArgs(logits.addr, ids.addr, t.addr if t is not None else 0, made[0].addr, made[1].addr, made[2].addr if k else 0,
+                           made[3].addr if k else 0, 0, 0, logits.sr, t.sr if t is not None else 0, rows, vocab, k, 0)
+  need, scratch = ctypes.c_uint64(), None
+  _lib.call("logprobs_scratch", ctypes.byref(args), ctypes.byref(need))
+  if need.value:
+    scratch = Storage(rt, need.value)
+    args.scratch, args.scratch_bytes = scratch.addr, need.value
+  rt.run("logprobs", "logprobs", ctypes.byref(args), reads=4 * vocab * rows)
+  del scratch
+  return tuple(made)
 
 
 class Stream:

@@ -453,6 +453,22 @@ typedef struct {
 int bt_verify_scratch(const bt_verify_args *args, uint64_t *bytes);
 int bt_verify(bt_runtime *rt, const bt_verify_args *args);
 
+/* ---- log probabilities of given tokens: no counterpart in the reference's greedy heads (serve.py:43-63) -----------------
+ *
+ * For each row of logits (fp32, `vocab` of them, row stride in elements), with p = softmax(t x) and t the row's inverse temperature
+ * (0: all 1; below 0 or NaN: 0; infinite: the first largest alone): logprobs[row] = log p[ids[row]], 0 for an id outside
+ * [0, vocab); entropy[row] = -sum p log p; and of its k (0 to 64) largest logits, equal ones in column order, values[row, j] = log p
+ * and labels[row, j] = the column, -inf and -1 where fewer are over -inf. A logit of NaN counts as -inf, +inf as the largest finite
+ * number; a row of nothing else has log probabilities of -inf and entropy 0. In fp32; every result is whole and contiguous, and
+ * the same from call to call. */
+typedef struct {
+  uint64_t logits, ids, t, logprobs, entropy, values, labels, scratch, scratch_bytes;
+  int64_t logits_sr, t_sr;
+  int32_t rows, vocab, k, pad_;
+} bt_logprobs_args;
+int bt_logprobs_scratch(const bt_logprobs_args *args, uint64_t *bytes);
+int bt_logprobs(bt_runtime *rt, const bt_logprobs_args *args);
+
 #ifdef __cplusplus
 }
 #endif
