@@ -232,6 +232,7 @@ template <int HD> struct Block4 {
   uint32_t k[4][KW];
   uint32_t ks;
   u32x4 v[HD / 32], vs[2];
+  bool seen;  // whether the values' page is one
 };
 // The weights of a block's 16 pairs, times the values' scales, as bf16: rounded to nearest, since the second product's operand is
 // bf16. l sums them in 32 bits before either, so that a row's weights add up to 1 but for that rounding.
@@ -308,69 +309,80 @@ __device__ __forceinline__ void fold4(const Query<HD, HD / 4> (&q)[QT], Running<
   }
 }
 
+// The blocks b, b + step .. below b1 of request r's keys, by a wave: a block's keys are requested while the block before weighs its
+// scores, its values while it multiplies. ONCE: nobody else reads them, so past the caches.
+template <int HD, int QT, bool ONE, bool ONCE>
+__device__ __forceinline__ void walk4(const AttendArgs &a, int r, int kvh, int b, int b1, int step, const int lane,
+                                      const Query<HD, HD / 4> (&q)[QT], Running<HD> (&st)[QT]) {
+  using R = Record<HD>;
+  if (b >= b1) return;
+  const int n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  int p0 = b * KB >> lg;
+  int ids = page_ids(a, r, p0, lane);
+  Block4<HD> x;
+  const auto load = [](auto *p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    else return gload(p);
+  };
+  const uint32_t krow = ((ONE ? 16 * (n >> 2) : 0) + (n & 3)) * R::ROW + R::ROW / 4 * g;
+  const uint32_t kscale = (ONE ? (n >> 2) * (HD / 2) : 0) + (HD == 128 ? g : g >> 1) * 16 + (n & 3) * 4;
+  const uint32_t vrow = (ONE ? g * 16 * R::ROW : 0) + 16 * n, vscale = ONE ? 32 * g : 0;
+  const auto fetch_keys = [&](int b) {
+    const int key = b * KB + (ONE ? 0 : 16 * (n >> 2)), in = key & mask;
+    const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh), *k = rec + in * R::ROW;
+#pragma unroll
+    for (int kt = 0; kt < 4; kt++) {
+      if constexpr (HD == 128) {
+        const u32x4 w = load((const u32x4 *)(k + (krow + 4 * kt * R::ROW)));
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++) x.k[kt][j] = w[j];
+      } else {
+        const u32x2 w = load((const u32x2 *)(k + (krow + 4 * kt * R::ROW)));
+#pragma unroll
+        for (int j = 0; j < HD / 32; j++) x.k[kt][j] = w[j];
+      }
+    }
+    x.ks = load((const uint32_t *)(rec + R::key_scales(lg) + in * (HD / 32) + kscale));
+  };
+  const auto fetch_values = [&](int b) {
+    const int key = b * KB + (ONE ? 0 : 16 * g), in = key & mask, id = page_of<ONE>(ids, p0, key, lg);
+    const uint8_t *rec = record_of<HD>(a.c, max(id, 0), kvh), *v = rec + R::values(lg) + in * R::ROW;
+    const u32x4 *vs = (const u32x4 *)(rec + R::value_scales(lg) + 2 * in + vscale);
+    x.seen = id >= 0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) x.vs[i] = load(vs + i);
+#pragma unroll
+    for (int c = 0; c < HD / 32; c++) x.v[c] = load((const u32x4 *)(v + 256 * c + vrow));
+  };
+  fetch_keys(b), fetch_values(b);
+  for (; b < b1; b += step) {
+    const int next = b + step;
+    const bool more = next < b1;
+    fold4<HD, QT>(q, st, b * KB + 16 * g, x.seen, x.ks, x.vs, [&](int kt, int j) { return x.k[kt][j]; },
+                  [&](int c) { return x.v[c]; }, [&] {
+                    if (!more) return;
+                    // the 64 pages that its keys lie in, if they are not there yet
+                    if (((next * KB + KB - 1) >> lg) - p0 >= 64) p0 = next * KB >> lg, ids = page_ids(a, r, p0, lane);
+                    fetch_keys(next);
+                  });
+    if (more) fetch_values(next);
+  }
+}
+
 // Few query pairs a request, a part a block of NW waves, as few_pairs in pages.hip.
 template <int HD, int QT, int NW, bool ONE>
 __device__ __forceinline__ void few_pairs4(const AttendArgs &a, const int block, const int tid, FewLds<HD, QT, NW> &lds) {
-  constexpr int KW = HD / 32, V = HD / 32;
-  using R = Record<HD>;
-  const int lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  const int lane = tid & 63;
   Part p;
   take_part<HD, QT, NW>(a, block, tid, &p);
-  const int kvh = p.kvh, b0 = p.b0, b1 = p.b1;
   Query<HD, HD / 4> q[QT];
   Running<HD> st[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    if (p.real) q[t].load(a, p, kvh, p.pair0 + 16 * t + n, g);
+    if (p.real) q[t].load(a, p, p.kvh, p.pair0 + 16 * t + (lane & 15), lane >> 4);
     st[t].clear();
   }
-  if (b0 < b1) {
-    int p0 = b0 * KB >> lg;
-    int ids = page_ids(a, p.r, p0, lane);
-    Block4<HD> x;
-    const auto turn = [&](int b) {  // the 64 pages that block b's keys lie in, if they are not there yet
-      if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, ids = page_ids(a, p.r, p0, lane);
-    };
-    const uint32_t krow = ((ONE ? 16 * (n >> 2) : 0) + (n & 3)) * R::ROW + R::ROW / 4 * g;
-    const uint32_t kscale = (ONE ? (n >> 2) * (HD / 2) : 0) + (HD == 128 ? g : g >> 1) * 16 + (n & 3) * 4;
-    const uint32_t vrow = (ONE ? g * 16 * R::ROW : 0) + 16 * n, vscale = ONE ? 32 * g : 0;
-    const auto fetch_keys = [&](int b) {
-      const int key = b * KB + (ONE ? 0 : 16 * (n >> 2)), in = key & mask;
-      const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh), *k = rec + in * R::ROW;
-#pragma unroll
-      for (int kt = 0; kt < 4; kt++) {
-        if constexpr (HD == 128) {
-          const u32x4 w = __builtin_nontemporal_load((const u32x4 *)(k + (krow + 4 * kt * R::ROW)));
-#pragma unroll
-          for (int j = 0; j < KW; j++) x.k[kt][j] = w[j];
-        } else {
-          const u32x2 w = __builtin_nontemporal_load((const u32x2 *)(k + (krow + 4 * kt * R::ROW)));
-#pragma unroll
-          for (int j = 0; j < KW; j++) x.k[kt][j] = w[j];
-        }
-      }
-      x.ks = __builtin_nontemporal_load((const uint32_t *)(rec + R::key_scales(lg) + in * (HD / 32) + kscale));
-    };
-    const auto fetch_values = [&](int b) {
-      const int key = b * KB + (ONE ? 0 : 16 * g), in = key & mask;
-      const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh), *v = rec + R::values(lg) + in * R::ROW;
-      const u32x4 *vs = (const u32x4 *)(rec + R::value_scales(lg) + 2 * in + vscale);
-#pragma unroll
-      for (int i = 0; i < 2; i++) x.vs[i] = __builtin_nontemporal_load(vs + i);
-#pragma unroll
-      for (int c = 0; c < V; c++) x.v[c] = __builtin_nontemporal_load((const u32x4 *)(v + 256 * c + vrow));
-    };
-    fetch_keys(b0), fetch_values(b0);
-    for (int b = b0; b < b1; b += NW) {
-      const bool more = b + NW < b1;
-      const bool seen = page_of<ONE>(ids, p0, b * KB + (ONE ? 0 : 16 * g), lg) >= 0;
-      fold4<HD, QT>(q, st, b * KB + 16 * g, seen, x.ks, x.vs, [&](int kt, int j) { return x.k[kt][j]; },
-                    [&](int c) { return x.v[c]; }, [&] {
-                      if (more) turn(b + NW), fetch_keys(b + NW);
-                    });
-      if (more) fetch_values(b + NW);
-    }
-  }
+  walk4<HD, QT, ONE, true>(a, p.r, p.kvh, p.b0, p.b1, NW, lane, q, st);
   finish_part<HD, QT, NW>(a, p, tid, st, lds);
 }
 
@@ -380,17 +392,15 @@ __global__ void __launch_bounds__(64 * NW, 2) pages4_few_kernel(const AttendArgs
   few_pairs4<HD, QT, NW, ONE>(a, blockIdx.x, threadIdx.x, lds);
 }
 
-// Many query pairs a request, 128 of one key head a block, as many_pairs in pages.hip: blocks of keys pass through LDS as codes
-// (8 KB a block of 64 keys and heads of 128), their scales straight into registers. Keys' 16-byte units are placed so that the 16
-// lanes of a read meet distinct banks: unit u of row r at u ^ r / 16 (heads of 64: 8-byte units); values' lie as they are read.
+// Many query pairs a request, 128 of one key head a block: 8 waves, two halves of 4 that take every other block of keys, each wave
+// 32 pairs. Every wave loads its keys as the parts' do, four of them the same, from the caches: 4 bits are few enough for that
+// (a block of 64 keys and heads of 128 is 8.4 KB), and the waves keep no step with each other.
 template <int HD> struct Many4Lds {
-  __attribute__((aligned(16))) uint8_t k[2][2][KB * HD / 2], v[2][2][KB * HD / 2];  // [half][stage]
+  f32x4 joined[4 * (HD / 16) * 64];
   float sums[8 * 64];
 };
 template <int HD, bool ONE> __device__ __forceinline__ void many_pairs4(const AttendArgs &a, const int block, Many4Lds<HD> &lds) {
-  using R = Record<HD>;
-  constexpr int UNITS = 2 * HD, NU = 2 * UNITS / 256;  // 16-byte units of a block's keys (its values as many), of both a thread
-  const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2, mask = (1 << lg) - 1;
+  const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
   const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = block % a.c.kv, unit = block / a.c.kv, split = unit % a.splits;
   const int slot = a.tiles - 1 - unit / a.splits;  // the longest rows first
@@ -409,75 +419,10 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs4(const At
     const int each = (b1 - b0 + a.splits - 1) / a.splits;
     b0 += split * each, b1 = min(b0 + each, b1);
   }
-  // the wave's own keys: blocks outside them it only helps to bring in
-  const int wlo = low(place(mine0)), whi = mine0 < pairs ? place(mine0 + 32 - 1) : -1;
-  int p0 = b0 * KB >> lg;
-  int ids = page_ids(a, p.r, p0, lane);
-  u32x4 r[NU], vs[2];
-  uint32_t ks = 0;
-  const uint32_t kscale = (ONE ? (n >> 2) * (HD / 2) : 0) + (HD == 128 ? g : g >> 1) * 16 + (n & 3) * 4, vscale = ONE ? 32 * g : 0;
-  const auto fetch = [&](int b) {  // the block's codes, the thread's units
-    if (((b * KB + KB - 1) >> lg) - p0 >= 64) p0 = b * KB >> lg, ids = page_ids(a, p.r, p0, lane);
-#pragma unroll
-    for (int i = 0; i < NU; i++) {
-      const int u = tid + 256 * i, e = u % UNITS, token = ONE ? 0 : e / (HD / 2) * 16;
-      const int key = b * KB + token, in = key & mask;
-      const uint8_t *rec = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh) + (u < UNITS ? 0 : R::values(lg));
-      r[i] = gload((const u32x4 *)(rec + (in - token) * R::ROW + 16 * e));
-    }
-  };
-  const auto fetch_scales = [&](int b) {
-    const int key = b * KB + (ONE ? 0 : 16 * (n >> 2)), value = b * KB + (ONE ? 0 : 16 * g);
-    const uint8_t *kr = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, key, lg), 0), kvh);
-    const uint8_t *vr = record_of<HD>(a.c, max(page_of<ONE>(ids, p0, value, lg), 0), kvh);
-    ks = gload((const uint32_t *)(kr + R::key_scales(lg) + (key & mask) * (HD / 32) + kscale));
-    const u32x4 *v = (const u32x4 *)(vr + R::value_scales(lg) + 2 * (value & mask) + vscale);
-    vs[0] = gload(v), vs[1] = gload(v + 1);
-  };
-  const auto store = [&](int to) {
-#pragma unroll
-    for (int i = 0; i < NU; i++) {
-      const int u = tid + 256 * i, e = u % UNITS;
-      if (u >= UNITS) {
-        *(u32x4 *)(lds.v[half][to] + 16 * e) = r[i];
-      } else if constexpr (HD == 128) {
-        *(u32x4 *)(lds.k[half][to] + e / 4 * R::ROW + 16 * (e % 4 ^ e >> 6)) = r[i];
-      } else {  // two units of 8 bytes
-        const int row = e / 2, at = row >> 4;
-        const u32x4 x = at & 1 ? u32x4{r[i][2], r[i][3], r[i][0], r[i][1]} : r[i];
-        *(u32x4 *)(lds.k[half][to] + row * R::ROW + 16 * (e % 2 ^ at >> 1)) = x;
-      }
-    }
-  };
-  if (b0 + half < b1) fetch(b0 + half), store(0);
-  __syncthreads();
-  for (int b = b0 + half, now = 0; b - half < b1; b += 2, now ^= 1) {
-    const bool mine = b < b1 && b * KB <= whi && b * KB + KB > wlo;
-    bool seen = false;
-    if (mine) fetch_scales(b), seen = page_of<ONE>(ids, p0, b * KB + (ONE ? 0 : 16 * g), lg) >= 0;
-    if (b + 2 < b1) fetch(b + 2);
-    if (mine) {
-      const uint8_t *k = lds.k[half][now], *v = lds.v[half][now];
-      u32x4 row;
-      fold4<HD, 2>(q, st, b * KB + 16 * g, seen, ks, vs,
-                   [&](int kt, int j) {
-                     if (j == 0) {
-                       const uint8_t *at = k + (16 * (n >> 2) + 4 * kt + (n & 3)) * R::ROW;
-                       if constexpr (HD == 128) {
-                         row = *(const u32x4 *)(at + 16 * (g ^ n >> 2));
-                       } else {
-                         const u32x2 w = *(const u32x2 *)(at + 8 * (g ^ n >> 2));
-                         row[0] = w[0], row[1] = w[1];
-                       }
-                     }
-                     return row[j];
-                   },
-                   [&](int c) { return *(const u32x4 *)(v + g * 16 * R::ROW + 256 * c + 16 * n); }, [] {});
-    }
-    if (b + 2 < b1) store(now ^ 1);
-    __syncthreads();
-  }
-  finish_tile<HD>(a, p, {slot, kvh, split}, half, wave, lane, st, (f32x4 *)lds.k, lds.sums);
+  // the wave's own keys among them
+  b0 = max(b0, low(place(mine0)) / KB), b1 = mine0 < pairs ? min(b1, place(mine0 + 32 - 1) / KB + 1) : 0;
+  walk4<HD, 2, ONE, false>(a, p.r, kvh, b0 + half, b1, 2, lane, q, st);
+  finish_tile<HD>(a, p, {slot, kvh, split}, half, wave, lane, st, lds.joined, lds.sums);
 }
 
 // A batch that may hold both, as pages_mixed_kernel in pages.hip.
