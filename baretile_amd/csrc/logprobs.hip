@@ -2,13 +2,14 @@
 //
 // With p = softmax(t x) of a row, m its largest logit, y_j = t (x_j - m), S = sum exp(y_j): log p_j = y_j - log S, and the entropy
 // -sum p_j log p_j = log S - sum exp(y_j) y_j / S (no difference of large numbers: both terms are at most log(vocab)). Rows are cut
-// into chunks, a block each, whose logits stay in registers: one read gives the chunk's maximum, then its sums against that, and
-// its k largest. A second launch joins a row's chunks; rows of one chunk need none.
+// into segments, a block each, which walk through them a chunk at a time: a chunk's logits stay in registers while they are
+// summed against the wave's running maximum and held against a bound. A second launch joins a row's segments; rows of one need none.
 //
-// The k largest of a chunk: at least k of its threads have a largest value of at least T, so all of the k largest are at least T,
-// the largest such T found by halving over the threads' largest values (one wave's ballots), and few others are; these go to LDS
-// and rank themselves by counting, equal values by their column, so the order in which they came doesn't matter. Where more
-// threads tie at T than that is made for, only the columns up to the one that completes k threads count.
+// The k largest: whatever is at least the bound goes to LDS, and where that gets full it ranks itself by counting, equal values by
+// their column (so the order in which they came doesn't matter); the k first stay, and the last of them is the new bound. The
+// first bound, and any that lets too much through, comes from a chunk's threads: where k of them have a largest value of T or
+// more, so do the k largest of all, T found by halving over the threads' largest values (one wave's ballots). Where more threads
+// tie at T than that is made for, only the columns up to the one that completes k threads count.
 #include "common.h"
 #include <algorithm>
 
@@ -35,7 +36,7 @@ struct LogprobArgs {
   float *top_values;             // [rows][chunks][k], -inf and column -1 where there are fewer
   int32_t *top_columns;
   int64_t logits_sr, t_sr;
-  int32_t vocab, k, chunks;
+  int32_t vocab, k, chunks, turns;  // chunks: a row's segments of `turns` chunks
 };
 
 // A logit as it counts: NaN as -inf, +inf as the largest finite.
@@ -78,12 +79,15 @@ constexpr uint32_t LEAST_ORDERED = 0x00800000u;  // the one above -inf
 
 // The threads whose values may go on, k at least and so many at most.
 __host__ __device__ constexpr int limit_of(int k) { return k + k / 2 + 8; }
+// Values in LDS past which they are ranked: the k that stayed, and as many again.
+__device__ __forceinline__ int full_of(int k) { return 2 * k + 16; }
+constexpr int ROOM = 2 * MOST_K + 16 + PER * limit_of(MOST_K);  // what is there, and one chunk's within the limit
 template <int NT> struct TopLds {
-  uint64_t found[PER * limit_of(MOST_K)];
+  uint64_t found[ROOM], best[MOST_K];
   uint32_t tops[NT];
   int32_t first[NT];
-  uint32_t least;
-  int32_t upto, count;
+  float least;
+  int32_t upto, came[3];  // (a chunk's count, while the last one's is read and the next one's cleared)
 };
 
 // By the first wave: T, from the threads' largest values in LDS. Returns whether more than the limit tie at it.
@@ -131,170 +135,246 @@ template <int NT> __device__ __forceinline__ int find_upto(TopLds<NT> &lds, int 
   return hi;
 }
 
-// The k largest of the block's values v (-inf: none), column(i) thread-wise theirs, by every thread: emit(rank, value, column), with
-// -inf and -1 for the ranks there is nothing for. `between` runs beside the search for T.
-template <int NT, class Column, class Between, class Emit>
-__device__ __forceinline__ void select_top(TopLds<NT> &lds, const float (&v)[PER], int k, Column column, Between between, Emit emit) {
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  float top = v[0];
-#pragma unroll
-  for (int i = 1; i < PER; i++) top = fmaxf(top, v[i]);
-  lds.tops[tid] = ordered(top);
-  if (tid == 0) lds.count = 0;
-  __syncthreads();
-  if (wave == 0) {
-    uint32_t least;
-    const bool ties = find_least<NT>(lds, k, &least);
-    if (tid == 0) lds.least = least, lds.upto = ties ? -1 : NOWHERE;
-  }
-  between();
-  __syncthreads();
-  const uint32_t least = lds.least;
-  int upto = lds.upto;
-  if (upto < 0) {
-    int first = NOWHERE;
-#pragma unroll
-    for (int i = 0; i < PER; i++)
-      if (ordered(v[i]) == least) first = min(first, column(i));
-    lds.first[tid] = first;
+// The k largest of what the block's threads show it, by all of them together: chunks, then finish.
+template <int NT> struct Top {
+  TopLds<NT> &lds;
+  int k, n = 0, turn = 0;  // values in LDS, by turns of the counts
+  float least = NONE;      // what a value has to pass
+
+  // Ahead of a chunk, where there are fewer than k yet: its bound, from the threads' largest values, by the first wave alone.
+  __device__ __forceinline__ void begin(float top) {
+    const int tid = threadIdx.x;
+    lds.tops[tid] = ordered(top);
     __syncthreads();
-    if (wave == 0) {
-      upto = find_upto<NT>(lds, k, least);
-      if (tid == 0) lds.upto = upto;
-    }
-    __syncthreads();
-    upto = lds.upto;
+    if (tid >= 64) return;
+    uint32_t bound;
+    const bool ties = find_least<NT>(lds, k, &bound);
+    if (tid == 0) lds.least = value_of(bound), lds.upto = ties ? -1 : NOWHERE, lds.came[turn] = 0;
   }
+  // A chunk's values v (-inf and NaN: none), the thread's largest among them, their columns (past every column before, or any order
+  // in the first chunk), and whether another follows.
+  template <class Column> __device__ __forceinline__ void chunk(const float (&v)[PER], float top, Column column, bool more) {
+    if (n < k) {  // begun
+      bounded(v, top, column);
+    } else {
+      push(v, top, column, [&](float x, int) { return x > least; });
+      __syncthreads();
+      const int came = lds.came[turn];
+      if (n + came > ROOM) {  // all of it again, within the limit
+        begin(top);
+        bounded(v, top, column);
+      } else {
+        n += came;
+        turn = turn == 2 ? 0 : turn + 1;
+      }
+    }
+    if (more && (n > full_of(k) || (n >= k && least == NONE))) keep();
+  }
+  template <class Column, class In> __device__ __forceinline__ void push(const float (&v)[PER], float top, Column column, In in) {
+    if (threadIdx.x == 0) lds.came[turn == 2 ? 0 : turn + 1] = 0;
+    if (in(top, -1))  // (of most waves no thread, or a few)
 #pragma unroll
-  for (int i = 0; i < PER; i++) {
-    const uint32_t u = ordered(v[i]);
-    if (u >= least) {
-      const int c = column(i);
-      if (u > least || c <= upto) lds.found[atomicAdd(&lds.count, 1)] = (uint64_t)u << 32 | (uint32_t)~c;
+      for (int i = 0; i < PER; i++)
+        if (in(v[i], -1)) {
+          const int c = column(i);
+          if (in(v[i], c)) {
+            const int at = n + atomicAdd(&lds.came[turn], 1);
+            if (at < ROOM) lds.found[at] = (uint64_t)ordered(v[i]) << 32 | (uint32_t)~c;
+          }
+        }
+  }
+  // What of a chunk is at least its own bound (and passes the one there was).
+  template <class Column> __device__ __forceinline__ void bounded(const float (&v)[PER], float top, Column column) {
+    const int tid = threadIdx.x;
+    __syncthreads();
+    const float bound = lds.least;
+    int upto = lds.upto;
+    if (upto < 0) {
+      int first = NOWHERE;
+#pragma unroll
+      for (int i = 0; i < PER; i++)
+        if (v[i] == bound) first = min(first, column(i));
+      lds.first[tid] = first;
+      __syncthreads();
+      if (tid < 64) {
+        upto = find_upto<NT>(lds, k, ordered(bound));
+        if (tid == 0) lds.upto = upto;
+      }
+      __syncthreads();
+      upto = lds.upto;
+    }
+    push(v, top, column, [&](float x, int c) { return x > least && x >= bound && (c <= upto || x > bound); });
+    __syncthreads();
+    n += lds.came[turn], turn = turn == 2 ? 0 : turn + 1;
+  }
+  // to(rank, value in LDS) for the k first by rank; behind a barrier.
+  template <class To> __device__ __forceinline__ void ranked(To to) {
+    for (int i = threadIdx.x; i < n; i += NT) {
+      const uint64_t mine = lds.found[i];
+      int rank = 0;
+      for (int j = 0; j < n; j++) rank += lds.found[j] > mine;
+      if (rank < k) to(rank, mine);
     }
   }
-  __syncthreads();
-  const int n = lds.count;
-  for (int i = tid; i < n; i += NT) {
-    const uint64_t mine = lds.found[i];
-    int rank = 0;
-    for (int j = 0; j < n; j++) rank += lds.found[j] > mine;
-    if (rank < k) emit(rank, value_of((uint32_t)(mine >> 32)), (int)~(uint32_t)mine);
+  // Only the k first stay, and there is a bound from then on.
+  __device__ __forceinline__ void keep() {
+    ranked([&](int rank, uint64_t x) { lds.best[rank] = x; });
+    __syncthreads();
+    n = min(n, k);
+    for (int i = threadIdx.x; i < n; i += NT) lds.found[i] = lds.best[i];
+    if (n == k) least = value_of((uint32_t)(lds.best[k - 1] >> 32));
+    __syncthreads();
   }
-  for (int i = n + tid; i < k; i += NT) emit(i, NONE, -1);
-}
+  // emit(rank, value, column), with -inf and -1 for the ranks there is nothing for.
+  template <class Emit> __device__ __forceinline__ void finish(Emit emit) {
+    ranked([&](int rank, uint64_t x) { emit(rank, value_of((uint32_t)(x >> 32)), (int)~(uint32_t)x); });
+    for (int i = n + threadIdx.x; i < k; i += NT) emit(i, NONE, -1);
+  }
+};
 
 // A row's largest logit and the logarithm of its sum, once they are known.
 struct RowSums {
   float m, lse, entropy;
   int at;
 };
-__device__ __forceinline__ RowSums row_sums(float m, float s, float e, int at, bool greedy) {
-  const float lse = logf(s);
-  if (m == NONE || greedy) return {m, 0.0f, 0.0f, at};
-  return {m, lse, lse - e / s * LN2, at};
+__device__ __forceinline__ RowSums row_sums(const ChunkSums &r, bool greedy) {
+  const float lse = logf(r.s);
+  if (r.m == NONE || greedy) return {r.m, 0.0f, 0.0f, r.at};
+  return {r.m, lse, lse - r.e / r.s * LN2, r.at};
+}
+// A block's waves' sums as one.
+template <int W> __device__ __forceinline__ ChunkSums together(const ChunkSums (&waves)[W], const Inverse &t) {
+  ChunkSums r = {NONE, 0.0f, 0.0f, NOWHERE};
+#pragma unroll
+  for (int i = 0; i < W; i++) r.m = fmaxf(r.m, waves[i].m);
+#pragma unroll
+  for (int i = 0; i < W; i++) {
+    const ChunkSums w = waves[i];
+    const float d = log2_weight(w.m, r.m, t.log2), by = __builtin_amdgcn_exp2f(d);
+    r.s = __builtin_fmaf(w.s, by, r.s), r.e = __builtin_fmaf(__builtin_fmaf(d, w.s, w.e), by, r.e);
+    if (w.m == r.m) r.at = min(r.at, w.at);
+  }
+  return r;
 }
 __device__ __forceinline__ float logprob(float x, int column, const RowSums &r, const Inverse &t) {
   if (x == NONE || (t.greedy && column != r.at)) return NONE;
   return t.greedy ? 0.0f : half_less(x, r.m) * t.t * 2.0f - r.lse;
 }
-__device__ __forceinline__ void store_row(const LogprobArgs &a, int row, const RowSums &r, const Inverse &t) {
-  const int id = gload(a.ids + row);
-  const bool is = (uint32_t)id < (uint32_t)a.vocab;
-  const float x = is ? logit(gload(a.logits + row * a.logits_sr + id)) : NONE;
-  a.logprobs[row] = is ? logprob(x, id, r, t) : 0.0f;
+// The row's given token, requested ahead of the rest.
+struct Given {
+  int id;
+  float x;
+  bool is;
+};
+__device__ __forceinline__ Given given(const LogprobArgs &a, int row) {
+  Given g;
+  g.id = gload(a.ids + row), g.is = (uint32_t)g.id < (uint32_t)a.vocab;
+  g.x = gload(a.logits + row * a.logits_sr + (g.is ? g.id : 0));
+  return g;
+}
+__device__ __forceinline__ void store_row(const LogprobArgs &a, int row, const Given &g, const RowSums &r, const Inverse &t) {
+  a.logprobs[row] = g.is ? logprob(logit(g.x), g.id, r, t) : 0.0f;
   a.entropy[row] = r.entropy;
 }
 
-// A block: PER NT logits of a row.
-template <int NT, bool WIDE> __global__ void __launch_bounds__(NT) logprobs_kernel(const LogprobArgs a) {
-  constexpr int W = NT / 64;
-  __shared__ TopLds<NT> lds;
-  __shared__ float tops[W], ss[W], es[W];
-  __shared__ int at;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int row = blockIdx.x / a.chunks, chunk = blockIdx.x - row * a.chunks, v0 = chunk * (PER * NT);
-  const float *x = a.logits + row * a.logits_sr;
-  const auto column = [&](int i) { return v0 + (WIDE ? i / 4 * (4 * NT) + 4 * tid + i % 4 : i * NT + tid); };
-  float v[PER];
-  if constexpr (WIDE) {  // rows end on 16 bytes too
-#pragma unroll
-    for (int i = 0; i < PER; i += 4) {
-      f32x4 w = {NONE, NONE, NONE, NONE};
-      if (column(i) < a.vocab) w = gload((const f32x4 *)(x + column(i)));
-#pragma unroll
-      for (int j = 0; j < 4; j++) v[i + j] = w[j];
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < PER; i++) v[i] = column(i) < a.vocab ? gload(x + column(i)) : NONE;
-  }
-  const Inverse t = inverse(a, row);
-  float top = NONE;
-#pragma unroll
-  for (int i = 0; i < PER; i++) top = fmaxf(top, v[i] = logit(v[i]));
-  top = wave_max(top);
-  if (lane == 0) tops[wave] = top;
-  if (tid == 0) at = NOWHERE;
-  float m = NONE;
-  const auto sums = [&] {  // (behind a barrier)
-#pragma unroll
-    for (int i = 0; i < W; i++) m = fmaxf(m, tops[i]);
-    float s = 0.0f, e = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const float y = log2_weight(v[i], m, t.log2), w = __builtin_amdgcn_exp2f(y);
-      s += w, e = __builtin_fmaf(w, y, e);
-    }
-    s = wave_sum(s), e = wave_sum(e);
-    if (lane == 0) ss[wave] = s, es[wave] = e;
-    if (t.greedy)
-#pragma unroll
-      for (int i = 0; i < PER; i++)
-        if (v[i] == m) atomicMin(&at, column(i));
-  };
-  const auto whole = [&] {  // (behind another)
-    float s = 0.0f, e = 0.0f;
-#pragma unroll
-    for (int i = 0; i < W; i++) s += ss[i], e += es[i];
-    return ChunkSums{m, s, e, at};
-  };
-  const int64_t unit = (int64_t)row * a.chunks + chunk;
-  if (a.k) {
-    RowSums r;
-    bool known = false;
-    select_top<NT>(lds, v, a.k, column, sums, [&](int rank, float value, int c) {
-      if (a.chunks > 1) {
-        a.top_values[unit * a.k + rank] = value, a.top_columns[unit * a.k + rank] = c;
-        return;
-      }
-      if (!known) {
-        const ChunkSums k = whole();
-        r = row_sums(k.m, k.s, k.e, k.at, t.greedy), known = true;
-      }
-      a.values[(int64_t)row * a.k + rank] = logprob(value, c, r, t), a.labels[(int64_t)row * a.k + rank] = c;
-    });
-  } else {
-    __syncthreads();
-    sums();
-    __syncthreads();
-  }
-  if (tid) return;
-  const ChunkSums k = whole();
-  if (a.chunks > 1) a.sums[unit] = k;
-  else store_row(a, row, row_sums(k.m, k.s, k.e, k.at, t.greedy), t);
+// A wave's sums, from its lanes'.
+__device__ __forceinline__ void store_sums(ChunkSums r, const Inverse &t, ChunkSums *to) {
+  r.s = wave_sum(r.s), r.e = wave_sum(r.e);
+  if (t.greedy)
+    for (int d = 1; d < 64; d *= 2) r.at = min(r.at, __shfl_xor(r.at, d, 64));
+  if ((threadIdx.x & 63) == 0) *to = r;
 }
 
-// A block: a row's chunks, up to 256, and their k largest, up to PER NT in all.
+// A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against its wave's running maximum; of the
+// chunk that makes the bound they are made while the first wave looks for it.
+// Memory bounds it where rows are many: 512 rows of 131072 with 20 alternatives (268 MB) 47 us, 5.7 TB/s, and a join of 5.2; 777 rows of
+// 49152 without (153 MB) 23.8 us, 6.4 TB/s. One row of 49152 is latency: 5.7 us and a join of 4.4, 32 rows of 131072 8.9 and 5.1.
+// Dropped: ranks counted over 4 or 8 values at once (the 47 us 49 and more), a wave a chunk with no barrier (one row 5.4 us, but
+// 32 13).
+template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) logprobs_kernel(const LogprobArgs a) {
+  constexpr int W = NT / 64, CHUNK = PER * NT;
+  __shared__ TopLds<NT> lds;
+  __shared__ ChunkSums sums[W];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int row = blockIdx.x / a.chunks, segment = blockIdx.x - row * a.chunks, from = segment * a.turns;
+  const float *x = a.logits + row * a.logits_sr;
+  const Inverse t = inverse(a, row);
+  Given g = {};
+  if (a.chunks == 1) g = given(a, row);
+  Top<NT> largest{lds, a.k};
+  ChunkSums r = {NONE, 0.0f, 0.0f, NOWHERE};
+  const int end = min(from + a.turns, (a.vocab + CHUNK - 1) / CHUNK);
+  for (int c = from; c < end; c++) {
+    const int v0 = c * CHUNK;
+    const auto column = [&](int i) { return v0 + (WIDE ? i / 4 * (4 * NT) + 4 * tid + i % 4 : i * NT + tid); };
+    float v[PER];
+    if constexpr (WIDE) {  // rows end on 16 bytes too
+#pragma unroll
+      for (int i = 0; i < PER; i += 4) {
+        f32x4 w = {NONE, NONE, NONE, NONE};
+        if (column(i) < a.vocab) w = gload((const f32x4 *)(x + column(i)));
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[i + j] = w[j];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; i++) v[i] = column(i) < a.vocab ? gload(x + column(i)) : NONE;
+    }
+    float top = NONE;  // NaNs count for nothing: not for a maximum, nor against a bound, nor as a weight
+#pragma unroll
+    for (int i = 0; i < PER; i++) top = fmaxf(top, v[i]);
+    const float wave_top = wave_max(top);
+    if (wave_top > LARGEST) {  // there are infinities
+#pragma unroll
+      for (int i = 0; i < PER; i++) v[i] = logit(v[i]);
+      top = fminf(top, LARGEST);
+    }
+    if (a.k && largest.n < a.k) largest.begin(top);
+    if (wave_top > r.m) {
+      const float m = fminf(wave_top, LARGEST), d = log2_weight(r.m, m, t.log2), by = __builtin_amdgcn_exp2f(d);
+      r.e = __builtin_fmaf(d, r.s, r.e) * by, r.s *= by;
+      if (m > r.m) r.at = NOWHERE;
+      r.m = m;
+    }
+    if (t.greedy && r.at == NOWHERE)
+#pragma unroll
+      for (int i = PER - 1; i >= 0; i--)
+        if (v[i] == r.m) r.at = column(i);  // the thread's first in this chunk: columns rise with i
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+      const float y = log2_weight(v[i], r.m, t.log2), w = __builtin_amdgcn_exp2f(y);
+      r.s += w, r.e = __builtin_fmaf(w, y, r.e);
+    }
+    if (c + 1 == end) store_sums(r, t, &sums[wave]);
+    if (a.k) largest.chunk(v, top, column, c + 1 < end);
+  }
+  if (a.k == 0) __syncthreads();
+  const int64_t unit = (int64_t)row * a.chunks + segment;
+  if (a.chunks > 1) {
+    if (tid == 0) a.sums[unit] = together(sums, t);
+    if (a.k)
+      largest.finish([&](int rank, float value, int c) {
+        a.top_values[unit * a.k + rank] = value, a.top_columns[unit * a.k + rank] = c;
+      });
+    return;
+  }
+  const RowSums sum = row_sums(together(sums, t), t.greedy);
+  if (tid == 0) store_row(a, row, g, sum, t);
+  if (a.k)
+    largest.finish([&](int rank, float value, int c) {
+      a.values[(int64_t)row * a.k + rank] = logprob(value, c, sum, t), a.labels[(int64_t)row * a.k + rank] = c;
+    });
+}
+
+// A block: a row's segments, up to 256, and their k largest, up to PER JOIN in all.
 constexpr int JOIN = 256;
 __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(const LogprobArgs a) {
   constexpr int W = JOIN / 64;
   __shared__ TopLds<JOIN> lds;
-  __shared__ float tops[W], ss[W], es[W];
-  __shared__ int at;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
-  ChunkSums k = {NONE, 0.0f, 0.0f, NOWHERE};
-  if (tid < a.chunks) k = a.sums[(int64_t)row * a.chunks + tid];
+  __shared__ ChunkSums sums[W];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), row = blockIdx.x;
+  ChunkSums r = {NONE, 0.0f, 0.0f, NOWHERE};
+  if (tid < a.chunks) r = a.sums[(int64_t)row * a.chunks + tid];
   const int n = a.chunks * a.k;
   float v[PER];
   int columns[PER];
@@ -305,33 +385,45 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(const LogprobArgs a
     if (e < n) v[i] = gload(a.top_values + (int64_t)row * n + e), columns[i] = gload(a.top_columns + (int64_t)row * n + e);
   }
   const Inverse t = inverse(a, row);
-  const float top = wave_max(k.m);
-  if (lane == 0) tops[wave] = top;
-  if (tid == 0) at = NOWHERE;
-  __syncthreads();
-  float m = NONE;
+  const Given g = given(a, row);
+  Top<JOIN> largest{lds, a.k};
+  const float m = wave_max(r.m), d = log2_weight(r.m, m, t.log2), by = __builtin_amdgcn_exp2f(d);
+  if (r.m < m) r.at = NOWHERE;
+  r.e = __builtin_fmaf(d, r.s, r.e) * by, r.s *= by, r.m = m;
+  store_sums(r, t, &sums[wave]);
+  if (a.k) {
+    float top = NONE;
 #pragma unroll
-  for (int i = 0; i < W; i++) m = fmaxf(m, tops[i]);
-  const float y = log2_weight(k.m, m, t.log2), by = __builtin_amdgcn_exp2f(y);
-  const float s = wave_sum(k.s * by), e = wave_sum(__builtin_fmaf(y, k.s, k.e) * by);
-  if (lane == 0) ss[wave] = s, es[wave] = e;
-  if (t.greedy && k.m == m) atomicMin(&at, k.at);
-  __syncthreads();
-  float s_all = 0.0f, e_all = 0.0f;
-#pragma unroll
-  for (int i = 0; i < W; i++) s_all += ss[i], e_all += es[i];
-  const RowSums r = row_sums(m, s_all, e_all, at, t.greedy);
-  if (tid == 0) store_row(a, row, r, t);
+    for (int i = 0; i < PER; i++) top = fmaxf(top, v[i]);
+    largest.begin(top);
+    largest.chunk(v, top, [&](int i) { return columns[i]; }, false);
+  } else {
+    __syncthreads();
+  }
+  const RowSums sum = row_sums(together(sums, t), t.greedy);
+  if (tid == 0) store_row(a, row, g, sum, t);
   if (a.k == 0) return;
-  select_top<JOIN>(lds, v, a.k, [&](int i) { return columns[i]; }, [] {}, [&](int rank, float value, int c) {
-    a.values[(int64_t)row * a.k + rank] = logprob(value, c, r, t), a.labels[(int64_t)row * a.k + rank] = c;
+  largest.finish([&](int rank, float value, int c) {
+    a.values[(int64_t)row * a.k + rank] = logprob(value, c, sum, t), a.labels[(int64_t)row * a.k + rank] = c;
   });
 }
 
+// Blocks that fill the card: eight of 256 threads on each of the 256 CUs.
+constexpr int BLOCKS = 2048;
+// Threads of a block: more where a row's chunks' k largest would pass what the join takes. (512 rows of 131072 with 20 alternatives, a
+// chunk a block: 55 us by 256, 59 by 512, 100 by 1024, 83 by 128 and 136 by 64, whose chunks each bring k values to rank.)
 static int logprobs_threads(const bt_logprobs_args *a) {
   return (int64_t)ceil_div(a->vocab, PER * 256) * std::max(a->k, 1) > PER * JOIN ? 1024 : 256;
 }
-static int logprobs_chunks(const bt_logprobs_args *a) { return ceil_div(a->vocab, PER * logprobs_threads(a)); }
+// Chunks of a segment: one, until there are more than fill the card, which then pass a bound that most of their values don't: 512 rows of
+// 131072 with 20 alternatives 61 us in 16384 segments, 47 in 2048, 55 in 4096, 52 in 1024. Without alternatives there is nothing to
+// gain (777 rows of 49152 23.8 us, in segments of 4 chunks 26.8).
+static int logprobs_turns(const bt_logprobs_args *a) {
+  const int64_t chunks = ceil_div(a->vocab, PER * logprobs_threads(a));
+  if (a->k == 0) return 1;
+  return (int)std::max<int64_t>(1, std::min(chunks, a->rows * chunks / BLOCKS));
+}
+static int logprobs_chunks(const bt_logprobs_args *a) { return ceil_div(a->vocab, PER * logprobs_threads(a) * logprobs_turns(a)); }
 static int check_logprobs(const bt_logprobs_args *a) {
   if (!a || !a->logits || !a->ids || !a->logprobs || !a->entropy || (a->k && (!a->values || !a->labels)))
     return fail(BT_EINVAL, "log probabilities need logits, ids and results");
@@ -340,7 +432,7 @@ static int check_logprobs(const bt_logprobs_args *a) {
   if (a->rows < 1 || a->rows > 1 << 20 || a->vocab < 1 || a->vocab > MOST_VOCAB || a->k < 0 || a->k > MOST_K)
     return fail(BT_EINVAL, "log probabilities of %d rows of %d logits (each 1 to 2^20) with %d alternatives (0 to %d)", a->rows, a->vocab,
                 a->k, MOST_K);
-  if ((int64_t)a->rows * logprobs_chunks(a) * logprobs_threads(a) > 0xFFFFFFFFll)  // a grid counts its threads in 32 bits
+  if ((int64_t)a->rows * a->vocab > 1ll << 36)  // (a block takes 2^12 at least, and a grid counts its threads in 32 bits)
     return fail(BT_EINVAL, "log probabilities of %d rows of %d logits are too large", a->rows, a->vocab);
   return BT_OK;
 }
@@ -373,18 +465,14 @@ int bt_logprobs(bt_runtime *rt, const bt_logprobs_args *a) {
   const auto f = [](uint64_t p) { return (float *)(uintptr_t)p; };
   k.logits = f(a->logits), k.t = f(a->t), k.ids = (const int32_t *)(uintptr_t)a->ids;
   k.logprobs = f(a->logprobs), k.entropy = f(a->entropy), k.values = f(a->values), k.labels = (int32_t *)(uintptr_t)a->labels;
-  k.chunks = logprobs_chunks(a), k.vocab = a->vocab, k.k = a->k, k.logits_sr = a->logits_sr, k.t_sr = a->t_sr;
+  k.chunks = logprobs_chunks(a), k.turns = logprobs_turns(a), k.vocab = a->vocab, k.k = a->k, k.logits_sr = a->logits_sr, k.t_sr = a->t_sr;
   const int64_t units = (int64_t)a->rows * k.chunks;
   k.sums = (ChunkSums *)(uintptr_t)a->scratch;
   k.top_values = (float *)(k.sums + units), k.top_columns = (int32_t *)(k.top_values + units * k.k);
   const bool wide = a->logits % 16 == 0 && a->logits_sr % 4 == 0 && a->vocab % 4 == 0;
-  if (logprobs_threads(a) == 256) {
-    if (wide) logprobs_kernel<256, true><<<(unsigned)units, 256, 0, r->stream>>>(k);
-    else logprobs_kernel<256, false><<<(unsigned)units, 256, 0, r->stream>>>(k);
-  } else {
-    if (wide) logprobs_kernel<1024, true><<<(unsigned)units, 1024, 0, r->stream>>>(k);
-    else logprobs_kernel<1024, false><<<(unsigned)units, 1024, 0, r->stream>>>(k);
-  }
+  const auto launch = [&](auto kernel, int threads) { kernel<<<(unsigned)units, threads, 0, r->stream>>>(k); };
+  if (logprobs_threads(a) == 256) wide ? launch(logprobs_kernel<256, true>, 256) : launch(logprobs_kernel<256, false>, 256);
+  else wide ? launch(logprobs_kernel<1024, true>, 1024) : launch(logprobs_kernel<1024, false>, 1024);
   BT_LAUNCHED("log probabilities");
   if (k.chunks > 1) {
     logprobs_join_kernel<<<(unsigned)a->rows, JOIN, 0, r->stream>>>(k);

@@ -339,37 +339,40 @@ __device__ __forceinline__ bool find_tile(const AttendArgs &a, int slot, int lan
 
 // The two halves of a tile's block, 4 waves of 32 pairs each, join a tile of pairs at a time: `joined` holds every wave of the
 // second half's O^T, `sums` its maxima and sums, where nothing is read any more. Then the rows, or the split's sums for the join.
+// HALVES: 1 where the block's 4 waves are all.
 struct TileAt {
   int slot, kvh, split;
 };
-template <int HD>
+template <int HD, int HALVES = 2>
 __device__ __forceinline__ void finish_tile(const AttendArgs &a, const Piece &p, const TileAt at, const int half, const int wave,
                                             const int lane, Running<HD> (&st)[2], f32x4 *joined, float *sums) {
   constexpr int C = HD / 16;
   const int n = lane & 15, g = lane >> 4, pairs = p.n * a.rep, pair0 = TILE * p.k, mine0 = pair0 + 32 * wave;
+  if constexpr (HALVES == 2) {
 #pragma unroll
-  for (int t = 0; t < 2; t++) {
-    if (half) {
+    for (int t = 0; t < 2; t++) {
+      if (half) {
 #pragma unroll
-      for (int c = 0; c < C; c++) joined[(wave * C + c) * 64 + lane] = st[t].o[c];
-      sums[(2 * wave) * 64 + lane] = st[t].m, sums[(2 * wave + 1) * 64 + lane] = st[t].l;
-    }
-    __syncthreads();
-    if (!half) {
-      const float m = sums[(2 * wave) * 64 + lane], top = fmaxf(st[t].m, m);
-      const float mine = st[t].m == -INF ? 0.0f : __builtin_amdgcn_exp2f(st[t].m - top);
-      const float other = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-      st[t].m = top, st[t].l = st[t].l * mine + sums[(2 * wave + 1) * 64 + lane] * other;
-#pragma unroll
-      for (int c = 0; c < C; c++) {
-        const f32x4 o = joined[(wave * C + c) * 64 + lane];
-#pragma unroll
-        for (int i = 0; i < 4; i++) st[t].o[c][i] = st[t].o[c][i] * mine + o[i] * other;
+        for (int c = 0; c < C; c++) joined[(wave * C + c) * 64 + lane] = st[t].o[c];
+        sums[(2 * wave) * 64 + lane] = st[t].m, sums[(2 * wave + 1) * 64 + lane] = st[t].l;
       }
+      __syncthreads();
+      if (!half) {
+        const float m = sums[(2 * wave) * 64 + lane], top = fmaxf(st[t].m, m);
+        const float mine = st[t].m == -INF ? 0.0f : __builtin_amdgcn_exp2f(st[t].m - top);
+        const float other = m == -INF ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+        st[t].m = top, st[t].l = st[t].l * mine + sums[(2 * wave + 1) * 64 + lane] * other;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+          const f32x4 o = joined[(wave * C + c) * 64 + lane];
+#pragma unroll
+          for (int i = 0; i < 4; i++) st[t].o[c][i] = st[t].o[c][i] * mine + o[i] * other;
+        }
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    if (half) return;
   }
-  if (half) return;
 #pragma unroll
   for (int t = 0; t < 2; t++) {
     const int pair = mine0 + 16 * t + n;

@@ -399,9 +399,10 @@ template <int HD> struct Many4Lds {
   f32x4 joined[4 * (HD / 16) * 64];
   float sums[8 * 64];
 };
-template <int HD, bool ONE> __device__ __forceinline__ void many_pairs4(const AttendArgs &a, const int block, Many4Lds<HD> &lds) {
+template <int HD, int HALVES, bool ONE>
+__device__ __forceinline__ void many_pairs4(const AttendArgs &a, const int block, Many4Lds<HD> &lds) {
   const int tid = threadIdx.x & 255, lane = tid & 63, n = lane & 15, g = lane >> 4, lg = a.c.page_log2;
-  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8), wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int half = HALVES == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int kvh = block % a.c.kv, unit = block / a.c.kv, split = unit % a.splits;
   const int slot = a.tiles - 1 - unit / a.splits;  // the longest rows first
   Piece p;
@@ -421,29 +422,40 @@ template <int HD, bool ONE> __device__ __forceinline__ void many_pairs4(const At
   }
   // the wave's own keys among them
   b0 = max(b0, low(place(mine0)) / KB), b1 = mine0 < pairs ? min(b1, place(mine0 + 32 - 1) / KB + 1) : 0;
-  walk4<HD, 2, ONE, false>(a, p.r, kvh, b0 + half, b1, 2, lane, q, st);
-  finish_tile<HD>(a, p, {slot, kvh, split}, half, wave, lane, st, lds.joined, lds.sums);
+  walk4<HD, 2, ONE, false>(a, p.r, kvh, b0 + half, b1, HALVES, lane, q, st);
+  finish_tile<HD, HALVES>(a, p, {slot, kvh, split}, half, wave, lane, st, lds.joined, lds.sums);
 }
 
 // A batch that may hold both, as pages_mixed_kernel in pages.hip.
-template <int HD, bool ONE> __global__ void __launch_bounds__(512, 2) pages4_mixed_kernel(const AttendArgs a) {
+template <int HD, int HALVES, bool ONE> __global__ void __launch_bounds__(256 * HALVES, 2) pages4_mixed_kernel(const AttendArgs a) {
   __shared__ union {
     Many4Lds<HD> many;
-    FewLds<HD, 2, 4> few[2];
+    FewLds<HD, 2, 4> few[HALVES];
   } lds;
   const int tiles = a.tiles * a.c.kv * a.splits;
-  if ((int)blockIdx.x < tiles) return many_pairs4<HD, ONE>(a, blockIdx.x, lds.many);
-  const int half = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
-  few_pairs4<HD, 2, 4, ONE>(a, 2 * (blockIdx.x - tiles) + half, threadIdx.x & 255, lds.few[half]);
+  if ((int)blockIdx.x < tiles) return many_pairs4<HD, HALVES, ONE>(a, blockIdx.x, lds.many);
+  const int half = HALVES == 2 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  few_pairs4<HD, 2, 4, ONE>(a, HALVES * (blockIdx.x - tiles) + half, threadIdx.x & 255, lds.few[half]);
 }
 
 // ---- entry points ----------------------------------------------------------------------------------------------------
 
+// Blocks of tiles past which each is 4 waves, so that two share a CU and one's start and end lie beside the other's work; up to it, 8:
+// prompts of 32 heads of 128, 8 of 300 rows (664 blocks) 71 us as 8 waves, 62 as 4; 4096 rows (1032) 183 and 156; 2048 (520) 61
+// and 63; 1536 (392) 40 and 47.
+constexpr unsigned HALVED = 640;
 template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;
-  if (p.many) pages4_mixed_kernel<HD, ONE><<<tiles * p.splits + (parts + 1) / 2, 512, 0, s>>>(a);
+  const unsigned blocks = tiles * p.splits;
+  // blocks of 8 waves where parts are long: heads of 64, whose registers leave room, 8 requests of 32768 keys of 3 heads 24.8 us by 4
+  // and 22.2 by 8, one of 8192 17.5 and 16.0, but 8 of 4096 14.0 and 14.6; of 128 only where all the parts there can be leave a CU
+  // one, one request of 131072 keys of 8 heads 34.5 and 32.8, of 65536 21.9 and 22.1, of 16384 14.0 and 15.0
+  const int64_t held = (int64_t)a.b.width << a.c.page_log2;
+  const bool long_parts = p.join && (HD == 64 ? held >= 8192 : held >= 131072 && MOST_PARTS * a.b.requests * a.c.kv <= 256);
+  if (p.many && blocks > HALVED) pages4_mixed_kernel<HD, 1, ONE><<<blocks + parts, 256, 0, s>>>(a);
+  else if (p.many) pages4_mixed_kernel<HD, 2, ONE><<<blocks + (parts + 1) / 2, 512, 0, s>>>(a);
   else if (p.tiles == 2) pages4_few_kernel<HD, 2, 4, ONE><<<parts, 256, 0, s>>>(a);
-  else if (p.waves == 8) pages4_few_kernel<HD, 1, 8, ONE><<<parts, 512, 0, s>>>(a);
+  else if (p.waves == 8 || long_parts) pages4_few_kernel<HD, 1, 8, ONE><<<parts, 512, 0, s>>>(a);
   else pages4_few_kernel<HD, 1, 4, ONE><<<parts, 256, 0, s>>>(a);
   BT_LAUNCHED("paged attention");
   return launch_pages_join(a, p, HD, s);
