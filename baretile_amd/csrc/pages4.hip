@@ -70,19 +70,24 @@ __device__ __forceinline__ float value_scale(float amax) {
 
 // ---- rows into pages ------------------------------------------------------------------------------------------------
 
-// A wave: the rows that one request puts into 16 tokens of one head. Rows are loaded once, all at once, and each one's scale is
-// made by its own lanes. Values turn by dimension in the wave's own LDS; tokens of the 16 that take no row keep their codes.
+// A wave: the rows that one request puts into 16 tokens of one head, a block's waves runs of 16 in a row. Rows are loaded once, all at
+// once, and each one's scale is made by its own lanes. Values turn by dimension in the wave's own LDS; tokens of the 16 that take no
+// row keep their codes.
+// Memory bounds it where there are many rows: 131072 of 16 heads of 128 (677 MB) 156 us, 4.3 TB/s (160 where a block's waves take
+// four heads of one run); a decode step's 32 rows are latency, 3.9 us, and 1500 rows of 3 requests 6.8 (the 8-bit cache's 5.2 and
+// 9.1). A row put alone reads and writes its 16 tokens' codes of a value head, 1 KB.
 template <int HD, int W>
 __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
                                                              int64_t x_sr, int each, int groups) {
   constexpr int U = HD / 8, RP = 64 / U, TURNS = 16 / RP;  // 16-byte units of a row, rows of a turn
-  constexpr int LINE = 20;                                 // bytes of a dim in LDS: 16 tokens, and 4 so that dims fall in distinct banks
+  // bytes of a dim in LDS, 16 tokens and 4 more, every 8th dim's in a row: what the lanes write at once falls in distinct banks
+  constexpr int LINE = 20;
   __shared__ __attribute__((aligned(16))) uint8_t turned[W][HD * LINE];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lg = c.page_log2;
-  const int at = blockIdx.x / groups, h = (blockIdx.x - at * groups) * W + w;
-  if (h >= 2 * c.kv) return;
+  const int heads = 2 * c.kv, h = blockIdx.x % heads, at = blockIdx.x / heads * W + w;
   Piece p;
   if (each) {  // pieces of every request
+    if (at / each >= b.requests) return;
     p = whole_piece(b, at / each);
     p.k = at - p.r * each;
   } else if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> 4) + 2 * i; }, &p)) {
@@ -135,9 +140,9 @@ __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, co
       }
       if (row < count) {
         const uint32_t codes = fp4_codes(f, 1.0f);
-        uint8_t *to = turned[w] + 8 * unit * LINE + token;
+        uint8_t *to = turned[w] + unit * LINE + token;
 #pragma unroll
-        for (int k = 0; k < 8; k++) to[k * LINE] = (uint8_t)(codes >> 4 * k & 15);
+        for (int k = 0; k < 8; k++) to[k * U * LINE] = (uint8_t)(codes >> 4 * k & 15);
         if (unit == 0) ((uint16_t *)(rec + Record<HD>::value_scales(lg)))[in + token] = (uint16_t)(__float_as_uint(s) >> 16);
       }
     }
@@ -150,7 +155,7 @@ __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, co
 #pragma unroll
   for (int i = 0; i < HD / 64; i++) {
     const int e = (HD / 64) * lane + i, dim = e >> 5 << 5 | (e & 1) << 4 | (e >> 1 & 15);
-    const uint32_t *line = (const uint32_t *)(turned[w] + dim * LINE);
+    const uint32_t *line = (const uint32_t *)(turned[w] + (dim % 8 * U + dim / 8) * LINE);
     uint32_t half[2];
 #pragma unroll
     for (int k = 0; k < 2; k++) {  // a byte a token to half a byte
@@ -163,7 +168,7 @@ __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, co
 }
 
 // A block: 64 tokens of a page (or all of a shorter one), keys' or values', of one key head as bf16 rows, 16 tokens a wave. Values
-// turn back through the wave's LDS.
+// turn back through the wave's LDS. 12.6 million values (32 MB read and written) 6.5 us, 270 million (680 MB) 127 us, 5.4 TB/s.
 template <int HD>
 __global__ void __launch_bounds__(256) read_pages4_kernel(const PoolArgs c, uint16_t *out, int runs) {
   constexpr int U = HD / 8, RP = 64 / U, LINE = HD + 8;  // (rows of LDS 16 bytes apart from a power of two)
@@ -369,7 +374,11 @@ __device__ __forceinline__ void walk4(const AttendArgs &a, int r, int kvh, int b
   }
 }
 
-// Few query pairs a request, a part a block of NW waves, as few_pairs in pages.hip.
+// Few query pairs a request, a part a block of NW waves, as few_pairs in pages.hip. Memory bounds it, less a launch's start and end: 32
+// requests of 4096 keys of 8 heads of 128 (140 MB) 26.4 us, 5.3 TB/s (8 bits, 269 MB: 44.8), 8 of up to 16383 (105 MB) 22.3. Dropped:
+// two blocks of keys ahead of the one at work (27 % more registers; the 26.4 us 28.2); scores from 8-bit products of q in two parts
+// with keys' codes as they are, which saves the keys' conversion (prompts 118 us for 122, but the 26.4 us 27.6, drafts 14.0 and
+// 16.2, a token 5.0 and 5.3: q's parts cost more than a few blocks' keys, and the product's own sums are less exact, 2^-17).
 template <int HD, int QT, int NW, bool ONE>
 __device__ __forceinline__ void few_pairs4(const AttendArgs &a, const int block, const int tid, FewLds<HD, QT, NW> &lds) {
   const int lane = tid & 63;
@@ -394,7 +403,9 @@ __global__ void __launch_bounds__(64 * NW, 2) pages4_few_kernel(const AttendArgs
 
 // Many query pairs a request, 128 of one key head a block: 8 waves, two halves of 4 that take every other block of keys, each wave
 // 32 pairs. Every wave loads its keys as the parts' do, four of them the same, from the caches: 4 bits are few enough for that
-// (a block of 64 keys and heads of 128 is 8.4 KB), and the waves keep no step with each other.
+// (a block of 64 keys and heads of 128 is 8.4 KB), and the waves keep no step with each other: two prompts of up to 2048 rows behind
+// cached ones 122 us, through LDS with a barrier a block, as the 8-bit cache's, 138 (that one's are 129); in blocks of one half 106. The
+// vector instructions beside the matrix ones bound it: a prompt of 4096 rows of 32 heads of 128 (137 GF) 156 us, 0.88 PFLOP/s.
 template <int HD> struct Many4Lds {
   f32x4 joined[4 * (HD / 16) * 64];
   float sums[8 * 64];
@@ -465,10 +476,11 @@ template <int HD> static int launch_put4(const PoolArgs &c, const BatchArgs &b, 
                                          hipStream_t s) {
   const int heads = 2 * c.kv, each = most == 1 ? 1 : most <= 16 ? 2 : 0;
   const int64_t pieces = each ? (int64_t)each * b.requests : (b.rows >> 4) + 2 * b.requests;
-  const int waves = pieces * heads <= 2048 ? 1 : 4, groups = (heads + waves - 1) / waves;
-  if (!grid_fits(pieces * groups, 64 * waves)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, heads);
-  if (waves == 1) put_pages4_kernel<HD, 1><<<(unsigned)(pieces * groups), 64, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
-  else put_pages4_kernel<HD, 4><<<(unsigned)(pieces * groups), 256, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
+  const int waves = pieces * heads <= 2048 ? 1 : 4, groups = heads;
+  const int64_t blocks = (pieces + waves - 1) / waves;
+  if (!grid_fits(blocks * groups, 64 * waves)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, heads);
+  if (waves == 1) put_pages4_kernel<HD, 1><<<(unsigned)(blocks * groups), 64, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
+  else put_pages4_kernel<HD, 4><<<(unsigned)(blocks * groups), 256, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
   BT_LAUNCHED("a paged put");
   return BT_OK;
 }
