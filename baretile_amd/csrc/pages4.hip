@@ -93,10 +93,11 @@ __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, co
   } else if (!find_piece(b, at, lane, [&](int i, int s) { return (s >> 4) + 2 * i; }, &p)) {
     return;  // request r owns pieces starts[r] / 16 + 2 r and on: at least as many as the 16 tokens its rows touch
   }
-  const int cached = p.len - p.n, token0 = ((cached >> 4) + p.k) << 4;
+  const int cached = p.len - p.n, run = (cached >> 4) + p.k, on = run >> (lg - 4);
+  if (on >= b.width) return;  // (before anything is counted in tokens, whatever lengths say)
+  const int token0 = run << 4, in = token0 & ((1 << lg) - 1);
   const int from = max(cached, token0), count = min(p.len, token0 + 16) - from, held = from - token0;
-  const int on = token0 >> lg, in = token0 & ((1 << lg) - 1);
-  if (count <= 0 || on >= b.width) return;
+  if (count <= 0) return;
   const int id = gload(b.tables + p.r * b.tables_sr + on);  // the rows are requested before it is looked at
   const int unit = lane % U, row0 = lane / U;
   const uint16_t *src = x + h * x_sb + (int64_t)(p.row0 + from - cached) * x_sr + 8 * unit;

@@ -93,6 +93,29 @@ def test_rows_in_order(rt, vocab, k):
   checked(rt, np.stack([up, -up, up % 0.1, np.where(blocks, 10 + up, up), np.where(np.arange(vocab) < 300, up + 3, up)]), [0, 1, 2, 3, 4], k)
 
 
+@pytest.mark.parametrize("rows, vocab", [(2100, 9002), (1100, 33000), (5000, 5000), (700, 70001)])
+@pytest.mark.parametrize("k", [0, 1, 20, 64])
+def test_rows_walked_a_chunk_at_a_time(rt, rows, vocab, k):
+  # rows enough that a block takes several chunks of one: rows whose every chunk passes the bound of the one before, rows that begin
+  # with nothing, or with fewer than k, ties within and across chunks, infinities and NaNs, among random ones
+  rng = np.random.default_rng(rows + k)
+  x = rng.normal(0, 2, (rows, vocab)).astype(np.float32)
+  at = np.arange(vocab)
+  some = [at / 64.0, -at / 64.0, np.where(at < vocab - 70, -INF, at / 8.0), np.where(at % 1000 == 5, 1.0, -INF), np.zeros(vocab), np.full(vocab, -INF),
+          np.where(at // 4096 % 2 == 1, 3.0, -INF), np.floor(at / 300.0), np.where(at >= vocab // 2, INF, at), np.where(at % 3 == 0, np.nan, at % 977),
+          np.where(at < 30, 50.0 - at, -at / 64.0), np.where(at == vocab - 1, 0.0, -INF)]
+  for i, a in enumerate(some): x[i::rows // 4][:4] = a
+  t = rng.uniform(0.3, 2, rows).astype(np.float32)
+  t[::7], t[1::50] = 1, INF
+  ids = rng.integers(-1, vocab, rows)
+  got = serve.logprobs(fp32(rt, x), row(rt, ids), k, fp32(rt, t[:, None]))
+  looked = np.unique(np.concatenate([np.arange(i, rows, rows // 4)[:4] for i in range(20)] + [np.arange(rows - 5, rows)]))
+  part = [back(v, np.int32 if v.dtype == "int32" else np.float32) for v in got]
+  want = L.logprobs(x[looked], ids[looked], k, t[looked])
+  assert near(part[0][0][looked], want[0], want[4]) and near(part[1][0][looked], want[1], want[5])
+  if k: assert np.array_equal(part[3][looked], want[3]) and near(part[2][looked], want[2], want[6])
+
+
 @pytest.mark.parametrize("vocab", [100, 4096, 30000])
 @pytest.mark.parametrize("k", [0, 1, 8, 64])
 def test_masked_rows(rt, vocab, k):

@@ -469,6 +469,40 @@ def test_stays_within_its_memory(rt, hd, page, lengths, new, window):
   kept(store, args.pages * kv * page * (hd + hd // 32 + 2))
 
 
+@pytest.mark.parametrize("new, most", [([1, 1, 1], 1), ([3, 9, 2], 9), ([40, 3, 20], None)])
+@pytest.mark.parametrize("hd, page", [(64, 16), (128, 64)])
+def test_stray_starts_and_lengths_touch_nothing_else(rt, hd, page, new, most):
+  # starts and lengths that no plan makes: any rows and places, but nothing outside the pool's and the results' memory
+  rng = np.random.default_rng(hd + sum(new))
+  kv, heads, rows, guard = 2, 4, sum(new) + 2, 1 << 16
+  pool, width = pool4(rt, 12, kv, hd, page), 4
+  store = Storage(rt, pool.storage.nbytes + 2 * guard)
+  rt.fill32(store.addr, 0xA5A5A5A5, store.nbytes // 4)
+  rt.fill32(store.addr + guard, 0, pool.storage.nbytes // 4)
+  args = _lib.PagesArgs(store.addr + guard, 0, 12, page, kv, hd)
+  tables = rng.permutation(12).reshape(3, 4)
+  b, _ = planned(rt, pool, tables, [5, 0, 7], new, [-1], rows, most=most)
+  x, q = Tensor.of(rt, bf16_rows(rng, 2 * kv, rows, hd)), Tensor.of(rt, B.bf16(rng.normal(0, 0.2, (heads, rows, hd))))
+  n = heads * rows * hd * 2
+  out = Storage(rt, n + 2 * guard)
+  rt.fill32(out.addr, 0xA5A5A5A5, out.nbytes // 4)
+  need = ctypes.c_uint64()
+  _lib.call("pages4_attend_scratch", ctypes.byref(args), ctypes.byref(b.args), heads, 0, ctypes.byref(need))
+  scratch = Storage(rt, max(need.value, 16))
+  big = 2 ** 31 - 1
+  for starts, lengths in (([0, 10, 9000, 9001], [5, 6, 7]), ([-5, 1, 2, 3], [0, -9, 40]), ([3, 1, 0, 2], [big, big - 3, -big]), ([0, 1, 2, 3], [big, big, big]),
+                          ([0, rows, rows, rows], [big, 0, 0]), ([big, -big, big, 0], [-1, big, 12]), ([0, 1, 2, 3], [width * page, width * page + 1, 1 << 30])):
+    b.starts.assign(row(rt, starts))
+    b.lengths.assign(row(rt, lengths))
+    rt.run("put", "pages4_put", ctypes.byref(args), ctypes.byref(b.args), x.addr, x.sb, x.sr)
+    rt.run("attend", "pages4_attend", ctypes.byref(args), ctypes.byref(b.args), q.addr, q.sb, q.sr, out.addr + guard, rows * hd, hd, heads, 0,
+           scratch.addr, need.value)
+    rt.wait()
+  for s, size in ((store, pool.storage.nbytes), (out, n)):
+    got = bytes(rt.download(s.addr, s.nbytes))
+    assert got[:guard] == b"\xa5" * guard and got[guard + size:] == b"\xa5" * (len(got) - guard - size)
+
+
 def numpy_step(L, ids, w, c, caches, plan, places):
   """Logits of every row as paged_forward gives them, over NumPy pages of 4 bits."""
   tables, starts, lengths = plan
