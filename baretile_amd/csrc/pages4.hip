@@ -453,10 +453,11 @@ template <int HD, int HALVES, bool ONE> __global__ void __launch_bounds__(256 * 
 
 // ---- entry points ----------------------------------------------------------------------------------------------------
 
-// Blocks of tiles past which each is 4 waves, so that two share a CU and one's start and end lie beside the other's work; up to it, 8:
-// prompts of 32 heads of 128, 8 of 300 rows (664 blocks) 71 us as 8 waves, 62 as 4; 4096 rows (1032) 183 and 156; 2048 (520) 61
-// and 63; 1536 (392) 40 and 47.
-constexpr unsigned HALVED = 640;
+// Blocks of tiles past which each is 4 waves, so that two share a CU and one's start and end lie beside the other's work; up to it, 8.
+// Prompts of 32 heads of 128, as 8 and as 4 waves: 4096 rows (1032 blocks) 183 and 153 us, 8 of 300 (664) 71 and 62, 16 of 128 (640)
+// 21.2 and 17.6, 2048 (520) 59 and 63, 1536 (392) 40 and 47; 200 requests of a row beside 8 of 300 (2264) 76 and 56, 16 of 5 rows beside
+// one of 256 (216) 50 and 58.
+constexpr unsigned HALVED = 600;
 template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;
   const unsigned blocks = tiles * p.splits;
