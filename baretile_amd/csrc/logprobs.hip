@@ -85,7 +85,7 @@ constexpr int ROOM = 2 * MOST_K + 16 + PER * limit_of(MOST_K);  // what is there
 template <int NT> struct TopLds {
   uint64_t found[ROOM], best[MOST_K];
   uint32_t tops[NT];
-  int32_t first[NT];
+  int32_t first[NT], counts[NT];
   float least;
   int32_t upto, came[3];  // (a chunk's count, while the last one's is read and the next one's cleared)
 };
@@ -207,14 +207,28 @@ template <int NT> struct Top {
     __syncthreads();
     n += lds.came[turn], turn = turn == 2 ? 0 : turn + 1;
   }
-  // to(rank, value in LDS) for the k first by rank; behind a barrier.
+  // to(rank, value in LDS) for the k first by rank; behind a barrier. More than a wave of them but no more than half the threads are
+  // counted by several threads each, a slice of the others a thread (512 rows of 131072 with 64 alternatives 72 us, so 66).
   template <class To> __device__ __forceinline__ void ranked(To to) {
-    for (int i = threadIdx.x; i < n; i += NT) {
+    const int span = n > 64 && n <= NT / 2 ? NT / 2 : NT, slices = NT / span, slice = threadIdx.x / span, i0 = threadIdx.x % span;
+    const int each = (n + slices - 1) / slices, from = slice * each, end = min(from + each, n);
+    for (int i = i0; i < n; i += span) {
       const uint64_t mine = lds.found[i];
       int rank = 0;
-      for (int j = 0; j < n; j++) rank += lds.found[j] > mine;
-      if (rank < k) to(rank, mine);
+#pragma unroll 4
+      for (int j = from; j < end; j++) rank += lds.found[j] > mine;
+      if (slices == 1) {
+        if (rank < k) to(rank, mine);
+      } else {
+        lds.counts[threadIdx.x] = rank;
+      }
     }
+    if (slices == 1) return;
+    __syncthreads();
+    if (slice || i0 >= n) return;
+    int rank = 0;
+    for (int l = 0; l < slices; l++) rank += lds.counts[l * span + i0];
+    if (rank < k) to(rank, lds.found[i0]);
   }
   // Only the k first stay, and there is a bound from then on.
   __device__ __forceinline__ void keep() {
@@ -287,10 +301,11 @@ __device__ __forceinline__ void store_sums(ChunkSums r, const Inverse &t, ChunkS
 
 // A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against its wave's running maximum; of the
 // chunk that makes the bound they are made while the first wave looks for it.
-// Memory bounds it where rows are many: 512 rows of 131072 with 20 alternatives (268 MB) 47 us, 5.7 TB/s, and a join of 5.2; 777 rows of
-// 49152 without (153 MB) 23.8 us, 6.4 TB/s. One row of 49152 is latency: 5.7 us and a join of 4.4, 32 rows of 131072 8.9 and 5.1.
+// Memory bounds it where rows are many: 512 rows of 131072 with 20 alternatives (268 MB) 47 us where half of them are in the Infinity
+// Cache, 57 where none is, 4.7 TB/s, and a join of 5.6 (with 64 64 and 6.4); 777 rows of 49152 without (153 MB) 23.8 and 27.4 us. One row of 49152 with 5 is latency: 5.9 us and a join of 4.8, 32
+// rows of 131072 with 20 8.5 and 5.9.
 // Dropped: ranks counted over 4 or 8 values at once (the 47 us 49 and more), a wave a chunk with no barrier (one row 5.4 us, but
-// 32 13).
+// 32 13), the next chunk requested ahead of the one at work (three quarters of the blocks; alike).
 template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) logprobs_kernel(const LogprobArgs a) {
   constexpr int W = NT / 64, CHUNK = PER * NT;
   __shared__ TopLds<NT> lds;
@@ -382,7 +397,12 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(const LogprobArgs a
   for (int i = 0; i < PER; i++) {
     const int e = tid + JOIN * i;
     v[i] = NONE, columns[i] = -1;
-    if (e < n) v[i] = gload(a.top_values + (int64_t)row * n + e), columns[i] = gload(a.top_columns + (int64_t)row * n + e);
+    if (JOIN * i < n && e < n) {
+      // each segment's are in order: turned by another step each, so that no thread gets the largest of many (of 32 segments' 64, whose
+      // largest would lie with four threads, the bound let 700 pass: 38 us)
+      const int s = e / a.k, at = s * a.k + (e - s * a.k + (int)((uint32_t)s * 0x9E3779B1u >> 20)) % a.k;
+      v[i] = gload(a.top_values + (int64_t)row * n + at), columns[i] = gload(a.top_columns + (int64_t)row * n + at);
+    }
   }
   const Inverse t = inverse(a, row);
   const Given g = given(a, row);
