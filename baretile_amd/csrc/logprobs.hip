@@ -1,15 +1,16 @@
 // Log probabilities of given tokens, each row's entropy and its likeliest tokens, from rows of logits.
 //
-// With p = softmax(t x) of a row, m its largest logit, y_j = t (x_j - m), S = sum exp(y_j): log p_j = y_j - log S, and the entropy
-// -sum p_j log p_j = log S - sum exp(y_j) y_j / S (no difference of large numbers: both terms are at most log(vocab)). Rows are cut
-// into segments, a block each, which walk through them a chunk at a time: a chunk's logits stay in registers while they are
-// summed against the wave's running maximum and held against a bound. A second launch joins a row's segments; rows of one need none.
+// With p = softmax(t x) of a row, m its largest logit, y_j = t (x_j - m), S = sum exp(y_j): log p_j = y_j - log S, and the
+// entropy -sum p_j log p_j = log S - sum exp(y_j) y_j / S (no difference of large numbers: both terms are at most
+// log(vocab)). Rows are cut into segments, a block each, which walk through them a chunk at a time: a chunk's logits stay in
+// registers while they are summed against the wave's running maximum and held against a bound. A second launch joins a row's
+// segments; rows of one need none.
 //
-// The k largest: whatever is at least the bound goes to LDS, and where that gets full it ranks itself by counting, equal values by
-// their column (so the order in which they came doesn't matter); the k first stay, and the last of them is the new bound. The
-// first bound, and any that lets too much through, comes from a chunk's threads: where k of them have a largest value of T or
-// more, so do the k largest of all, T found by halving over the threads' largest values (one wave's ballots). Where more threads
-// tie at T than that is made for, only the columns up to the one that completes k threads count.
+// The k largest: whatever is at least the bound goes to LDS, and where that gets full it ranks itself by counting, equal
+// values by their column (so the order in which they came doesn't matter); the k first stay, and the last of them is the new
+// bound. The first bound, and any that lets too much through, comes from a chunk's threads: where k of them have a largest
+// value of T or more, so do the k largest of all, T found by halving over the threads' largest values (one wave's ballots).
+// Where more threads tie at T than that is made for, only the columns up to the one that completes k threads count.
 #include "common.h"
 #include <algorithm>
 
@@ -42,8 +43,8 @@ struct LogprobArgs {
 // A logit as it counts: NaN as -inf, +inf as the largest finite.
 __device__ __forceinline__ float logit(float x) { return x != x ? NONE : fminf(x, LARGEST); }
 
-// A row's inverse temperature t, below 0 or NaN as 0. Differences of logits are taken halved, so that they don't pass the largest
-// number, and t is at least the smallest number there is, so that a t of 0 weighs every logit over -inf alike.
+// A row's inverse temperature t, below 0 or NaN as 0. Differences of logits are taken halved, so that they don't pass the
+// largest number, and t is at least the smallest number there is, so that a t of 0 weighs every logit over -inf alike.
 struct Inverse {
   float log2, t;  // (log2: 2 t log2(e))
   bool greedy;  // an infinite t: the first of the largest alone
@@ -299,13 +300,13 @@ __device__ __forceinline__ void store_sums(ChunkSums r, const Inverse &t, ChunkS
   if ((threadIdx.x & 63) == 0) *to = r;
 }
 
-// A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against its wave's running maximum; of the
-// chunk that makes the bound they are made while the first wave looks for it.
-// Memory bounds it where rows are many: 512 rows of 131072 with 20 alternatives (268 MB) 47 us where half of them are in the Infinity
-// Cache, 57 where none is, 4.7 TB/s, and a join of 5.6 (with 64 64 and 6.4); 777 rows of 49152 without (153 MB) 23.8 and 27.4 us. One row of 49152 with 5 is latency: 5.9 us and a join of 4.8, 32
-// rows of 131072 with 20 8.5 and 5.9.
-// Dropped: ranks counted over 4 or 8 values at once (the 47 us 49 and more), a wave a chunk with no barrier (one row 5.4 us, but
-// 32 13), the next chunk requested ahead of the one at work (three quarters of the blocks; alike).
+// A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against its wave's running maximum;
+// of the chunk that makes the bound they are made while the first wave looks for it. Memory bounds it where rows are many:
+// 512 rows of 131072 with 20 alternatives (268 MB) 47 us where half of them are in the Infinity Cache, 57 where none is, 4.7
+// TB/s, and a join of 5.6 (with 64 64 and 6.4); 777 rows of 49152 without (153 MB) 23.8 and 27.4 us. One row of 49152 with 5
+// is latency: 5.9 us and a join of 4.8, 32 rows of 131072 with 20 8.5 and 5.9. Dropped: ranks counted over 4 or 8 values at
+// once (the 47 us 49 and more), a wave a chunk with no barrier (one row 5.4 us, but 32 13), the next chunk requested ahead
+// of the one at work (three quarters of the blocks; alike).
 template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) logprobs_kernel(const LogprobArgs a) {
   constexpr int W = NT / 64, CHUNK = PER * NT;
   __shared__ TopLds<NT> lds;
@@ -430,14 +431,15 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(const LogprobArgs a
 
 // Blocks that fill the card: eight of 256 threads on each of the 256 CUs.
 constexpr int BLOCKS = 2048;
-// Threads of a block: more where a row's chunks' k largest would pass what the join takes. (512 rows of 131072 with 20 alternatives, a
-// chunk a block: 55 us by 256, 59 by 512, 100 by 1024, 83 by 128 and 136 by 64, whose chunks each bring k values to rank.)
+// Threads of a block: more where a row's chunks' k largest would pass what the join takes. (512 rows of 131072 with 20
+// alternatives, a chunk a block: 55 us by 256, 59 by 512, 100 by 1024, 83 by 128 and 136 by 64, whose chunks each bring k
+// values to rank.)
 static int logprobs_threads(const bt_logprobs_args *a) {
   return (int64_t)ceil_div(a->vocab, PER * 256) * std::max(a->k, 1) > PER * JOIN ? 1024 : 256;
 }
-// Chunks of a segment: one, until there are more than fill the card, which then pass a bound that most of their values don't: 512 rows of
-// 131072 with 20 alternatives 61 us in 16384 segments, 47 in 2048, 55 in 4096, 52 in 1024. Without alternatives there is nothing to
-// gain (777 rows of 49152 23.8 us, in segments of 4 chunks 26.8).
+// Chunks of a segment: one, until there are more than fill the card, which then pass a bound that most of their values
+// don't: 512 rows of 131072 with 20 alternatives 61 us in 16384 segments, 47 in 2048, 55 in 4096, 52 in 1024. Without
+// alternatives there is nothing to gain (777 rows of 49152 23.8 us, in segments of 4 chunks 26.8).
 static int logprobs_turns(const bt_logprobs_args *a) {
   const int64_t chunks = ceil_div(a->vocab, PER * logprobs_threads(a));
   if (a->k == 0) return 1;
@@ -452,7 +454,8 @@ static int check_logprobs(const bt_logprobs_args *a) {
   if (a->rows < 1 || a->rows > 1 << 20 || a->vocab < 1 || a->vocab > MOST_VOCAB || a->k < 0 || a->k > MOST_K)
     return fail(BT_EINVAL, "log probabilities of %d rows of %d logits (each 1 to 2^20) with %d alternatives (0 to %d)", a->rows, a->vocab,
                 a->k, MOST_K);
-  if ((int64_t)a->rows * a->vocab > 1ll << 36)  // (a block takes 2^12 at least, and a grid counts its threads in 32 bits)
+  // (a grid counts its threads in 32 bits)
+  if ((int64_t)a->rows * a->vocab > 1ll << 36 || (int64_t)a->rows * logprobs_chunks(a) * logprobs_threads(a) > 0xFFFFFFFFll)
     return fail(BT_EINVAL, "log probabilities of %d rows of %d logits are too large", a->rows, a->vocab);
   return BT_OK;
 }

@@ -1,23 +1,24 @@
 // The paged KV cache in 4 bits a value: rows put into their pages, attention over the pages, and the pages read back. Plans,
 // batches, parts, tiles and joins are the 8-bit cache's (pages.h, pages.hip).
 //
-// A value is a code of one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign (e2m1) times a scale. v_cvt_scalef32_pk_bf16_fp4 turns a byte
-// into two bf16 values times a power of two, so a key's scale, a power of two for 32 of its dims, costs nothing there. A value
-// row has one scale for all of its dims, which the weights of its key are multiplied by before they meet it: O = sum (p_t s_t) c_t.
-// That scale has two bits behind its leading one, since it costs the same (rows of uneven channels: their rounding's error 0.126 of
-// their size for 0.150 under powers of two; 0.126 and 0.127 are a key's under one scale of full precision and under a power of
-// two for each 32 dims). Every scale belongs to one row, so a row's codes are final when it is put: no page is rounded again as it
-// fills, and what it holds doesn't depend on how its rows came.
+// A value is a code of one of 0, 1/2, 1, 3/2, 2, 3, 4, 6 and a sign (e2m1) times a scale. v_cvt_scalef32_pk_bf16_fp4 turns a
+// byte into two bf16 values times a power of two, so a key's scale, a power of two for 32 of its dims, costs nothing there.
+// A value row has one scale for all of its dims, which the weights of its key are multiplied by before they meet it: O = sum
+// (p_t s_t) c_t. That scale has two bits behind its leading one, since it costs the same (rows of uneven channels: their
+// rounding's error 0.126 of their size for 0.150 under powers of two; 0.126 and 0.127 are a key's under one scale of full
+// precision and under a power of two for each 32 dims). Every scale belongs to one row, so a row's codes are final when it
+// is put: no page is rounded again as it fills, and what it holds doesn't depend on how its rows came.
 //
 // A page is one run of bytes, for every key head (`kv` of them) a record of
 //   keys' codes    [page][HD / 2]              a row's dims in order, the even one in a byte's low half;
 //   keys' scales   [page / 16][HD / 32][4][4]  the exponent (biased by 127) of token 16 a + 4 j + i at [a][dims][i][j];
 //   values' codes  [page / 16][HD / 32][16][2][8]  16 tokens of dim 32 c + 16 j + n at [a][c][n][j], the even one in the low half;
 //   values' scales [page]                      bf16.
-// so that attention's operands lie as its lanes take them (pages.hip has the two products): lane (n, g) of a wave holds for tile
-// kt of a block of 64 keys the key 16 (n / 4) + 4 kt + n % 4, dims HD / 4 g and on, which are the codes of all four contraction
-// steps, in one load (the contraction takes dims in any order that both operands share), with the four tiles' exponents in a word; and
-// for dims 32 c .. + 31 the codes of its keys 16 g .. + 15 for dims 32 c + n and 32 c + 16 + n in another.
+// so that attention's operands lie as its lanes take them (pages.hip has the two products): lane (n, g) of a wave holds for
+// tile kt of a block of 64 keys the key 16 (n / 4) + 4 kt + n % 4, dims HD / 4 g and on, which are the codes of all four
+// contraction steps, in one load (the contraction takes dims in any order that both operands share), with the four tiles'
+// exponents in a word; and for dims 32 c .. + 31 the codes of its keys 16 g .. + 15 for dims 32 c + n and 32 c + 16 + n in
+// another.
 #include "pages.h"
 
 namespace bt {
@@ -70,12 +71,12 @@ __device__ __forceinline__ float value_scale(float amax) {
 
 // ---- rows into pages ------------------------------------------------------------------------------------------------
 
-// A wave: the rows that one request puts into 16 tokens of one head, a block's waves runs of 16 in a row. Rows are loaded once, all at
-// once, and each one's scale is made by its own lanes. Values turn by dimension in the wave's own LDS; tokens of the 16 that take no
-// row keep their codes.
-// Memory bounds it where there are many rows: 131072 of 16 heads of 128 (677 MB) 156 us, 4.3 TB/s (160 where a block's waves take
-// four heads of one run); a decode step's 32 rows are latency, 3.9 us, and 1500 rows of 3 requests 6.8 (the 8-bit cache's 5.2 and
-// 9.1). A row put alone reads and writes its 16 tokens' codes of a value head, 1 KB.
+// A wave: the rows that one request puts into 16 tokens of one head, a block's waves runs of 16 in a row. Rows are loaded
+// once, all at once, and each one's scale is made by its own lanes. Values turn by dimension in the wave's own LDS; tokens
+// of the 16 that take no row keep their codes. Memory bounds it where there are many rows: 131072 of 16 heads of 128 (677
+// MB) 156 us, 4.3 TB/s (160 where a block's waves take four heads of one run); a decode step's 32 rows are latency, 3.9 us,
+// and 1500 rows of 3 requests 6.8 (the 8-bit cache's 5.2 and 9.1). A row put alone reads and writes its 16 tokens' codes of
+// a value head, 1 KB.
 template <int HD, int W>
 __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
                                                              int64_t x_sr, int each, int groups) {
@@ -168,8 +169,9 @@ __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, co
   }
 }
 
-// A block: 64 tokens of a page (or all of a shorter one), keys' or values', of one key head as bf16 rows, 16 tokens a wave. Values
-// turn back through the wave's LDS. 12.6 million values (32 MB read and written) 6.5 us, 270 million (680 MB) 127 us, 5.4 TB/s.
+// A block: 64 tokens of a page (or all of a shorter one), keys' or values', of one key head as bf16 rows, 16 tokens a wave.
+// Values turn back through the wave's LDS. 12.6 million values (32 MB read and written) 6.5 us, 270 million (680 MB) 127 us,
+// 5.4 TB/s.
 template <int HD>
 __global__ void __launch_bounds__(256) read_pages4_kernel(const PoolArgs c, uint16_t *out, int runs) {
   constexpr int U = HD / 8, RP = 64 / U, LINE = HD + 8;  // (rows of LDS 16 bytes apart from a power of two)
@@ -240,8 +242,8 @@ template <int HD> struct Block4 {
   u32x4 v[HD / 32], vs[2];
   bool seen;  // whether the values' page is one
 };
-// The weights of a block's 16 pairs, times the values' scales, as bf16: rounded to nearest, since the second product's operand is
-// bf16. l sums them in 32 bits before either, so that a row's weights add up to 1 but for that rounding.
+// The weights of a block's 16 pairs, times the values' scales, as bf16: rounded to nearest, since the second product's
+// operand is bf16. l sums them in 32 bits before either, so that a row's weights add up to 1 but for that rounding.
 template <int HD>
 __device__ __forceinline__ void weigh4(Running<HD> &st, const f32x4 (&s)[4], const u32x4 (&vs)[2], bf16x8 (&p)[2]) {
   const float ref = st.reference(s);
@@ -259,8 +261,8 @@ __device__ __forceinline__ void weigh4(Running<HD> &st, const f32x4 (&s)[4], con
   p[0] = __builtin_bit_cast(bf16x8, w[0]), p[1] = __builtin_bit_cast(bf16x8, w[1]);
 }
 
-// One block of 64 keys against QT tiles of pairs, as fold_block in pages.hip. key: the lane's first key, seen: whether their page is
-// one; values(c): the lane's codes of dims 32 c ..; between: run once the scores are made.
+// One block of 64 keys against QT tiles of pairs, as fold_block in pages.hip. key: the lane's first key, seen: whether their
+// page is one; values(c): the lane's codes of dims 32 c ..; between: run once the scores are made.
 template <int HD, int QT, class Keys, class Values, class Between>
 __device__ __forceinline__ void fold4(const Query<HD, HD / 4> (&q)[QT], Running<HD> (&st)[QT], int key, bool seen, uint32_t ks,
                                       const u32x4 (&vs)[2], Keys keys, Values values, Between between) {
@@ -315,8 +317,8 @@ __device__ __forceinline__ void fold4(const Query<HD, HD / 4> (&q)[QT], Running<
   }
 }
 
-// The blocks b, b + step .. below b1 of request r's keys, by a wave: a block's keys are requested while the block before weighs its
-// scores, its values while it multiplies. ONCE: nobody else reads them, so past the caches.
+// The blocks b, b + step .. below b1 of request r's keys, by a wave: a block's keys are requested while the block before
+// weighs its scores, its values while it multiplies. ONCE: nobody else reads them, so past the caches.
 template <int HD, int QT, bool ONE, bool ONCE>
 __device__ __forceinline__ void walk4(const AttendArgs &a, int r, int kvh, int b, int b1, int step, const int lane,
                                       const Query<HD, HD / 4> (&q)[QT], Running<HD> (&st)[QT]) {
@@ -375,11 +377,12 @@ __device__ __forceinline__ void walk4(const AttendArgs &a, int r, int kvh, int b
   }
 }
 
-// Few query pairs a request, a part a block of NW waves, as few_pairs in pages.hip. Memory bounds it, less a launch's start and end: 32
-// requests of 4096 keys of 8 heads of 128 (140 MB) 26.4 us, 5.3 TB/s (8 bits, 269 MB: 44.8), 8 of up to 16383 (105 MB) 22.3. Dropped:
-// two blocks of keys ahead of the one at work (27 % more registers; the 26.4 us 28.2); scores from 8-bit products of q in two parts
-// with keys' codes as they are, which saves the keys' conversion (prompts 118 us for 122, but the 26.4 us 27.6, drafts 14.0 and
-// 16.2, a token 5.0 and 5.3: q's parts cost more than a few blocks' keys, and the product's own sums are less exact, 2^-17).
+// Few query pairs a request, a part a block of NW waves, as few_pairs in pages.hip. Memory bounds it, less a launch's start
+// and end: 32 requests of 4096 keys of 8 heads of 128 (140 MB) 26.4 us, 5.3 TB/s (8 bits, 269 MB: 44.8), 8 of up to 16383
+// (105 MB) 22.3. Dropped: two blocks of keys ahead of the one at work (27 % more registers; the 26.4 us 28.2); scores from
+// 8-bit products of q in two parts with keys' codes as they are, which saves the keys' conversion (prompts 118 us for 122,
+// but the 26.4 us 27.6, drafts 14.0 and 16.2, a token 5.0 and 5.3: q's parts cost more than a few blocks' keys, and the
+// product's own sums are less exact, 2^-17).
 template <int HD, int QT, int NW, bool ONE>
 __device__ __forceinline__ void few_pairs4(const AttendArgs &a, const int block, const int tid, FewLds<HD, QT, NW> &lds) {
   const int lane = tid & 63;
@@ -402,12 +405,13 @@ __global__ void __launch_bounds__(64 * NW, 2) pages4_few_kernel(const AttendArgs
   few_pairs4<HD, QT, NW, ONE>(a, blockIdx.x, threadIdx.x, lds);
 }
 
-// Many query pairs a request, 128 of one key head a block: 8 waves, two halves of 4 that take every other block of keys, each wave
-// 32 pairs. Every wave loads its keys as the parts' do, four of them the same, from the caches: 4 bits are few enough for that
-// (a block of 64 keys and heads of 128 is 8.4 KB), and the waves keep no step with each other: two prompts of up to 2048 rows behind
-// cached ones 122 us, through LDS with a barrier a block, as the 8-bit cache's, 138 (that one's are 129); in blocks of one half 106. The
-// vector instructions beside the matrix ones bound it: a prompt of 4096 rows of 32 heads of 128 (137 GF) 153 us, 0.90 PFLOP/s; of 8192 563,
-// 0.98. Dropped: queries in LDS and values requested a step later, for three waves a SIMD (27 registers spilled; the 153 us 258).
+// Many query pairs a request, 128 of one key head a block: 8 waves, two halves of 4 that take every other block of keys,
+// each wave 32 pairs. Every wave loads its keys as the parts' do, four of them the same, from the caches: 4 bits are few
+// enough for that (a block of 64 keys and heads of 128 is 8.4 KB), and the waves keep no step with each other: two prompts
+// of up to 2048 rows behind cached ones 122 us, through LDS with a barrier a block, as the 8-bit cache's, 138 (that one's
+// are 129); in blocks of one half 106. The vector instructions beside the matrix ones bound it: a prompt of 4096 rows of 32
+// heads of 128 (137 GF) 153 us, 0.90 PFLOP/s; of 8192 563, 0.98. Dropped: queries in LDS and values requested a step later,
+// for three waves a SIMD (27 registers spilled; the 153 us 258).
 template <int HD> struct Many4Lds {
   f32x4 joined[4 * (HD / 16) * 64];
   float sums[8 * 64];
@@ -453,10 +457,10 @@ template <int HD, int HALVES, bool ONE> __global__ void __launch_bounds__(256 * 
 
 // ---- entry points ----------------------------------------------------------------------------------------------------
 
-// Blocks of tiles past which each is 4 waves, so that two share a CU and one's start and end lie beside the other's work; up to it, 8.
-// Prompts of 32 heads of 128, as 8 and as 4 waves: 4096 rows (1032 blocks) 183 and 153 us, 8 of 300 (664) 71 and 62, 16 of 128 (640)
-// 21.2 and 17.6, 2048 (520) 59 and 63, 1536 (392) 40 and 47; 200 requests of a row beside 8 of 300 (2264) 76 and 56, 16 of 5 rows beside
-// one of 256 (216) 50 and 58.
+// Blocks of tiles past which each is 4 waves, so that two share a CU and one's start and end lie beside the other's work; up
+// to it, 8. Prompts of 32 heads of 128, as 8 and as 4 waves: 4096 rows (1032 blocks) 183 and 153 us, 8 of 300 (664) 71 and
+// 62, 16 of 128 (640) 21.2 and 17.6, 2048 (520) 59 and 63, 1536 (392) 40 and 47; 200 requests of a row beside 8 of 300
+// (2264) 76 and 56, 16 of 5 rows beside one of 256 (216) 50 and 58.
 constexpr unsigned HALVED = 600;
 template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;

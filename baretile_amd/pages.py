@@ -1,5 +1,5 @@
-"""A paged KV cache of 8 or 4 bits a value: requests share a pool of pages through block tables, and a step's tables, row starts, places and
-slots are made on the device from request lengths, so the whole step can be recorded and replayed.
+"""A paged KV cache of 8 or 4 bits a value: requests share a pool of pages through block tables, and a step's tables, row
+starts, places and slots are made on the device from request lengths, so the whole step can be recorded and replayed.
 
 The reference keeps a fixed region a slot (llama.py:293-373), as models.serve.Engine does; here a request holds the pages
 its tokens fill. A page holds the tokens of every key and value head, a head's as 8-bit floats (4 exponent and 3 mantissa bits)
@@ -11,7 +11,7 @@ A step over several requests, each with any number of new tokens (a token, a tok
 the last drafts[r] of request r are drafts (0: none; -1: no token follows yet, as behind a chunk that does not end its prompt,
 or the request brings no row):
 
-  batch = pool.plan(tables, cached, new, free, rows)   # once a step; every block's pool of the same shape shares it
+  batch = pool.plan(tables, cached, new, free, rows)   # once a step; every block's pool of its shape shares it, of either width
   pool.put(batch, x)                                   # each block's keys and values
   o = pool.attend(q, batch)                            # and its attention
   tokens, counts = serve.verify(logits, ids, batch.starts, uniforms, drafts=drafts)
@@ -119,8 +119,8 @@ class Pages:
     448; where a page that holds rows needs a larger one, those are rounded again under it. It stays so until the page is begun
     again, also where it was a refused draft's value that needed it. In 4 bits each row has scales of its own, the smallest under
     which its largest value is at most 7 (a power of two for 32 dims of a key, one of 4 to 7 quarters of one for a value), and
-    what a page holds doesn't depend on the puts that its rows came in. Rows without a page are dropped. Requests may share pages that they
-    only read; a page that takes rows is one request's."""
+    what a page holds doesn't depend on the puts that its rows came in. Rows without a page are dropped. Requests may share pages
+    that they only read; a page that takes rows is one request's."""
     self._fits(batch)
     if not (isinstance(x, Tensor) and x.rt is self.rt and x.dtype == "bf16" and
             (x.batch, x.rows, x.cols) == (2 * self.kv, batch.rows, self.head)):
@@ -135,8 +135,8 @@ class Pages:
 
   def attend(self, q, batch, window=0, merged=False):
     """softmax(q @ k^T + mask) @ v over each row's request (bt_pages_attend, bt_pages4_attend): q (heads, rows, head) bf16, heads a
-    multiple of kv; a row sees its request's keys up to its own place and, with window, the last `window` of them. RoPE scales q beforehand.
-    Rows behind the last request's come back as zeros. merged gives the result as merge() of it, (rows, heads * head)."""
+    multiple of kv; a row sees its request's keys up to its own place and, with window, the last `window` of them. RoPE scales q
+    beforehand. Rows behind the last request's come back as zeros. merged gives the result as merge() of it, (rows, heads * head)."""
     self._fits(batch)
     window = operator.index(window)
     if not 0 <= window < 1 << 31: raise ValueError(f"attention needs a nonnegative window of less than 2^31, not {window}")

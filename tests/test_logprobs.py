@@ -32,7 +32,7 @@ def test_by_torch():
 
 
 @pytest.mark.parametrize("kw", [dict(logits=0), dict(ids=0), dict(logprobs=0), dict(entropy=0), dict(k=3), dict(k=65), dict(k=-1), dict(rows=0),
-                                dict(vocab=0), dict(vocab=(1 << 20) + 1), dict(rows=(1 << 20) + 1), dict(t=2), dict(rows=1 << 20, vocab=1 << 20)])
+                                dict(vocab=0), dict(vocab=(1 << 20) + 1), dict(rows=(1 << 20) + 1), dict(t=2), dict(rows=1 << 20, vocab=1 << 20), dict(rows=1 << 20, vocab=61441)])
 def test_refused(kw):
   args = _lib.LogprobsArgs(**(dict(logits=16, ids=16, logprobs=16, entropy=16, rows=4, vocab=50) | kw))
   with pytest.raises(ValueError): _lib.call("logprobs_scratch", ctypes.byref(args), ctypes.byref(ctypes.c_uint64()))
