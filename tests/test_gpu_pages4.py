@@ -206,6 +206,29 @@ def test_many_requests(rt, requests):
   attended(rt, rng, 4, 2, 64, 16, lengths.tolist(), new.tolist())
 
 
+@pytest.mark.parametrize("hd, page", [(64, 16), (64, 64), (128, 16), (128, 64)])
+def test_many_requests_beside_prompts(rt, hd, page):
+  # tiles enough that each is a block of 4 waves, most of them of requests with few rows, whose parts lie behind them
+  rng = np.random.default_rng(hd + page)
+  lengths = rng.integers(0, 70, 330)
+  new = np.minimum(lengths, rng.choice([0, 1, 3], 330))
+  lengths[[5, 200, 329]], new[[5, 200, 329]] = [150, 90, 300], [100, 70, 130]
+  attended(rt, rng, 4, 2, hd, page, lengths.tolist(), new.tolist(), spare=3)
+
+
+def test_puts_of_many_rows_of_wide_heads(rt):
+  # blocks of four waves, for heads of 128
+  rng = np.random.default_rng(21)
+  filled_pool, values, _ = filled(rt, rng, 4, 128, 64, [5000, 17, 900, 1, 0, 333])
+  assert np.array_equal(whole(filled_pool), values)
+
+
+def test_a_long_cache_of_wide_heads(rt):
+  # parts long enough for blocks of 8 waves
+  attended(rt, np.random.default_rng(22), 4, 1, 128, 256, [140000, 5], [1, 1], most=1)
+  attended(rt, np.random.default_rng(23), 2, 2, 64, 64, [9000, 70], [2, 1], most=2)
+
+
 @pytest.mark.parametrize("window", [1, 7, 64, 100, 1000])
 @pytest.mark.parametrize("lengths, new", [([300, 40], [1, 3]), ([400, 150], [100, 70])])
 def test_attend_window(rt, window, lengths, new):
