@@ -3,7 +3,7 @@
 // With p = softmax(t x) of a row, m its largest logit, y_j = t (x_j - m), S = sum exp(y_j): log p_j = y_j - log S, and the
 // entropy -sum p_j log p_j = log S - sum exp(y_j) y_j / S (no difference of large numbers: both terms are at most
 // log(vocab)). Rows are cut into segments, a block each, which walk through them a chunk at a time: a chunk's logits stay in
-// registers while they are summed against the wave's running maximum and held against a bound. A second launch joins a row's
+// registers while they are summed against a running maximum of the wave's and held against a bound. A second launch joins a row's
 // segments; rows of one need none.
 //
 // The k largest: whatever is at least the bound goes to LDS, and where that gets full it ranks itself by counting, equal
@@ -300,8 +300,8 @@ __device__ __forceinline__ void store_sums(ChunkSums r, const Inverse &t, ChunkS
   if ((threadIdx.x & 63) == 0) *to = r;
 }
 
-// A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against its wave's running maximum;
-// of the chunk that makes the bound they are made while the first wave looks for it. Memory bounds it where rows are many:
+// A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against a running maximum of its
+// wave's; of the chunk that makes the bound they are made while the first wave looks for it. Memory bounds it where rows are many:
 // 512 rows of 131072 with 20 alternatives (268 MB) 47 us where half of them are in the Infinity Cache, 57 where none is, 4.7
 // TB/s, and a join of 5.6 (with 64 64 and 6.4); 777 rows of 49152 without (153 MB) 23.8 and 27.4 us. One row of 49152 with 5
 // is latency: 5.9 us and a join of 4.8, 32 rows of 131072 with 20 8.5 and 5.9. Dropped: ranks counted over 4 or 8 values at
@@ -319,6 +319,16 @@ template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8
   if (a.chunks == 1) g = given(a, row);
   Top<NT> largest{lds, a.k};
   ChunkSums r = {NONE, 0.0f, 0.0f, NOWHERE};
+  // A chunk's 16 weights are summed in 32 bits, the thread's chunks in 64, so that the error doesn't grow with them (of equal
+  // weights in 256 chunks 6 in 10^5, so 1 in 10^6; 512 rows of 131071 with 20 alternatives 2 % slower, the others alike). Weights are
+  // against `ref`, which the wave's maximum passes by a factor of two before what was summed is moved to it: where it creeps up
+  // from chunk to chunk the sums are rounded once a doubling.
+  double s = 0.0, e = 0.0;
+  float ref = NONE;
+  const auto move = [&](float m) {
+    const float d = log2_weight(ref, m, t.log2), by = __builtin_amdgcn_exp2f(d);
+    e = (e + d * s) * by, s *= by, ref = m;
+  };
   const int end = min(from + a.turns, (a.vocab + CHUNK - 1) / CHUNK);
   for (int c = from; c < end; c++) {
     const int v0 = c * CHUNK;
@@ -347,21 +357,27 @@ template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8
     }
     if (a.k && largest.n < a.k) largest.begin(top);
     if (wave_top > r.m) {
-      const float m = fminf(wave_top, LARGEST), d = log2_weight(r.m, m, t.log2), by = __builtin_amdgcn_exp2f(d);
-      r.e = __builtin_fmaf(d, r.s, r.e) * by, r.s *= by;
+      const float m = fminf(wave_top, LARGEST);
       if (m > r.m) r.at = NOWHERE;
       r.m = m;
+      if (log2_weight(ref, m, t.log2) < -1.0f) move(m);
     }
     if (t.greedy && r.at == NOWHERE)
 #pragma unroll
       for (int i = PER - 1; i >= 0; i--)
         if (v[i] == r.m) r.at = column(i);  // the thread's first in this chunk: columns rise with i
+    float chunk_s = 0.0f, chunk_e = 0.0f;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
-      const float y = log2_weight(v[i], r.m, t.log2), w = __builtin_amdgcn_exp2f(y);
-      r.s += w, r.e = __builtin_fmaf(w, y, r.e);
+      const float y = log2_weight(v[i], ref, t.log2), w = __builtin_amdgcn_exp2f(y);
+      chunk_s += w, chunk_e = __builtin_fmaf(w, y, chunk_e);
     }
-    if (c + 1 == end) store_sums(r, t, &sums[wave]);
+    s += chunk_s, e += chunk_e;
+    if (c + 1 == end) {
+      if (ref != r.m) move(r.m);
+      r.s = (float)s, r.e = (float)e;
+      store_sums(r, t, &sums[wave]);
+    }
     if (a.k) largest.chunk(v, top, column, c + 1 < end);
   }
   if (a.k == 0) __syncthreads();

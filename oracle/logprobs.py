@@ -28,12 +28,17 @@ def logprobs(logits, ids, k=0, t=None):
         p, size = w / w.sum(), np.where(real, -y, 0)
         p = np.where(real, p, 0)
         entropy[r] = lse + (p * size).sum()
-        # a weight's exponent has three roundings and its power two units, a sum of 16, 6 of a wave's lanes, up to 16 waves' and the
-        # chunks' likewise about 50; then the logarithm's two units
+        # Roundings of half a unit, eps: a weight's exponent four (relative to it), its power two; a chunk's 16 weights 15, the sum of a
+        # thread's chunks one (it is of 64 bits), its move to the wave's largest logit two; 64 lanes' six, up to 16 waves' by a power each
+        # 18, then the segments' likewise three, six and six: 59. A sum against a reference is moved to another only where that is twice
+        # as far at least, two roundings each time: at most 2 / log(2) a unit of the weight's own distance from the largest, and
+        # two, as the reference may lie a factor of two below. Then the logarithm's two units. The entropy's products have four more, its
+        # quotient and the change of the logarithm's base three, and against a reference that is passed by two a chunk's 16 products may
+        # be that much larger.
         with np.errstate(invalid="ignore"):
           mean = (p * size).sum()
-          slack = eps * (3 * mean + 54 + 4 * lse)
-          off_entropy[r] = slack + eps * (np.nansum(p * size * (3 * size + 58)) + 4 * entropy[r])
+          slack = eps * (7 * mean + 61 + 4 * lse)
+          off_entropy[r] = slack + eps * (np.nansum(p * size * (7 * size + 68)) + 16 + 4 * entropy[r])
     def allowed(at): return 0.0 if logs[at] == -np.inf or t[r] == np.inf else slack + eps * (3 * -y[at] + 2 * abs(logs[at]))
     if 0 <= ids[r] < vocab: given[r], off[r] = logs[ids[r]], allowed(ids[r])
     order = [c for c in np.argsort(-(x[r] + 0.0), kind="stable")[:k] if real[c]]

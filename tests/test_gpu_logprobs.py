@@ -259,3 +259,33 @@ def test_refusals(rt):
              dict(vocab=9000, scratch=x.addr, scratch_bytes=16), dict(vocab=9000, scratch=x.addr + 8, scratch_bytes=1 << 20),
              dict(rows=1 << 20, vocab=1 << 20)):
     with pytest.raises(ValueError): rt.run("refused", "logprobs", ctypes.byref(ok(**kw)))
+
+
+@pytest.mark.parametrize("vocab", [131072, 1 << 20])
+@pytest.mark.parametrize("k", [1, 20, 64])
+def test_sums_of_many_chunks(rt, vocab, k):
+  # rows enough that a block takes 32 to 256 chunks of one, all of them the same row in memory: equal weights whose sum rounds the same
+  # way again and again, nearly equal ones, and largest logits that creep up from chunk to chunk
+  rng = np.random.default_rng(vocab + k)
+  rows, at = 2048, np.arange(vocab)
+  def flat(x):  # with a largest logit that each wave meets in its first chunk
+    return np.where((at < 16384) & (at % 64 == 0), 0.0, x)
+  ids = np.resize([7, vocab // 2, vocab - 1, -1], rows)
+  given, many = row(rt, ids), (rows, k)
+  for x in (flat(-0.58), flat(-0.75), flat(-1.49), np.where(at == vocab - 1, 0.0, -1.2), flat(-1.2 + 1e-3 * rng.normal(0, 1, vocab)),
+            at * (0.02 / 4096), at * (1e-4 / 4096)):
+    x = x.astype(np.float32)
+    logits = fp32(rt, x[None])
+    out = [Tensor(rt, 1, rows, dtype="fp32"), Tensor(rt, 1, rows, dtype="fp32"), Tensor(rt, *many, dtype="fp32"), Tensor(rt, *many, dtype="int32")]
+    args = _lib.LogprobsArgs(logits.addr, given.addr, 0, *(t.addr for t in out), 0, 0, 0, 0, rows, vocab, k, 0)
+    need = ctypes.c_uint64()
+    _lib.call("logprobs_scratch", ctypes.byref(args), ctypes.byref(need))
+    scratch = Storage(rt, max(need.value, 16))
+    args.scratch, args.scratch_bytes = scratch.addr, need.value
+    rt.run("logprobs", "logprobs", ctypes.byref(args))
+    lp, h, values, labels = back(out[0])[0], back(out[1])[0], back(out[2]), back(out[3], np.int32)
+    want = L.logprobs(np.repeat(x[None], 4, 0), ids[:4], k)
+    assert near(lp[:4], want[0], want[4]), (lp[:4], want[0], want[4])
+    assert near(h[:4], want[1], want[5]), (h[:4], want[1], want[5])
+    assert near(values[:4], want[2], want[6]) and np.array_equal(labels[:4], want[3])
+    assert np.array_equal(lp, np.resize(lp[:4], rows)) and np.all(h == h[0]) and np.all(values == values[0]) and np.all(labels == labels[0])
