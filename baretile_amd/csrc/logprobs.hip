@@ -44,20 +44,26 @@ struct LogprobArgs {
 __device__ __forceinline__ float logit(float x) { return x != x ? NONE : fminf(x, LARGEST); }
 
 // A row's inverse temperature t, below 0 or NaN as 0. Differences of logits are taken halved, so that they don't pass the
-// largest number, and t is at least the smallest number there is, so that a t of 0 weighs every logit over -inf alike.
+// largest number, and t is at least the smallest number there is, so that a t of 0 weighs every logit over -inf alike. Past FAR
+// the factor 2 t log2(e) would pass the largest number: there it is a quarter of that, and the 4 comes after it.
+constexpr float FAR = 0x1p126f;
 struct Inverse {
-  float log2, t;  // (log2: 2 t log2(e))
+  float log2, t;  // (log2: 2 t log2(e), or t log2(e) / 2 past FAR)
   bool greedy;  // an infinite t: the first of the largest alone
+  __device__ __forceinline__ bool far() const { return t > FAR; }
 };
 __device__ __forceinline__ Inverse inverse(const LogprobArgs &a, int row) {
   float t = a.t ? gload(a.t + row * a.t_sr) : 1.0f;
   t = t > 0.0f ? t : 0.0f;
   constexpr float least = 1.401298464e-45f;
-  return {fmaxf(fminf(t * (2.0f * LOG2E), LARGEST), least), fmaxf(t, least), t > LARGEST};
+  return {fmaxf(fminf(t * (t > FAR ? 0.5f * LOG2E : 2.0f * LOG2E), LARGEST), least), fmaxf(t, least), t > LARGEST};
 }
 __device__ __forceinline__ float half_less(float x, float m) { return __builtin_fmaf(x, 0.5f, -0.5f * m); }
 // log2 of a weight, down to where it is 0. (-inf - -inf and NaN: 0 weight.)
-__device__ __forceinline__ float log2_weight(float x, float m, float t2) { return fmaxf(half_less(x, m) * t2, -200.0f); }
+__device__ __forceinline__ float log2_near(float x, float m, const Inverse &t) { return fmaxf(half_less(x, m) * t.log2, -200.0f); }
+__device__ __forceinline__ float log2_weight(float x, float m, const Inverse &t) {
+  return t.far() ? fmaxf(half_less(x, m) * t.log2 * 4.0f, -200.0f) : log2_near(x, m, t);
+}
 
 __device__ __forceinline__ float wave_max(float x) {  // as wave_sum in common.h
   const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -265,7 +271,7 @@ template <int W> __device__ __forceinline__ ChunkSums together(const ChunkSums (
 #pragma unroll
   for (int i = 0; i < W; i++) {
     const ChunkSums w = waves[i];
-    const float d = log2_weight(w.m, r.m, t.log2), by = __builtin_amdgcn_exp2f(d);
+    const float d = log2_weight(w.m, r.m, t), by = __builtin_amdgcn_exp2f(d);
     r.s = __builtin_fmaf(w.s, by, r.s), r.e = __builtin_fmaf(__builtin_fmaf(d, w.s, w.e), by, r.e);
     if (w.m == r.m) r.at = min(r.at, w.at);
   }
@@ -320,13 +326,13 @@ template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8
   Top<NT> largest{lds, a.k};
   ChunkSums r = {NONE, 0.0f, 0.0f, NOWHERE};
   // A chunk's 16 weights are summed in 32 bits, the thread's chunks in 64, so that the error doesn't grow with them (of equal
-  // weights in 256 chunks 6 in 10^5, so 1 in 10^6; 512 rows of 131071 with 20 alternatives 2 % slower, the others alike). Weights are
+  // weights in 256 chunks 6 in 10^5, so 1 in 10^6; no case is slower). Weights are
   // against `ref`, which the wave's maximum passes by a factor of two before what was summed is moved to it: where it creeps up
   // from chunk to chunk the sums are rounded once a doubling.
   double s = 0.0, e = 0.0;
   float ref = NONE;
   const auto move = [&](float m) {
-    const float d = log2_weight(ref, m, t.log2), by = __builtin_amdgcn_exp2f(d);
+    const float d = log2_weight(ref, m, t), by = __builtin_amdgcn_exp2f(d);
     e = (e + d * s) * by, s *= by, ref = m;
   };
   const int end = min(from + a.turns, (a.vocab + CHUNK - 1) / CHUNK);
@@ -360,18 +366,22 @@ template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8
       const float m = fminf(wave_top, LARGEST);
       if (m > r.m) r.at = NOWHERE;
       r.m = m;
-      if (log2_weight(ref, m, t.log2) < -1.0f) move(m);
+      if (log2_weight(ref, m, t) < -1.0f) move(m);
     }
     if (t.greedy && r.at == NOWHERE)
 #pragma unroll
       for (int i = PER - 1; i >= 0; i--)
         if (v[i] == r.m) r.at = column(i);  // the thread's first in this chunk: columns rise with i
     float chunk_s = 0.0f, chunk_e = 0.0f;
+    const auto weigh = [&](auto log2) {
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-      const float y = log2_weight(v[i], ref, t.log2), w = __builtin_amdgcn_exp2f(y);
-      chunk_s += w, chunk_e = __builtin_fmaf(w, y, chunk_e);
-    }
+      for (int i = 0; i < PER; i++) {
+        const float y = log2(v[i], ref, t), w = __builtin_amdgcn_exp2f(y);
+        chunk_s += w, chunk_e = __builtin_fmaf(w, y, chunk_e);
+      }
+    };
+    if (__any(t.far())) weigh(log2_weight);  // (one t a row, so the wave's branch: a factor more for all of them costs 1 %)
+    else weigh(log2_near);
     s += chunk_s, e += chunk_e;
     if (c + 1 == end) {
       if (ref != r.m) move(r.m);
@@ -424,7 +434,7 @@ __global__ void __launch_bounds__(JOIN) logprobs_join_kernel(const LogprobArgs a
   const Inverse t = inverse(a, row);
   const Given g = given(a, row);
   Top<JOIN> largest{lds, a.k};
-  const float m = wave_max(r.m), d = log2_weight(r.m, m, t.log2), by = __builtin_amdgcn_exp2f(d);
+  const float m = wave_max(r.m), d = log2_weight(r.m, m, t), by = __builtin_amdgcn_exp2f(d);
   if (r.m < m) r.at = NOWHERE;
   r.e = __builtin_fmaf(d, r.s, r.e) * by, r.s *= by, r.m = m;
   store_sums(r, t, &sums[wave]);

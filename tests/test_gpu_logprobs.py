@@ -289,3 +289,14 @@ def test_sums_of_many_chunks(rt, vocab, k):
     assert near(h[:4], want[1], want[5]), (h[:4], want[1], want[5])
     assert near(values[:4], want[2], want[6]) and np.array_equal(labels[:4], want[3])
     assert np.array_equal(lp, np.resize(lp[:4], rows)) and np.all(h == h[0]) and np.all(values == values[0]) and np.all(labels == labels[0])
+
+
+@pytest.mark.parametrize("vocab", [50, 9000])
+def test_the_largest_temperatures(rt, vocab):
+  # inverse temperatures up to the largest number, over logits so close that they still tell them apart
+  rng = np.random.default_rng(vocab)
+  t = np.array([5e37, 1e38, 1.2e38, 2e38, 3e38, np.finfo(np.float32).max, 3e38], np.float32)
+  x = (rng.normal(0, 1, (len(t), vocab)) / t[:, None]).astype(np.float32)
+  x[-1, ::2] = -3e38
+  for ids in (np.argmax(x, 1), rng.integers(0, vocab, len(t))):
+    for k in (0, 6): checked(rt, x, ids, k, t)
