@@ -459,8 +459,11 @@ template <int HD, int HALVES, bool ONE> __global__ void __launch_bounds__(256 * 
 
 // Blocks of tiles past which each is 4 waves, so that two share a CU and one's start and end lie beside the other's work; up
 // to it, 8. Prompts of 32 heads of 128, as 8 and as 4 waves: 4096 rows (1032 blocks) 183 and 153 us, 8 of 300 (664) 71 and
-// 62, 16 of 128 (640) 21.2 and 17.6, 2048 (520) 59 and 63, 1536 (392) 40 and 47; 200 requests of a row beside 8 of 300
-// (2264) 76 and 56, 16 of 5 rows beside one of 256 (216) 50 and 58.
+// 62, 16 of 128 (640) 28 and 22, 2048 (520) 59 and 62, 1024 (264) 27.6 and 29.5; 16 of 5 rows beside one of 256 (216) 50 and
+// 58. Every request counts as a block, also one with few rows, whose tile is empty: where they are many their parts are most of
+// the work, and those go faster beside each other in blocks of their own. A prompt of 256 rows beside 128 of a row and 500 keys
+// (1128 blocks, 64 of them tiles) 34.9 and 28.2 us, of 100 beside 200 (1680, 32) 49.5 and 38.9, beside 200 of 3000 keys 166 and
+// 138, of 2000 beside 200 (2152, 504) 112 and 86; 16 rows of two requests each over 16384 keys, cut in 32 (768, 512) 43 and 33.
 constexpr unsigned HALVED = 600;
 template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;

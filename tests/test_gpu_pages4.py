@@ -588,3 +588,10 @@ def test_refusals(rt):
   with pytest.raises(ValueError): rt.run("refused", "pages4_read", args[0], 0)
   none = _lib.PagesArgs(0, 0, 10, 16, 2, 64)
   with pytest.raises(ValueError, match="values"): rt.run("refused", "pages4_put", ctypes.byref(none), args[1], x.addr, x.sb, x.sr)
+
+
+@pytest.mark.parametrize("hd, page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("new", [[15, 17], [28, 4]])
+def test_tiles_of_4_waves_whose_keys_are_cut(rt, hd, page, new):
+  # a tile of pairs and a block for each request, times 8 heads and 32 pieces of the keys
+  attended(rt, np.random.default_rng(24), 32, 8, hd, page, [16400, 40], new)
