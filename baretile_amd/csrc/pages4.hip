@@ -468,11 +468,18 @@ constexpr unsigned HALVED = 600;
 template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const AttendPlan &p, hipStream_t s) {
   const unsigned parts = p.items * a.c.kv * p.groups + (a.b.rows + 15) / 16, tiles = p.many_tiles * a.c.kv;
   const unsigned blocks = tiles * p.splits;
-  // blocks of 8 waves where parts are long: heads of 64, whose registers leave room, 8 requests of 32768 keys of 3 heads 24.8 us by 4
-  // and 22.2 by 8, one of 8192 17.5 and 16.0, but 8 of 4096 14.0 and 14.6; of 128 only where all the parts there can be leave a CU
-  // one, one request of 131072 keys of 8 heads 34.5 and 32.8, of 65536 21.9 and 22.1, of 16384 14.0 and 15.0
-  const int64_t held = (int64_t)a.b.width << a.c.page_log2;
-  const bool long_parts = p.join && (HD == 64 ? held >= 8192 : held >= 131072 && MOST_PARTS * a.b.requests * a.c.kv <= 256);
+  // Blocks of 8 waves where parts are long, by what tables can hold: for heads of 64 from where a request's most parts have a block of
+  // keys for each wave, for heads of 128, whose registers leave a CU one such block, where the parts there can be are no more than
+  // the CUs, and the longer the more they are. Times by 4 and by 8 waves, caches from memory:
+  //   128, parts at most: 32 (one key head): 32768 keys 14.5 and 14.9 us, 65536 19.4 and 17.9, 524288 87 and 66; 128: 32768 15.2 and
+  //        15.5, 49152 18.1 and 18.3, 65536 20.5 and 18.5, 262144 50 and 40; 192: 49152 18.8 and 18.2, 65536 21.1 and 20.2, 98304
+  //        25.8 and 23.1; 256 (8 key heads): 32768 16.4 and 17.8, 65536 21.9 and 22.5, 98304 27.5 and 27.4, 131072 33.5 and
+  //        32.6, 524288 100 and 94; 512: 16384 17.6 and 21.0, 131072 52 and 57, 524288 176 and 178
+  //   64: 8192 keys 15.7 and 16.0 (one request of 3 key heads), 27.4 and 27.8 (32), 15.7 and 16.0 (one of 8); 16384 17.9 and 17.6, 41.8
+  //        and 41.7, 17.8 and 17.0; 131072 33.1 and 28.2 (one of 3)
+  // A recorded step whose tables hold more than its caches do is cut by its tables: 16384 keys of 8 heads of 128 14.8 and 15.3.
+  const int64_t held = (int64_t)a.b.width << a.c.page_log2, most = (int64_t)MOST_PARTS * a.b.requests * a.c.kv;
+  const bool long_parts = p.join && (HD == 64 ? held >= 8 * KB * MOST_PARTS : most <= 256 && held >= std::max<int64_t>(65536, 512 * most));
   if (p.many && blocks > HALVED) pages4_mixed_kernel<HD, 1, ONE><<<blocks + parts, 256, 0, s>>>(a);
   else if (p.many) pages4_mixed_kernel<HD, 2, ONE><<<blocks + (parts + 1) / 2, 512, 0, s>>>(a);
   else if (p.tiles == 2) pages4_few_kernel<HD, 2, 4, ONE><<<parts, 256, 0, s>>>(a);

@@ -595,3 +595,10 @@ def test_refusals(rt):
 def test_tiles_of_4_waves_whose_keys_are_cut(rt, hd, page, new):
   # a tile of pairs and a block for each request, times 8 heads and 32 pieces of the keys
   attended(rt, np.random.default_rng(24), 32, 8, hd, page, [16400, 40], new)
+
+
+def test_parts_of_4_and_of_8_waves(rt):
+  # on both sides of the lengths from which a part is a block of 8 waves, by the most parts there can be
+  for i, (heads, kv, hd, page, length, requests) in enumerate([(2, 1, 128, 64, 65535 - 64, 1), (2, 1, 128, 64, 65536, 1), (2, 1, 128, 256, 65530, 5),
+                                                               (2, 1, 128, 128, 81920, 5), (4, 1, 64, 64, 16383 - 64, 2), (4, 1, 64, 64, 16384, 2)]):
+    attended(rt, np.random.default_rng(30 + i), heads, kv, hd, page, [length] + [9] * (requests - 1), [1] * requests, most=1)
