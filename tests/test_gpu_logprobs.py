@@ -300,3 +300,26 @@ def test_the_largest_temperatures(rt, vocab):
   x[-1, ::2] = -3e38
   for ids in (np.argmax(x, 1), rng.integers(0, vocab, len(t))):
     for k in (0, 6): checked(rt, x, ids, k, t)
+
+
+@pytest.mark.parametrize("bits", [8, 4])
+def test_each_tokens_log_probability_over_pages(rt, bits):
+  # a prompt through a model whose logits its cache decides: every token's log probability against the oracle's over a cache of the same
+  # width, within what a broken cache, or the other width's, is past twice over (test_cache_cost.py)
+  import test_cache_cost as M
+  from baretile_amd.models import llama
+  c, w, prompt, ids = M.model()
+  dc = llama.model(**M.CONFIG)
+  dw = llama.upload(rt, {n: v for n, v in w.items() if n not in ("cos", "sin", "turn", "embed.T")}, dc, places=96)
+  caches = llama.paged_cache(rt, dc, 5, M.PAGE, bits=bits)
+  want = M.logits(c, w, prompt, bits)
+  for steps in ([M.ROWS], [30, 1, 1, 5, 13]):  # whole, and in pieces, some of one token
+    tables, at, taken, got = Tensor.of(rt, np.full((1, 4), -1), "int32"), 0, None, []
+    for n in steps:
+      b = caches[0].plan(tables, row(rt, [at]), row(rt, [n]), row(rt, [3, 0, 4, 1]), n, taken)
+      x = llama.paged_forward(row(rt, prompt[at:at + n]), b, dw, dc, caches)
+      out = serve.logprobs(x, row(rt, ids[at:at + n]), 5)
+      same_as_oracle(out, np.frombuffer(x.tobytes(), np.float32).reshape(n, 256), ids[at:at + n], 5, None)
+      got.append(back(out[0])[0])
+      at, taken = at + n, b.taken
+    assert np.abs(np.concatenate(got)[:-1] - M.given(want, ids)).max() <= M.allowed(want)
