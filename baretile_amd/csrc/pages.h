@@ -391,9 +391,11 @@ __device__ __forceinline__ void finish_tile(const AttendArgs &a, const Piece &p,
 
 // ---- a call's checks and plan ----------------------------------------------------------------------------------------
 
-// A pool of 8 bits a value has its scales beside its values; one of 4 bits among them.
+// A pool of 8 bits a value has its scales beside its values; one of 4 bits among them, and `scales` is not looked at.
 inline int check_pool(const bt_pages *c, int bits, PoolArgs *out) {
-  if (!c || !c->values || (bits == 8 && !c->scales)) return fail(BT_EINVAL, "a paged cache needs its values and scales");
+  const uint64_t scales = c && bits == 8 ? c->scales : 0;
+  if (!c || !c->values || (bits == 8 && !scales))
+    return fail(BT_EINVAL, "a paged cache needs its %s", bits == 8 ? "values and scales" : "values");
   if (c->head_dim != 64 && c->head_dim != 128)
     return fail(BT_EINVAL, "a paged cache's heads are 64 or 128 wide, not %d", c->head_dim);
   int lg = 0;
@@ -401,8 +403,8 @@ inline int check_pool(const bt_pages *c, int bits, PoolArgs *out) {
   if (lg < 4 || lg > 8) return fail(BT_EINVAL, "a page holds 16, 32, 64, 128 or 256 tokens, not %d", c->page);
   if (c->kv < 1 || c->kv > 1024 || c->pages < 1 || (int64_t)c->pages * c->page > 0x7FFFFFFFll)
     return fail(BT_EINVAL, "a paged cache of %d pages of %d tokens and %d key heads", c->pages, c->page, c->kv);
-  if (c->values % 16 || c->scales % 4) return fail(BT_EINVAL, "a paged cache's values are 16-byte aligned, its scales 4-byte");
-  if (out) *out = PoolArgs{(uint8_t *)(uintptr_t)c->values, (float *)(uintptr_t)c->scales, c->pages, lg, c->kv};
+  if (c->values % 16 || scales % 4) return fail(BT_EINVAL, "a paged cache's values are 16-byte aligned, its scales 4-byte");
+  if (out) *out = PoolArgs{(uint8_t *)(uintptr_t)c->values, (float *)(uintptr_t)scales, c->pages, lg, c->kv};
   return BT_OK;
 }
 

@@ -78,3 +78,15 @@ def test_scratch_is_the_8_bit_caches():
         _lib.call("pages4_attend_scratch", ctypes.byref(_lib.PagesArgs(16, 0, 9, page, 4, hd)), ctypes.byref(batch), bad, 0, ctypes.byref(a))
     with pytest.raises(ValueError):
       _lib.call("pages4_attend_scratch", ctypes.byref(_lib.PagesArgs(16, 0, 9, page, 4, hd)), ctypes.byref(batch), heads, -1, ctypes.byref(a))
+
+
+@pytest.mark.parametrize("scales", [0, 1, 2, 16, 2 ** 64 - 1])
+def test_scales_of_a_pool_of_4_bits_are_not_looked_at(scales):
+  need = ctypes.c_uint64()
+  pool, batch = _lib.PagesArgs(16, scales, 9, 64, 4, 64), _lib.BatchArgs(16, 16, 16, 16, 40, 5, 40, 9, 3)
+  _lib.call("pages4_bytes", ctypes.byref(pool), ctypes.byref(need))
+  assert need.value == 9 * 4 * 64 * 68
+  _lib.call("pages4_attend_scratch", ctypes.byref(pool), ctypes.byref(batch), 8, 0, ctypes.byref(need))
+  with pytest.raises(ValueError): _lib.call("pages4_attend_scratch", ctypes.byref(_lib.PagesArgs(8, scales, 9, 64, 4, 64)), ctypes.byref(batch), 8, 0, ctypes.byref(need))
+  if scales % 4:  # in 8 bits they are
+    with pytest.raises(ValueError): _lib.call("pages_attend_scratch", ctypes.byref(pool), ctypes.byref(batch), 8, 0, ctypes.byref(need))
