@@ -79,7 +79,7 @@ __device__ __forceinline__ float value_scale(float amax) {
 // a value head, 1 KB.
 template <int HD, int W>
 __global__ void __launch_bounds__(64 * W) put_pages4_kernel(const PoolArgs c, const BatchArgs b, const uint16_t *x, int64_t x_sb,
-                                                             int64_t x_sr, int each, int groups) {
+                                                             int64_t x_sr, int each) {
   constexpr int U = HD / 8, RP = 64 / U, TURNS = 16 / RP;  // 16-byte units of a row, rows of a turn
   // bytes of a dim in LDS, 16 tokens and 4 more, every 8th dim's in a row: what the lanes write at once falls in distinct banks
   constexpr int LINE = 20;
@@ -492,12 +492,15 @@ template <int HD, bool ONE> static int launch_attend4(const AttendArgs &a, const
 template <int HD> static int launch_put4(const PoolArgs &c, const BatchArgs &b, const uint16_t *x, int64_t x_sb, int64_t x_sr, int most,
                                          hipStream_t s) {
   const int heads = 2 * c.kv, each = most == 1 ? 1 : most <= 16 ? 2 : 0;
+  // A wave a block while there are few, so that they spread over the CUs; past that four runs of a head, whose codes lie in a row. By
+  // 1 and by 4, pieces of all heads: 192 3.4 and 3.6 us, 768 3.3 and 3.5 (128 requests of a row), 1520 7.0 and 7.3 (1500 rows), 2080 6.6 and
+  // 7.1, 3072 5.2 and 4.3 (256 requests of 5 rows), 4128 9.0 and 8.5, 8192 9.1 and 7.6, 16384 12.3 and 11.6, 132096 151 and 154.
   const int64_t pieces = each ? (int64_t)each * b.requests : (b.rows >> 4) + 2 * b.requests;
-  const int waves = pieces * heads <= 2048 ? 1 : 4, groups = heads;
+  const int waves = pieces * heads <= 2048 ? 1 : 4;
   const int64_t blocks = (pieces + waves - 1) / waves;
-  if (!grid_fits(blocks * groups, 64 * waves)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, heads);
-  if (waves == 1) put_pages4_kernel<HD, 1><<<(unsigned)(blocks * groups), 64, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
-  else put_pages4_kernel<HD, 4><<<(unsigned)(blocks * groups), 256, 0, s>>>(c, b, x, x_sb, x_sr, each, groups);
+  if (!grid_fits(blocks * heads, 64 * waves)) return fail(BT_EINVAL, "a put of %d rows of %d heads is too large", b.rows, heads);
+  if (waves == 1) put_pages4_kernel<HD, 1><<<(unsigned)(blocks * heads), 64, 0, s>>>(c, b, x, x_sb, x_sr, each);
+  else put_pages4_kernel<HD, 4><<<(unsigned)(blocks * heads), 256, 0, s>>>(c, b, x, x_sb, x_sr, each);
   BT_LAUNCHED("a paged put");
   return BT_OK;
 }
