@@ -215,7 +215,7 @@ template <int NT> struct Top {
     n += lds.came[turn], turn = turn == 2 ? 0 : turn + 1;
   }
   // to(rank, value in LDS) for the k first by rank; behind a barrier. More than a wave of them but no more than half the threads are
-  // counted by several threads each, a slice of the others a thread (512 rows of 131072 with 64 alternatives 72 us, so 66).
+  // counted by several threads each, a slice of the others a thread (the join of 512 rows of 131072 with 64 alternatives 7.4 us, so 6.3).
   template <class To> __device__ __forceinline__ void ranked(To to) {
     const int span = n > 64 && n <= NT / 2 ? NT / 2 : NT, slices = NT / span, slice = threadIdx.x / span, i0 = threadIdx.x % span;
     const int each = (n + slices - 1) / slices, from = slice * each, end = min(from + each, n);
@@ -308,11 +308,11 @@ __device__ __forceinline__ void store_sums(ChunkSums r, const Inverse &t, ChunkS
 
 // A block: a segment of a row, `turns` chunks of PER NT logits. Sums are a thread's own, against a running maximum of its
 // wave's; of the chunk that makes the bound they are made while the first wave looks for it. Memory bounds it where rows are many:
-// 512 rows of 131072 with 20 alternatives (268 MB) 47 us where half of them are in the Infinity Cache, 57 where none is, 4.7
-// TB/s, and a join of 5.6 (with 64 64 and 6.4); 777 rows of 49152 without (153 MB) 23.8 and 27.4 us. One row of 49152 with 5
-// is latency: 5.9 us and a join of 4.8, 32 rows of 131072 with 20 8.5 and 5.9. Dropped: ranks counted over 4 or 8 values at
-// once (the 47 us 49 and more), a wave a chunk with no barrier (one row 5.4 us, but 32 13), the next chunk requested ahead
-// of the one at work (three quarters of the blocks; alike).
+// 512 rows of 131072 with 20 alternatives (268 MB) 49 us where half of them are in the Infinity Cache, 59 where none is, 4.6
+// TB/s, and a join of 5.8 and 6.4 (with 64 66 and 70, 6.3 and 7.0); 777 rows of 49152 without (153 MB) 24.3 and 27.2 us. One row of
+// 49152 with 5 is latency: 5.9 us and a join of 4.5, 32 rows of 131072 with 20 9.2 and 11.2, and 6.2. Dropped: ranks counted over 4
+// or 8 values at once (2 us more on the 49), a wave a chunk with no barrier (one row 5.4 us, but 32 13), the next chunk requested
+// ahead of the one at work (three quarters of the blocks; alike).
 template <int NT, bool WIDE> __global__ void __launch_bounds__(NT, NT == 256 ? 8 : 1) logprobs_kernel(const LogprobArgs a) {
   constexpr int W = NT / 64, CHUNK = PER * NT;
   __shared__ TopLds<NT> lds;

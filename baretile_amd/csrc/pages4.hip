@@ -409,8 +409,10 @@ __global__ void __launch_bounds__(64 * NW, 2) pages4_few_kernel(const AttendArgs
 // each wave 32 pairs. Every wave loads its keys as the parts' do, four of them the same, from the caches: 4 bits are few
 // enough for that (a block of 64 keys and heads of 128 is 8.4 KB), and the waves keep no step with each other: two prompts
 // of up to 2048 rows behind cached ones 122 us, through LDS with a barrier a block, as the 8-bit cache's, 138 (that one's
-// are 129); in blocks of one half 106. The vector instructions beside the matrix ones bound it: a prompt of 4096 rows of 32
-// heads of 128 (137 GF) 153 us, 0.90 PFLOP/s; of 8192 563, 0.98. Dropped: queries in LDS and values requested a step later,
+// are 129); in blocks of one half 106. The vector instructions beside the matrix ones bound it, at work 0.70 of the
+// time, matrix ones 0.35: a prompt of 4096 rows of 32 heads of 128 (137 GF) 154 us, 0.89 PFLOP/s; of 8192 563, 0.98. Heads of 64 have
+// half the products for the same weights, vector instructions 0.73 and matrix ones 0.23: 4096 rows of 32 118 us, 0.58, of 8192 389,
+// 0.71. Dropped: queries in LDS and values requested a step later,
 // for three waves a SIMD (27 registers spilled; the 153 us 258).
 template <int HD> struct Many4Lds {
   f32x4 joined[4 * (HD / 16) * 64];
