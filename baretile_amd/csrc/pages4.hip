@@ -496,7 +496,7 @@ template <int HD> static int launch_put4(const PoolArgs &c, const BatchArgs &b, 
   const int heads = 2 * c.kv, each = most == 1 ? 1 : most <= 16 ? 2 : 0;
   // A wave a block while there are few, so that they spread over the CUs; past that four runs of a head, whose codes lie in a row. By
   // 1 and by 4, pieces of all heads: 192 3.4 and 3.6 us, 768 3.3 and 3.5 (128 requests of a row), 1520 7.0 and 7.3 (1500 rows), 2080 6.6 and
-  // 7.1, 3072 5.2 and 4.3 (256 requests of 5 rows), 4128 9.0 and 8.5, 8192 9.1 and 7.6, 16384 12.3 and 11.6, 132096 151 and 154.
+  // 7.1, 3088 7.5 and 7.4, 4128 9.0 and 8.5, 8192 9.1 and 7.6 (256 requests of 5 rows), 16384 12.3 and 11.6, 132096 151 and 154.
   const int64_t pieces = each ? (int64_t)each * b.requests : (b.rows >> 4) + 2 * b.requests;
   const int waves = pieces * heads <= 2048 ? 1 : 4;
   const int64_t blocks = (pieces + waves - 1) / waves;
